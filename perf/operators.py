@@ -218,7 +218,7 @@ def _own_rope(s):
     qkv = s["qkv"]
     q = ops.rope_append(qkv[:, :H * D], qkv[:, H * D:(H + KV) * D], qkv[:, (H + KV) * D:], s["k"], s["v"], s["cu"],
                         s["kv"], s["table"], s["freq"], interleaved=c["layout"] == "interleaved", mscale=s["m"],
-                        q_norm=s.get("qn"), k_norm=s.get("kn"), eps=1e-6, max_q=s["max_q"])
+                        q_norm=s.get("qn"), k_norm=s.get("kn"), eps=1e-6)
     return q, s["k"], s["v"]
 
 
