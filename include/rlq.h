@@ -319,6 +319,101 @@ int rlq_moe_native(const void *x, int x_stride, const float *logits, int logit_s
 int rlq_moe_swiglu(const float *gu, int gu_stride, int A, int I, const float *cs, void *act, int act_stride,
                    void *stream);
 
+/* ---------------------------------------------------------------- positions and cache */
+
+/* The paged key/value cache that rlq_rope_append writes and rlq_attention reads. k_cache and
+ * v_cache are device arrays of 16-bit elements (RLQ_F16 or RLQ_BF16), 16-byte aligned,
+ * [n_pages][kv_heads][page_size][D]; page_size is a multiple of 32, D (the head size) 64, 128
+ * or 256. The [page_size][D] elements of a page and head are blocks of 32 positions, each in
+ * matrix-operand order:
+ *   keys    [D/16][2][32][8]: element (s, h, p, i) is dimension 16 s + 8 h + i of position p;
+ *   values  [D/32][2][2][32][2][4]: element (u, t, h, d, a, b) is dimension 32 u + d of
+ *           position 16 t + 8 a + 4 h + b.
+ * A call's rows belong to B sequences: rows cu_q[b] .. cu_q[b+1]-1 (int32 [B+1], rising, from 0) are
+ * the last tokens of sequence b, which then holds kv_len[b] tokens (int32 [B]), its position p
+ * on page table[b][p / page_size] (int32 [B][table_stride], table_width entries used). Row i of a
+ * sequence with n rows has position kv_len[b] - n + i. All four arrays are device memory, so a
+ * captured graph follows them. Rows from cu_q[B] on belong to no sequence: nothing is read
+ * from them and nothing written to them. A table entry outside [0, n_pages), such as -1 for a
+ * page given back behind a sliding window, and positions past the table's width name no page:
+ * nothing is written there and no row sees those keys. Nothing is read from pages that no entry
+ * names, or from a page behind a sequence's last token into a result. A sequence holds at most
+ * 2^29 tokens. */
+
+/* Frequencies of rotary positions, freq[i] (host memory, rot/2 doubles, radians per token) for
+ * the pair i of `rot` rotated dimensions: base^(-2i/rot), and for contexts longer than the
+ * model's own by `factor` >= 1:
+ *   RLQ_ROPE_LINEAR  divided by factor;
+ *   RLQ_ROPE_NTK     with base * factor^(rot/(rot-2)): the fastest pair stays, the slowest is
+ *                    divided by factor;
+ *   RLQ_ROPE_PARTS   by the turns a pair makes over the `original` context: at most `low` turns
+ *                    divided by factor, at least `high` kept, mixed linearly between.
+ * low, high and original are read for PARTS only, factor not for PLAIN. */
+enum { RLQ_ROPE_PLAIN = 0, RLQ_ROPE_LINEAR = 1, RLQ_ROPE_NTK = 2, RLQ_ROPE_PARTS = 3 };
+int rlq_rope_frequencies(int scaling, int rot, double base, double factor, double low, double high, double original,
+                         double *freq);
+
+/* The rows of a layer's q, k and v projections into rotated queries and the paged cache
+ * (kernels/ops.metal:468-519, dispatched by src/engine.mm:1176-1186). q fp32 [T][q_stride] with
+ * heads * D elements a row, k and v fp32 with kv_heads * D (slices of one stacked product, say);
+ * q_out 16-bit (dtype) [T][q_out_stride]. Per head of q and k:
+ *   x = x * (1 / sqrt(mean x^2 + eps)) * q_norm (k_norm), fp32 [D], where that is not NULL;
+ *   then each pair (x1, x2) of the first rot dimensions turned by position * freq[i] and scaled:
+ *   mscale * (x1 cos - x2 sin, x1 sin + x2 cos); pairs (i, i + rot/2), or (2i, 2i+1) with
+ *   `interleaved`. freq: device memory, rot/2 doubles. rot = 0 turns nothing.
+ * v is stored as it is. Values are rounded once, to dtype. T at most 2^26, B at most 2^20; heads a
+ * multiple of kv_heads, query head h shares key/value head h / (heads / kv_heads). No two
+ * tokens of a call may name the same position of the same page. */
+int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, const float *v, int v_stride, int T,
+                    const double *freq, int rot, int interleaved, float mscale, const float *q_norm,
+                    const float *k_norm, float eps, int heads, int kv_heads, int D, int dtype, void *q_out,
+                    int q_out_stride, void *k_cache, void *v_cache, int n_pages, int page_size, const int *cu_q,
+                    const int *kv_len, const int *table, int table_stride, int table_width, int B, void *stream);
+
+/* ---------------------------------------------------------------- attention */
+
+/* Causal attention of the call's rows over their sequences' cached keys and values, the rows'
+ * own among them (append them first), as attn_flash and attn_combine
+ * (kernels/flash.metal:132,339):
+ *   s_j = scale * q . k_j, with softcap > 0: softcap * tanh(s_j / softcap);
+ *   out = sum_j softmax(s)_j v_j over the keys j <= position, and j > position - window where
+ *   window > 0. A row that sees no key is zero. Infinities and NaN in keys and values that a
+ *   row does not see do not reach it.
+ * q 16-bit (dtype, the cache's) [T][q_stride]; out 16-bit (out_dtype) [T][out_stride], as the o
+ * linear takes its rows. Products, softmax and sums in fp32; weights are rounded to dtype for
+ * the second product, to two terms of it where the cache is RLQ_BF16 and the output RLQ_F16.
+ * max_q and max_kv (host) bound the new and all tokens of a sequence: the kernels and the split
+ * of the keys over workgroups are chosen from them, and results stay right past them. Both
+ * given as they are, calls of the same sizes give the same bits.
+ * The workspace (rlq_attention_workspace_bytes, may be 0; 16-byte aligned, no initialisation)
+ * holds the sums of a split call's parts; calls that overlap must not share it. */
+size_t rlq_attention_workspace_bytes(int T, int heads, int kv_heads, int D, int B, int max_q, int max_kv, int window);
+int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, int D, int dtype, const void *k_cache,
+                  const void *v_cache, int n_pages, int page_size, const int *cu_q, const int *kv_len,
+                  const int *table, int table_stride, int table_width, int B, int max_q, int max_kv, float scale,
+                  int window, float softcap, void *out, int out_stride, int out_dtype, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------- logits */
+
+/* Adjusts rows of logits before a token is chosen from them (rl_top_k_device, rl_argmax); out may
+ * be logits. For token v of a row, with `said` whether v is among the row's tokens and `made`
+ * how many of its tokens from index n_prompt on are v:
+ *   l = said ? (l > 0 ? l / repetition : l * repetition) : l
+ *   l = made ? l - frequency * made - presence : l
+ *   l = l + the sum of the row's biases for v
+ *   l = -inf where the row's mask has bit v % 32 of word v / 32 clear, whatever l was.
+ * tokens int32 [rows][token_stride], max_tokens entries of which n_tokens[row] (NULL: all) count;
+ * n_prompt[row] (NULL: 0); repetition, presence, frequency fp32 [rows] (NULL: 1, 0, 0). bias_ids int32
+ * and bias fp32 [rows][bias_stride], n_bias <= 1024 entries; an id that comes twice adds both.
+ * allowed uint32 [rows][allowed_stride] (NULL: every token). Strides in elements; 0 for tokens,
+ * biases or the mask gives every row the same. Ids outside [0, vocab) are passed over. */
+int rlq_adjust_logits(const float *logits, int64_t stride, int rows, int vocab, const int *tokens,
+                      int64_t token_stride, int max_tokens, const int *n_tokens, const int *n_prompt,
+                      const float *repetition, const float *presence, const float *frequency, const int *bias_ids,
+                      const float *bias, int n_bias, int64_t bias_stride, const uint32_t *allowed,
+                      int64_t allowed_stride, float *out, int64_t out_stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,872 @@
+// Attention of new tokens over the paged cache: the step between rope_append and the o linear.
+// Plays the part of attn_flash and attn_combine (kernels/flash.metal:132,339).
+//
+//   s = scale * q . k            (a cap: s = cap * tanh(s / cap))
+//   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)   over the keys j a row sees:
+//       pos - window < j <= pos, pos = kv_len - q_len + i for row i of its sequence
+//
+// One pass over the keys with a running reference m and running sums in fp32. Rows are (token,
+// query head) pairs of one key/value head, row r = (token r / G, head r % G): the G heads that
+// share a key/value head read it once, and a tile of rows spans few positions.
+// Two kernels: few_rows_kernel (a sequence with at most 32 rows a head: decoding, drafts) is bound
+// by the stream of keys and values, many_rows_kernel by the matrix cores and the exponentials.
+#include "paged.h"
+#include "../../include/rlq.h"
+
+#include <algorithm>
+
+namespace rlq {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kFewRows = 32;      // rows of a few_rows_kernel tile
+constexpr int kManyRows = 128;    // rows of a many_rows_kernel tile
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Weights are exp2(x - ref) with x the score in base-2 units. ref follows the largest score
+// seen, kRefBelow under it, and moves only when a score passes ref + kRefBelow + kRefSlack: most
+// steps then leave the accumulators alone. A weight is at most 2^15, inside fp16, and 2^-14, where
+// fp16 loses bits, lies 2^21 under the largest: what is lost there does not show in the sum.
+constexpr float kRefBelow = 7.0f, kRefSlack = 8.0f;
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+struct AttnArgs {
+  const void *q;
+  void *out;
+  PagedCache c;
+  int64_t q_stride, out_stride;
+  float *part, *part_ml;      // [splits][rows][heads][D] and [splits][rows][heads][2]: sums, (ref, weight sum)
+  int heads, group, window, out_bf16, q_wide, out_wide;
+  int splits, span;           // keys are split in runs of `span` positions (a multiple of 32)
+  int few_splits, few_span;   // the same for sequences of few rows
+  int few, many;              // which kernels this call launches
+  float scale_log2, cap_log2, inv_cap;
+};
+
+template <typename T>
+struct Mfma;
+template <>
+struct Mfma<_Float16> {
+  typedef half8 op;
+  static __device__ __forceinline__ f32x4 mul16(op a, op b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mul32(op a, op b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static constexpr unsigned kExp = 0x7C00u;
+};
+template <>
+struct Mfma<__bf16> {
+  typedef bf16x8 op;
+  static __device__ __forceinline__ f32x4 mul16(op a, op b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mul32(op a, op b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static constexpr unsigned kExp = 0x7F80u;
+};
+
+// A score in base-2 units. The cap's tanh y = 1 - 2 / (1 + e^2y) has an error of about 2^-23
+// absolute, times cap: far under what the weight's 16 bits keep.
+__device__ __forceinline__ float score(const AttnArgs &a, float s) {
+  if (a.cap_log2 == 0.0f) return s * a.scale_log2;
+  const float e = __builtin_amdgcn_exp2f(s * a.inv_cap);
+  return a.cap_log2 - 2.0f * a.cap_log2 * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// Eight weights as a matrix operand. TERMS 2 (bf16 keys, fp16 rows out): the rounding's remainder
+// as a second operand, so that no weight has fewer bits than the rows that leave.
+template <typename T, int TERMS>
+__device__ __forceinline__ void weights(const float (&p)[8], typename Mfma<T>::op (&w)[TERMS]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const T hi = static_cast<T>(p[e]);
+    w[0][e] = hi;
+    if constexpr (TERMS == 2) w[1][e] = static_cast<T>(p[e] - static_cast<float>(hi));
+  }
+}
+
+// Infinities and NaN among values that some row does not see would reach it as 0 * inf. In blocks
+// that are masked for some row the product is therefore formed without them (finite8), and those
+// of keys that some row does see are noted and added at the end to the rows that see them
+// (add_odd). `seen`: bit e, whether any row sees the run's key e; what lies behind a sequence's end
+// is never read into a result.
+template <typename T>
+__device__ __forceinline__ u32x4 finite8(u32x4 v, unsigned seen, bool &odd) {
+  constexpr unsigned E = Mfma<T>::kExp;
+  u32x4 r;
+  unsigned found = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (v[i] & E) == E, hi = (v[i] & (E << 16)) == E << 16;
+    found |= (lo ? 1u << 2 * i : 0u) | (hi ? 2u << 2 * i : 0u);
+    r[i] = (lo ? 0u : v[i] & 0xFFFFu) | (hi ? 0u : v[i] & 0xFFFF0000u);
+  }
+  odd |= (found & seen) != 0;
+  return r;
+}
+
+// What a sequence's rows are in this call.
+struct Seq {
+  int b, row0, tokens, kv, rows;   // rows: of one key/value head
+};
+
+__device__ __forceinline__ Seq sequence(const AttnArgs &a, int b) {
+  Seq s;
+  s.b = b;
+  s.row0 = row_start(a.c, b);
+  s.tokens = max(0, row_start(a.c, b + 1) - s.row0);
+  s.kv = cached(a.c, b);
+  s.rows = s.tokens * a.group;
+  return s;
+}
+
+// Which kernel takes a sequence: few_rows where both run and its rows fit one tile of it.
+__device__ __forceinline__ bool is_few(const AttnArgs &a, const Seq &s) {
+  return a.few && (!a.many || s.rows <= kFewRows);
+}
+
+// First position that any row of the sequence sees, to the block below; the runs of `span` keys
+// begin there.
+__device__ __forceinline__ int first_key(const AttnArgs &a, const Seq &s) {
+  return a.window ? max(0, s.kv - s.tokens + 1 - a.window) & ~(kBlockKeys - 1) : 0;
+}
+
+// Runs that hold keys of the sequence; one run's kernel writes the rows itself.
+__device__ __forceinline__ int runs_of(const AttnArgs &a, const Seq &s, bool few) {
+  const int span = few ? a.few_span : a.span, splits = few ? a.few_splits : a.splits;
+  return max(1, min(splits, (s.kv - first_key(a, s) + span - 1) / span));
+}
+
+__device__ __forceinline__ float *part_row(const AttnArgs &a, int split, int row, int head, int D) {
+  return a.part + ((static_cast<int64_t>(split) * a.c.rows + row) * a.heads + head) * D;
+}
+
+__device__ __forceinline__ float *part_stat(const AttnArgs &a, int split, int row, int head) {
+  return a.part_ml + ((static_cast<int64_t>(split) * a.c.rows + row) * a.heads + head) * 2;
+}
+
+// Adds the infinities and NaN among one block's values to o (o[i]: dimension dim(i)) for the keys
+// that a row sees.
+template <typename T, int D, int N, typename Dim>
+__device__ __forceinline__ void add_odd(const AttnArgs &a, int page, int head, int block, int lo, int hi, Dim dim,
+                                        float (&o)[N]) {
+  const unsigned short *v = static_cast<const unsigned short *>(a.c.v) + block_base(a.c, page, head, block, D);
+  for (int key = 0; key < kBlockKeys; ++key) {
+    const int at = block * kBlockKeys + key;
+    const bool seen = at >= lo && at <= hi;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const unsigned x = v[value_run(dim(i), key >> 4, key >> 2 & 1) + (key >> 3 & 1) * 4 + (key & 3)];
+      if (seen && (x & Mfma<T>::kExp) == Mfma<T>::kExp)
+        o[i] += static_cast<float>(__builtin_bit_cast(T, static_cast<unsigned short>(x)));
+    }
+  }
+}
+
+// Four neighbouring dimensions of a finished row.
+__device__ __forceinline__ void store4(const AttnArgs &a, int row, int col, f32x4 o) {
+  if (a.out_bf16) {
+    __bf16 *p = static_cast<__bf16 *>(a.out) + row * a.out_stride + col;
+    const bf16x4 y = __builtin_convertvector(o, bf16x4);
+    if (a.out_wide) {
+      *reinterpret_cast<bf16x4 *>(p) = y;
+    } else {
+      for (int i = 0; i < 4; ++i) p[i] = y[i];
+    }
+  } else {
+    _Float16 *p = static_cast<_Float16 *>(a.out) + row * a.out_stride + col;
+    const half4 y = __builtin_convertvector(o, half4);
+    if (a.out_wide) {
+      *reinterpret_cast<half4 *>(p) = y;
+    } else {
+      for (int i = 0; i < 4; ++i) p[i] = y[i];
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ typename Mfma<T>::op load_q(const AttnArgs &a, int row, int col) {
+  typedef typename Mfma<T>::op op;
+  const T *p = static_cast<const T *>(a.q) + row * a.q_stride + col;
+  if (a.q_wide) return *reinterpret_cast<const op *>(p);
+  op r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = p[i];
+  return r;
+}
+
+// ----------------------------------------------------------------------------- few rows
+
+// One workgroup: up to 16 * NT rows of one sequence and key/value head over one run of its keys.
+// Its four waves take blocks of 32 keys in turn, straight from memory into registers, each with
+// its own running sums, which meet in LDS at the end: nothing is shared until then, so a wave
+// never waits for another, and 8 waves a CU keep their next keys and values in flight.
+// v_mfma_f32_16x16x32: S^T (keys x rows) = K Q^T with the operand's row r standing for key
+// 16 (r / 8) + r % 8 (then + 8), so that a lane's eight weights belong to one 16-byte run of V.
+template <typename T, int D, int NT, int TERMS>
+__global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kernel(AttnArgs a) {
+  constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * NT;
+  typedef typename Mfma<T>::op op;
+  __shared__ int found[kThreads / 64];
+  __shared__ float stat[4][ROWS][2];
+  __shared__ float sums[2][ROWS][D + 4];
+  __shared__ op queries[NT][KS][64];
+
+  const int KV = a.c.kv_heads, head = blockIdx.x % KV, split = (blockIdx.x / KV) % a.few_splits;
+  const int64_t slot = blockIdx.x / KV / a.few_splits;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, r = lane & 15;
+  const int b = find_sequence<kThreads>(a.c, slot, a.group, ROWS, 1, found);
+  if (b < 0 || b >= a.c.batch) return;
+  const Seq s = sequence(a, b);
+  const int tile = (int)(slot - slot_base(a.c, b, a.group, ROWS, 1)) * ROWS;
+  if (tile < 0 || tile >= s.rows || !is_few(a, s)) return;
+  const int runs = runs_of(a, s, true);
+  if (split >= runs) return;
+
+  // rows of this lane's columns, and what they see
+  int lo[NT], hi[NT], row[NT], col[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int R = tile + n * 16 + r, tok = R / a.group;
+    const bool here = R < s.rows;
+    row[n] = here ? s.row0 + tok : -1;
+    col[n] = (head * a.group + R - tok * a.group) * D;
+    hi[n] = here ? s.kv - s.tokens + tok : -1;                       // last key seen
+    lo[n] = a.window ? max(0, hi[n] - a.window + 1) : 0;             // first
+    for (int k = wave; k < KS; k += 4)
+      queries[n][k][lane] = here ? load_q<T>(a, row[n], col[n] + 32 * k + 8 * g) : op{};
+  }
+  __syncthreads();
+  const int last = min(s.rows, tile + ROWS) - 1;
+  const int lo_any = a.window ? max(0, s.kv - s.tokens + tile / a.group - a.window + 1) : 0;
+  const int lo_all = a.window ? max(0, s.kv - s.tokens + last / a.group - a.window + 1) : 0;
+  const int hi_any = s.kv - s.tokens + last / a.group, hi_all = s.kv - s.tokens + tile / a.group;
+  const int base = first_key(a, s) + split * a.few_span;
+  const int end = min(hi_any + 1, split == a.few_splits - 1 ? hi_any + 1 : base + a.few_span);
+  const int blk0 = max(base, lo_any & ~(kBlockKeys - 1)) / kBlockKeys, blk1 = (end + kBlockKeys - 1) / kBlockKeys;
+
+  f32x4 o[NT][DT];
+  float ref[NT], sum[NT];
+  bool odd = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    ref[n] = -__builtin_inff(), sum[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[n][d] = f32x4{0, 0, 0, 0};
+  }
+
+  const T *kc = static_cast<const T *>(a.c.k), *vc = static_cast<const T *>(a.c.v);
+  // key 16 (r / 8) + r % 8 of a step of 32 dimensions: two operand steps of 16
+  const int koff = (g >> 1) * 512 + (g & 1) * 256 + (16 * (r >> 3) + (r & 7)) * 8;
+  const int voff = (g >> 1) * 512 + (g & 1) * 256 + r * 8;
+  const int key0 = 16 * (g >> 1) + 4 * (g & 1);   // this lane's keys: key0 + 8 j + i
+  op kr[KS][2];
+  u32x4 vr[DT];
+  int pages = -1;                                  // lane i: the page of this wave's i-th block from `from`
+  int from = 0;
+  const int nblk = max(0, blk1 - blk0), mine = nblk > wave ? (nblk - wave + 3) / 4 : 0;
+  auto page_at = [&](int i) {
+    if (i >= mine) return -1;
+    if (i - from >= 64 || i == 0) {
+      from = i;
+      const int blk = blk0 + wave + 4 * (i + lane);
+      pages = i + lane < mine ? page_of(a.c, b, blk) : -1;
+    }
+    return __builtin_amdgcn_readlane(pages, i - from);
+  };
+  auto load_k = [&](int page, int blk) {
+    const T *p = kc + block_base(a.c, page, head, blk, D) + koff;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      kr[k][0] = *reinterpret_cast<const op *>(p + k * 1024);
+      kr[k][1] = *reinterpret_cast<const op *>(p + k * 1024 + 64);
+    }
+  };
+  int page = page_at(0);
+  if (page >= 0) load_k(page, blk0 + wave);
+  for (int i = 0; i < mine; ++i) {
+    const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
+    const int next = page_at(i + 1);
+    if (page < 0) {
+      page = next;
+      if (page >= 0) load_k(page, blk + 4);
+      continue;
+    }
+    const T *vp = vc + block_base(a.c, page, head, blk, D) + voff;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      vr[d] = *reinterpret_cast<const u32x4 *>(vp + (d >> 1) * 1024 + (d & 1) * 128);
+
+    f32x4 sc[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sc[n][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) sc[n][j] = Mfma<T>::mul16(kr[k][j], queries[n][k][lane], sc[n][j]);
+      }
+    if (next >= 0) load_k(next, blk + 4);
+    page = next;
+
+    const bool masked = first < lo_all || first + kBlockKeys - 1 > hi_all || first + kBlockKeys > end;
+    op w[NT][TERMS];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float x[8], top = -__builtin_inff();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = score(a, sc[n][e >> 2][e & 3]);
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = first + key0 + 8 * (e >> 2) + (e & 3);
+          x[e] = key >= lo[n] && key <= hi[n] ? x[e] : -__builtin_inff();
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__any(top > ref[n] + (kRefBelow + kRefSlack))) {
+        const float to = top > ref[n] + (kRefBelow + kRefSlack) ? top - kRefBelow : ref[n];
+        const float f = ref[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref[n] - to);
+        ref[n] = to;
+        sum[n] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[n][d] *= f;
+      }
+      const float m = ref[n] == -__builtin_inff() ? 0.0f : ref[n];
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(x[e] - m);
+        sum[n] += p[e];
+      }
+      weights<T, TERMS>(p, w[n]);
+    }
+    if (masked) {
+      unsigned seen = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = first + key0 + 8 * (e >> 2) + (e & 3);
+        seen |= key >= lo_any && key <= hi_any ? 1u << e : 0u;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vr[d] = finite8<T>(vr[d], seen, odd);
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+          o[n][d] = Mfma<T>::mul16(__builtin_bit_cast(op, vr[d]), w[n][t], o[n][d]);
+  }
+
+  if (__builtin_expect(__any(odd), 0)) {
+    for (int i = 0; i < mine; ++i) {
+      const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
+      if (first >= lo_all && first + kBlockKeys - 1 <= hi_all && first + kBlockKeys <= end) continue;
+      const int at = page_of(a.c, b, blk);
+      if (at < 0) continue;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          float part[4] = {o[n][d][0], o[n][d][1], o[n][d][2], o[n][d][3]};
+          add_odd<T, D, 4>(a, at, head, blk, lo[n], hi[n], [&](int j) { return 16 * d + 4 * g + j; }, part);
+          o[n][d] = f32x4{part[0], part[1], part[2], part[3]};
+        }
+    }
+  }
+
+  // the waves' sums: the largest reference first, then each wave's share scaled to it
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    sum[n] += __shfl_xor(sum[n], 16);
+    sum[n] += __shfl_xor(sum[n], 32);
+    if (g == 0) stat[wave][n * 16 + r][0] = ref[n], stat[wave][n * 16 + r][1] = sum[n];
+  }
+  __syncthreads();
+  float total[NT], top[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    top[n] = -__builtin_inff(), total[n] = 0.0f;
+    for (int w2 = 0; w2 < 4; ++w2) top[n] = fmaxf(top[n], stat[w2][n * 16 + r][0]);
+    for (int w2 = 0; w2 < 4; ++w2) {
+      const float m = stat[w2][n * 16 + r][0];
+      total[n] += m == -__builtin_inff() ? 0.0f : stat[w2][n * 16 + r][1] * __builtin_amdgcn_exp2f(m - top[n]);
+    }
+    const float f = ref[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref[n] - top[n]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][d][i] = ref[n] == -__builtin_inff() ? 0.0f : o[n][d][i] * f;
+  }
+  // waves 2 and 3 hand theirs to waves 0 and 1, then wave 1 to wave 0
+  for (int step = 2; step; step >>= 1) {
+    if (wave >= step && wave < 2 * step) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          *reinterpret_cast<f32x4 *>(&sums[wave - step][n * 16 + r][d * 16 + 4 * g]) = o[n][d];
+    }
+    __syncthreads();
+    if (wave < step) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[n][d] += *reinterpret_cast<const f32x4 *>(&sums[wave][n * 16 + r][d * 16 + 4 * g]);
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (row[n] < 0) continue;
+    if (runs == 1) {
+      const float f = top[n] == -__builtin_inff() ? 0.0f : 1.0f / total[n];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = top[n] == -__builtin_inff() ? 0.0f : o[n][d][i] * f;
+        store4(a, row[n], col[n] + d * 16 + 4 * g, y);
+      }
+    } else {
+      float *p = part_row(a, split, row[n], col[n] / D, D);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p + d * 16 + 4 * g) = o[n][d];
+      if (g == 0) {
+        float *ml = part_stat(a, split, row[n], col[n] / D);
+        ml[0] = top[n], ml[1] = total[n];
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- many rows
+
+// One LDS-DMA: 16 bytes a lane into the kilobyte at lds + at.
+__device__ __forceinline__ void dma_kb(const void *src, unsigned char *lds, int at, int lane) {
+  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(src), (short)0, 1024, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + at), 16, 16 * lane, 0, 0,
+                                           0);
+}
+
+// One workgroup: 128 rows of one sequence and key/value head over one run of its keys; each of its
+// four waves holds 32 rows (Q^T as B operands, O^T accumulators) and takes every key. Keys and
+// values go through LDS in tiles of KB keys, copied as they lie (the cache's order is the
+// operands' order: no swizzle, no transpose, no bank conflicts), two stages deep, so that the
+// next tile's copy runs under this tile's products; one barrier a tile.
+template <typename T, int D, int TERMS>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(AttnArgs a) {
+  constexpr int KB = D == 256 ? 32 : 64, NB = KB / kBlockKeys, KS = D / 16, DT = D / 32;
+  constexpr int kBlockBytes = kBlockKeys * D * 2, kStage = 2 * NB * kBlockBytes, kPieces = kBlockBytes / 1024;
+  typedef typename Mfma<T>::op op;
+  extern __shared__ unsigned char lds[];   // two stages, then find_sequence's few words
+  int *found = reinterpret_cast<int *>(lds + 2 * kStage);
+
+  const int KV = a.c.kv_heads, head = blockIdx.x % KV, split = (blockIdx.x / KV) % a.splits;
+  const int64_t slots = gridDim.x / KV / a.splits, slot = slots - 1 - blockIdx.x / KV / a.splits;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, h = lane >> 5;
+  const int b = find_sequence<kThreads>(a.c, slot, a.group, kManyRows, 1, found);
+  if (b < 0 || b >= a.c.batch) return;
+  const Seq s = sequence(a, b);
+  const int tile = (int)(slot - slot_base(a.c, b, a.group, kManyRows, 1)) * kManyRows;
+  if (tile < 0 || tile >= s.rows || is_few(a, s)) return;
+  const int runs = runs_of(a, s, false);
+  if (split >= runs) return;
+
+  const int R = tile + wave * 32 + n32, tok = R / a.group;
+  const bool here = R < s.rows;
+  const int row = here ? s.row0 + tok : -1, col = (head * a.group + R - tok * a.group) * D;
+  const int hi = here ? s.kv - s.tokens + tok : -1, lo = a.window ? max(0, hi - a.window + 1) : 0;
+  op q[KS];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) q[k] = here ? load_q<T>(a, row, col + 16 * k + 8 * h) : op{};
+
+  // keys that any row of the tile sees, and that all of this wave's rows see
+  const int last = min(s.rows, tile + kManyRows) - 1, p0 = s.kv - s.tokens;
+  const int lo_any = a.window ? max(0, p0 + tile / a.group - a.window + 1) : 0, hi_any = p0 + last / a.group;
+  const int wfirst = min(tile + wave * 32, s.rows - 1), wlast = min(tile + wave * 32 + 31, s.rows - 1);
+  const int lo_all = a.window ? max(0, p0 + wlast / a.group - a.window + 1) : 0, hi_all = p0 + wfirst / a.group;
+  const int base = first_key(a, s) + split * a.span;
+  const int end = min(hi_any + 1, split == a.splits - 1 ? hi_any + 1 : base + a.span);
+  const int blk0 = max(base, lo_any & ~(kBlockKeys - 1)) / kBlockKeys, blk1 = (end + kBlockKeys - 1) / kBlockKeys;
+  const int nblk = max(0, blk1 - blk0), tiles = (nblk + NB - 1) / NB;
+
+  f32x16 o[DT];
+  float ref = -__builtin_inff(), sum = 0.0f;
+  bool odd = false;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+
+  const char *kc = static_cast<const char *>(a.c.k), *vc = static_cast<const char *>(a.c.v);
+  int pages = -1, from = 0;   // lane i: the page of block from + i of the run
+  auto page_at = [&](int i) {
+    if (i >= nblk) return -1;
+    if (i - from >= 64 || i == 0) {
+      from = i;
+      pages = i + lane < nblk ? page_of(a.c, b, blk0 + i + lane) : -1;
+    }
+    return __builtin_amdgcn_readlane(pages, i - from);
+  };
+  auto stage = [&](int kt, int buf, int (&page)[NB]) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      page[j] = page_at(kt * NB + j);
+      if (page[j] < 0) continue;
+      const int64_t at = block_base(a.c, page[j], head, blk0 + kt * NB + j, D) * 2;
+#pragma unroll
+      for (int i = wave; i < 2 * kPieces; i += 4)
+        dma_kb((i < kPieces ? kc : vc) + at + (i % kPieces) * 1024, lds,
+               buf * kStage + (i < kPieces ? 0 : NB * kBlockBytes) + j * kBlockBytes + (i % kPieces) * 1024, lane);
+    }
+  };
+
+  int page[NB], next[NB];
+  if (tiles) stage(0, 0, page);
+  for (int kt = 0; kt < tiles; ++kt) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's pieces of the tile have landed
+    __syncthreads();                      // and every wave's; the other stage's readers are done
+    if (kt + 1 < tiles) stage(kt + 1, (kt + 1) & 1, next);
+    const unsigned char *kl = lds + (kt & 1) * kStage + lane * 16, *vl = kl + NB * kBlockBytes;
+    const int first = (blk0 + kt * NB) * kBlockKeys;
+
+    bool masked = first < lo_all || first + KB - 1 > hi_all || first + KB > end;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) masked |= page[j] < 0;   // also the blocks behind the last
+    f32x16 sc[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[j][i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        sc[j] = Mfma<T>::mul32(*reinterpret_cast<const op *>(kl + j * kBlockBytes + k * 1024), q[k], sc[j]);
+    }
+    // (row, key) pairs: key of element i of block j, and whether the row sees it
+    auto sees = [&](int j, int i) {
+      const int key = first + 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
+      return key >= lo && key <= hi && page[j] >= 0;
+    };
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[j][i] = score(a, sc[j][i]);
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[j][i] = sees(j, i) ? sc[j][i] : -__builtin_inff();
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[j][i]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (__any(top > ref + (kRefBelow + kRefSlack))) {
+      const float to = top > ref + (kRefBelow + kRefSlack) ? top - kRefBelow : ref;
+      const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
+      ref = to;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+    const float m = ref == -__builtin_inff() ? 0.0f : ref;
+    op w[NB][2][TERMS];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(sc[j][8 * t + e] - m);
+          sum += p[e];
+        }
+        weights<T, TERMS>(p, w[j][t]);
+      }
+    auto value = [&](int j, int d, int t) {
+      return *reinterpret_cast<const u32x4 *>(vl + j * kBlockBytes + (2 * d + t) * 1024);
+    };
+    if (__builtin_expect(masked, 0)) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          unsigned seen = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = first + 32 * j + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+            seen |= key >= lo_any && key <= hi_any && page[j] >= 0 ? 1u << e : 0u;
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const op v = __builtin_bit_cast(op, finite8<T>(value(j, d, t), seen, odd));
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) o[d] = Mfma<T>::mul32(v, w[j][t][x], o[d]);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const op v = __builtin_bit_cast(op, value(j, d, t));
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) o[d] = Mfma<T>::mul32(v, w[j][t][x], o[d]);
+          }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) page[j] = next[j];
+  }
+
+  if (__builtin_expect(__any(odd), 0)) {
+    for (int i = 0; i < nblk; ++i) {
+      const int first = (blk0 + i / NB * NB) * kBlockKeys;   // of the tile, as above
+      const int at = page_of(a.c, b, blk0 + i);
+      if (at < 0) continue;
+      bool masked = first < lo_all || first + KB - 1 > hi_all || first + KB > end;
+      for (int j = 0; j < NB; ++j) masked |= i / NB * NB + j >= nblk || page_of(a.c, b, blk0 + i / NB * NB + j) < 0;
+      if (!masked) continue;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        float part[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[e] = o[d][e];
+        add_odd<T, D, 16>(a, at, head, blk0 + i, lo, hi,
+                          [&](int e) { return 32 * d + 8 * (e >> 2) + 4 * h + (e & 3); }, part);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = part[e];
+      }
+    }
+  }
+  sum += __shfl_xor(sum, 32);
+  if (row < 0) return;
+  const bool empty = ref == -__builtin_inff();
+  if (runs == 1) {
+    const float f = empty ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 y = {o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
+        store4(a, row, col + 32 * d + 8 * i + 4 * h, y);
+      }
+  } else {
+    float *p = part_row(a, split, row, col / D, D);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4 *>(p + 32 * d + 8 * i + 4 * h) =
+            f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    if (h == 0) {
+      float *ml = part_stat(a, split, row, col / D);
+      ml[0] = ref, ml[1] = sum;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- the runs' sums
+
+// One wave: one (token, head) row; adds its runs' sums in the runs' order.
+template <int D>
+__global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
+  constexpr int PER = D / 64;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int row = (int)(item / a.heads), head = (int)(item % a.heads);
+  if (row >= a.c.rows) return;
+  int b = 0;
+  for (int i = lane; i < a.c.batch; i += 64) b += row_start(a.c, i) <= row ? 1 : 0;
+  for (int off = 32; off; off >>= 1) b += __shfl_xor(b, off);
+  b -= 1;
+  if (b < 0 || row >= row_start(a.c, b + 1)) return;
+  const Seq s = sequence(a, b);
+  const int runs = runs_of(a, s, is_few(a, s));
+  if (runs == 1) return;
+  float top = -__builtin_inff();
+  for (int i = 0; i < runs; ++i) top = fmaxf(top, part_stat(a, i, row, head)[0]);
+  float total = 0.0f, o[PER] = {};
+  for (int i = 0; i < runs; ++i) {
+    const float *ml = part_stat(a, i, row, head);
+    if (ml[0] == -__builtin_inff()) continue;
+    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+    total += ml[1] * f;
+    const float *p = part_row(a, i, row, head, D) + lane * PER;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] += p[e] * f;
+  }
+  const float f = top == -__builtin_inff() ? 0.0f : 1.0f / total;
+  const int64_t at = row * a.out_stride + head * D + lane * PER;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if (a.out_bf16) static_cast<__bf16 *>(a.out)[at + e] = static_cast<__bf16>(o[e] * f);
+    else static_cast<_Float16 *>(a.out)[at + e] = static_cast<_Float16>(o[e] * f);
+  }
+}
+
+// ----------------------------------------------------------------------------- host
+
+// How a call is launched, from its sizes alone (max_q and max_kv bound the sequences' new and
+// cached tokens; they choose, they do not limit what is computed).
+struct Plan {
+  int few, many, splits, span, few_splits, few_span, few_tiles;
+  size_t bytes;
+};
+
+// Runs of keys for `tiles` workgroups over up to kv keys: enough workgroups for `want`, none with
+// fewer than `least` keys, and at most 64 runs.
+void split_keys(int64_t tiles, int kv, int want, int least, int *splits, int *span) {
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>({64, (want + tiles - 1) / tiles, (kv + least - 1) / least}));
+  const int step = 4 * kBlockKeys;
+  *span = (int)((kv + n * step - 1) / (n * step) * step);
+  *splits = (kv + *span - 1) / *span;
+}
+
+Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv, int window) {
+  Plan p{};
+  const int group = heads / kv_heads;
+  const int64_t rows = (int64_t)max_q * group;
+  p.many = rows > kFewRows;
+  p.few = !p.many || (B > 1 && (int64_t)B * max_q > T);
+  p.few_tiles = !p.many && rows <= 16 ? 1 : 2;
+  int kv = std::max(1, max_kv);
+  if (window && window < kMaxPositions && window < kv) kv = (int)std::min<int64_t>(kv, (int64_t)window + max_q + kBlockKeys);
+  p.splits = p.few_splits = 1;
+  p.span = p.few_span = (kv + 127) / 128 * 128;
+  if (p.few) {
+    const int64_t per = std::max<int64_t>(1, (rows + 16 * p.few_tiles - 1) / (16 * p.few_tiles));
+    split_keys((int64_t)B * (p.many ? 1 : per) * kv_heads, kv, 1024, 256, &p.few_splits, &p.few_span);
+  }
+  if (p.many) {
+    const int64_t tiles = ((int64_t)T * group + kManyRows - 1) / kManyRows * kv_heads;
+    split_keys(tiles, kv, 384, 1024, &p.splits, &p.span);
+  }
+  const int s = std::max(p.splits, p.few_splits);
+  p.bytes = s > 1 ? (size_t)s * T * heads * (D + 2) * sizeof(float) : 0;
+  return p;
+}
+
+template <typename T, int D, int TERMS>
+int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
+  const int64_t rows = (int64_t)a.c.rows * a.group;
+  if (p.few) {
+    const int64_t grid = (rows / (16 * p.few_tiles) + a.c.batch) * a.c.kv_heads * p.few_splits;
+    RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
+    if (p.few_tiles == 1) few_rows_kernel<T, D, 1, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
+    else few_rows_kernel<T, D, 2, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
+    RLQ_HIP(hipGetLastError());
+  }
+  if (p.many) {
+    constexpr int lds = 2 * 2 * (D == 256 ? 32 : 64) * D * 2 + 64;
+    const int64_t grid = (rows / kManyRows + a.c.batch) * a.c.kv_heads * p.splits;
+    RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
+    static LdsOptIn opt;
+    auto fn = many_rows_kernel<T, D, TERMS>;
+    if (int rc = allow_large_lds(reinterpret_cast<const void *>(fn), opt)) return rc;
+    fn<<<(unsigned)grid, kThreads, lds, st>>>(a);
+    RLQ_HIP(hipGetLastError());
+  }
+  if (p.splits > 1 || p.few_splits > 1) {
+    const int64_t grid = ((int64_t)a.c.rows * a.heads + 3) / 4;
+    RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
+    join_runs_kernel<D><<<(unsigned)grid, kThreads, 0, st>>>(a);
+    RLQ_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+template <typename T, int TERMS>
+int launch_size(const AttnArgs &a, const Plan &p, int D, hipStream_t st) {
+  if (D == 64) return launch_attn<T, 64, TERMS>(a, p, st);
+  if (D == 128) return launch_attn<T, 128, TERMS>(a, p, st);
+  return launch_attn<T, 256, TERMS>(a, p, st);
+}
+
+bool sizes_ok(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv, int window) {
+  return T >= 0 && T <= (1 << 26) && B >= 0 && B <= (1 << 20) && kv_heads >= 1 && heads >= kv_heads &&
+         heads % kv_heads == 0 && (int64_t)heads * D <= INT32_MAX && (int64_t)T * heads <= INT32_MAX / 2 && (D == 64 || D == 128 || D == 256) && max_q >= 0 &&
+         max_kv >= 0 && max_kv <= kMaxPositions && window >= 0;
+}
+
+}  // namespace
+}  // namespace rlq
+
+extern "C" {
+
+size_t rlq_attention_workspace_bytes(int T, int heads, int kv_heads, int D, int B, int max_q, int max_kv, int window) {
+  if (!rlq::sizes_ok(T, B, heads, kv_heads, D, max_q, max_kv, window) || T == 0 || B == 0) return 0;
+  return rlq::plan_of(T, B, heads, kv_heads, D, max_q, max_kv, window).bytes;
+}
+
+int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, int D, int dtype, const void *k_cache,
+                  const void *v_cache, int n_pages, int page_size, const int *cu_q, const int *kv_len,
+                  const int *table, int table_stride, int table_width, int B, int max_q, int max_kv, float scale,
+                  int window, float softcap, void *out, int out_stride, int out_dtype, void *workspace,
+                  size_t workspace_bytes, void *stream) {
+  using namespace rlq;
+  RLQ_REQUIRE(D == 64 || D == 128 || D == 256, "rlq_attention: head size %d is not 64, 128 or 256", D);
+  RLQ_REQUIRE(dtype == RLQ_F16 || dtype == RLQ_BF16, "rlq_attention: unknown dtype %d", dtype);
+  RLQ_REQUIRE(out_dtype == RLQ_F16 || out_dtype == RLQ_BF16, "rlq_attention: unknown output dtype %d", out_dtype);
+  RLQ_REQUIRE(kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0,
+              "rlq_attention: %d heads do not share %d key/value heads evenly", heads, kv_heads);
+  RLQ_REQUIRE(page_size >= 32 && page_size % 32 == 0, "rlq_attention: page_size=%d is not a multiple of 32", page_size);
+  RLQ_REQUIRE(n_pages >= 0 && table_width >= 0 && table_stride >= table_width,
+              "rlq_attention: n_pages=%d, table_width=%d, table_stride=%d", n_pages, table_width, table_stride);
+  RLQ_REQUIRE((int64_t)table_width * page_size <= kMaxPositions,
+              "rlq_attention: a table of %d pages of %d holds more than 2^29 positions", table_width, page_size);
+  RLQ_REQUIRE(scale > 0 && scale < __builtin_inff(), "rlq_attention: scale=%g must be positive", scale);
+  RLQ_REQUIRE(softcap >= 0 && softcap < __builtin_inff(), "rlq_attention: softcap=%g must be 0 or positive", softcap);
+  RLQ_REQUIRE(sizes_ok(T, B, heads, kv_heads, D, max_q, max_kv, window),
+              "rlq_attention: T=%d, B=%d, heads=%d, max_q=%d, max_kv=%d or window=%d is out of range", T, B, heads, max_q,
+              max_kv, window);
+  if (T == 0 || B == 0) return 0;
+  RLQ_REQUIRE(q && out && cu_q && kv_len, "rlq_attention: null pointer");
+  RLQ_REQUIRE((k_cache && v_cache) || n_pages == 0, "rlq_attention: null cache");
+  RLQ_REQUIRE(table || table_width == 0, "rlq_attention: null table");
+  RLQ_REQUIRE(q_stride >= heads * D && out_stride >= heads * D,
+              "rlq_attention: a row stride (q %d, out %d) is shorter than %d heads of %d", q_stride, out_stride, heads, D);
+  RLQ_REQUIRE(aligned(k_cache, 16) && aligned(v_cache, 16), "rlq_attention: the cache must be 16-byte aligned");
+  const Plan p = plan_of(T, B, heads, kv_heads, D, max_q, max_kv, window);
+  RLQ_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 16)),
+              "rlq_attention: needs %zu bytes of 16-byte aligned workspace (got %zu)", p.bytes, workspace_bytes);
+  AttnArgs a{};
+  a.q = q, a.out = out;
+  a.c = {const_cast<void *>(k_cache), const_cast<void *>(v_cache), cu_q, kv_len, table, n_pages, page_size / kBlockKeys,
+         kv_heads, B, T, table_stride, table_width};
+  a.q_stride = q_stride, a.out_stride = out_stride;
+  a.part = static_cast<float *>(workspace);
+  if (p.bytes) a.part_ml = a.part + (size_t)std::max(p.splits, p.few_splits) * T * heads * D;
+  a.heads = heads, a.group = heads / kv_heads, a.window = window < kMaxPositions ? window : 0, a.out_bf16 = out_dtype == RLQ_BF16;
+  a.q_wide = aligned(q, 16) && q_stride % 8 == 0;
+  a.out_wide = aligned(out, 8) && out_stride % 4 == 0;
+  a.splits = p.splits, a.span = p.span, a.few_splits = p.few_splits, a.few_span = p.few_span;
+  a.few = p.few, a.many = p.many;
+  a.scale_log2 = scale * kLog2e;
+  a.cap_log2 = softcap * kLog2e;
+  a.inv_cap = softcap > 0 ? 2.0f * kLog2e * scale / softcap : 0.0f;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == RLQ_F16) return launch_size<_Float16, 1>(a, p, D, st);
+  if (out_dtype == RLQ_BF16) return launch_size<__bf16, 1>(a, p, D, st);
+  return launch_size<__bf16, 2>(a, p, D, st);
+}
+
+}  // extern "C"

@@ -17,6 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libraceline_amd.so"
 
 c_int, c_size_t, c_void_p, c_char_p = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p
+c_int64, c_float, c_double = ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 # name -> (restype, argtypes); the whole exported surface of include/rlq.h
 SIGNATURES = {
@@ -76,6 +77,17 @@ SIGNATURES = {
                                        c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "rlq_moe": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
                         c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "rlq_rope_frequencies": (c_int, [c_int, c_int, c_double, c_double, c_double, c_double, c_double, c_void_p]),
+    "rlq_rope_append": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_float,
+                                c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                                c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "rlq_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "rlq_attention": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+                              c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_float,
+                              c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "rlq_adjust_logits": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64,
+                                  c_void_p, c_int64, c_void_p]),
     # include/rl_engine.h: the model file reader and the engine layer
     "rlm_open": (c_void_p, [c_char_p]),
     "rlm_close": (None, [c_void_p]),

@@ -513,3 +513,221 @@ def moe_native(x: torch.Tensor, logits: torch.Tensor, gu: MoeNativeStack, dn: Mo
         act = moe_swiglu(moe_linear_native(x, gu, slots, r, True, stream=stream), gu.Ne // 2, cs, stream=stream)
     y = moe_linear_native(act, dn, slots, r, False, stream=stream)
     return moe_combine(y, r, h, stream=stream)
+
+
+# ------------------------------------------------------------------ positions, cache, attention
+
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "ntk": 2, "parts": 3}   # include/rlq.h RLQ_ROPE_*
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, scaling: str = "plain", factor: float = 1.0, low: float = 1.0,
+                     high: float = 32.0, original: int = 0, device="cuda") -> torch.Tensor:
+    """Radians per token of the rot/2 rotated pairs, float64 (rlq_rope_frequencies): what
+    rope_append takes as freq, kept by the program."""
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if rot < 0 or rot % 2:
+        raise ValueError(f"rot={rot} must be even and not negative")
+    f = torch.empty(rot // 2, dtype=torch.float64)
+    host = f if rot else torch.empty(1, dtype=torch.float64)
+    lib.call("rlq_rope_frequencies", ROPE_SCALINGS[scaling], rot, base, factor, low, high, float(original),
+             host.data_ptr())
+    return f.to(device)
+
+
+def kv_cache(n_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dtype: torch.dtype = torch.float16,
+             device="cuda"):
+    """The two arrays of a paged key/value cache, [n_pages][kv_heads][page_size][head_dim]
+    (include/rlq.h has the order of a page's elements). They need no filling: what was not
+    written is never read into a result."""
+    scale_code(dtype)
+    if page_size < 32 or page_size % 32 or head_dim not in (64, 128, 256):
+        raise ValueError(f"page_size={page_size} must be a multiple of 32, head_dim={head_dim} 64, 128 or 256")
+    shape = (n_pages, kv_heads, page_size, head_dim)
+    return torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+
+
+def _check_paged(k_cache, v_cache, cu_q, kv_len, table):
+    """Shapes, types and places of a cache and its sequences; (code, B)."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError("k_cache and v_cache must be alike, [n_pages][kv_heads][page_size][head_dim]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache and v_cache must be contiguous")
+    if not (cu_q.dtype == kv_len.dtype == table.dtype == torch.int32):
+        raise TypeError("cu_q, kv_len and table must be int32")
+    B = kv_len.numel()
+    if kv_len.dim() != 1 or cu_q.dim() != 1 or cu_q.numel() != B + 1 or not (cu_q.is_contiguous() and kv_len.is_contiguous()):
+        raise ValueError("kv_len must be a contiguous vector [B], cu_q [B + 1]")
+    if table.dim() != 2 or table.shape[0] < B or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be a row-major matrix [B][pages of a sequence]")
+    dev = k_cache.device
+    if not (v_cache.device == cu_q.device == kv_len.device == table.device == dev):
+        raise ValueError("the cache and its sequences must be on one device")
+    return scale_code(k_cache.dtype), B
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _call_on(device: torch.device, stream, name: str, *args):
+    """lib.call on the device its tensors live on, whichever is current."""
+    if device.type != "cuda":
+        raise ValueError(f"{name} needs tensors on the GPU, not on {device}")
+    if stream is None and (_current_device is None or device.index != _current_device()):
+        with torch.cuda.device(device):
+            return lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    if stream is not None and stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
+    if stream is not None and (_current_device is None or device.index != _current_device()):
+        with torch.cuda.device(device):
+            return lib.call(name, *args, stream.cuda_stream)
+    return lib.call(name, *args, _stream(stream))
+
+
+def _new(shape, dtype, device, stream) -> torch.Tensor:
+    """An output or scratch tensor that the caching allocator keeps until `stream` is through."""
+    t = torch.empty(shape, dtype=dtype, device=device)
+    if stream is not None:
+        t.record_stream(stream)
+    return t
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                cu_q: torch.Tensor, kv_len: torch.Tensor, table: torch.Tensor, freq: torch.Tensor | None,
+                interleaved: bool = False, mscale: float = 1.0, q_norm: torch.Tensor | None = None,
+                k_norm: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None,
+                stream=None) -> torch.Tensor:
+    """Rows of a layer's q, k and v (fp32, slices of the stacked linear's rows, say) -> rotated
+    queries [T][heads * head_dim] in the cache's dtype, and keys and values in the cache
+    (rlq_rope_append). Row i of a sequence's n new rows has position kv_len - n + i; freq:
+    rope_frequencies, None turns nothing. Rows from cu_q[B] on are left as they were in `out`."""
+    code, B = _check_paged(k_cache, v_cache, cu_q, kv_len, table)
+    n_pages, kv_heads, page, D = k_cache.shape
+    dev = k_cache.device
+    for t in (q, k, v):
+        if t.dtype != torch.float32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or t.device != dev:
+            raise ValueError("q, k and v must be row-major float32 matrices on the cache's device")
+    T = q.shape[0]
+    if k.shape != (T, kv_heads * D) or v.shape != k.shape or q.shape[1] % (kv_heads * D) or q.shape[1] == 0:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match {kv_heads} "
+                         f"key/value heads of {D}")
+    rot = 0
+    if freq is not None:
+        if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous() or freq.device != dev:
+            raise ValueError("freq must be a contiguous float64 vector on the cache's device")
+        rot = 2 * freq.numel()
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous() or w.device != dev):
+            raise ValueError(f"q_norm and k_norm must be contiguous float32 vectors of {D} on the cache's device")
+    if out is None:
+        out = _new((T, q.shape[1]), k_cache.dtype, dev, stream)
+    elif out.dtype != k_cache.dtype or out.shape != q.shape or out.stride(1) != 1 or out.device != dev:
+        raise ValueError(f"out must be a row-major {k_cache.dtype} matrix shaped like q")
+    _call_on(dev, stream, "rlq_rope_append", _ptr(q), _row_stride(q), _ptr(k), _row_stride(k), _ptr(v), _row_stride(v), T,
+             _ptr(freq), rot, 1 if interleaved else 0, mscale, _ptr(q_norm), _ptr(k_norm), eps, q.shape[1] // D, kv_heads,
+             D, code, _ptr(out), _row_stride(out), _ptr(k_cache), _ptr(v_cache), n_pages, page, _ptr(cu_q), _ptr(kv_len),
+             _ptr(table), max(table.stride(0), table.shape[1]), table.shape[1], B)
+    return out
+
+
+def attention_workspace_bytes(T: int, heads: int, kv_heads: int, head_dim: int, B: int, max_q: int, max_kv: int,
+                              window: int = 0) -> int:
+    return int(lib.load().rlq_attention_workspace_bytes(T, heads, kv_heads, head_dim, B, max_q, max_kv, window))
+
+
+def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+              table: torch.Tensor, max_q: int, max_kv: int, scale: float | None = None, window: int = 0,
+              softcap: float = 0.0, out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float16,
+              workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Causal attention of new rows q [T][heads * head_dim] (the cache's dtype) over their
+    sequences' pages, the rows' own keys among them (rlq_attention) -> [T][heads * head_dim] in
+    out_dtype. max_q and max_kv bound a sequence's new and all tokens; scale: 1 / sqrt(head_dim)
+    by default; window: the last positions a row sees (0: all); softcap: 0 for none. Rows from
+    cu_q[B] on are left as they were in `out`. workspace: scratch to use in place of a new
+    tensor; calls that overlap must not share it."""
+    code, B = _check_paged(k_cache, v_cache, cu_q, kv_len, table)
+    n_pages, kv_heads, page, D = k_cache.shape
+    dev = k_cache.device
+    if q.dtype != k_cache.dtype or q.dim() != 2 or q.stride(1) != 1 or q.device != dev:
+        raise ValueError(f"q must be a row-major {k_cache.dtype} matrix on the cache's device")
+    T, width = q.shape
+    if width == 0 or width % (kv_heads * D):
+        raise ValueError(f"q rows of {width} are no whole number of {D}-wide heads a key/value head")
+    if out is None:
+        out = _new((T, width), out_dtype, dev, stream)
+    elif out.shape != q.shape or out.stride(1) != 1 or out.device != dev:
+        raise ValueError("out must be a row-major matrix shaped like q")
+    H = width // D
+    nbytes = int(lib.load().rlq_attention_workspace_bytes(T, H, kv_heads, D, B, max_q, max_kv, window))
+    if workspace is not None and workspace.device != dev:
+        raise ValueError("the workspace must be on the cache's device")
+    if nbytes and workspace is None:
+        workspace = _new(nbytes, torch.uint8, dev, stream)
+    _call_on(dev, stream, "rlq_attention", _ptr(q), _row_stride(q), T, H, kv_heads, D, code, _ptr(k_cache), _ptr(v_cache),
+             n_pages, page, _ptr(cu_q), _ptr(kv_len), _ptr(table), max(table.stride(0), table.shape[1]), table.shape[1],
+             B, max_q, max_kv, D ** -0.5 if scale is None else scale, window, softcap, _ptr(out), _row_stride(out),
+             scale_code(out.dtype), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size())
+    return out
+
+
+# ------------------------------------------------------------------ logits
+
+def _check_row_vector(t, rows, dtype, what, dev):
+    if t is not None and (t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous() or t.device != dev):
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of {rows} rows on the logits' device")
+
+
+def _shared_rows(t, rows, dtype, what, dev) -> int:
+    """Row stride of a matrix with a row per row of logits, or of one row (or a vector) for all: 0."""
+    if t.dtype != dtype or t.dim() not in (1, 2) or (t.shape[-1] > 1 and t.stride(-1) != 1) or t.device != dev:
+        raise ValueError(f"{what} must be a row-major {dtype} matrix (or one row) on the logits' device")
+    if t.dim() == 1:
+        return 0
+    if t.shape[0] != rows and t.shape[0] != 1:
+        raise ValueError(f"{what} has {t.shape[0]} rows, the logits have {rows}")
+    return t.stride(0) if t.shape[0] == rows else 0
+
+
+def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, n_tokens: torch.Tensor | None = None,
+                  n_prompt: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                  presence: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                  bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                  allowed: torch.Tensor | None = None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Penalties, biases and a mask on rows of logits (fp32 [rows][vocab]) before a token is
+    chosen from them (rlq_adjust_logits) -> out (may be logits; a new tensor by default).
+    tokens int32 [rows][n], the first n_tokens of a row count: any of them for `repetition`,
+    those from n_prompt on for `presence` and `frequency` (fp32 [rows]); bias_ids int32 and bias
+    fp32 [rows][n]; allowed int32 or uint32 [rows][words], bit v % 32 of word v / 32 set where
+    token v may follow. tokens, biases and the mask may be one row for all."""
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be a row-major float32 matrix")
+    rows, vocab = logits.shape
+    dev = logits.device
+    if out is None:
+        out = _new((rows, vocab), torch.float32, dev, stream)
+    elif out.dtype != torch.float32 or out.shape != logits.shape or (vocab > 1 and out.stride(1) != 1) or out.device != dev:
+        raise ValueError("out must be a row-major float32 matrix shaped like logits")
+    ts = n = bs = nb = ms = 0
+    if tokens is not None:
+        ts, n = _shared_rows(tokens, rows, torch.int32, "tokens", dev), tokens.shape[-1]
+    _check_row_vector(n_tokens, rows, torch.int32, "n_tokens", dev)
+    _check_row_vector(n_prompt, rows, torch.int32, "n_prompt", dev)
+    _check_row_vector(repetition, rows, torch.float32, "repetition", dev)
+    _check_row_vector(presence, rows, torch.float32, "presence", dev)
+    _check_row_vector(frequency, rows, torch.float32, "frequency", dev)
+    if (bias is None) != (bias_ids is None):
+        raise ValueError("bias and bias_ids come together")
+    if bias is not None:
+        bs, nb = _shared_rows(bias, rows, torch.float32, "bias", dev), bias.shape[-1]
+        if bias_ids.shape != bias.shape or _shared_rows(bias_ids, rows, torch.int32, "bias_ids", dev) != bs:
+            raise ValueError("bias_ids must be shaped like bias")
+    if allowed is not None:
+        ms = _shared_rows(allowed, rows, allowed.dtype if allowed.dtype in (torch.int32, torch.uint32) else torch.int32,
+                          "allowed", dev)
+        if allowed.shape[-1] < (vocab + 31) // 32:
+            raise ValueError(f"a mask row of {allowed.shape[-1]} words is shorter than the vocabulary")
+    _call_on(dev, stream, "rlq_adjust_logits", _ptr(logits), _row_stride(logits), rows, vocab, _ptr(tokens), ts, n,
+             _ptr(n_tokens), _ptr(n_prompt), _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_ids), _ptr(bias),
+             nb, bs, _ptr(allowed), ms, _ptr(out), _row_stride(out))
+    return out
