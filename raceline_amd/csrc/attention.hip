@@ -14,6 +14,7 @@
 #include "../../include/rlq.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace rlq {
 namespace {
@@ -38,12 +39,15 @@ struct AttnArgs {
   void *out;
   PagedCache c;
   int64_t q_stride, out_stride;
-  float *part, *part_ml;      // [splits][rows][heads][D] and [splits][rows][heads][2]: sums, (ref, weight sum)
+  float *part;                // [splits][rows][heads][D]: a run's sums, not divided; null where no run is split
+  float2 *part_stat;          // [splits][rows][heads]: (ref, sum of weights)
+  int *part_runs;             // [rows][heads]: runs of the row
   int heads, group, window, out_bf16, q_wide, out_wide;
   int splits, span;           // keys are split in runs of `span` positions (a multiple of 32)
   int few_splits, few_span;   // the same for sequences of few rows
   int few, many;              // which kernels this call launches
-  float scale_log2, cap_log2, inv_cap;
+  int join_few;               // join_runs_kernel: only sequences of few rows have more than one run
+  float unit, cap_log2, inv_cap;   // unit: base-2 units of a score as the product gives it, or of a capped one (1)
 };
 
 template <typename T>
@@ -71,12 +75,17 @@ struct Mfma<__bf16> {
   static constexpr unsigned kExp = 0x7F80u;
 };
 
-// A score in base-2 units. The cap's tanh y = 1 - 2 / (1 + e^2y) has an error of about 2^-23
-// absolute, times cap: far under what the weight's 16 bits keep.
-__device__ __forceinline__ float score(const AttnArgs &a, float s) {
-  if (a.cap_log2 == 0.0f) return s * a.scale_log2;
+// A capped score in base-2 units. tanh y = 1 - 2 / (1 + e^2y) has an error of about 2^-23 absolute,
+// times cap: far under what the weight's 16 bits keep.
+__device__ __forceinline__ float capped(const AttnArgs &a, float s) {
   const float e = __builtin_amdgcn_exp2f(s * a.inv_cap);
   return a.cap_log2 - 2.0f * a.cap_log2 * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+__device__ __forceinline__ float max_halves(float x) {
+  const unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Eight weights as a matrix operand. TERMS 2 (bf16 keys, fp16 rows out): the rounding's remainder
@@ -111,34 +120,19 @@ __device__ __forceinline__ u32x4 finite8(u32x4 v, unsigned seen, bool &odd) {
   return r;
 }
 
-// What a sequence's rows are in this call.
-struct Seq {
-  int b, row0, tokens, kv, rows;   // rows: of one key/value head
-};
-
-__device__ __forceinline__ Seq sequence(const AttnArgs &a, int b) {
-  Seq s;
-  s.b = b;
-  s.row0 = row_start(a.c, b);
-  s.tokens = max(0, row_start(a.c, b + 1) - s.row0);
-  s.kv = cached(a.c, b);
-  s.rows = s.tokens * a.group;
-  return s;
-}
-
 // Which kernel takes a sequence: few_rows where both run and its rows fit one tile of it.
-__device__ __forceinline__ bool is_few(const AttnArgs &a, const Seq &s) {
-  return a.few && (!a.many || s.rows <= kFewRows);
+__device__ __forceinline__ bool is_few(const AttnArgs &a, const Sequence &s) {
+  return a.few && (!a.many || s.tokens * a.group <= kFewRows);
 }
 
 // First position that any row of the sequence sees, to the block below; the runs of `span` keys
 // begin there.
-__device__ __forceinline__ int first_key(const AttnArgs &a, const Seq &s) {
+__device__ __forceinline__ int first_key(const AttnArgs &a, const Sequence &s) {
   return a.window ? max(0, s.kv - s.tokens + 1 - a.window) & ~(kBlockKeys - 1) : 0;
 }
 
 // Runs that hold keys of the sequence; one run's kernel writes the rows itself.
-__device__ __forceinline__ int runs_of(const AttnArgs &a, const Seq &s, bool few) {
+__device__ __forceinline__ int runs_of(const AttnArgs &a, const Sequence &s, bool few) {
   const int span = few ? a.few_span : a.span, splits = few ? a.few_splits : a.splits;
   return max(1, min(splits, (s.kv - first_key(a, s) + span - 1) / span));
 }
@@ -147,8 +141,12 @@ __device__ __forceinline__ float *part_row(const AttnArgs &a, int split, int row
   return a.part + ((static_cast<int64_t>(split) * a.c.rows + row) * a.heads + head) * D;
 }
 
-__device__ __forceinline__ float *part_stat(const AttnArgs &a, int split, int row, int head) {
-  return a.part_ml + ((static_cast<int64_t>(split) * a.c.rows + row) * a.heads + head) * 2;
+__device__ __forceinline__ float2 &part_stat(const AttnArgs &a, int split, int row, int head) {
+  return a.part_stat[(static_cast<int64_t>(split) * a.c.rows + row) * a.heads + head];
+}
+
+__device__ __forceinline__ int &run_count(const AttnArgs &a, int row, int head) {
+  return a.part_runs[static_cast<int64_t>(row) * a.heads + head];
 }
 
 // Adds the infinities and NaN among one block's values to o (o[i]: dimension dim(i)) for the keys
@@ -213,7 +211,6 @@ template <typename T, int D, int NT, int TERMS>
 __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kernel(AttnArgs a) {
   constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * NT;
   typedef typename Mfma<T>::op op;
-  __shared__ int found[kThreads / 64];
   __shared__ float stat[4][ROWS][2];
   __shared__ float sums[2][ROWS][D + 4];
   __shared__ op queries[NT][KS][64];
@@ -221,11 +218,10 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
   const int KV = a.c.kv_heads, head = blockIdx.x % KV, split = (blockIdx.x / KV) % a.few_splits;
   const int64_t slot = blockIdx.x / KV / a.few_splits;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, r = lane & 15;
-  const int b = find_sequence<kThreads>(a.c, slot, a.group, ROWS, 1, found);
-  if (b < 0 || b >= a.c.batch) return;
-  const Seq s = sequence(a, b);
-  const int tile = (int)(slot - slot_base(a.c, b, a.group, ROWS, 1)) * ROWS;
-  if (tile < 0 || tile >= s.rows || !is_few(a, s)) return;
+  // beside many_rows_kernel a sequence of few rows is one tile: items are the sequences
+  const Sequence s = find_sequence(a.c, slot, a.many ? 0 : a.group, ROWS, 1);
+  const int b = s.b, tile = s.item * ROWS, rows = s.tokens * a.group;
+  if (b < 0 || tile < 0 || tile >= rows || !is_few(a, s)) return;
   const int runs = runs_of(a, s, true);
   if (split >= runs) return;
 
@@ -234,7 +230,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int R = tile + n * 16 + r, tok = R / a.group;
-    const bool here = R < s.rows;
+    const bool here = R < rows;
     row[n] = here ? s.row0 + tok : -1;
     col[n] = (head * a.group + R - tok * a.group) * D;
     hi[n] = here ? s.kv - s.tokens + tok : -1;                       // last key seen
@@ -243,7 +239,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       queries[n][k][lane] = here ? load_q<T>(a, row[n], col[n] + 32 * k + 8 * g) : op{};
   }
   __syncthreads();
-  const int last = min(s.rows, tile + ROWS) - 1;
+  const int last = min(rows, tile + ROWS) - 1;
   const int lo_any = a.window ? max(0, s.kv - s.tokens + tile / a.group - a.window + 1) : 0;
   const int lo_all = a.window ? max(0, s.kv - s.tokens + last / a.group - a.window + 1) : 0;
   const int hi_any = s.kv - s.tokens + last / a.group, hi_all = s.kv - s.tokens + tile / a.group;
@@ -284,8 +280,8 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     const T *p = kc + block_base(a.c, page, head, blk, D) + koff;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      kr[k][0] = *reinterpret_cast<const op *>(p + k * 1024);
-      kr[k][1] = *reinterpret_cast<const op *>(p + k * 1024 + 64);
+      kr[k][0] = __builtin_nontemporal_load(reinterpret_cast<const op *>(p + k * 1024));
+      kr[k][1] = __builtin_nontemporal_load(reinterpret_cast<const op *>(p + k * 1024 + 64));
     }
   };
   int page = page_at(0);
@@ -301,7 +297,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     const T *vp = vc + block_base(a.c, page, head, blk, D) + voff;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      vr[d] = *reinterpret_cast<const u32x4 *>(vp + (d >> 1) * 1024 + (d & 1) * 128);
+      vr[d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp + (d >> 1) * 1024 + (d & 1) * 128));
 
     f32x4 sc[NT][2];
 #pragma unroll
@@ -321,7 +317,11 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     for (int n = 0; n < NT; ++n) {
       float x[8], top = -__builtin_inff();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = score(a, sc[n][e >> 2][e & 3]);
+      for (int e = 0; e < 8; ++e) x[e] = sc[n][e >> 2][e & 3];
+      if (a.cap_log2 != 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = capped(a, x[e]);
+      }
       if (masked) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
       top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = max_halves(top) * a.unit;
       if (__any(top > ref[n] + (kRefBelow + kRefSlack))) {
         const float to = top > ref[n] + (kRefBelow + kRefSlack) ? top - kRefBelow : ref[n];
         const float f = ref[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref[n] - to);
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(x[e] - m);
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.unit, -m));
         sum[n] += p[e];
       }
       weights<T, TERMS>(p, w[n]);
@@ -445,11 +445,9 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       float *p = part_row(a, split, row[n], col[n] / D, D);
 #pragma unroll
       for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p + d * 16 + 4 * g) = o[n][d];
-      if (g == 0) {
-        float *ml = part_stat(a, split, row[n], col[n] / D);
-        ml[0] = top[n], ml[1] = total[n];
-      }
+      if (g == 0) part_stat(a, split, row[n], col[n] / D) = make_float2(top[n], total[n]);
     }
+    if (split == 0 && g == 0 && a.part) run_count(a, row[n], col[n] / D) = runs;
   }
 }
 
@@ -463,43 +461,67 @@ __device__ __forceinline__ void dma_kb(const void *src, unsigned char *lds, int 
 }
 
 // One workgroup: 128 rows of one sequence and key/value head over one run of its keys; each of its
-// four waves holds 32 rows (Q^T as B operands, O^T accumulators) and takes every key. Keys and
-// values go through LDS in tiles of KB keys, copied as they lie (the cache's order is the
+// four waves holds 32 rows (Q^T as B operands, O^T accumulators) and takes every key.
+// Keys and values go through LDS in tiles of KB keys, copied as they lie (the cache's order is the
 // operands' order: no swizzle, no transpose, no bank conflicts), two stages deep, so that the
-// next tile's copy runs under this tile's products; one barrier a tile.
+// next tile's copy runs under this tile's products; one barrier a tile. 64 rows a wave (half the
+// LDS reads, one wave a SIMD) were slower: 69 us against 60 for 333 rows over 20,011 keys in
+// heads of 64, and did not fit the registers in heads of 256.
+template <int N, int AHEAD, int READS, int PER, int VALU>
+__device__ __forceinline__ void feed_step() {
+  if constexpr (N < READS * PER) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if constexpr (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+    if constexpr (N % PER == 0 && N / PER + AHEAD < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    feed_step<N + 1, AHEAD, READS, PER, VALU>();
+  }
+}
+
+// The order of a run of products whose A operands come from LDS: AHEAD reads first, then
+// after each operand's PER products the next read, VALU operations of the softmax between
+// them. Left to itself the compiler reads two operands, waits for both, and multiplies.
+template <int AHEAD, int READS, int PER, int VALU>
+__device__ __forceinline__ void feed_products() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+  feed_step<0, AHEAD, READS, PER, VALU>();
+}
+
+constexpr int kAhead = 4;
+
+template <int D>
+constexpr int kTileKeys = D >= 128 ? 32 : 64;
+
 template <typename T, int D, int TERMS>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(AttnArgs a) {
-  constexpr int KB = D == 256 ? 32 : 64, NB = KB / kBlockKeys, KS = D / 16, DT = D / 32;
+__global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
+  constexpr int KB = kTileKeys<D>, NB = KB / kBlockKeys, KS = D / 16, DT = D / 32, ROWS = kManyRows;
   constexpr int kBlockBytes = kBlockKeys * D * 2, kStage = 2 * NB * kBlockBytes, kPieces = kBlockBytes / 1024;
   typedef typename Mfma<T>::op op;
-  extern __shared__ unsigned char lds[];   // two stages, then find_sequence's few words
-  int *found = reinterpret_cast<int *>(lds + 2 * kStage);
+  extern __shared__ unsigned char lds[];   // two stages, then a flag
+  int *odd = reinterpret_cast<int *>(lds + 2 * kStage);
 
   const int KV = a.c.kv_heads, head = blockIdx.x % KV, split = (blockIdx.x / KV) % a.splits;
   const int64_t slots = gridDim.x / KV / a.splits, slot = slots - 1 - blockIdx.x / KV / a.splits;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
-  const int b = find_sequence<kThreads>(a.c, slot, a.group, kManyRows, 1, found);
-  if (b < 0 || b >= a.c.batch) return;
-  const Seq s = sequence(a, b);
-  const int tile = (int)(slot - slot_base(a.c, b, a.group, kManyRows, 1)) * kManyRows;
-  if (tile < 0 || tile >= s.rows || is_few(a, s)) return;
+  const Sequence s = find_sequence(a.c, slot, a.group, ROWS, 1);
+  const int b = s.b, tile = s.item * ROWS, rows = s.tokens * a.group;
+  if (b < 0 || tile < 0 || tile >= rows || is_few(a, s)) return;
   const int runs = runs_of(a, s, false);
   if (split >= runs) return;
 
+  // this lane's rows and what they see
+  const int p0 = s.kv - s.tokens;
   const int R = tile + wave * 32 + n32, tok = R / a.group;
-  const bool here = R < s.rows;
+  const bool here = R < rows;
   const int row = here ? s.row0 + tok : -1, col = (head * a.group + R - tok * a.group) * D;
-  const int hi = here ? s.kv - s.tokens + tok : -1, lo = a.window ? max(0, hi - a.window + 1) : 0;
+  const int hi = here ? p0 + tok : -1, lo = a.window ? max(0, hi - a.window + 1) : 0;
   op q[KS];
 #pragma unroll
   for (int k = 0; k < KS; ++k) q[k] = here ? load_q<T>(a, row, col + 16 * k + 8 * h) : op{};
-
-  // keys that any row of the tile sees, and that all of this wave's rows see
-  const int last = min(s.rows, tile + kManyRows) - 1, p0 = s.kv - s.tokens;
+  // keys that any row of the tile sees, and that all of its rows see
+  const int last = min(rows, tile + ROWS) - 1;
   const int lo_any = a.window ? max(0, p0 + tile / a.group - a.window + 1) : 0, hi_any = p0 + last / a.group;
-  const int wfirst = min(tile + wave * 32, s.rows - 1), wlast = min(tile + wave * 32 + 31, s.rows - 1);
-  const int lo_all = a.window ? max(0, p0 + wlast / a.group - a.window + 1) : 0, hi_all = p0 + wfirst / a.group;
+  const int lo_all = a.window ? max(0, p0 + last / a.group - a.window + 1) : 0, hi_all = p0 + tile / a.group;
   const int base = first_key(a, s) + split * a.span;
   const int end = min(hi_any + 1, split == a.splits - 1 ? hi_any + 1 : base + a.span);
   const int blk0 = max(base, lo_any & ~(kBlockKeys - 1)) / kBlockKeys, blk1 = (end + kBlockKeys - 1) / kBlockKeys;
@@ -507,7 +529,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
 
   f32x16 o[DT];
   float ref = -__builtin_inff(), sum = 0.0f;
-  bool odd = false;
+  if (tid == 0) *odd = 0;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -542,42 +564,65 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's pieces of the tile have landed
     __syncthreads();                      // and every wave's; the other stage's readers are done
     if (kt + 1 < tiles) stage(kt + 1, (kt + 1) & 1, next);
-    const unsigned char *kl = lds + (kt & 1) * kStage + lane * 16, *vl = kl + NB * kBlockBytes;
+    unsigned char *kl = lds + (kt & 1) * kStage + lane * 16, *vl = kl + NB * kBlockBytes;
     const int first = (blk0 + kt * NB) * kBlockKeys;
 
     bool masked = first < lo_all || first + KB - 1 > hi_all || first + KB > end;
 #pragma unroll
     for (int j = 0; j < NB; ++j) masked |= page[j] < 0;   // also the blocks behind the last
-    f32x16 sc[NB];
+    if (masked) {   // for the workgroup as a whole: take out what finite8 takes out, once for all waves
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
+      for (int j = 0; j < NB; ++j)
+        for (int i = wave; i < kPieces; i += 4) {
+          unsigned seen = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[j][i] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        sc[j] = Mfma<T>::mul32(*reinterpret_cast<const op *>(kl + j * kBlockBytes + k * 1024), q[k], sc[j]);
+          for (int e = 0; e < 8; ++e) {
+            const int key = first + 32 * j + 16 * (i & 1) + 8 * (e >> 2) + 4 * h + (e & 3);
+            seen |= key >= lo_any && key <= hi_any && page[j] >= 0 ? 1u << e : 0u;
+          }
+          bool here = false;
+          u32x4 *v = reinterpret_cast<u32x4 *>(vl + j * kBlockBytes + i * 1024);
+          *v = finite8<T>(*v, seen, here);
+          if (here) *odd = 1;
+        }
+      __syncthreads();
     }
-    // (row, key) pairs: key of element i of block j, and whether the row sees it
-    auto sees = [&](int j, int i) {
-      const int key = first + 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
-      return key >= lo && key <= hi && page[j] >= 0;
-    };
+    f32x16 sc[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[j][i] = score(a, sc[j][i]);
+      for (int i = 0; i < 16; ++i) sc[j][i] = 0.0f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const op key = *reinterpret_cast<const op *>(kl + j * kBlockBytes + k * 1024);
+        sc[j] = Mfma<T>::mul32(key, q[k], sc[j]);
+      }
+    feed_products<kAhead, NB * KS, 1, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (a.cap_log2 != 0.0f) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[j][i] = capped(a, sc[j][i]);
+    }
     if (masked) {
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[j][i] = sees(j, i) ? sc[j][i] : -__builtin_inff();
+        for (int i = 0; i < 16; ++i) {
+          const int key = first + 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
+          sc[j][i] = key >= lo && key <= hi && page[j] >= 0 ? sc[j][i] : -__builtin_inff();
+        }
     }
     float top = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[j][i]);
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = max_halves(top) * a.unit;
     if (__any(top > ref + (kRefBelow + kRefSlack))) {
       const float to = top > ref + (kRefBelow + kRefSlack) ? top - kRefBelow : ref;
       const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
@@ -587,57 +632,43 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
       for (int d = 0; d < DT; ++d) o[d] *= f;
     }
     const float m = ref == -__builtin_inff() ? 0.0f : ref;
+    // weights of block j, and the products of block j - 1 between them
+    __builtin_amdgcn_sched_barrier(0);
     op w[NB][2][TERMS];
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(sc[j][8 * t + e] - m);
-          sum += p[e];
-        }
-        weights<T, TERMS>(p, w[j][t]);
-      }
-    auto value = [&](int j, int d, int t) {
-      return *reinterpret_cast<const u32x4 *>(vl + j * kBlockBytes + (2 * d + t) * 1024);
-    };
-    if (__builtin_expect(masked, 0)) {
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
+    for (int j = 0; j <= NB; ++j) {
+      if (j < NB) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          unsigned seen = 0;
+          float p[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int key = first + 32 * j + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-            seen |= key >= lo_any && key <= hi_any && page[j] >= 0 ? 1u << e : 0u;
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][8 * t + e], a.unit, -m));
+            sum += p[e];
           }
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const op v = __builtin_bit_cast(op, finite8<T>(value(j, d, t), seen, odd));
-#pragma unroll
-            for (int x = 0; x < TERMS; ++x) o[d] = Mfma<T>::mul32(v, w[j][t][x], o[d]);
-          }
+          weights<T, TERMS>(p, w[j][t]);
         }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
+      }
+      if (j > 0) {
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const op v = __builtin_bit_cast(op, value(j, d, t));
+            const op v = *reinterpret_cast<const op *>(vl + (j - 1) * kBlockBytes + (2 * d + t) * 1024);
 #pragma unroll
-            for (int x = 0; x < TERMS; ++x) o[d] = Mfma<T>::mul32(v, w[j][t][x], o[d]);
+            for (int x = 0; x < TERMS; ++x) o[d] = Mfma<T>::mul32(v, w[j - 1][t][x], o[d]);
           }
+        if (j < NB) feed_products<kAhead, 2 * DT, TERMS, 32 / (DT * TERMS) + 1>();
+        else feed_products<kAhead, 2 * DT, TERMS, 0>();
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) page[j] = next[j];
   }
 
-  if (__builtin_expect(__any(odd), 0)) {
+  __syncthreads();
+  if (__builtin_expect(*odd, 0)) {
     for (int i = 0; i < nblk; ++i) {
       const int first = (blk0 + i / NB * NB) * kBlockKeys;   // of the tile, as above
       const int at = page_of(a.c, b, blk0 + i);
@@ -657,18 +688,16 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
       }
     }
   }
-  sum += __shfl_xor(sum, 32);
+  const float total = sum + __shfl_xor(sum, 32);
   if (row < 0) return;
-  const bool empty = ref == -__builtin_inff();
   if (runs == 1) {
-    const float f = empty ? 0.0f : 1.0f / sum;
+    const float f = ref == -__builtin_inff() ? 0.0f : 1.0f / total;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 y = {o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
-        store4(a, row, col + 32 * d + 8 * i + 4 * h, y);
-      }
+      for (int i = 0; i < 4; ++i)
+        store4(a, row, col + 32 * d + 8 * i + 4 * h,
+               f32x4{o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f});
   } else {
     float *p = part_row(a, split, row, col / D, D);
 #pragma unroll
@@ -677,42 +706,54 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void many_rows_kernel(A
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f32x4 *>(p + 32 * d + 8 * i + 4 * h) =
             f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-    if (h == 0) {
-      float *ml = part_stat(a, split, row, col / D);
-      ml[0] = ref, ml[1] = sum;
-    }
+    if (h == 0) part_stat(a, split, row, col / D) = make_float2(ref, total);
   }
+  if (split == 0 && h == 0 && a.part) run_count(a, row, col / D) = runs;
 }
 
 // ----------------------------------------------------------------------------- the runs' sums
 
-// One wave: one (token, head) row; adds its runs' sums in the runs' order.
+// One wave: one (token, head) row; adds its runs' sums in the runs' order. How many runs a row has
+// its first run's workgroup wrote, so that the wave does not look for its sequence again; the
+// statistics of all runs come with one load (at most 64 runs), the sums eight runs at a time.
 template <int D>
 __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
   constexpr int PER = D / 64;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+  typedef float fvec __attribute__((ext_vector_type(PER)));
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  const int row = (int)(item / a.heads), head = (int)(item % a.heads);
-  if (row >= a.c.rows) return;
-  int b = 0;
-  for (int i = lane; i < a.c.batch; i += 64) b += row_start(a.c, i) <= row ? 1 : 0;
-  for (int off = 32; off; off >>= 1) b += __shfl_xor(b, off);
-  b -= 1;
-  if (b < 0 || row >= row_start(a.c, b + 1)) return;
-  const Seq s = sequence(a, b);
-  const int runs = runs_of(a, s, is_few(a, s));
-  if (runs == 1) return;
-  float top = -__builtin_inff();
-  for (int i = 0; i < runs; ++i) top = fmaxf(top, part_stat(a, i, row, head)[0]);
-  float total = 0.0f, o[PER] = {};
-  for (int i = 0; i < runs; ++i) {
-    const float *ml = part_stat(a, i, row, head);
-    if (ml[0] == -__builtin_inff()) continue;
-    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-    total += ml[1] * f;
-    const float *p = part_row(a, i, row, head, D) + lane * PER;
+  if (item >= (a.join_few ? static_cast<int64_t>(a.c.batch) * a.c.kv_heads * kFewRows
+                          : static_cast<int64_t>(a.c.rows) * a.heads)) return;
+  int row = (int)(item / a.heads), head = (int)(item - (int64_t)row * a.heads);
+  if (a.join_few) {   // only sequences of few rows were split: 32 items for each of them and its heads
+    const int r = (int)item % kFewRows, kvh = (int)(item / kFewRows) % a.c.kv_heads;
+    const int b = (int)(item / kFewRows / a.c.kv_heads), row0 = row_start(a.c, b);
+    const int rows = (row_start(a.c, b + 1) - row0) * a.group;
+    if (r >= rows || rows > kFewRows) return;
+    row = row0 + r / a.group, head = kvh * a.group + r % a.group;
+  }
+  const int most = max(a.splits, a.few_splits);
+  const float2 stat = part_stat(a, min(lane, most - 1), row, head);
+  const int runs = __builtin_amdgcn_readfirstlane(min(run_count(a, row, head), most));
+  if (row < row_start(a.c, 0) || row >= row_start(a.c, a.c.batch) || runs <= 1) return;
+  float top = lane < runs ? stat.x : -__builtin_inff();
+  for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float mine = lane < runs && stat.x != -__builtin_inff() ? __builtin_amdgcn_exp2f(stat.x - top) : 0.0f;
+  float total = 0.0f;
+  fvec o = {};
+  for (int i0 = 0; i0 < runs; i0 += 8) {
+    fvec p[8];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] += p[e] * f;
+    for (int i = 0; i < 8; ++i)
+      p[i] = *reinterpret_cast<const fvec *>(part_row(a, min(i0 + i, runs - 1), row, head, D) + lane * PER);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= runs) break;
+      const float f = __shfl(mine, i0 + i);
+      if (f == 0.0f) continue;                     // a run in which the row saw nothing, or next to nothing
+      total += __shfl(stat.y, i0 + i) * f;
+      o += p[i] * f;
+    }
   }
   const float f = top == -__builtin_inff() ? 0.0f : 1.0f / total;
   const int64_t at = row * a.out_stride + head * D + lane * PER;
@@ -741,6 +782,22 @@ void split_keys(int64_t tiles, int kv, int want, int least, int *splits, int *sp
   *splits = (kv + *span - 1) / *span;
 }
 
+// many_rows_kernel: the number of runs with the least estimated time. A workgroup takes `per_key` for
+// a key while its CU holds as many workgroups as fit (2, 3 or 4); fewer share the CU's units less.
+// Joining writes and reads the runs' sums once and costs a launch.
+void split_many(int64_t tiles, int kv, double out_elems, int D, int *splits, int *span) {
+  const double slots = 256.0 * (D == 256 ? 2 : D == 128 ? 3 : 4), per_key = D == 256 ? 0.10 : D == 128 ? 0.08 : 0.07;
+  double best = 0;
+  for (int n = 1; n <= 64 && (n == 1 || kv / n >= 512); ++n) {
+    const int run = (kv + n * kBlockKeys - 1) / (n * kBlockKeys) * kBlockKeys, runs = (kv + run - 1) / run;
+    if (runs != n) continue;
+    const double full = tiles * runs / slots;
+    const double us = run * per_key * (full > 1 ? std::ceil(full) : std::max(0.5, full)) +
+                      (n > 1 ? 5 + runs * out_elems * 8 / 4e6 : 0);
+    if (n == 1 || us < best) best = us, *splits = runs, *span = run;
+  }
+}
+
 Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv, int window) {
   Plan p{};
   const int group = heads / kv_heads;
@@ -754,14 +811,14 @@ Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv
   p.span = p.few_span = (kv + 127) / 128 * 128;
   if (p.few) {
     const int64_t per = std::max<int64_t>(1, (rows + 16 * p.few_tiles - 1) / (16 * p.few_tiles));
-    split_keys((int64_t)B * (p.many ? 1 : per) * kv_heads, kv, 1024, 256, &p.few_splits, &p.few_span);
+    split_keys((int64_t)B * (p.many ? 1 : per) * kv_heads, kv, 512, 128, &p.few_splits, &p.few_span);
   }
   if (p.many) {
-    const int64_t tiles = ((int64_t)T * group + kManyRows - 1) / kManyRows * kv_heads;
-    split_keys(tiles, kv, 384, 1024, &p.splits, &p.span);
+    split_many(((int64_t)T * group + kManyRows - 1) / kManyRows * kv_heads, kv, (double)T * heads * D, D, &p.splits,
+               &p.span);
   }
   const int s = std::max(p.splits, p.few_splits);
-  p.bytes = s > 1 ? (size_t)s * T * heads * (D + 2) * sizeof(float) : 0;
+  p.bytes = s > 1 ? (size_t)T * heads * ((size_t)s * (D + 2) + 1) * sizeof(float) : 0;
   return p;
 }
 
@@ -769,14 +826,15 @@ template <typename T, int D, int TERMS>
 int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
   const int64_t rows = (int64_t)a.c.rows * a.group;
   if (p.few) {
-    const int64_t grid = (rows / (16 * p.few_tiles) + a.c.batch) * a.c.kv_heads * p.few_splits;
+    const int64_t slots = (p.many ? 0 : rows / (16 * p.few_tiles)) + a.c.batch;
+    const int64_t grid = slots * a.c.kv_heads * p.few_splits;
     RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
     if (p.few_tiles == 1) few_rows_kernel<T, D, 1, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
     else few_rows_kernel<T, D, 2, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
   }
   if (p.many) {
-    constexpr int lds = 2 * 2 * (D == 256 ? 32 : 64) * D * 2 + 64;
+    constexpr int lds = 2 * 2 * kTileKeys<D> * D * 2 + 64;
     const int64_t grid = (rows / kManyRows + a.c.batch) * a.c.kv_heads * p.splits;
     RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
     static LdsOptIn opt;
@@ -786,7 +844,8 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
     RLQ_HIP(hipGetLastError());
   }
   if (p.splits > 1 || p.few_splits > 1) {
-    const int64_t grid = ((int64_t)a.c.rows * a.heads + 3) / 4;
+    const int64_t items = a.join_few ? (int64_t)a.c.batch * a.c.kv_heads * kFewRows : (int64_t)a.c.rows * a.heads;
+    const int64_t grid = (items + 3) / 4;
     RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
     join_runs_kernel<D><<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
@@ -853,14 +912,18 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   a.c = {const_cast<void *>(k_cache), const_cast<void *>(v_cache), cu_q, kv_len, table, n_pages, page_size / kBlockKeys,
          kv_heads, B, T, table_stride, table_width};
   a.q_stride = q_stride, a.out_stride = out_stride;
-  a.part = static_cast<float *>(workspace);
-  if (p.bytes) a.part_ml = a.part + (size_t)std::max(p.splits, p.few_splits) * T * heads * D;
+  if (p.bytes) {
+    const size_t n = (size_t)std::max(p.splits, p.few_splits) * T * heads;
+    a.part = static_cast<float *>(workspace);
+    a.part_stat = reinterpret_cast<float2 *>(a.part + n * D);
+    a.part_runs = reinterpret_cast<int *>(a.part_stat + n);
+  }
   a.heads = heads, a.group = heads / kv_heads, a.window = window < kMaxPositions ? window : 0, a.out_bf16 = out_dtype == RLQ_BF16;
   a.q_wide = aligned(q, 16) && q_stride % 8 == 0;
   a.out_wide = aligned(out, 8) && out_stride % 4 == 0;
   a.splits = p.splits, a.span = p.span, a.few_splits = p.few_splits, a.few_span = p.few_span;
-  a.few = p.few, a.many = p.many;
-  a.scale_log2 = scale * kLog2e;
+  a.few = p.few, a.many = p.many, a.join_few = p.many && p.splits == 1;
+  a.unit = softcap > 0 ? 1.0f : scale * kLog2e;
   a.cap_log2 = softcap * kLog2e;
   a.inv_cap = softcap > 0 ? 2.0f * kLog2e * scale / softcap : 0.0f;
   hipStream_t st = static_cast<hipStream_t>(stream);

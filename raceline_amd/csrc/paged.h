@@ -65,26 +65,47 @@ __device__ __forceinline__ int cached(const PagedCache &c, int seq) {
 
 // Work items are numbered without a prefix sum over the sequences' own counts: sequence b begins
 // at (first row * mul) / div + extra * b, which leaves room for its items (a sequence of n rows
-// takes at most ceil(n * mul / div) + extra - 1), and a few numbers without an item. Every
-// thread takes part; returns the sequence whose range holds `slot`, or -1. One round trip to
-// memory for up to blockDim.x sequences, against log2(batch) for a binary search.
-__device__ __forceinline__ int64_t slot_base(const PagedCache &c, int seq, int mul, int div, int extra) {
-  return static_cast<int64_t>(row_start(c, seq)) * mul / div + static_cast<int64_t>(extra) * seq;
+// takes at most ceil(n * mul / div) + extra - 1), and a few numbers without an item.
+struct Sequence {
+  int b, row0, tokens, kv;   // b < 0: none; kv: tokens in the cache, the call's own among them
+  int item;                  // number of the item among the sequence's
+};
+
+__device__ __forceinline__ int64_t first_item(int row0, int seq, int mul, int div, int extra) {
+  return static_cast<int64_t>(row0) * mul / div + static_cast<int64_t>(extra) * seq;
 }
 
-template <int THREADS>
-__device__ __forceinline__ int find_sequence(const PagedCache &c, int64_t slot, int mul, int div, int extra,
-                                             int *shared) {
-  int below = 0;
-  for (int i = threadIdx.x; i < c.batch; i += THREADS) below += slot_base(c, i, mul, div, extra) <= slot ? 1 : 0;
-  for (int off = 32; off; off >>= 1) below += __shfl_xor(below, off);
-  if (THREADS > 64) {
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = below;
-    __syncthreads();
-    below = 0;
-    for (int i = 0; i < THREADS / 64; ++i) below += shared[i];
+// The sequence whose range holds item `slot`; the same in every lane of a wave. A wave looks over
+// 64 sequences with one load of a lane (one round trip to memory, against log2(batch) for a
+// binary search), and up to 63 sequences take the rest of what it returns from the same loads.
+__device__ __forceinline__ Sequence find_sequence(const PagedCache &c, int64_t slot, int mul, int div, int extra) {
+  const int lane = threadIdx.x & 63;
+  Sequence s;
+  if (c.batch < 64) {
+    const int row = row_start(c, min(lane, c.batch)), kv = cached(c, min(lane, c.batch - 1));
+    const bool below = lane < c.batch && first_item(row, lane, mul, div, extra) <= slot;
+    s.b = __popcll(__ballot(below)) - 1;
+    const int at = max(s.b, 0);
+    s.row0 = __builtin_amdgcn_readlane(row, at);
+    s.tokens = __builtin_amdgcn_readlane(row, at + 1) - s.row0;
+    s.kv = __builtin_amdgcn_readlane(kv, at);
+  } else {
+    int below = 0;
+    for (int i = lane; i < c.batch; i += 64) below += first_item(row_start(c, i), i, mul, div, extra) <= slot ? 1 : 0;
+    for (int off = 32; off; off >>= 1) below += __shfl_xor(below, off);
+    s.b = __builtin_amdgcn_readfirstlane(below) - 1;
+    const int at = max(s.b, 0);
+    s.row0 = row_start(c, at);
+    s.tokens = row_start(c, at + 1) - s.row0;
+    s.kv = cached(c, at);
   }
-  return below - 1;
+  // in scalar registers: what follows from them (page ids, addresses of copies) has to stay there
+  s.b = __builtin_amdgcn_readfirstlane(s.b);
+  s.row0 = __builtin_amdgcn_readfirstlane(s.row0);
+  s.tokens = max(0, __builtin_amdgcn_readfirstlane(s.tokens));
+  s.kv = __builtin_amdgcn_readfirstlane(s.kv);
+  s.item = __builtin_amdgcn_readfirstlane(static_cast<int>(slot - first_item(s.row0, max(s.b, 0), mul, div, extra)));
+  return s;
 }
 
 }  // namespace rlq

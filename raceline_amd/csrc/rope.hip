@@ -20,6 +20,7 @@ struct RopeArgs {
   PagedCache c;
   int64_t q_stride, k_stride, v_stride, out_stride;
   int heads, rot, interleaved, wide;   // wide: every row starts on 16 bytes
+  int heads_per;                       // of a key/value head's query heads and its key, those of one workgroup
   float mscale, eps;
 };
 
@@ -47,8 +48,9 @@ __device__ __forceinline__ void load8(const float *p, bool wide, float (&x)[8]) 
   }
 }
 
-// One workgroup: the tokens of one sequence that fall into one block of 32 positions, one
-// key/value head and the query heads that share it.
+// One workgroup: the tokens of one sequence that fall into one block of 32 positions, and some (in
+// small calls one, in large ones all) of the heads of one key/value head: the query heads that
+// share it, then its key, with which go its values.
 //   angle   a = pos * f, reduced to a fraction of a turn in 64 bits (a far position times a
 //           32-bit frequency would be off by more than the rounding of the result), then
 //           sincospi in 32; once per token and pair, kept in LDS for all heads.
@@ -57,49 +59,54 @@ __device__ __forceinline__ void load8(const float *p, bool wide, float (&x)[8]) 
 template <typename T, int D>
 __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
   constexpr int kChunks = D / 8, kRowStep = kRopeThreads / kChunks, kPad = D + 8;
-  __shared__ int found[kRopeThreads / 64];
-  __shared__ float2 turn[kBlockKeys * (D / 2)];
-  __shared__ T vals[kBlockKeys * kPad];
+  extern __shared__ float2 turn[];   // [32][rot / 2], then the values, [32][kPad]
   typedef typename Pack8<T>::type pack8;
 
   const int slot = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
-  const int b = find_sequence<kRopeThreads>(a.c, slot, 1, kBlockKeys, 2, found);
-  if (b < 0 || b >= a.c.batch) return;
-  const int row0 = row_start(a.c, b), n = row_start(a.c, b + 1) - row0, p0 = cached(a.c, b) - n;
-  const int block = (p0 >> 5) + (int)(slot - slot_base(a.c, b, 1, kBlockKeys, 2));
-  const int first = max(p0, block * kBlockKeys), tokens = min(p0 + n, (block + 1) * kBlockKeys) - first;
-  if (n <= 0 || tokens <= 0) return;
-  const int row = row0 + first - p0, lane_key = first - block * kBlockKeys;
-  const int page = page_of(a.c, b, block);
+  const Sequence s = find_sequence(a.c, slot, 1, kBlockKeys, 2);
+  const int p0 = s.kv - s.tokens, block = (p0 >> 5) + s.item;
+  const int first = max(p0, block * kBlockKeys), tokens = min(s.kv, (block + 1) * kBlockKeys) - first;
+  if (s.b < 0 || tokens <= 0) return;
+  const int row = s.row0 + first - p0, lane_key = first - block * kBlockKeys;
+  const int page = page_of(a.c, s.b, block);
 
-  const int half = a.rot >> 1;
+  const int group = a.heads / a.c.kv_heads, half = a.rot >> 1, chunk = tid % kChunks, d0 = chunk * 8;
+  const int head0 = blockIdx.z * a.heads_per, heads = min(a.heads_per, group + 1 - head0);
+  const bool with_key = head0 + heads == group + 1;
+  T *vals = reinterpret_cast<T *>(turn + kBlockKeys * half);
+  auto row_of = [&](int i) {   // item i: head head0 + i / tokens (group: the key), token i % tokens
+    const int h = head0 + i / tokens, t = i % tokens;
+    return h < group ? a.q + (row + t) * a.q_stride + (head * group + h) * D : a.k + (row + t) * a.k_stride + head * D;
+  };
+  float next[8] = {};
+  if (tid / kChunks < tokens * heads) load8(row_of(tid / kChunks) + d0, a.wide, next);
   for (int i = tid; i < tokens * half; i += kRopeThreads) {
     const int t = i / half, p = i - t * half;
     double x = (first + t) * (a.freq[p] * 0.15915494309189533577);   // turns
     x -= rint(x);
-    float s, c;
-    sincospif(2.0f * static_cast<float>(x), &s, &c);
-    turn[t * half + p] = make_float2(c * a.mscale, s * a.mscale);
+    float sin, cos;
+    sincospif(2.0f * static_cast<float>(x), &sin, &cos);
+    turn[t * half + p] = make_float2(cos * a.mscale, sin * a.mscale);
   }
-  const int chunk = tid % kChunks, d0 = chunk * 8;
-  for (int t = tid / kChunks; t < tokens; t += kRowStep) {
-    float x[8];
-    load8(a.v + (row + t) * a.v_stride + head * D + d0, a.wide, x);
-    *reinterpret_cast<pack8 *>(vals + (lane_key + t) * kPad + d0) = narrow8<T>(x);
+  if (with_key) {
+    for (int t = tid / kChunks; t < tokens; t += kRowStep) {
+      float x[8];
+      load8(a.v + (row + t) * a.v_stride + head * D + d0, a.wide, x);
+      *reinterpret_cast<pack8 *>(vals + (lane_key + t) * kPad + d0) = narrow8<T>(x);
+    }
   }
   __syncthreads();
 
   T *kb = page < 0 ? nullptr : static_cast<T *>(a.c.k) + block_base(a.c, page, head, block, D);
   T *vb = page < 0 ? nullptr : static_cast<T *>(a.c.v) + block_base(a.c, page, head, block, D);
-  const int group = a.heads / a.c.kv_heads;
-  for (int i = tid / kChunks; i < tokens * (group + 1); i += kRowStep) {
-    const int h = i / tokens, t = i - h * tokens;   // heads 0 .. group-1: queries, then the key
+  for (int i = tid / kChunks; i < tokens * heads; i += kRowStep) {
+    const int h = head0 + i / tokens, t = i % tokens;
     const bool is_q = h < group;
-    const float *src = is_q ? a.q + (row + t) * a.q_stride + (head * group + h) * D
-                            : a.k + (row + t) * a.k_stride + head * D;
-    const float *w = is_q ? a.q_norm : a.k_norm;
+    const float *src = row_of(i), *w = is_q ? a.q_norm : a.k_norm;
     float x[8], r = 1.0f;
-    load8(src + d0, a.wide, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = next[j];
+    if (i + kRowStep < tokens * heads) load8(row_of(i + kRowStep) + d0, a.wide, next);
     if (w) {
       float ss = 0.0f;
 #pragma unroll
@@ -155,7 +162,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
       *reinterpret_cast<pack8 *>(kb + key_offset(lane_key + t, d0)) = y;
     }
   }
-  if (!vb) return;
+  if (!vb || !with_key) return;
   for (int i = tid; i < D * 4; i += kRopeThreads) {
     const int d = (i & 31) | ((i >> 7) << 5), t = (i >> 6) & 1, h = (i >> 5) & 1;
     T *dst = vb + value_run(d, t, h);
@@ -179,14 +186,24 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
   }
 }
 
-template <typename T>
-int launch_rope(const RopeArgs &a, int D, hipStream_t st) {
-  const dim3 grid((unsigned)(a.c.rows / kBlockKeys + 2 * a.c.batch), (unsigned)a.c.kv_heads);
-  if (D == 64) rope_append_kernel<T, 64><<<grid, kRopeThreads, 0, st>>>(a);
-  if (D == 128) rope_append_kernel<T, 128><<<grid, kRopeThreads, 0, st>>>(a);
-  if (D == 256) rope_append_kernel<T, 256><<<grid, kRopeThreads, 0, st>>>(a);
+template <typename T, int D>
+int launch_size(RopeArgs a, hipStream_t st) {
+  const int64_t blocks = a.c.rows / kBlockKeys + 2 * (int64_t)a.c.batch;
+  const int group = a.heads / a.c.kv_heads;
+  a.heads_per = blocks * a.c.kv_heads < 1024 ? 1 : group + 1;
+  const dim3 grid((unsigned)blocks, (unsigned)a.c.kv_heads, (unsigned)((group + a.heads_per) / a.heads_per));
+  const int lds = kBlockKeys * ((a.rot / 2) * (int)sizeof(float2) + (D + 8) * (int)sizeof(T));
+  RLQ_REQUIRE(grid.z <= 65535, "rlq_rope_append: %d heads share a key/value head, more than 65534", group);
+  rope_append_kernel<T, D><<<grid, kRopeThreads, lds, st>>>(a);
   RLQ_HIP(hipGetLastError());
   return 0;
+}
+
+template <typename T>
+int launch_rope(const RopeArgs &a, int D, hipStream_t st) {
+  if (D == 64) return launch_size<T, 64>(a, st);
+  if (D == 128) return launch_size<T, 128>(a, st);
+  return launch_size<T, 256>(a, st);
 }
 
 }  // namespace

@@ -13,6 +13,7 @@ stream (see include/rlq.h); the dequantized value of every weight is unchanged.
 
 from __future__ import annotations
 
+import functools
 import threading
 from dataclasses import dataclass, field
 
@@ -547,48 +548,63 @@ def kv_cache(n_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, dt
     return torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
 
 
+# Dtypes are compared by identity and devices by number here: a serving step makes these calls for
+# every layer, and the checks are half of what a call costs the host.
+_CODES = {torch.float16: F16, torch.bfloat16: BF16}
+
+
 def _check_paged(k_cache, v_cache, cu_q, kv_len, table):
-    """Shapes, types and places of a cache and its sequences; (code, B)."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+    """Shapes, types and places of a cache and its sequences -> (n_pages, kv_heads, page_size,
+    head_dim), the type's code, the device's number, B."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
         raise ValueError("k_cache and v_cache must be alike, [n_pages][kv_heads][page_size][head_dim]")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache and v_cache must be contiguous")
-    if not (cu_q.dtype == kv_len.dtype == table.dtype == torch.int32):
+    code = _CODES.get(k_cache.dtype)
+    if code is None:
+        raise ValueError(f"the cache must be float16 or bfloat16, not {k_cache.dtype}")
+    i32 = torch.int32
+    if cu_q.dtype is not i32 or kv_len.dtype is not i32 or table.dtype is not i32:
         raise TypeError("cu_q, kv_len and table must be int32")
     B = kv_len.numel()
-    if kv_len.dim() != 1 or cu_q.dim() != 1 or cu_q.numel() != B + 1 or not (cu_q.is_contiguous() and kv_len.is_contiguous()):
+    if kv_len.shape != (B,) or cu_q.shape != (B + 1,) or not (cu_q.is_contiguous() and kv_len.is_contiguous()):
         raise ValueError("kv_len must be a contiguous vector [B], cu_q [B + 1]")
-    if table.dim() != 2 or table.shape[0] < B or (table.shape[1] > 1 and table.stride(1) != 1):
+    rows = table.shape
+    if len(rows) != 2 or rows[0] < B or (rows[1] > 1 and table.stride(1) != 1):
         raise ValueError("table must be a row-major matrix [B][pages of a sequence]")
-    dev = k_cache.device
-    if not (v_cache.device == cu_q.device == kv_len.device == table.device == dev):
+    dev = k_cache.get_device()
+    if v_cache.get_device() != dev or cu_q.get_device() != dev or kv_len.get_device() != dev or table.get_device() != dev:
         raise ValueError("the cache and its sequences must be on one device")
-    return scale_code(k_cache.dtype), B
+    return shape, code, dev, B
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _rows(t, dtype, dev, what):
+    """(rows, columns, row stride) of a row-major matrix of a type on a device."""
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{what} must be {dtype} on the device of the call's other tensors")
+    shape = t.shape
+    if len(shape) != 2 or (shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be a row-major matrix")
+    return shape[0], shape[1], t.stride(0) if shape[0] > 1 else max(t.stride(0), shape[1])
 
 
-def _call_on(device: torch.device, stream, name: str, *args):
+def _call_on(dev: int, stream, name: str, *args):
     """lib.call on the device its tensors live on, whichever is current."""
-    if device.type != "cuda":
-        raise ValueError(f"{name} needs tensors on the GPU, not on {device}")
-    if stream is None and (_current_device is None or device.index != _current_device()):
-        with torch.cuda.device(device):
-            return lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
-    if stream is not None and stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
-    if stream is not None and (_current_device is None or device.index != _current_device()):
-        with torch.cuda.device(device):
-            return lib.call(name, *args, stream.cuda_stream)
-    return lib.call(name, *args, _stream(stream))
+    if dev < 0:
+        raise ValueError(f"{name} needs tensors on the GPU")
+    if stream is not None and stream.device_index != dev:
+        raise ValueError(f"{name}: the stream is on device {stream.device_index}, the tensors on {dev}")
+    if _raw_stream is None or _current_device is None or _current_device() != dev:
+        with torch.cuda.device(dev):
+            return lib.call(name, *args, _stream(stream))
+    return lib.call(name, *args, _raw_stream(dev) if stream is None else stream.cuda_stream)
 
 
-def _new(shape, dtype, device, stream) -> torch.Tensor:
+def _new(like, shape, dtype, stream) -> torch.Tensor:
     """An output or scratch tensor that the caching allocator keeps until `stream` is through."""
-    t = torch.empty(shape, dtype=dtype, device=device)
-    if stream is not None:
+    t = torch.empty(shape, dtype=dtype, device=like.device)
+    if stream is not None and t.is_cuda:
         t.record_stream(stream)
     return t
 
@@ -602,35 +618,37 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     queries [T][heads * head_dim] in the cache's dtype, and keys and values in the cache
     (rlq_rope_append). Row i of a sequence's n new rows has position kv_len - n + i; freq:
     rope_frequencies, None turns nothing. Rows from cu_q[B] on are left as they were in `out`."""
-    code, B = _check_paged(k_cache, v_cache, cu_q, kv_len, table)
-    n_pages, kv_heads, page, D = k_cache.shape
-    dev = k_cache.device
-    for t in (q, k, v):
-        if t.dtype != torch.float32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or t.device != dev:
-            raise ValueError("q, k and v must be row-major float32 matrices on the cache's device")
-    T = q.shape[0]
-    if k.shape != (T, kv_heads * D) or v.shape != k.shape or q.shape[1] % (kv_heads * D) or q.shape[1] == 0:
+    (n_pages, kv_heads, page, D), code, dev, B = _check_paged(k_cache, v_cache, cu_q, kv_len, table)
+    f32 = torch.float32
+    T, width, qs = _rows(q, f32, dev, "q")
+    Tk, kw, ks = _rows(k, f32, dev, "k")
+    Tv, vw, vs = _rows(v, f32, dev, "v")
+    if Tk != T or Tv != T or kw != kv_heads * D or vw != kw or width % max(kw, 1) or not width:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match {kv_heads} "
                          f"key/value heads of {D}")
     rot = 0
     if freq is not None:
-        if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous() or freq.device != dev:
+        if freq.dtype is not torch.float64 or freq.dim() != 1 or not freq.is_contiguous() or freq.get_device() != dev:
             raise ValueError("freq must be a contiguous float64 vector on the cache's device")
         rot = 2 * freq.numel()
     for w in (q_norm, k_norm):
-        if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous() or w.device != dev):
+        if w is not None and (w.dtype is not f32 or w.shape != (D,) or not w.is_contiguous() or w.get_device() != dev):
             raise ValueError(f"q_norm and k_norm must be contiguous float32 vectors of {D} on the cache's device")
     if out is None:
-        out = _new((T, q.shape[1]), k_cache.dtype, dev, stream)
-    elif out.dtype != k_cache.dtype or out.shape != q.shape or out.stride(1) != 1 or out.device != dev:
-        raise ValueError(f"out must be a row-major {k_cache.dtype} matrix shaped like q")
-    _call_on(dev, stream, "rlq_rope_append", _ptr(q), _row_stride(q), _ptr(k), _row_stride(k), _ptr(v), _row_stride(v), T,
-             _ptr(freq), rot, 1 if interleaved else 0, mscale, _ptr(q_norm), _ptr(k_norm), eps, q.shape[1] // D, kv_heads,
-             D, code, _ptr(out), _row_stride(out), _ptr(k_cache), _ptr(v_cache), n_pages, page, _ptr(cu_q), _ptr(kv_len),
-             _ptr(table), max(table.stride(0), table.shape[1]), table.shape[1], B)
+        out = _new(q, (T, width), k_cache.dtype, stream)
+        os = width
+    else:
+        To, ow, os = _rows(out, k_cache.dtype, dev, "out")
+        if To != T or ow != width:
+            raise ValueError("out must be shaped like q")
+    _call_on(dev, stream, "rlq_rope_append", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, T, _ptr(freq), rot,
+             1 if interleaved else 0, mscale, _ptr(q_norm), _ptr(k_norm), eps, width // D, kv_heads, D, code,
+             out.data_ptr(), os, k_cache.data_ptr(), v_cache.data_ptr(), n_pages, page, cu_q.data_ptr(),
+             kv_len.data_ptr(), table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1], B)
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_workspace_bytes(T: int, heads: int, kv_heads: int, head_dim: int, B: int, max_q: int, max_kv: int,
                               window: int = 0) -> int:
     return int(lib.load().rlq_attention_workspace_bytes(T, heads, kv_heads, head_dim, B, max_q, max_kv, window))
@@ -646,47 +664,60 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_
     by default; window: the last positions a row sees (0: all); softcap: 0 for none. Rows from
     cu_q[B] on are left as they were in `out`. workspace: scratch to use in place of a new
     tensor; calls that overlap must not share it."""
-    code, B = _check_paged(k_cache, v_cache, cu_q, kv_len, table)
-    n_pages, kv_heads, page, D = k_cache.shape
-    dev = k_cache.device
-    if q.dtype != k_cache.dtype or q.dim() != 2 or q.stride(1) != 1 or q.device != dev:
-        raise ValueError(f"q must be a row-major {k_cache.dtype} matrix on the cache's device")
-    T, width = q.shape
-    if width == 0 or width % (kv_heads * D):
+    (n_pages, kv_heads, page, D), code, dev, B = _check_paged(k_cache, v_cache, cu_q, kv_len, table)
+    T, width, qs = _rows(q, k_cache.dtype, dev, "q")
+    if not width or width % max(kv_heads * D, 1):
         raise ValueError(f"q rows of {width} are no whole number of {D}-wide heads a key/value head")
     if out is None:
-        out = _new((T, width), out_dtype, dev, stream)
-    elif out.shape != q.shape or out.stride(1) != 1 or out.device != dev:
-        raise ValueError("out must be a row-major matrix shaped like q")
+        out = _new(q, (T, width), out_dtype, stream)
+        os = width
+    else:
+        To, ow, os = _rows(out, out.dtype, dev, "out")
+        if To != T or ow != width:
+            raise ValueError("out must be shaped like q")
+    out_code = _CODES.get(out.dtype)
+    if out_code is None:
+        raise ValueError(f"out must be float16 or bfloat16, not {out.dtype}")
     H = width // D
-    nbytes = int(lib.load().rlq_attention_workspace_bytes(T, H, kv_heads, D, B, max_q, max_kv, window))
-    if workspace is not None and workspace.device != dev:
-        raise ValueError("the workspace must be on the cache's device")
-    if nbytes and workspace is None:
-        workspace = _new(nbytes, torch.uint8, dev, stream)
-    _call_on(dev, stream, "rlq_attention", _ptr(q), _row_stride(q), T, H, kv_heads, D, code, _ptr(k_cache), _ptr(v_cache),
-             n_pages, page, _ptr(cu_q), _ptr(kv_len), _ptr(table), max(table.stride(0), table.shape[1]), table.shape[1],
-             B, max_q, max_kv, D ** -0.5 if scale is None else scale, window, softcap, _ptr(out), _row_stride(out),
-             scale_code(out.dtype), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size())
+    nbytes = attention_workspace_bytes(T, H, kv_heads, D, B, max_q, max_kv, window)
+    if workspace is None:
+        if nbytes:
+            workspace = _new(q, nbytes, torch.uint8, stream)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous, on the cache's device")
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+    _call_on(dev, stream, "rlq_attention", q.data_ptr(), qs, T, H, kv_heads, D, code, k_cache.data_ptr(),
+             v_cache.data_ptr(), n_pages, page, cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
+             max(table.stride(0), table.shape[1]), table.shape[1], B, max_q, max_kv, D ** -0.5 if scale is None else scale,
+             window, softcap, out.data_ptr(), os, out_code, _ptr(workspace), nbytes)
     return out
 
 
 # ------------------------------------------------------------------ logits
 
-def _check_row_vector(t, rows, dtype, what, dev):
-    if t is not None and (t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous() or t.device != dev):
-        raise ValueError(f"{what} must be a contiguous {dtype} vector of {rows} rows on the logits' device")
-
-
-def _shared_rows(t, rows, dtype, what, dev) -> int:
-    """Row stride of a matrix with a row per row of logits, or of one row (or a vector) for all: 0."""
-    if t.dtype != dtype or t.dim() not in (1, 2) or (t.shape[-1] > 1 and t.stride(-1) != 1) or t.device != dev:
-        raise ValueError(f"{what} must be a row-major {dtype} matrix (or one row) on the logits' device")
-    if t.dim() == 1:
+def _row_vector(t, rows, dtype, what, dev) -> int:
+    if t is None:
         return 0
-    if t.shape[0] != rows and t.shape[0] != 1:
-        raise ValueError(f"{what} has {t.shape[0]} rows, the logits have {rows}")
-    return t.stride(0) if t.shape[0] == rows else 0
+    if t.dtype is not dtype or t.shape != (rows,) or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of {rows} rows on the logits' device")
+    return t.data_ptr()
+
+
+def _shared_rows(t, rows, dtypes, what, dev):
+    """(pointer, row stride, columns) of a matrix with a row per row of logits, or of one row (or
+    a vector) for all: stride 0."""
+    shape = t.shape
+    if t.dtype not in dtypes or len(shape) not in (1, 2) or (shape[-1] > 1 and t.stride(-1) != 1) or t.get_device() != dev:
+        raise ValueError(f"{what} must be a row-major {dtypes[0]} matrix (or one row) on the logits' device")
+    if len(shape) == 1:
+        return t.data_ptr(), 0, shape[0]
+    if shape[0] != rows and shape[0] != 1:
+        raise ValueError(f"{what} has {shape[0]} rows, the logits have {rows}")
+    return t.data_ptr(), t.stride(0) if shape[0] > 1 else 0, shape[1]
+
+
+_I32, _F32, _BITS = (torch.int32,), (torch.float32,), (torch.int32, torch.uint32)
 
 
 def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, n_tokens: torch.Tensor | None = None,
@@ -700,34 +731,33 @@ def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, n_to
     those from n_prompt on for `presence` and `frequency` (fp32 [rows]); bias_ids int32 and bias
     fp32 [rows][n]; allowed int32 or uint32 [rows][words], bit v % 32 of word v / 32 set where
     token v may follow. tokens, biases and the mask may be one row for all."""
-    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits must be a row-major float32 matrix")
-    rows, vocab = logits.shape
-    dev = logits.device
+    dev = logits.get_device()
+    rows, vocab, xs = _rows(logits, torch.float32, dev, "logits")
     if out is None:
-        out = _new((rows, vocab), torch.float32, dev, stream)
-    elif out.dtype != torch.float32 or out.shape != logits.shape or (vocab > 1 and out.stride(1) != 1) or out.device != dev:
-        raise ValueError("out must be a row-major float32 matrix shaped like logits")
-    ts = n = bs = nb = ms = 0
+        out = _new(logits, (rows, vocab), torch.float32, stream)
+        ys = vocab
+    else:
+        orows, ovocab, ys = _rows(out, torch.float32, dev, "out")
+        if orows != rows or ovocab != vocab:
+            raise ValueError("out must be shaped like logits")
+    tp = ts = n = ip = bp = bs = nb = mp = ms = 0
     if tokens is not None:
-        ts, n = _shared_rows(tokens, rows, torch.int32, "tokens", dev), tokens.shape[-1]
-    _check_row_vector(n_tokens, rows, torch.int32, "n_tokens", dev)
-    _check_row_vector(n_prompt, rows, torch.int32, "n_prompt", dev)
-    _check_row_vector(repetition, rows, torch.float32, "repetition", dev)
-    _check_row_vector(presence, rows, torch.float32, "presence", dev)
-    _check_row_vector(frequency, rows, torch.float32, "frequency", dev)
+        tp, ts, n = _shared_rows(tokens, rows, _I32, "tokens", dev)
     if (bias is None) != (bias_ids is None):
         raise ValueError("bias and bias_ids come together")
     if bias is not None:
-        bs, nb = _shared_rows(bias, rows, torch.float32, "bias", dev), bias.shape[-1]
-        if bias_ids.shape != bias.shape or _shared_rows(bias_ids, rows, torch.int32, "bias_ids", dev) != bs:
-            raise ValueError("bias_ids must be shaped like bias")
+        bp, bs, nb = _shared_rows(bias, rows, _F32, "bias", dev)
+        ip, ids_stride, ids_n = _shared_rows(bias_ids, rows, _I32, "bias_ids", dev)
+        if ids_n != nb or ids_stride != bs:
+            raise ValueError("bias_ids must be laid out like bias")
     if allowed is not None:
-        ms = _shared_rows(allowed, rows, allowed.dtype if allowed.dtype in (torch.int32, torch.uint32) else torch.int32,
-                          "allowed", dev)
-        if allowed.shape[-1] < (vocab + 31) // 32:
-            raise ValueError(f"a mask row of {allowed.shape[-1]} words is shorter than the vocabulary")
-    _call_on(dev, stream, "rlq_adjust_logits", _ptr(logits), _row_stride(logits), rows, vocab, _ptr(tokens), ts, n,
-             _ptr(n_tokens), _ptr(n_prompt), _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_ids), _ptr(bias),
-             nb, bs, _ptr(allowed), ms, _ptr(out), _row_stride(out))
+        mp, ms, words = _shared_rows(allowed, rows, _BITS, "allowed", dev)
+        if words < (vocab + 31) // 32:
+            raise ValueError(f"a mask row of {words} words is shorter than the vocabulary")
+    _call_on(dev, stream, "rlq_adjust_logits", logits.data_ptr(), xs, rows, vocab, tp, ts, n,
+             _row_vector(n_tokens, rows, torch.int32, "n_tokens", dev),
+             _row_vector(n_prompt, rows, torch.int32, "n_prompt", dev),
+             _row_vector(repetition, rows, torch.float32, "repetition", dev),
+             _row_vector(presence, rows, torch.float32, "presence", dev),
+             _row_vector(frequency, rows, torch.float32, "frequency", dev), ip, bp, nb, bs, mp, ms, out.data_ptr(), ys)
     return out
