@@ -43,8 +43,8 @@ struct AttnArgs {
   float2 *part_stat;          // [splits][rows][heads]: (ref, sum of weights)
   int *part_runs;             // [rows][heads]: runs of the row
   int heads, group, window, out_bf16, q_wide, out_wide;
-  int splits, span;           // keys are split in runs of `span` positions (a multiple of 32)
-  int few_splits, few_span;   // the same for sequences of few rows
+  int whole, splits, span;    // the `whole` longest tiles of a head are not split, the others' keys in runs of `span` (a multiple of 32)
+  int few_splits, few_span;   // the same for sequences of few rows, all of them
   int few, many;              // which kernels this call launches
   int join_few;               // join_runs_kernel: only sequences of few rows have more than one run
   float unit, cap_log2, inv_cap;   // unit: base-2 units of a score as the product gives it, or of a capped one (1)
@@ -131,10 +131,67 @@ __device__ __forceinline__ int first_key(const AttnArgs &a, const Sequence &s) {
   return a.window ? max(0, s.kv - s.tokens + 1 - a.window) & ~(kBlockKeys - 1) : 0;
 }
 
-// Runs that hold keys of the sequence; one run's kernel writes the rows itself.
-__device__ __forceinline__ int runs_of(const AttnArgs &a, const Sequence &s, bool few) {
-  const int span = few ? a.few_span : a.span, splits = few ? a.few_splits : a.splits;
+// Runs that hold keys of the sequence; where there is one, its workgroup finishes the rows itself.
+__device__ __forceinline__ int runs_of(const AttnArgs &a, const Sequence &s, int splits, int span) {
   return max(1, min(splits, (s.kv - first_key(a, s) + span - 1) / span));
+}
+
+// many_rows_kernel's tile of a rank, longest first: a chip that is given its last long tile late
+// waits for it (six prompts of up to 1537 tokens in the order of the batch, the longest last:
+// 87 us, in this order RANKED us). Tile d of a sequence counts as long as the sequence before the
+// call's rows and (d + 1) * 128 / group of them; 64 lanes try 64 lengths at a time for the one past
+// which lie as many tiles as the rank says. 64 sequences and more go in the order of the batch, last
+// tile first.
+__device__ __forceinline__ Sequence find_tile(const AttnArgs &a, int rank, int slots) {
+  if (a.c.batch >= 64) return find_sequence(a.c, slots - 1 - rank, a.group, kManyRows, 1);
+  const int lane = threadIdx.x & 63, batch = a.c.batch;
+  const int row = row_start(a.c, min(lane, batch)), kv = cached(a.c, min(lane, batch - 1));
+  const int tokens = max(0, __shfl(row, lane + 1) - row);
+  int tiles = lane < batch ? (tokens * a.group + kManyRows - 1) / kManyRows : 0;
+  if (a.few && tokens * a.group <= kFewRows) tiles = 0;   // few_rows_kernel's
+  const int before = kv - tokens;
+  auto shorter = [&](int length, int b) {                  // tiles of sequence b no longer than that
+    const int64_t x = static_cast<int64_t>(length - __builtin_amdgcn_readlane(before, b)) * a.group;
+    const int most = __builtin_amdgcn_readlane(tiles, b);
+    return static_cast<int>(max<int64_t>(0, min<int64_t>(x / kManyRows, most)));
+  };
+  auto longer = [&](int length) {                          // of all sequences, longer
+    int n = 0;
+    for (int b = 0; b < batch; ++b) n += __builtin_amdgcn_readlane(tiles, b) - shorter(length, b);
+    return n;
+  };
+  Sequence s = {-1, 0, 0, 0, 0};
+  // no tile is longer than `most`, and none is as short as `least`
+  int least = kMaxPositions, most = 0;
+  for (int b = 0; b < batch; ++b) {
+    const int from = __builtin_amdgcn_readlane(before, b), n = __builtin_amdgcn_readlane(tiles, b);
+    if (!n) continue;
+    least = min(least, from);
+    most = max(most, from + static_cast<int>((static_cast<int64_t>(n) * kManyRows + a.group - 1) / a.group));
+  }
+  if (rank >= longer(least)) return s;
+  while (most - least > 1) {                               // longer(most) <= rank < longer(least)
+    const int step = (most - least + 63) / 64, at = min(most, least + (lane + 1) * step);
+    const uint64_t low = __ballot(longer(at) <= rank);
+    const int first = __builtin_ctzll(low);                // the last lane's length is `most`
+    most = min(most, least + (first + 1) * step);
+    least = least + first * step;
+  }
+  int left = rank - __builtin_amdgcn_readfirstlane(longer(most));
+  for (int b = 0; b < batch; ++b) {
+    const int upto = __builtin_amdgcn_readfirstlane(shorter(most, b));
+    const int n = upto - __builtin_amdgcn_readfirstlane(shorter(most - 1, b));
+    if (left < n) {
+      s.b = b;
+      s.item = upto - 1 - left;
+      s.row0 = __builtin_amdgcn_readlane(row, b);
+      s.tokens = __builtin_amdgcn_readlane(tokens, b);
+      s.kv = __builtin_amdgcn_readlane(kv, b);
+      break;
+    }
+    left -= n;
+  }
+  return s;
 }
 
 __device__ __forceinline__ float *part_row(const AttnArgs &a, int split, int row, int head, int D) {
@@ -149,15 +206,13 @@ __device__ __forceinline__ int &run_count(const AttnArgs &a, int row, int head) 
   return a.part_runs[static_cast<int64_t>(row) * a.heads + head];
 }
 
-// Adds the infinities and NaN among one block's values to o (o[i]: dimension dim(i)) for the keys
-// that a row sees.
+// Adds the infinities and NaN among the values of block `at` (its first key `first`) to o (o[i]:
+// dimension dim(i)) for the keys that a row sees.
 template <typename T, int D, int N, typename Dim>
-__device__ __forceinline__ void add_odd(const AttnArgs &a, int page, int head, int block, int lo, int hi, Dim dim,
-                                        float (&o)[N]) {
-  const unsigned short *v = static_cast<const unsigned short *>(a.c.v) + block_base(a.c, page, head, block, D);
+__device__ __forceinline__ void add_odd(const AttnArgs &a, int at, int first, int lo, int hi, Dim dim, float (&o)[N]) {
+  const unsigned short *v = static_cast<const unsigned short *>(a.c.v) + static_cast<int64_t>(at) * (kBlockKeys * D);
   for (int key = 0; key < kBlockKeys; ++key) {
-    const int at = block * kBlockKeys + key;
-    const bool seen = at >= lo && at <= hi;
+    const bool seen = first + key >= lo && first + key <= hi;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const unsigned x = v[value_run(dim(i), key >> 4, key >> 2 & 1) + (key >> 3 & 1) * 4 + (key & 3)];
@@ -222,7 +277,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
   const Sequence s = find_sequence(a.c, slot, a.many ? 0 : a.group, ROWS, 1);
   const int b = s.b, tile = s.item * ROWS, rows = s.tokens * a.group;
   if (b < 0 || tile < 0 || tile >= rows || !is_few(a, s)) return;
-  const int runs = runs_of(a, s, true);
+  const int runs = runs_of(a, s, a.few_splits, a.few_span);
   if (split >= runs) return;
 
   // rows of this lane's columns, and what they see
@@ -264,7 +319,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
   const int key0 = 16 * (g >> 1) + 4 * (g & 1);   // this lane's keys: key0 + 8 j + i
   op kr[KS][2];
   u32x4 vr[DT];
-  int pages = -1;                                  // lane i: the page of this wave's i-th block from `from`
+  int pages = -1;                                  // lane i: this wave's block from + i, by its number in the cache
   int from = 0;
   const int nblk = max(0, blk1 - blk0), mine = nblk > wave ? (nblk - wave + 3) / 4 : 0;
   auto page_at = [&](int i) {
@@ -272,12 +327,12 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     if (i - from >= 64 || i == 0) {
       from = i;
       const int blk = blk0 + wave + 4 * (i + lane);
-      pages = i + lane < mine ? page_of(a.c, b, blk) : -1;
+      pages = i + lane < mine ? block_at(a.c, b, head, blk) : -1;
     }
     return __builtin_amdgcn_readlane(pages, i - from);
   };
-  auto load_k = [&](int page, int blk) {
-    const T *p = kc + block_base(a.c, page, head, blk, D) + koff;
+  auto load_k = [&](int at) {
+    const T *p = kc + static_cast<int64_t>(at) * (kBlockKeys * D) + koff;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       kr[k][0] = __builtin_nontemporal_load(reinterpret_cast<const op *>(p + k * 1024));
@@ -285,16 +340,16 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     }
   };
   int page = page_at(0);
-  if (page >= 0) load_k(page, blk0 + wave);
+  if (page >= 0) load_k(page);
   for (int i = 0; i < mine; ++i) {
     const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
     const int next = page_at(i + 1);
     if (page < 0) {
       page = next;
-      if (page >= 0) load_k(page, blk + 4);
+      if (page >= 0) load_k(page);
       continue;
     }
-    const T *vp = vc + block_base(a.c, page, head, blk, D) + voff;
+    const T *vp = vc + static_cast<int64_t>(page) * (kBlockKeys * D) + voff;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
       vr[d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp + (d >> 1) * 1024 + (d & 1) * 128));
@@ -308,7 +363,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
 #pragma unroll
         for (int k = 0; k < KS; ++k) sc[n][j] = Mfma<T>::mul16(kr[k][j], queries[n][k][lane], sc[n][j]);
       }
-    if (next >= 0) load_k(next, blk + 4);
+    if (next >= 0) load_k(next);
     page = next;
 
     const bool masked = first < lo_all || first + kBlockKeys - 1 > hi_all || first + kBlockKeys > end;
@@ -373,14 +428,14 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     for (int i = 0; i < mine; ++i) {
       const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
       if (first >= lo_all && first + kBlockKeys - 1 <= hi_all && first + kBlockKeys <= end) continue;
-      const int at = page_of(a.c, b, blk);
+      const int at = block_at(a.c, b, head, blk);
       if (at < 0) continue;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           float part[4] = {o[n][d][0], o[n][d][1], o[n][d][2], o[n][d][3]};
-          add_odd<T, D, 4>(a, at, head, blk, lo[n], hi[n], [&](int j) { return 16 * d + 4 * g + j; }, part);
+          add_odd<T, D, 4>(a, at, first, lo[n], hi[n], [&](int j) { return 16 * d + 4 * g + j; }, part);
           o[n][d] = f32x4{part[0], part[1], part[2], part[3]};
         }
     }
@@ -453,20 +508,16 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
 
 // ----------------------------------------------------------------------------- many rows
 
-// One LDS-DMA: 16 bytes a lane into the kilobyte at lds + at.
-__device__ __forceinline__ void dma_kb(const void *src, unsigned char *lds, int at, int lane) {
-  __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(src), (short)0, 1024, 0x00020000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + at), 16, 16 * lane, 0, 0,
-                                           0);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const void *p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, bytes, 0x00020000);
 }
 
-// One workgroup: 128 rows of one sequence and key/value head over one run of its keys; each of its
-// four waves holds 32 rows (Q^T as B operands, O^T accumulators) and takes every key.
-// Keys and values go through LDS in tiles of KB keys, copied as they lie (the cache's order is the
-// operands' order: no swizzle, no transpose, no bank conflicts), two stages deep, so that the
-// next tile's copy runs under this tile's products; one barrier a tile. 64 rows a wave (half the
-// LDS reads, one wave a SIMD) were slower: 69 us against 60 for 333 rows over 20,011 keys in
-// heads of 64, and did not fit the registers in heads of 256.
+// One LDS-DMA: 16 bytes a lane into the kilobyte at lds + at. (Not a template: in one, the host
+// pass refuses the 16-byte size.)
+__device__ __forceinline__ void dma_kb(__amdgpu_buffer_rsrc_t r, unsigned char *lds, int at, int voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + at), 16, voff, soff, 0, 0);
+}
+
 template <int N, int AHEAD, int READS, int PER, int VALU>
 __device__ __forceinline__ void feed_step() {
   if constexpr (N < READS * PER) {
@@ -499,14 +550,15 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
   extern __shared__ unsigned char lds[];   // two stages, then a flag
   int *odd = reinterpret_cast<int *>(lds + 2 * kStage);
 
-  const int KV = a.c.kv_heads, head = blockIdx.x % KV, split = (blockIdx.x / KV) % a.splits;
-  const int64_t slots = gridDim.x / KV / a.splits, slot = slots - 1 - blockIdx.x / KV / a.splits;
+  const int KV = a.c.kv_heads, head = blockIdx.x % KV, item = blockIdx.x / KV, slots = a.c.rows * a.group / kManyRows + a.c.batch;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
-  const Sequence s = find_sequence(a.c, slot, a.group, ROWS, 1);
-  const int b = s.b, tile = s.item * ROWS, rows = s.tokens * a.group;
+  const bool whole = item < a.whole;
+  const int splits = whole ? 1 : a.splits, split = whole ? 0 : (item - a.whole) % splits;
+  const Sequence s = find_tile(a, whole ? item : a.whole + (item - a.whole) / splits, slots);
+  const int b = s.b, tile = s.item * kManyRows, rows = s.tokens * a.group;
   if (b < 0 || tile < 0 || tile >= rows || is_few(a, s)) return;
-  const int runs = runs_of(a, s, false);
+  const int runs = runs_of(a, s, splits, a.span);
   if (split >= runs) return;
 
   // this lane's rows and what they see
@@ -523,7 +575,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
   const int lo_any = a.window ? max(0, p0 + tile / a.group - a.window + 1) : 0, hi_any = p0 + last / a.group;
   const int lo_all = a.window ? max(0, p0 + last / a.group - a.window + 1) : 0, hi_all = p0 + tile / a.group;
   const int base = first_key(a, s) + split * a.span;
-  const int end = min(hi_any + 1, split == a.splits - 1 ? hi_any + 1 : base + a.span);
+  const int end = min(hi_any + 1, split == splits - 1 ? hi_any + 1 : base + a.span);
   const int blk0 = max(base, lo_any & ~(kBlockKeys - 1)) / kBlockKeys, blk1 = (end + kBlockKeys - 1) / kBlockKeys;
   const int nblk = max(0, blk1 - blk0), tiles = (nblk + NB - 1) / NB;
 
@@ -536,12 +588,12 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
   const char *kc = static_cast<const char *>(a.c.k), *vc = static_cast<const char *>(a.c.v);
-  int pages = -1, from = 0;   // lane i: the page of block from + i of the run
+  int pages = -1, from = 0;   // lane i: block from + i of the run, by its number in the cache
   auto page_at = [&](int i) {
     if (i >= nblk) return -1;
     if (i - from >= 64 || i == 0) {
       from = i;
-      pages = i + lane < nblk ? page_of(a.c, b, blk0 + i + lane) : -1;
+      pages = i + lane < nblk ? block_at(a.c, b, head, blk0 + i + lane) : -1;
     }
     return __builtin_amdgcn_readlane(pages, i - from);
   };
@@ -550,11 +602,14 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
     for (int j = 0; j < NB; ++j) {
       page[j] = page_at(kt * NB + j);
       if (page[j] < 0) continue;
-      const int64_t at = block_base(a.c, page[j], head, blk0 + kt * NB + j, D) * 2;
+      const int64_t at = static_cast<int64_t>(page[j]) * kBlockBytes;
+      const int to = buf * kStage + j * kBlockBytes + wave * 1024;
+      const __amdgpu_buffer_rsrc_t kr = block_rsrc(kc + at, kBlockBytes), vr = block_rsrc(vc + at, kBlockBytes);
 #pragma unroll
-      for (int i = wave; i < 2 * kPieces; i += 4)
-        dma_kb((i < kPieces ? kc : vc) + at + (i % kPieces) * 1024, lds,
-               buf * kStage + (i < kPieces ? 0 : NB * kBlockBytes) + j * kBlockBytes + (i % kPieces) * 1024, lane);
+      for (int i = 0; i < kPieces / 4; ++i) dma_kb(kr, lds, to + i * 4096, 16 * lane, wave * 1024 + i * 4096);
+#pragma unroll
+      for (int i = 0; i < kPieces / 4; ++i)
+        dma_kb(vr, lds, to + NB * kBlockBytes + i * 4096, 16 * lane, wave * 1024 + i * 4096);
     }
   };
 
@@ -617,6 +672,10 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
           sc[j][i] = key >= lo && key <= hi && page[j] >= 0 ? sc[j][i] : -__builtin_inff();
         }
     }
+    op va[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) va[i] = *reinterpret_cast<const op *>(vl + i * 1024);
+    __builtin_amdgcn_sched_barrier(0);
     float top = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < NB; ++j)
@@ -654,11 +713,12 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const op v = *reinterpret_cast<const op *>(vl + (j - 1) * kBlockBytes + (2 * d + t) * 1024);
+            const op v = j == 1 && 2 * d + t < kAhead ? va[(2 * d + t) % kAhead] : *reinterpret_cast<const op *>(vl + (j - 1) * kBlockBytes + (2 * d + t) * 1024);
 #pragma unroll
             for (int x = 0; x < TERMS; ++x) o[d] = Mfma<T>::mul32(v, w[j - 1][t][x], o[d]);
           }
-        if (j < NB) feed_products<kAhead, 2 * DT, TERMS, 32 / (DT * TERMS) + 1>();
+        if (j < NB) feed_products<0, 2 * DT, TERMS, 32 / (DT * TERMS) + 1>();
+        else if (NB == 1) feed_products<0, 2 * DT, TERMS, 0>();
         else feed_products<kAhead, 2 * DT, TERMS, 0>();
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -671,17 +731,17 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
   if (__builtin_expect(*odd, 0)) {
     for (int i = 0; i < nblk; ++i) {
       const int first = (blk0 + i / NB * NB) * kBlockKeys;   // of the tile, as above
-      const int at = page_of(a.c, b, blk0 + i);
+      const int at = block_at(a.c, b, head, blk0 + i);
       if (at < 0) continue;
       bool masked = first < lo_all || first + KB - 1 > hi_all || first + KB > end;
-      for (int j = 0; j < NB; ++j) masked |= i / NB * NB + j >= nblk || page_of(a.c, b, blk0 + i / NB * NB + j) < 0;
+      for (int j = 0; j < NB; ++j) masked |= i / NB * NB + j >= nblk || block_at(a.c, b, head, blk0 + i / NB * NB + j) < 0;
       if (!masked) continue;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         float part[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) part[e] = o[d][e];
-        add_odd<T, D, 16>(a, at, head, blk0 + i, lo, hi,
+        add_odd<T, D, 16>(a, at, (blk0 + i) * kBlockKeys, lo, hi,
                           [&](int e) { return 32 * d + 8 * (e >> 2) + 4 * h + (e & 3); }, part);
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = part[e];
@@ -769,7 +829,7 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
 // How a call is launched, from its sizes alone (max_q and max_kv bound the sequences' new and
 // cached tokens; they choose, they do not limit what is computed).
 struct Plan {
-  int few, many, splits, span, few_splits, few_span, few_tiles;
+  int few, many, whole, splits, span, few_splits, few_span, few_tiles;
   size_t bytes;
 };
 
@@ -782,19 +842,57 @@ void split_keys(int64_t tiles, int kv, int want, int least, int *splits, int *sp
   *splits = (kv + *span - 1) / *span;
 }
 
-// many_rows_kernel: the number of runs with the least estimated time. A workgroup takes `per_key` for
-// a key while its CU holds as many workgroups as fit (2, 3 or 4); fewer share the CU's units less.
-// Joining writes and reads the runs' sums once and costs a launch.
-void split_many(int64_t tiles, int kv, double out_elems, int D, int *splits, int *span) {
-  const double slots = 256.0 * (D == 256 ? 2 : D == 128 ? 3 : 4), per_key = D == 256 ? 0.10 : D == 128 ? 0.08 : 0.07;
-  double best = 0;
-  for (int n = 1; n <= 64 && (n == 1 || kv / n >= 512); ++n) {
-    const int run = (kv + n * kBlockKeys - 1) / (n * kBlockKeys) * kBlockKeys, runs = (kv + run - 1) / run;
-    if (runs != n) continue;
-    const double full = tiles * runs / slots;
-    const double us = run * per_key * (full > 1 ? std::ceil(full) : std::max(0.5, full)) +
-                      (n > 1 ? 5 + runs * out_elems * 8 / 4e6 : 0);
-    if (n == 1 || us < best) best = us, *splits = runs, *span = run;
+// many_rows_kernel's microseconds a key for one of 1, 2, .. workgroups that share a CU (measured over
+// 8192 keys, whole chips of them); as many as its registers let in.
+struct Rates {
+  int most;
+  double key[4];
+};
+const Rates &rates(int D) {
+  static const Rates r64 = {4, {0.0163, 0.0232, 0.0319, 0.0404}}, r128 = {3, {0.0256, 0.0344, 0.0496}},
+                     r256 = {2, {0.0403, 0.0644}};
+  return D == 64 ? r64 : D == 128 ? r128 : r256;
+}
+
+// Microseconds of a CU that gets `whole` tiles of `keys` keys and then `pieces` of `run` keys, as
+// they come to an end.
+double cu_time(const Rates &r, int whole, int keys, int pieces, int run) {
+  double left[4] = {}, t = 0;
+  int held = 0;
+  for (;;) {
+    while (held < r.most && whole + pieces > 0) left[held++] = whole > 0 ? (--whole, keys) : (--pieces, run);
+    if (!held) return t;
+    const double least = *std::min_element(left, left + held);
+    t += least * r.key[held - 1];
+    int kept = 0;
+    for (int i = 0; i < held; ++i)
+      if (left[i] > least) left[kept++] = left[i] - least;
+    held = kept;
+  }
+}
+
+// many_rows_kernel: which tiles are split into how many runs, by the least estimated time of a CU
+// (256 of them). Not all tiles alike: 320 tiles leave a quarter of the CUs with two, so 256 stay
+// whole and the other 64 are split in four; splitting writes and reads the runs' sums once, and
+// joining costs a launch.
+void split_many(int64_t tiles, int kv_heads, int kv, int D, int *whole, int *splits, int *span) {
+  const Rates &r = rates(D);
+  const int64_t per_head = (tiles + kv_heads - 1) / kv_heads;
+  *whole = (int)std::min<int64_t>(per_head, INT32_MAX), *splits = 1, *span = (kv + kBlockKeys - 1) / kBlockKeys * kBlockKeys;
+  if (tiles > 256 * r.most * 3) return;          // the last round is short beside the others
+  double best = cu_time(r, (int)((tiles + 255) / 256), kv, 0, 0);
+  for (int pass = 0; pass < 2; ++pass) {
+    const int64_t keep = pass ? tiles / 256 * 256 / kv_heads : 0, rest = tiles - keep * kv_heads;
+    if ((pass && !keep) || rest <= 0) continue;
+    for (int pieces = 1; pieces <= 12; ++pieces) {   // of a CU; as many runs as make no CU have more
+      const int64_t n = std::min<int64_t>(64, pieces * 256 / rest);
+      if (n < 2) continue;
+      if (kv / n < 256) break;
+      const int run = (int)((kv + n * kBlockKeys - 1) / (n * kBlockKeys) * kBlockKeys), runs = (kv + run - 1) / run;
+      const double us = cu_time(r, (int)((keep * kv_heads + 255) / 256), kv, pieces, run) + 5 +
+                        (double)rest * runs * kManyRows * D * 8 / 4.2e6;
+      if (us < best) best = us, *whole = (int)keep, *splits = runs, *span = run;
+    }
   }
 }
 
@@ -814,8 +912,7 @@ Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv
     split_keys((int64_t)B * (p.many ? 1 : per) * kv_heads, kv, 512, 128, &p.few_splits, &p.few_span);
   }
   if (p.many) {
-    split_many(((int64_t)T * group + kManyRows - 1) / kManyRows * kv_heads, kv, (double)T * heads * D, D, &p.splits,
-               &p.span);
+    split_many(((int64_t)T * group + kManyRows - 1) / kManyRows * kv_heads, kv_heads, kv, D, &p.whole, &p.splits, &p.span);
   }
   const int s = std::max(p.splits, p.few_splits);
   p.bytes = s > 1 ? (size_t)T * heads * ((size_t)s * (D + 2) + 1) * sizeof(float) : 0;
@@ -835,7 +932,8 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
   }
   if (p.many) {
     constexpr int lds = 2 * 2 * kTileKeys<D> * D * 2 + 64;
-    const int64_t grid = (rows / kManyRows + a.c.batch) * a.c.kv_heads * p.splits;
+    const int64_t slots = rows / kManyRows + a.c.batch, whole = std::min<int64_t>(p.whole, slots);
+    const int64_t grid = (whole + (slots - whole) * p.splits) * a.c.kv_heads;
     RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
     static LdsOptIn opt;
     auto fn = many_rows_kernel<T, D, TERMS>;
@@ -890,6 +988,8 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   RLQ_REQUIRE(page_size >= 32 && page_size % 32 == 0, "rlq_attention: page_size=%d is not a multiple of 32", page_size);
   RLQ_REQUIRE(n_pages >= 0 && table_width >= 0 && table_stride >= table_width,
               "rlq_attention: n_pages=%d, table_width=%d, table_stride=%d", n_pages, table_width, table_stride);
+  RLQ_REQUIRE((int64_t)n_pages * kv_heads * (page_size / 32) <= INT32_MAX,
+              "rlq_attention: a cache of %d pages of %d holds more than 2^31 blocks", n_pages, page_size);
   RLQ_REQUIRE((int64_t)table_width * page_size <= kMaxPositions,
               "rlq_attention: a table of %d pages of %d holds more than 2^29 positions", table_width, page_size);
   RLQ_REQUIRE(scale > 0 && scale < __builtin_inff(), "rlq_attention: scale=%g must be positive", scale);
@@ -921,7 +1021,7 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   a.heads = heads, a.group = heads / kv_heads, a.window = window < kMaxPositions ? window : 0, a.out_bf16 = out_dtype == RLQ_BF16;
   a.q_wide = aligned(q, 16) && q_stride % 8 == 0;
   a.out_wide = aligned(out, 8) && out_stride % 4 == 0;
-  a.splits = p.splits, a.span = p.span, a.few_splits = p.few_splits, a.few_span = p.few_span;
+  a.whole = p.splits > 1 ? p.whole : INT32_MAX, a.splits = p.splits, a.span = p.span, a.few_splits = p.few_splits, a.few_span = p.few_span;
   a.few = p.few, a.many = p.many, a.join_few = p.many && p.splits == 1;
   a.unit = softcap > 0 ? 1.0f : scale * kLog2e;
   a.cap_log2 = softcap * kLog2e;

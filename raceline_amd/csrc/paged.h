@@ -35,19 +35,15 @@ __device__ __forceinline__ int value_run(int d, int t, int h) {
   return (d >> 5) * 1024 + t * 512 + h * 256 + (d & 31) * 8;
 }
 
-// First element of a block.
-__device__ __forceinline__ int64_t block_base(const PagedCache &c, int page, int head, int block, int D) {
-  return ((static_cast<int64_t>(page) * c.kv_heads + head) * c.blocks_per_page + block % c.blocks_per_page) *
-         (kBlockKeys * D);
-}
-
-// The page of a sequence's block, or -1: a block past the table's row, or an entry that names no
-// page (its keys are then seen by nobody, and nothing is written there).
-__device__ __forceinline__ int page_of(const PagedCache &c, int seq, int block) {
+// Number of a sequence's block of one head among all blocks of the cache, or -1 where it names no
+// page: a block past the table's row, or an entry outside the cache (nobody sees its keys, and
+// nothing is written there).
+__device__ __forceinline__ int block_at(const PagedCache &c, int seq, int head, int block) {
   const int at = block / c.blocks_per_page;
   if (block < 0 || at >= c.table_width) return -1;
   const int page = c.table[static_cast<int64_t>(seq) * c.table_stride + at];
-  return page >= 0 && page < c.n_pages ? page : -1;
+  if (page < 0 || page >= c.n_pages) return -1;
+  return (page * c.kv_heads + head) * c.blocks_per_page + block - at * c.blocks_per_page;
 }
 
 // First row of a sequence, inside the call's rows whatever the array holds.

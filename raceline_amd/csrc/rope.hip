@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
   const int first = max(p0, block * kBlockKeys), tokens = min(s.kv, (block + 1) * kBlockKeys) - first;
   if (s.b < 0 || tokens <= 0) return;
   const int row = s.row0 + first - p0, lane_key = first - block * kBlockKeys;
-  const int page = page_of(a.c, s.b, block);
+  const int at = block_at(a.c, s.b, head, block);
 
   const int group = a.heads / a.c.kv_heads, half = a.rot >> 1, chunk = tid % kChunks, d0 = chunk * 8;
   const int head0 = blockIdx.z * a.heads_per, heads = min(a.heads_per, group + 1 - head0);
@@ -97,8 +97,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
   }
   __syncthreads();
 
-  T *kb = page < 0 ? nullptr : static_cast<T *>(a.c.k) + block_base(a.c, page, head, block, D);
-  T *vb = page < 0 ? nullptr : static_cast<T *>(a.c.v) + block_base(a.c, page, head, block, D);
+  T *kb = at < 0 ? nullptr : static_cast<T *>(a.c.k) + static_cast<int64_t>(at) * (kBlockKeys * D);
+  T *vb = at < 0 ? nullptr : static_cast<T *>(a.c.v) + static_cast<int64_t>(at) * (kBlockKeys * D);
   for (int i = tid / kChunks; i < tokens * heads; i += kRowStep) {
     const int h = head0 + i / tokens, t = i % tokens;
     const bool is_q = h < group;
@@ -253,6 +253,8 @@ int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, 
               page_size);
   RLQ_REQUIRE(n_pages >= 0 && table_width >= 0 && table_stride >= table_width,
               "rlq_rope_append: n_pages=%d, table_width=%d, table_stride=%d", n_pages, table_width, table_stride);
+  RLQ_REQUIRE((int64_t)n_pages * kv_heads * (page_size / 32) <= INT32_MAX,
+              "rlq_rope_append: a cache of %d pages of %d holds more than 2^31 blocks", n_pages, page_size);
   RLQ_REQUIRE((int64_t)table_width * page_size <= rlq::kMaxPositions,
               "rlq_rope_append: a table of %d pages of %d holds more than 2^29 positions", table_width, page_size);
   RLQ_REQUIRE(T <= (1 << 26) && B <= (1 << 20), "rlq_rope_append: T=%d or B=%d is too large", T, B);
