@@ -138,7 +138,7 @@ __device__ __forceinline__ int runs_of(const AttnArgs &a, const Sequence &s, int
 
 // many_rows_kernel's tile of a rank, longest first: a chip that is given its last long tile late
 // waits for it (six prompts of up to 1537 tokens in the order of the batch, the longest last:
-// 87 us, in this order RANKED us). Tile d of a sequence counts as long as the sequence before the
+// 87 us, in this order 77). Tile d of a sequence counts as long as the sequence before the
 // call's rows and (d + 1) * 128 / group of them; 64 lanes try 64 lengths at a time for the one past
 // which lie as many tiles as the rank says. 64 sequences and more go in the order of the batch, last
 // tile first.
@@ -901,7 +901,10 @@ Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv
   const int group = heads / kv_heads;
   const int64_t rows = (int64_t)max_q * group;
   p.many = rows > kFewRows;
-  p.few = !p.many || (B > 1 && (int64_t)B * max_q > T);
+  // sequences of few rows beside long ones: their own kernel where they may be long in keys; up to
+  // 2048, a tile of them takes no longer than its neighbours, and the launches it saves (the kernel's
+  // and the join's) are 8 us
+  p.few = !p.many || (B > 1 && (int64_t)B * max_q > T && max_kv > 2048);
   p.few_tiles = !p.many && rows <= 16 ? 1 : 2;
   int kv = std::max(1, max_kv);
   if (window && window < kMaxPositions && window < kv) kv = (int)std::min<int64_t>(kv, (int64_t)window + max_q + kBlockKeys);
