@@ -74,12 +74,14 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
   const int head0 = blockIdx.z * a.heads_per, heads = min(a.heads_per, group + 1 - head0);
   const bool with_key = head0 + heads == group + 1;
   T *vals = reinterpret_cast<T *>(turn + kBlockKeys * half);
-  auto row_of = [&](int i) {   // item i: head head0 + i / tokens (group: the key), token i % tokens
-    const int h = head0 + i / tokens, t = i % tokens;
+  // a thread's items: head h (group: the key) of token t, kRowStep tokens on each time
+  auto source = [&](int h, int t) {
     return h < group ? a.q + (row + t) * a.q_stride + (head * group + h) * D : a.k + (row + t) * a.k_stride + head * D;
   };
+  int h = head0 + tid / kChunks / tokens, t = tid / kChunks % tokens;
+  const float *src = source(h, t);
   float next[8] = {};
-  if (tid / kChunks < tokens * heads) load8(row_of(tid / kChunks) + d0, a.wide, next);
+  if (h < head0 + heads) load8(src + d0, a.wide, next);
   for (int i = tid; i < tokens * half; i += kRopeThreads) {
     const int t = i / half, p = i - t * half;
     double x = (first + t) * (a.freq[p] * 0.15915494309189533577);   // turns
@@ -99,14 +101,16 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
 
   T *kb = at < 0 ? nullptr : static_cast<T *>(a.c.k) + static_cast<int64_t>(at) * (kBlockKeys * D);
   T *vb = at < 0 ? nullptr : static_cast<T *>(a.c.v) + static_cast<int64_t>(at) * (kBlockKeys * D);
-  for (int i = tid / kChunks; i < tokens * heads; i += kRowStep) {
-    const int h = head0 + i / tokens, t = i % tokens;
+  while (h < head0 + heads) {
     const bool is_q = h < group;
-    const float *src = row_of(i), *w = is_q ? a.q_norm : a.k_norm;
+    const float *w = is_q ? a.q_norm : a.k_norm, *from = src;
+    const int token = t, q_head = head * group + h;
     float x[8], r = 1.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = next[j];
-    if (i + kRowStep < tokens * heads) load8(row_of(i + kRowStep) + d0, a.wide, next);
+    for (t += kRowStep; t >= tokens; t -= tokens) ++h;
+    src = source(h, t);
+    if (h < head0 + heads) load8(src + d0, a.wide, next);
     if (w) {
       float ss = 0.0f;
 #pragma unroll
@@ -122,7 +126,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           if (d0 + j >= a.rot) break;
-          const float2 cs = turn[t * half + ((d0 + j) >> 1)];
+          const float2 cs = turn[token * half + ((d0 + j) >> 1)];
           const float u = x[j], v = x[j + 1];
           x[j] = u * cs.x - v * cs.y;
           x[j + 1] = u * cs.y + v * cs.x;
@@ -138,20 +142,20 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int d = d0 + j, e = d < half ? d + half : d - half;
-          o[j] = d < a.rot ? src[e] * (w ? r * w[e] : 1.0f) : 0.0f;
+          o[j] = d < a.rot ? from[e] * (w ? r * w[e] : 1.0f) : 0.0f;
         }
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int d = d0 + j;
         if (d >= a.rot) break;
-        const float2 cs = turn[t * half + (d < half ? d : d - half)];
+        const float2 cs = turn[token * half + (d < half ? d : d - half)];
         x[j] = d < half ? x[j] * cs.x - o[j] * cs.y : o[j] * cs.y + x[j] * cs.x;
       }
     }
     const pack8 y = narrow8<T>(x);
     if (is_q) {
-      T *dst = static_cast<T *>(a.q_out) + (row + t) * a.out_stride + (head * group + h) * D + d0;
+      T *dst = static_cast<T *>(a.q_out) + (row + token) * a.out_stride + q_head * D + d0;
       if (a.wide) {
         *reinterpret_cast<pack8 *>(dst) = y;
       } else {
@@ -159,7 +163,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
         for (int j = 0; j < 8; ++j) dst[j] = y[j];
       }
     } else if (kb) {
-      *reinterpret_cast<pack8 *>(kb + key_offset(lane_key + t, d0)) = y;
+      *reinterpret_cast<pack8 *>(kb + key_offset(lane_key + token, d0)) = y;
     }
   }
   if (!vb || !with_key) return;
