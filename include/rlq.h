@@ -380,7 +380,7 @@ int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, 
  *   window > 0. A row that sees no key is zero. Infinities and NaN in keys and values that a
  *   row does not see do not reach it.
  * q 16-bit (dtype, the cache's) [T][q_stride]; out 16-bit (out_dtype) [T][out_stride], as the o
- * linear takes its rows. Products, softmax and sums in fp32; weights are rounded to dtype for
+ * linear takes its rows; with q's type and stride it may take q's place. Products, softmax and sums in fp32; weights are rounded to dtype for
  * the second product, to two terms of it where the cache is RLQ_BF16 and the output RLQ_F16.
  * max_q and max_kv (host) bound the new and all tokens of a sequence: the kernels and the split
  * of the keys over workgroups are chosen from them, and results stay right past them. Both

@@ -833,6 +833,8 @@ struct Plan {
   size_t bytes;
 };
 
+constexpr int64_t kMaxGrid = (int64_t)UINT32_MAX / kThreads;   // a launch counts its threads in 32 bits
+
 // Runs of keys for `tiles` workgroups over up to kv keys: enough workgroups for `want`, none with
 // fewer than `least` keys, and at most 64 runs.
 void split_keys(int64_t tiles, int kv, int want, int least, int *splits, int *span) {
@@ -928,7 +930,7 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
   if (p.few) {
     const int64_t slots = (p.many ? 0 : rows / (16 * p.few_tiles)) + a.c.batch;
     const int64_t grid = slots * a.c.kv_heads * p.few_splits;
-    RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
+    RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     if (p.few_tiles == 1) few_rows_kernel<T, D, 1, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
     else few_rows_kernel<T, D, 2, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
@@ -937,7 +939,7 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
     constexpr int lds = 2 * 2 * kTileKeys<D> * D * 2 + 64;
     const int64_t slots = rows / kManyRows + a.c.batch, whole = std::min<int64_t>(p.whole, slots);
     const int64_t grid = (whole + (slots - whole) * p.splits) * a.c.kv_heads;
-    RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
+    RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     static LdsOptIn opt;
     auto fn = many_rows_kernel<T, D, TERMS>;
     if (int rc = allow_large_lds(reinterpret_cast<const void *>(fn), opt)) return rc;
@@ -947,7 +949,7 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
   if (p.splits > 1 || p.few_splits > 1) {
     const int64_t items = a.join_few ? (int64_t)a.c.batch * a.c.kv_heads * kFewRows : (int64_t)a.c.rows * a.heads;
     const int64_t grid = (items + 3) / 4;
-    RLQ_REQUIRE(grid <= INT32_MAX, "rlq_attention: too many workgroups");
+    RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     join_runs_kernel<D><<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
   }
@@ -1000,6 +1002,8 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   RLQ_REQUIRE(sizes_ok(T, B, heads, kv_heads, D, max_q, max_kv, window),
               "rlq_attention: T=%d, B=%d, heads=%d, max_q=%d, max_kv=%d or window=%d is out of range", T, B, heads, max_q,
               max_kv, window);
+  const float inv_cap = softcap > 0 ? 2.0f * kLog2e * scale / softcap : 0.0f;
+  RLQ_REQUIRE(inv_cap < __builtin_inff(), "rlq_attention: scale=%g over softcap=%g passes fp32", scale, softcap);
   if (T == 0 || B == 0) return 0;
   RLQ_REQUIRE(q && out && cu_q && kv_len, "rlq_attention: null pointer");
   RLQ_REQUIRE((k_cache && v_cache) || n_pages == 0, "rlq_attention: null cache");
@@ -1028,7 +1032,7 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   a.few = p.few, a.many = p.many, a.join_few = p.many && p.splits == 1;
   a.unit = softcap > 0 ? 1.0f : scale * kLog2e;
   a.cap_log2 = softcap * kLog2e;
-  a.inv_cap = softcap > 0 ? 2.0f * kLog2e * scale / softcap : 0.0f;
+  a.inv_cap = inv_cap;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == RLQ_F16) return launch_size<_Float16, 1>(a, p, D, st);
   if (out_dtype == RLQ_BF16) return launch_size<__bf16, 1>(a, p, D, st);

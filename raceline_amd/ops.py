@@ -679,6 +679,8 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_
     if out_code is None:
         raise ValueError(f"out must be float16 or bfloat16, not {out.dtype}")
     H = width // D
+    most = 2**31 - 1                      # past what a position can be: no window, no bound
+    max_q, max_kv, window = min(max_q, most), min(max_kv, 2**29), min(window, most)
     nbytes = attention_workspace_bytes(T, H, kv_heads, D, B, max_q, max_kv, window)
     if workspace is None:
         if nbytes:

@@ -267,3 +267,99 @@ def test_graph_follows_lengths_and_pages(gpu, lens):
         assert torch.equal(out, eager), f"shortened by {shorten}"
         if not shorten:
             check(s, out)
+
+
+@pytest.mark.parametrize("lens", [[(1, 1 + 7 * i % 400) for i in range(100)],
+                                  [(1 + 11 * i % 60, 100 + 11 * i % 60) for i in range(70)],
+                                  [(1 + 11 * i % 60, 100 + 37 * i % 3000) for i in range(70)],
+                                  [(1 + i, 1 + i) for i in range(63)]], ids=["few", "many", "both", "63"])
+def test_many_sequences(gpu, lens):
+    """More sequences than a wave's lanes, and as many as it has."""
+    s = make(gpu, lens, 4, 2, 64, page=32)
+    check(s, run(s, gpu))
+
+
+def test_more_shared_heads_than_a_tile_has_rows(gpu):
+    s = make(gpu, [(3, 40), (2, 90)], 160, 1, 64)
+    check(s, run(s, gpu))
+
+
+def test_sequences_that_share_pages(gpu):
+    """Two sequences with one prompt's pages, and their own after it."""
+    s = make(gpu, [(1, 192), (40, 192)], 4, 2, 128)
+    s.table[1, :2] = s.table[0, :2]
+    for b in (0, 1):
+        s.keys[b][:128], s.values[b][:128] = s.keys[0][:128], s.values[0][:128]
+    check(s, run(s, gpu))
+
+
+def test_no_pages_and_no_table(gpu):
+    from raceline_amd import ops
+
+    s = make(gpu, [(2, 50), (40, 90)], 4, 2, 64)
+    cu, kv, table = s.dev(gpu)
+    for k, v, t in ((s.kc, s.vc, table[:, :0]), (s.kc[:0], s.vc[:0], table), (s.kc[:0], s.vc[:0], table[:, :0])):
+        out = ops.attention(s.dq, k, v, cu, kv, t, s.max_q, s.max_kv)
+        assert (out == 0).all()
+    empty = torch.zeros(1, dtype=torch.int32, device=gpu)
+    out = ops.attention(s.dq[:0], s.kc, s.vc, empty, empty[:0], table[:0], 0, 0)
+    assert out.shape == (0, 256)
+    seven = torch.full_like(s.dq, 7.0)
+    ops.attention(s.dq, s.kc, s.vc, empty, empty[:0], table[:0], 1, 1, out=seven)
+    assert (seven == 7).all()
+
+
+def test_the_rows_may_take_the_queries_place(gpu):
+    for lens in ([(1, 50), (3, 600)], [(70, 300)], [(1, 6000)], [(50, 6000)]):
+        s = make(gpu, lens, 4, 2, 64)
+        q = s.dq.clone()
+        assert run(s, gpu, q=q, out=q) is q
+        check(s, q)
+
+
+def test_two_streams_at_once(gpu):
+    from raceline_amd import ops
+
+    work = [make(gpu, lens, 4, 1, 128, seed=i) for i, lens in enumerate([[(1, 9000)], [(60, 5000)]])]
+    args = [(s.dq, s.kc, s.vc, *s.dev(gpu), s.max_q, s.max_kv) for s in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(ops.attention(*args[i]))
+    torch.cuda.synchronize()
+    for s, os in zip(work, outs):
+        for o in os:
+            check(s, o)
+
+
+def test_two_graphs_at_once(gpu):
+    """Each graph keeps its own scratch."""
+    from raceline_amd import ops
+
+    work = [make(gpu, [(1, 9000 - 500 * i)], 4, 1, 128, seed=i) for i in range(2)]
+    args = [(s.dq, s.kc, s.vc, *s.dev(gpu), s.max_q, s.max_kv) for s in work]
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in work], []
+    for g, a in zip(graphs, args):
+        ops.attention(*a)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            outs.append(ops.attention(*a))
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for s, o in zip(work, outs):
+            check(s, o)
+
+
+def test_windows_past_32_bits_are_none(gpu):
+    s = make(gpu, [(1, 200), (40, 128)], 4, 2, 64)
+    check(s, run(s, gpu, window=2**32 + 5, max_kv=2**40))

@@ -152,3 +152,29 @@ def test_graph_and_stream(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_masks_of_unsigned_words_and_one_row_for_all(gpu):
+    from raceline_amd import ops
+
+    x = torch.randn((3, 100), device=gpu)
+    bits = np.array([0xF0F0F0F0, 1, 0x80000000, 0xF], np.uint32)
+    want = np.where(np.unpackbits(bits.view(np.uint8), bitorder="little")[:100] == 1, x.cpu().numpy(), -np.inf)
+    signed = torch.from_numpy(bits.view(np.int32)).to(gpu)
+    for allowed in (signed, signed[None], signed.view(torch.uint32), signed.repeat(3, 1)):
+        assert np.array_equal(ops.adjust_logits(x, allowed=allowed).cpu().numpy(), want)
+
+
+def test_more_biases_than_threads_share_one_id(gpu):
+    """1024 entries for one token add up in list order, in fp32."""
+    from raceline_amd import ops
+
+    rng = np.random.default_rng(5)
+    b = rng.standard_normal(1024).astype(np.float32)
+    total = np.float32(0)
+    for v in b:
+        total = np.float32(total + v)
+    x = torch.zeros((1, 50), device=gpu)
+    out = ops.adjust_logits(x, bias_ids=torch.full((1, 1024), 7, dtype=torch.int32, device=gpu),
+                            bias=torch.from_numpy(b[None]).to(gpu)).cpu().numpy()
+    assert out[0, 7] == total and (np.delete(out[0], 7) == 0).all()

@@ -152,3 +152,40 @@ def test_graph_follows_lengths(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager) and torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+
+
+def test_no_pages_no_table_and_no_rows(gpu):
+    """Without pages the queries are turned and nothing is stored."""
+    from raceline_amd import ops
+
+    s = Sequences([(2, 50), (40, 90)], 64)
+    cu, kv, table = s.dev(gpu)
+    x = torch.randn((42, 6 * 64), device=gpu)
+    kc, vc = ops.kv_cache(s.n_pages, 1, 64, 64, F16, gpu)
+    freq = ops.rope_frequencies(64, device=gpu)
+    parts = x[:, :256], x[:, 256:320], x[:, 320:]
+    want = ops.rope_append(*parts, kc, vc, cu, kv, table, freq)
+    kc.fill_(3), vc.fill_(5)
+    for k, v, t in ((kc, vc, table[:, :0]), (kc[:0], vc[:0], table)):
+        assert torch.equal(ops.rope_append(*parts, k, v, cu, kv, t, freq), want)
+    assert (kc == 3).all() and (vc == 5).all()
+    empty = torch.zeros(1, dtype=torch.int32, device=gpu)
+    none = [p[:0] for p in parts]
+    assert ops.rope_append(*none, kc, vc, empty, empty[:0], table[:0], freq).shape == (0, 256)
+
+
+@pytest.mark.parametrize("H,KV", [(1, 1), (40, 1), (7, 7)])
+def test_heads(gpu, H, KV):
+    check(gpu, [(1, 33), (40, 40)], H, KV, 64, norm=True)
+
+
+def test_infinities_and_nan_stay_in_their_head(gpu):
+    from raceline_amd import ops
+
+    s = Sequences([(3, 3)], 32)
+    x = torch.randn((3, 4 * 64), device=gpu)
+    x[1, 5], x[2, 64 + 7] = float("inf"), float("nan")
+    kc, vc = ops.kv_cache(s.n_pages, 1, 64, 32, F16, gpu)
+    q = ops.rope_append(x[:, :128], x[:, 128:192], x[:, 192:], kc, vc, *s.dev(gpu), ops.rope_frequencies(32, device=gpu))
+    bad = (~q.isfinite()).cpu().numpy()
+    assert set(zip(*np.nonzero(bad))) == {(1, 5), (1, 21), (2, 64 + 7), (2, 64 + 23)}

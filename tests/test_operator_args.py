@@ -27,6 +27,7 @@ LOGITS = dict(logits=16, stride=1000, rows=2, vocab=1000, tokens=16, token_strid
     (dict(kv_heads=0), "evenly"), (dict(rot=63), "rot=63"), (dict(rot=66), "rot=66"), (dict(rot=-2), "rot=-2"),
     (dict(page_size=48), "page_size=48"), (dict(page_size=0), "page_size=0"), (dict(table_stride=1), "table_stride=1"),
     (dict(table_width=1 << 24, table_stride=1 << 24), "2.29 positions"), (dict(q=None), "null pointer"),
+    (dict(n_pages=1 << 30, page_size=128), "2.31 blocks"),
     (dict(freq=None), "null pointer"), (dict(kv_len=None), "null pointer"), (dict(k_cache=None), "null cache"),
     (dict(table=None), "null table"), (dict(q_stride=255), "stride"), (dict(v_stride=127), "stride"),
     (dict(q_out_stride=0), "stride"), (dict(k_cache=24), "16-byte aligned"), (dict(T=-1), "T=-1"), (dict(B=-1), "B=-1"),
@@ -41,7 +42,8 @@ def test_rope_append_refuses(change, message):
     (dict(heads=3), "evenly"), (dict(page_size=16), "page_size=16"), (dict(table_width=3), "table_width=3"),
     (dict(table_width=1 << 24, table_stride=1 << 24), "2.29 positions"), (dict(scale=0.0), "scale"),
     (dict(scale=-1.0), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"),
-    (dict(softcap=-1.0), "softcap"), (dict(softcap=math.nan), "softcap"), (dict(window=-1), "window=-1"),
+    (dict(softcap=-1.0), "softcap"), (dict(softcap=math.nan), "softcap"), (dict(softcap=1e-40), "passes fp32"),
+    (dict(n_pages=1 << 30, page_size=128), "2.31 blocks"), (dict(window=-1), "window=-1"),
     (dict(max_q=-1), "max_q=-1"), (dict(max_kv=-1), "max_kv=-1"), (dict(T=-4), "T=-4"), (dict(q=None), "null pointer"),
     (dict(out=None), "null pointer"), (dict(v_cache=None), "null cache"), (dict(table=None), "null table"),
     (dict(q_stride=128), "stride"), (dict(out_stride=128), "stride"), (dict(v_cache=8), "16-byte aligned"),
