@@ -6,6 +6,8 @@
  * dispatch kernels/linear.metal and kernels/moe.metal with the POD parameter blocks of
  * kernels/params.h:6-32. Here the same operations are plain C functions over device
  * pointers, so an engine, ctypes (raceline/engine.py:67-125 style) or a test can call them.
+ * At the end: the operators of a decoding step between those products (rotary positions with
+ * the write into a paged cache, attention, adjustments of logits).
  *
  * Conventions
  *  - Every pointer argument is device memory (hipMalloc'd or a torch CUDA tensor), except
