@@ -32,7 +32,6 @@ constexpr float kRefBelow = 7.0f, kRefSlack = 8.0f;
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 struct AttnArgs {
   const void *q;
