@@ -834,13 +834,23 @@ struct Plan {
 
 constexpr int64_t kMaxGrid = (int64_t)UINT32_MAX / kThreads;   // a launch counts its threads in 32 bits
 
-// Runs of keys for `tiles` workgroups over up to kv keys: enough workgroups for `want`, none with
-// fewer than `least` keys, and at most 64 runs.
-void split_keys(int64_t tiles, int kv, int want, int least, int *splits, int *span) {
-  const int64_t n = std::max<int64_t>(1, std::min<int64_t>({64, (want + tiles - 1) / tiles, (kv + least - 1) / least}));
-  const int step = 4 * kBlockKeys;
-  *span = (int)((kv + n * step - 1) / (n * step) * step);
-  *splits = (kv + *span - 1) / *span;
+// few_rows_kernel: how the keys are split into runs (of whole blocks for the four waves, 64 at most).
+// Where the keys and values take 8 us or more at 5.5 TB/s, as many runs as give 512 workgroups, two a
+// CU: fewer leave memory idle and sequences of different lengths uneven (nine sequences' drafts 29.6
+// us with 576 workgroups, 35 with 288). Below that a call is a chain of latencies: a run of 128 keys
+// (a block a wave) takes `first`, each further 128 keys `step`, joining 2.5 us and 0.14 a run, and
+// the least sum is taken. So one token of 1024 keys in heads of 64 is one run (7.7 us, eight runs 7.8),
+// in heads of 256 eight (10.1, one run 15.5), and of 4096 keys 16 (12.4, 32 runs 14.2).
+void split_few(int64_t tiles, int kv, int D, int *splits, int *span) {
+  const double first = D == 256 ? 7.5 : D == 128 ? 5.5 : 4.5, step = D == 256 ? 1.15 : D == 128 ? 0.56 : 0.45;
+  const bool streams = (double)tiles * kv * D * 4 / 5.5e6 >= 8;
+  const int block = 4 * kBlockKeys, most = (int)std::min<int64_t>(64, (511 + tiles) / tiles);
+  double best = 0;
+  for (int n = streams ? most : 1; n <= most; ++n) {
+    const int run = (int)(((int64_t)kv + (int64_t)n * block - 1) / ((int64_t)n * block) * block), runs = (kv + run - 1) / run;
+    const double us = first + step * (run / block - 1) + (runs > 1 ? 2.5 + 0.14 * runs : 0);
+    if (best == 0 || us < best) best = us, *splits = runs, *span = run;
+  }
 }
 
 // many_rows_kernel's microseconds a key for one of 1, 2, .. workgroups that share a CU (measured over
@@ -913,7 +923,7 @@ Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv
   p.span = p.few_span = (kv + 127) / 128 * 128;
   if (p.few) {
     const int64_t per = std::max<int64_t>(1, (rows + 16 * p.few_tiles - 1) / (16 * p.few_tiles));
-    split_keys((int64_t)B * (p.many ? 1 : per) * kv_heads, kv, 512, 128, &p.few_splits, &p.few_span);
+    split_few((int64_t)B * (p.many ? 1 : per) * kv_heads, kv, D, &p.few_splits, &p.few_span);
   }
   if (p.many) {
     split_many(((int64_t)T * group + kManyRows - 1) / kManyRows * kv_heads, kv_heads, kv, D, &p.whole, &p.splits, &p.span);
