@@ -189,3 +189,24 @@ def test_infinities_and_nan_stay_in_their_head(gpu):
     q = ops.rope_append(x[:, :128], x[:, 128:192], x[:, 192:], kc, vc, *s.dev(gpu), ops.rope_frequencies(32, device=gpu))
     bad = (~q.isfinite()).cpu().numpy()
     assert set(zip(*np.nonzero(bad))) == {(1, 5), (1, 21), (2, 64 + 7), (2, 64 + 23)}
+
+
+def test_offsets_past_32_bits(gpu):
+    """The same rows into pages at the end of a cache of 4.6e9 elements (9.2 GB) an array."""
+    from raceline_amd import ops
+
+    s = Sequences([(1, 130), (40, 70)], 64)
+    cu, kv, table = s.dev(gpu)
+    x = torch.randn((41, 12 * 256), device=gpu)
+    parts = x[:, :1024], x[:, 1024:2048], x[:, 2048:]
+    freq = ops.rope_frequencies(64, device=gpu)
+    small = [c.fill_(3) for c in ops.kv_cache(s.n_pages, 4, 256, 64, F16, gpu)]
+    n = 70000
+    large = ops.kv_cache(n, 4, 256, 64, F16, gpu)
+    for c in large:
+        c[n - s.n_pages:] = 3
+    q = ops.rope_append(*parts, *small, cu, kv, table, freq)
+    q2 = ops.rope_append(*parts, *large, cu, kv, table + (n - s.n_pages), freq)
+    assert torch.equal(q, q2)
+    for a, b in zip(small, large):
+        assert torch.equal(a, b[n - s.n_pages:])
