@@ -571,7 +571,8 @@ def _check_paged(k_cache, v_cache, cu_q, kv_len, table):
     if kv_len.shape != (B,) or cu_q.shape != (B + 1,) or not (cu_q.is_contiguous() and kv_len.is_contiguous()):
         raise ValueError("kv_len must be a contiguous vector [B], cu_q [B + 1]")
     rows = table.shape
-    if len(rows) != 2 or rows[0] < B or (rows[1] > 1 and table.stride(1) != 1):
+    if len(rows) != 2 or rows[0] < B or (rows[1] > 1 and table.stride(1) != 1) or (
+            rows[0] > 1 and table.stride(0) < rows[1]):
         raise ValueError("table must be a row-major matrix [B][pages of a sequence]")
     dev = k_cache.get_device()
     if v_cache.get_device() != dev or cu_q.get_device() != dev or kv_len.get_device() != dev or table.get_device() != dev:

@@ -2,6 +2,7 @@
 device work (pointers are placeholders), the Python layer before it calls them. And the rotary
 frequencies, which are formed on the host."""
 
+import contextlib
 import math
 
 import numpy as np
@@ -85,6 +86,14 @@ def paged(B=2, KV=2, D=64, page=64, dtype=torch.float16):
             torch.zeros((B, 2), dtype=torch.int32)]
 
 
+@contextlib.contextmanager
+def refused():
+    """A refusal of the arguments, not of where they are."""
+    with pytest.raises((ValueError, TypeError, lib.RlqError)) as e:
+        yield
+    assert "on the GPU" not in str(e.value)
+
+
 def change(args, at, value):
     args = list(args)
     args[at] = value
@@ -95,11 +104,11 @@ def test_python_layer_refuses_caches_and_sequences():
     q, args = torch.zeros((4, 256), dtype=torch.float16), paged()
     bad = [(0, args[0][:2]), (0, args[0].bfloat16()), (1, args[1].transpose(2, 3)), (0, args[0].float()), (0, args[0][0]),
            (2, args[2].long()), (3, args[3].long()), (4, args[4].long()), (2, args[2][:2]), (3, torch.zeros((2, 1), dtype=torch.int32)),
-           (4, args[4][:1]), (4, args[4][0]), (4, torch.zeros((2, 4), dtype=torch.int32)[:, ::2])]
+           (4, args[4][:1]), (4, args[4][:1].expand(2, 2)), (4, args[4][0]), (4, torch.zeros((2, 4), dtype=torch.int32)[:, ::2])]
     for at, value in bad:
-        with pytest.raises((ValueError, TypeError)):
+        with refused():
             ops.attention(q, *change(args, at, value), max_q=4, max_kv=10)
-        with pytest.raises((ValueError, TypeError)):
+        with refused():
             ops.rope_append(torch.zeros((4, 256)), torch.zeros((4, 128)), torch.zeros((4, 128)),
                             *change(args, at, value), None)
 
@@ -107,11 +116,11 @@ def test_python_layer_refuses_caches_and_sequences():
 def test_python_layer_refuses_rows():
     args = paged()
     q = torch.zeros((4, 256), dtype=torch.float16)
-    for bad in (q.float(), q.bfloat16(), q[:, :200], q[:, :0], q[:, ::2], q[0]):
-        with pytest.raises((ValueError, RuntimeError)):
+    for bad in (q.float(), q.bfloat16(), q[:, :200], q[:, :0], q[:, ::2], q[0], q.t()):
+        with refused():
             ops.attention(bad, *args, max_q=4, max_kv=10)
     for out in (q[:3], torch.zeros((4, 512), dtype=torch.float16)[:, ::2], q.float()):
-        with pytest.raises(ValueError):
+        with refused():
             ops.attention(q, *args, max_q=4, max_kv=10, out=out)
     q, k = torch.zeros((4, 256)), torch.zeros((4, 128))
     freq = torch.zeros(32, dtype=torch.float64)
@@ -120,7 +129,7 @@ def test_python_layer_refuses_rows():
                 dict(freq=freq.float()), dict(freq=torch.zeros(64, dtype=torch.float64)[::2]), dict(q_norm=torch.zeros(63)),
                 dict(k_norm=torch.zeros(64, dtype=torch.float64)), dict(out=torch.zeros((4, 256)))):
         a = {**ok, **bad}
-        with pytest.raises((ValueError, lib.RlqError)):
+        with refused():
             ops.rope_append(a.pop("q"), a.pop("k"), a.pop("v"), *args, a.pop("freq"), **a)
 
 
@@ -132,9 +141,9 @@ def test_python_layer_refuses_logits():
                 dict(bias=torch.zeros((2, 3)), bias_ids=torch.zeros((2, 4), **i)),
                 dict(bias=torch.zeros((2, 3)), bias_ids=torch.zeros((1, 3), **i)), dict(allowed=torch.zeros((2, 3), **i)),
                 dict(allowed=torch.zeros((2, 4))), dict(out=torch.zeros((2, 99))), dict(out=x.double())):
-        with pytest.raises(ValueError):
+        with refused():
             ops.adjust_logits(x, **bad)
-    with pytest.raises(ValueError):
+    with refused():
         ops.adjust_logits(x.half())
 
 
