@@ -224,6 +224,10 @@ __device__ __forceinline__ void add_odd(const AttnArgs &a, int at, int first, in
   }
 }
 
+// What a finished row is multiplied by. A row that found no score above -inf has a sum of 0 and is
+// zero; what it saw being NaN shows in the sum alone (a maximum passes NaN over).
+__device__ __forceinline__ float over_sum(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+
 // Four neighbouring dimensions of a finished row.
 __device__ __forceinline__ void store4(const AttnArgs &a, int row, int col, f32x4 o) {
   if (a.out_bf16) {
@@ -445,7 +449,8 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     }
   }
 
-  // the waves' sums: the largest reference first, then each wave's share scaled to it
+  // the waves' sums: the largest reference first, then each wave's share scaled to it (exp2 of -inf, 0,
+  // where the wave found no score: its sums are 0, or NaN where what it saw was)
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     sum[n] += __shfl_xor(sum[n], 16);
@@ -458,15 +463,12 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
   for (int n = 0; n < NT; ++n) {
     top[n] = -__builtin_inff(), total[n] = 0.0f;
     for (int w2 = 0; w2 < 4; ++w2) top[n] = fmaxf(top[n], stat[w2][n * 16 + r][0]);
-    for (int w2 = 0; w2 < 4; ++w2) {
-      const float m = stat[w2][n * 16 + r][0];
-      total[n] += m == -__builtin_inff() ? 0.0f : stat[w2][n * 16 + r][1] * __builtin_amdgcn_exp2f(m - top[n]);
-    }
-    const float f = ref[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref[n] - top[n]);
+    const float m = top[n] == -__builtin_inff() ? 0.0f : top[n];
+    for (int w2 = 0; w2 < 4; ++w2)
+      total[n] += stat[w2][n * 16 + r][1] * __builtin_amdgcn_exp2f(stat[w2][n * 16 + r][0] - m);
+    const float f = __builtin_amdgcn_exp2f(ref[n] - m);
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][d][i] = ref[n] == -__builtin_inff() ? 0.0f : o[n][d][i] * f;
+    for (int d = 0; d < DT; ++d) o[n][d] *= f;
   }
   // waves 2 and 3 hand theirs to waves 0 and 1, then wave 1 to wave 0
   for (int step = 2; step; step >>= 1) {
@@ -492,14 +494,9 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
   for (int n = 0; n < NT; ++n) {
     if (row[n] < 0) continue;
     if (runs == 1) {
-      const float f = top[n] == -__builtin_inff() ? 0.0f : 1.0f / total[n];
+      const float f = over_sum(total[n]);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        f32x4 y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = top[n] == -__builtin_inff() ? 0.0f : o[n][d][i] * f;
-        store4(a, row[n], col[n] + d * 16 + 4 * g, y);
-      }
+      for (int d = 0; d < DT; ++d) store4(a, row[n], col[n] + d * 16 + 4 * g, o[n][d] * f);
     } else {
       float *p = part_row(a, split, row[n], col[n] / D, D);
 #pragma unroll
@@ -755,7 +752,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
   const float total = sum + __shfl_xor(sum, 32);
   if (row < 0) return;
   if (runs == 1) {
-    const float f = ref == -__builtin_inff() ? 0.0f : 1.0f / total;
+    const float f = over_sum(total);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -777,7 +774,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
 
 // ----------------------------------------------------------------------------- the runs' sums
 
-// One wave: one (token, head) row; adds its runs' sums in the runs' order. How many runs a row has
+// One wave: one (token, head) row; adds its runs' sums, always in the same order. How many runs a row has
 // its first run's workgroup wrote, so that the wave does not look for its sequence again; the
 // statistics of all runs come with one load (at most 64 runs), the sums eight runs at a time.
 template <int D>
@@ -802,8 +799,10 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
   if (row < row_start(a.c, 0) || row >= row_start(a.c, a.c.batch) || runs <= 1) return;
   float top = lane < runs ? stat.x : -__builtin_inff();
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  const float mine = lane < runs && stat.x != -__builtin_inff() ? __builtin_amdgcn_exp2f(stat.x - top) : 0.0f;
-  float total = 0.0f;
+  // a run in which the row found no score counts exp2(-inf) = 0 times its sums: 0, or NaN as they are
+  const float mine = lane < runs ? __builtin_amdgcn_exp2f(stat.x - (top == -__builtin_inff() ? 0.0f : top)) : 0.0f;
+  float total = lane < runs ? stat.y * mine : 0.0f;
+  for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off);
   fvec o = {};
   for (int i0 = 0; i0 < runs; i0 += 8) {
     fvec p[8];
@@ -812,14 +811,12 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
       p[i] = *reinterpret_cast<const fvec *>(part_row(a, min(i0 + i, runs - 1), row, head, D) + lane * PER);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i0 + i >= runs) break;
-      const float f = __shfl(mine, i0 + i);
-      if (f == 0.0f) continue;                     // a run in which the row saw nothing, or next to nothing
-      total += __shfl(stat.y, i0 + i) * f;
-      o += p[i] * f;
+      const fvec add = p[i] * __shfl(mine, i0 + i);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] += i0 + i < runs ? add[e] : 0.0f;
     }
   }
-  const float f = top == -__builtin_inff() ? 0.0f : 1.0f / total;
+  const float f = over_sum(total);
   const int64_t at = row * a.out_stride + head * D + lane * PER;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
