@@ -380,8 +380,8 @@ int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, 
  *   s_j = scale * q . k_j, with softcap > 0: softcap * tanh(s_j / softcap);
  *   out = sum_j softmax(s)_j v_j over the keys j <= position, and j > position - window where
  *   window > 0. A row that sees no key, or none with a score above -inf, is zero; one that sees a
- *   score that is NaN is NaN. Infinities and NaN in keys and values that a row does not see do not
- *   reach it.
+ *   score that is NaN is NaN. An infinite value makes the rows that see it infinite, whatever
+ *   its weight. Infinities and NaN in keys and values that a row does not see do not reach it.
  * q 16-bit (dtype, the cache's) [T][q_stride]; out 16-bit (out_dtype) [T][out_stride], as the o
  * linear takes its rows; with q's type and stride it may take q's place. Products, softmax and sums in fp32; weights are rounded to dtype for
  * the second product, to two terms of it where the cache is RLQ_BF16 and the output RLQ_F16.

@@ -100,10 +100,12 @@ __device__ __forceinline__ void weights(const float (&p)[8], typename Mfma<T>::o
 }
 
 // Infinities and NaN among values that some row does not see would reach it as 0 * inf. In blocks
-// that are masked for some row the product is therefore formed without them (finite8), and those
-// of keys that some row does see are noted and added at the end to the rows that see them
-// (add_odd). `seen`: bit e, whether any row sees the run's key e; what lies behind a sequence's end
-// is never read into a result.
+// that are masked for some row the product is therefore formed without them (finite8), and whether
+// some row does see one is noted. `seen`: bit e, whether any row sees the run's key e; what lies
+// behind a sequence's end is never read into a result. In blocks that every row sees the product is
+// formed with them, and is NaN where a weight, or its second term, rounds to 0 or below. In both
+// cases they are added at the end to the rows that see them (add_odd), whose sums they alone
+// decide: an infinity makes the rows that see it infinite, wherever it lies.
 template <typename T>
 __device__ __forceinline__ u32x4 finite8(u32x4 v, unsigned seen, bool &odd) {
   constexpr unsigned E = Mfma<T>::kExp;
@@ -206,6 +208,12 @@ __device__ __forceinline__ float2 &part_stat(const AttnArgs &a, int split, int r
 
 __device__ __forceinline__ int &run_count(const AttnArgs &a, int row, int head) {
   return a.part_runs[static_cast<int64_t>(row) * a.heads + head];
+}
+
+// What sums over the reference `ref` are multiplied by to join others over m. Never 0, so that an infinity
+// among them stays one; 2^-126 of finite sums is 2^-90 of the others or less.
+__device__ __forceinline__ float share(float ref, float m) {
+  return fmaxf(__builtin_amdgcn_exp2f(ref - m), 0x1p-126f);
 }
 
 // Adds the infinities and NaN among the values of block `at` (its first key `first`) to o (o[i]:
@@ -432,10 +440,26 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
           o[n][d] = Mfma<T>::mul16(__builtin_bit_cast(op, vr[d]), w[n][t], o[n][d]);
   }
 
+  // NaN beside a sum of weights that is not is one that a value made
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    sum[n] += __shfl_xor(sum[n], 16);
+    sum[n] += __shfl_xor(sum[n], 32);
+    const bool plain = row[n] >= 0 && !__builtin_isnan(sum[n]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) odd |= plain && __builtin_isnan(o[n][d][i]);
+  }
   if (__builtin_expect(__any(odd), 0)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][d][i] = __builtin_isnan(o[n][d][i]) && !__builtin_isnan(sum[n]) ? 0.0f : o[n][d][i];
     for (int i = 0; i < mine; ++i) {
       const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
-      if (first >= lo_all && first + kBlockKeys - 1 <= hi_all && first + kBlockKeys <= end) continue;
       const int at = block_at(a.c, b, head, blk);
       if (at < 0) continue;
 #pragma unroll
@@ -443,18 +467,16 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           float part[4] = {o[n][d][0], o[n][d][1], o[n][d][2], o[n][d][3]};
-          add_odd<T, D, 4>(a, at, first, lo[n], hi[n], [&](int j) { return 16 * d + 4 * g + j; }, part);
+          add_odd<T, D, 4>(a, at, first, lo[n], min(hi[n], end - 1), [&](int j) { return 16 * d + 4 * g + j; }, part);
           o[n][d] = f32x4{part[0], part[1], part[2], part[3]};
         }
     }
   }
 
-  // the waves' sums: the largest reference first, then each wave's share scaled to it (exp2 of -inf, 0,
-  // where the wave found no score: its sums are 0, or NaN where what it saw was)
+  // the waves' sums: the largest reference first, then each wave's share scaled to it (where the wave
+  // found no score, its sums are 0, or NaN where what it saw was)
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    sum[n] += __shfl_xor(sum[n], 16);
-    sum[n] += __shfl_xor(sum[n], 32);
     if (g == 0) stat[wave][n * 16 + r][0] = ref[n], stat[wave][n * 16 + r][1] = sum[n];
   }
   __syncthreads();
@@ -465,8 +487,8 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     for (int w2 = 0; w2 < 4; ++w2) top[n] = fmaxf(top[n], stat[w2][n * 16 + r][0]);
     const float m = top[n] == -__builtin_inff() ? 0.0f : top[n];
     for (int w2 = 0; w2 < 4; ++w2)
-      total[n] += stat[w2][n * 16 + r][1] * __builtin_amdgcn_exp2f(stat[w2][n * 16 + r][0] - m);
-    const float f = __builtin_amdgcn_exp2f(ref[n] - m);
+      total[n] += stat[w2][n * 16 + r][1] * share(stat[w2][n * 16 + r][0], m);
+    const float f = share(ref[n], m);
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[n][d] *= f;
   }
@@ -728,28 +750,34 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
     for (int j = 0; j < NB; ++j) page[j] = next[j];
   }
 
+  const float total = sum + __shfl_xor(sum, 32);
   __syncthreads();
-  if (__builtin_expect(*odd, 0)) {
+  bool found = *odd != 0;
+  const bool plain = row >= 0 && !__builtin_isnan(total);   // NaN beside it is one that a value made
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) found |= plain && __builtin_isnan(o[d][i]);
+  if (__builtin_expect(__any(found), 0)) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = plain && __builtin_isnan(o[d][i]) ? 0.0f : o[d][i];
     for (int i = 0; i < nblk; ++i) {
-      const int first = (blk0 + i / NB * NB) * kBlockKeys;   // of the tile, as above
       const int at = block_at(a.c, b, head, blk0 + i);
       if (at < 0) continue;
-      bool masked = first < lo_all || first + KB - 1 > hi_all || first + KB > end;
-      for (int j = 0; j < NB; ++j) masked |= i / NB * NB + j >= nblk || block_at(a.c, b, head, blk0 + i / NB * NB + j) < 0;
-      if (!masked) continue;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         float part[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) part[e] = o[d][e];
-        add_odd<T, D, 16>(a, at, (blk0 + i) * kBlockKeys, lo, hi,
+        add_odd<T, D, 16>(a, at, (blk0 + i) * kBlockKeys, lo, min(hi, end - 1),
                           [&](int e) { return 32 * d + 8 * (e >> 2) + 4 * h + (e & 3); }, part);
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = part[e];
       }
     }
   }
-  const float total = sum + __shfl_xor(sum, 32);
   if (row < 0) return;
   if (runs == 1) {
     const float f = over_sum(total);
@@ -799,8 +827,7 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
   if (row < row_start(a.c, 0) || row >= row_start(a.c, a.c.batch) || runs <= 1) return;
   float top = lane < runs ? stat.x : -__builtin_inff();
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  // a run in which the row found no score counts exp2(-inf) = 0 times its sums: 0, or NaN as they are
-  const float mine = lane < runs ? __builtin_amdgcn_exp2f(stat.x - (top == -__builtin_inff() ? 0.0f : top)) : 0.0f;
+  const float mine = lane < runs ? share(stat.x, top == -__builtin_inff() ? 0.0f : top) : 0.0f;
   float total = lane < runs ? stat.y * mine : 0.0f;
   for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off);
   fvec o = {};

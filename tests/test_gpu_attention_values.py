@@ -88,3 +88,66 @@ def test_a_block_of_nan_keys_reaches_the_rows_that_see_it(gpu, plan):
         assert np.isnan(got[:, hit]).all()
         rest = np.delete(np.arange(4), hit)
         assert (np.abs(got - ref) <= tol)[:, rest].all()
+
+
+TYPES = [(F16, F16), (BF16, F16), (BF16, BF16), (F16, BF16)]
+INF = float("inf")
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=["f16", "bf16-f16", "bf16", "f16-bf16"])
+@pytest.mark.parametrize("plan", PLANS)
+def test_an_infinite_value_is_infinite_in_the_rows_that_see_it(gpu, plan, dtype, out_dtype):
+    """In a block that all rows see, and in the newest, that they see in part; two of them with different
+    signs are NaN."""
+    s = planned(gpu, plan, 64, dtype)
+    n, kv = s.lens[0]
+    put(s, 0, 40, 3, INF)
+    put(s, 0, 41, 4, -INF)
+    put(s, 0, 40, 9, INF)
+    put(s, 0, 45, 9, -INF)
+    put(s, 0, kv - 1, 17, -INF)                              # the last row alone
+    for b, (got, ref, tol) in enumerate(rows_of(s, run(s, gpu, out_dtype=out_dtype), out_dtype)):
+        if b == 0:
+            assert (got[:, :, 3] == INF).all() and (got[:, :, 4] == -INF).all() and np.isnan(got[:, :, 9]).all()
+            assert (got[-1, :, 17] == -INF).all()
+            ok = np.abs(got - ref) <= tol
+            ok[:, :, [3, 4, 9]] = ok[-1, :, 17] = True
+            assert ok.all()
+        else:
+            assert (np.abs(got - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=["f16", "bf16-f16", "bf16", "f16-bf16"])
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("below", [-6, -20])
+def test_an_infinite_value_of_a_small_weight_is_infinite(gpu, plan, below, dtype, out_dtype):
+    """The keys of positions 32 to 63 (one wave's) score 48 or 160 under the others: weights of 2^-69 and
+    2^-230, under what 16 and 32 bits hold and over nothing."""
+    s = planned(gpu, plan, 64, dtype)
+    s.dq.fill_(1.0), s.q.fill(1.0)
+    for pos in range(32, 64):
+        for d in range(64):
+            put(s, 0, pos, d, float(below), keys=True)
+        s.keys[0][pos] = below
+    put(s, 0, 40, 3, INF)
+    for b, (got, ref, tol) in enumerate(rows_of(s, run(s, gpu, out_dtype=out_dtype), out_dtype)):
+        if b == 0:
+            assert (got[:, :, 3] == INF).all()
+            got, ref, tol = (np.delete(x, 3, -1) for x in (got, ref, tol))
+        assert (np.abs(got - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("plan", ["few-split", "many-split"])
+def test_an_infinite_value_of_a_run_of_small_weights_is_infinite(gpu, plan):
+    """As above, with the first 2560 keys, more than a workgroup's run."""
+    s = planned(gpu, plan, 64)
+    s.dq.fill_(1.0), s.q.fill(1.0)
+    for pos in range(0, 2560, s.page):
+        s.kc[int(s.table[0, pos // s.page])] = -20.0
+    s.keys[0][:2560] = -20.0
+    put(s, 0, 40, 3, INF)
+    for b, (got, ref, tol) in enumerate(rows_of(s, run(s, gpu))):
+        if b == 0:
+            assert (got[:, :, 3] == INF).all()
+            got, ref, tol = (np.delete(x, 3, -1) for x in (got, ref, tol))
+        assert (np.abs(got - ref) <= tol).all()
