@@ -383,8 +383,11 @@ int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, 
  *   score that is NaN is NaN. An infinite value makes the rows that see it infinite, whatever
  *   its weight. Infinities and NaN in keys and values that a row does not see do not reach it.
  * q 16-bit (dtype, the cache's) [T][q_stride]; out 16-bit (out_dtype) [T][out_stride], as the o
- * linear takes its rows; with q's type and stride it may take q's place. Products, softmax and sums in fp32; weights are rounded to dtype for
- * the second product, to two terms of it where the cache is RLQ_BF16 and the output RLQ_F16.
+ * linear takes its rows; with q's type and stride it may take q's place. Products, softmax and
+ * sums in fp32. For the second product weights are rounded to two terms of dtype (2^-16 of a
+ * weight for bf16, 2^-21 for fp16) where a sequence has at most 32 rows a key/value head (tokens
+ * times query heads that share it) and where the cache is RLQ_BF16 and the output RLQ_F16; in
+ * other calls to one term.
  * max_q and max_kv (host) bound the new and all tokens of a sequence: the kernels and the split
  * of the keys over workgroups are chosen from them, and results stay right past them. Both
  * given as they are, calls of the same sizes give the same bits.

@@ -87,8 +87,13 @@ __device__ __forceinline__ float max_halves(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Eight weights as a matrix operand. TERMS 2 (bf16 keys, fp16 rows out): the rounding's remainder
-// as a second operand, so that no weight has fewer bits than the rows that leave.
+// Eight weights as a matrix operand. TERMS 2: the rounding's remainder as a second operand, 16 bits
+// of a weight for bf16 and 22 for fp16. few_rows_kernel always has it, since it waits for memory (32
+// sequences of up to 16384 tokens 218 us with one term and with two, off by 2.8e-4 of the rows and by
+// 2.07e-4, which is the rows' own rounding to fp16). many_rows_kernel has it where one term would have
+// fewer bits than the rows that leave (bf16 keys, fp16 rows); elsewhere its rounding is as large as the
+// rows' own (2.9e-4 against 2.07e-4, bf16 2.07e-3 against 1.63e-3), and half of the matrix products more
+// cost 33 to 40% (a 27B layer's chunk 351 us against 468, six capped prompts 84 against 113).
 template <typename T, int TERMS>
 __device__ __forceinline__ void weights(const float (&p)[8], typename Mfma<T>::op (&w)[TERMS]) {
 #pragma unroll
@@ -278,9 +283,9 @@ __device__ __forceinline__ typename Mfma<T>::op load_q(const AttnArgs &a, int ro
 // 16 (r / 8) + r % 8 (then + 8), so that a lane's eight weights belong to one 16-byte run of V.
 // Bound by the stream of keys and values, read past the caches: 32 sequences of up to 16384 tokens, 4
 // heads of 256, 1.21 GB in 212 us, 5.7 TB/s (229 us through the L2; a plain read gets 6.9 TB/s).
-template <typename T, int D, int NT, int TERMS>
+template <typename T, int D, int NT>
 __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kernel(AttnArgs a) {
-  constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * NT;
+  constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * NT, TERMS = 2;
   typedef typename Mfma<T>::op op;
   __shared__ float stat[4][ROWS][2];
   __shared__ float sums[2][ROWS][D + 4];
@@ -968,8 +973,8 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
     const int64_t slots = (p.many ? 0 : rows / (16 * p.few_tiles)) + a.c.batch;
     const int64_t grid = slots * a.c.kv_heads * p.few_splits;
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
-    if (p.few_tiles == 1) few_rows_kernel<T, D, 1, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
-    else few_rows_kernel<T, D, 2, TERMS><<<(unsigned)grid, kThreads, 0, st>>>(a);
+    if (p.few_tiles == 1) few_rows_kernel<T, D, 1><<<(unsigned)grid, kThreads, 0, st>>>(a);
+    else few_rows_kernel<T, D, 2><<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
   }
   if (p.many) {

@@ -151,3 +151,28 @@ def test_an_infinite_value_of_a_run_of_small_weights_is_infinite(gpu, plan):
             assert (got[:, :, 3] == INF).all()
             got, ref, tol = (np.delete(x, 3, -1) for x in (got, ref, tol))
         assert (np.abs(got - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=["f16", "bf16-f16", "bf16", "f16-bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 1), (1, 700), (1, 65)], [(5, 333), (8, 900)], [(2, 6000)]],
+                         ids=["tokens", "drafts", "split"])
+def test_weights_of_few_rows_keep_more_bits_than_the_rows(gpu, lens, D, dtype, out_dtype):
+    """Queries with one dimension, so that a score is one product, exact in fp32 but for two roundings of
+    2^-24 of at most 16 (base 2): 2^-19; exp2 2^-22; weights of two terms 2^-16 (bf16) or 2^-21 (fp16); the sum
+    over at most 6000 keys, whose partial sums of 4 x 4 x 32 keys and runs are short, 2^-17. The rows are off by half
+    a step of their own, by its size there, and those."""
+    s = make(gpu, lens, 4, 2, D, dtype=dtype)
+    keep = np.arange(s.T * 4).reshape(s.T, 4, 1) * 7 % D == np.arange(D)
+    s.q = np.where(keep, np.clip(s.q, -3, 3), 0.0)
+    s.dq = torch.from_numpy(s.q.reshape(s.T, 4 * D)).to(dtype).to(gpu)
+    s.q = s.dq.double().cpu().numpy().reshape(s.T, 4, D)
+    out = run(s, gpu, scale=0.5, out_dtype=out_dtype).double().cpu().numpy().reshape(s.T, 4, D)
+    bits = 10 if out_dtype == F16 else 7
+    for b, (n, kv) in enumerate(lens):
+        r = slice(s.cu[b], s.cu[b] + n)
+        ref, size = attend(s.q[r], s.keys[b], s.values[b], kv, 0.5)
+        off = (2.0 ** -16 if dtype == BF16 else 2.0 ** -21) + 2.0 ** -18 + 2.0 ** -22 + 2.0 ** -17
+        _, e = np.frexp(np.abs(ref) + off * size)
+        half_step = 2.0 ** np.maximum(e - 2 - bits, -25 if out_dtype == F16 else -134)
+        assert (np.abs(out[r] - ref) <= half_step + off * size).all(), np.max((np.abs(out[r] - ref) - half_step) / size)
