@@ -46,7 +46,10 @@ struct AttnArgs {
   int few_splits, few_span;   // the same for sequences of few rows, all of them
   int few, many;              // which kernels this call launches
   int join_few;               // join_runs_kernel: only sequences of few rows have more than one run
-  float unit, cap_log2, inv_cap;   // unit: base-2 units of a score as the product gives it, or of a capped one (1)
+  float unit;                 // base-2 units of a score as the product gives it, or of a capped one (1)
+  float cap_log2;             // the cap in base-2 units, 0 for none
+  float over_cap, exp_cap;    // score / cap, and the same in the power of tanh's exponential
+  float near_cap[6];          // a capped score in base-2 units over the score, in powers of (score / cap)^2
 };
 
 template <typename T>
@@ -74,11 +77,49 @@ struct Mfma<__bf16> {
   static constexpr unsigned kExp = 0x7F80u;
 };
 
-// A capped score in base-2 units. tanh y = 1 - 2 / (1 + e^2y) has an error of about 2^-23 absolute,
-// times cap: far under what the weight's 16 bits keep.
-__device__ __forceinline__ float capped(const AttnArgs &a, float s) {
-  const float e = __builtin_amdgcn_exp2f(s * a.inv_cap);
+// Capped scores in base-2 units, cap tanh(y) with y = score / cap. 1 - 2 / (1 + e^2y) is off by 2^-21.5
+// times the cap wherever y lies, so that a cap of 10^4 would cost the weights of small scores their
+// bits and one of 10^7 all of them. It serves for caps up to 88 (128 in base 2), where that is 2^-15 of a
+// weight, an eighth of what an fp16 row is rounded by. Under larger ones tanh(y) / y is a polynomial
+// in y^2 up to |y| = 0.6 (fitted to the least relative error, 2^-24.4), so that a score is off by its
+// own roundings; past 0.6 the form above is off by 2^-20.6 of what it gives, and a wave with no
+// such score skips it. The polynomial alone would take longer (six prompts capped at 30: 89 to 92 us against
+// 85): two exponential-class operations cost less than its eight others.
+constexpr float kFarCap = 0.6f, kSmallCap = 128.0f;   // of a score over the cap, of a cap in base 2
+
+__device__ __forceinline__ float far_capped(const AttnArgs &a, float s) {
+  const float e = __builtin_amdgcn_exp2f(s * a.exp_cap);
   return a.cap_log2 - 2.0f * a.cap_log2 * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+__device__ __forceinline__ float near_capped(const AttnArgs &a, float s, float y) {
+  const float z = y * y;
+  float r = a.near_cap[5];
+#pragma unroll
+  for (int i = 4; i >= 0; --i) r = __builtin_fmaf(r, z, a.near_cap[i]);
+  return s * r;
+}
+
+template <int N, typename Scores>
+__device__ __forceinline__ void cap_scores(const AttnArgs &a, Scores &x) {
+  if (a.cap_log2 <= kSmallCap) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = far_capped(a, x[i]);
+    return;
+  }
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(x[i]));
+  if (__any(most * a.over_cap > kFarCap)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = x[i] * a.over_cap;
+      x[i] = fabsf(y) <= kFarCap ? near_capped(a, x[i], y) : far_capped(a, x[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = near_capped(a, x[i], x[i] * a.over_cap);
+  }
 }
 
 __device__ __forceinline__ float max_halves(float x) {
@@ -394,10 +435,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       float x[8], top = -__builtin_inff();
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = sc[n][e >> 2][e & 3];
-      if (a.cap_log2 != 0.0f) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = capped(a, x[e]);
-      }
+      if (a.cap_log2 != 0.0f) cap_scores<8>(a, x);
       if (masked) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -570,8 +608,12 @@ constexpr int kAhead = 4;
 template <int D>
 constexpr int kTileKeys = D >= 128 ? 32 : 64;
 
+// Workgroups of many_rows_kernel that a CU holds, by its registers.
+template <int D, int TERMS>
+constexpr int kManyHeld = D == 64 ? (TERMS == 1 ? 4 : 3) : D == 128 && TERMS == 1 ? 3 : 2;
+
 template <typename T, int D, int TERMS>
-__global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_kernel(AttnArgs a) {
   constexpr int KB = kTileKeys<D>, NB = KB / kBlockKeys, KS = D / 16, DT = D / 32, ROWS = kManyRows;
   constexpr int kBlockBytes = kBlockKeys * D * 2, kStage = 2 * NB * kBlockBytes, kPieces = kBlockBytes / 1024;
   typedef typename Mfma<T>::op op;
@@ -687,9 +729,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_rows_kernel(AttnArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     if (a.cap_log2 != 0.0f) {
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[j][i] = capped(a, sc[j][i]);
+      for (int j = 0; j < NB; ++j) cap_scores<16>(a, sc[j]);
     }
     if (masked) {
 #pragma unroll
@@ -1044,8 +1084,8 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   RLQ_REQUIRE(sizes_ok(T, B, heads, kv_heads, D, max_q, max_kv, window),
               "rlq_attention: T=%d, B=%d, heads=%d, max_q=%d, max_kv=%d or window=%d is out of range", T, B, heads, max_q,
               max_kv, window);
-  const float inv_cap = softcap > 0 ? 2.0f * kLog2e * scale / softcap : 0.0f;
-  RLQ_REQUIRE(inv_cap < __builtin_inff(), "rlq_attention: scale=%g over softcap=%g passes fp32", scale, softcap);
+  const float exp_cap = softcap > 0 ? 2.0f * kLog2e * scale / softcap : 0.0f;
+  RLQ_REQUIRE(exp_cap < __builtin_inff(), "rlq_attention: scale=%g over softcap=%g passes fp32", scale, softcap);
   if (T == 0 || B == 0) return 0;
   RLQ_REQUIRE(q && out && cu_q && kv_len, "rlq_attention: null pointer");
   RLQ_REQUIRE((k_cache && v_cache) || n_pages == 0, "rlq_attention: null cache");
@@ -1073,8 +1113,12 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   a.whole = p.splits > 1 ? p.whole : INT32_MAX, a.splits = p.splits, a.span = p.span, a.few_splits = p.few_splits, a.few_span = p.few_span;
   a.few = p.few, a.many = p.many, a.join_few = p.many && p.splits == 1;
   a.unit = softcap > 0 ? 1.0f : scale * kLog2e;
-  a.cap_log2 = softcap * kLog2e;
-  a.inv_cap = inv_cap;
+  if (softcap > 0) {
+    constexpr float tanh_over_y[6] = {1.0f, -0.33333284f, 0.13331689f, -0.053768702f, 0.020753626f, -0.0058521652f};
+    a.cap_log2 = std::min(softcap, 1e38f) * kLog2e;   // twice that is finite
+    a.over_cap = scale / softcap, a.exp_cap = exp_cap;
+    for (int i = 0; i < 6; ++i) a.near_cap[i] = tanh_over_y[i] * (scale * kLog2e);
+  }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == RLQ_F16) return launch_size<_Float16, 1>(a, p, D, st);
   if (out_dtype == RLQ_BF16) return launch_size<__bf16, 1>(a, p, D, st);

@@ -176,3 +176,31 @@ def test_weights_of_few_rows_keep_more_bits_than_the_rows(gpu, lens, D, dtype, o
         _, e = np.frexp(np.abs(ref) + off * size)
         half_step = 2.0 ** np.maximum(e - 2 - bits, -25 if out_dtype == F16 else -134)
         assert (np.abs(out[r] - ref) <= half_step + off * size).all(), np.max((np.abs(out[r] - ref) - half_step) / size)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("n,q_scale", [(2, 1.5), (60, 1.5), (2, 12.0), (60, 12.0)], ids=["few", "many", "few-wide", "many-wide"])
+@pytest.mark.parametrize("cap", [0.25, 2.0, 12.0, 30.0, 88.0, 89.0, 1e3, 1e4, 1e5, 1e6, 1e8, 1e12, 1e30, 1e38, 3.4e38])
+def test_a_cap_of_any_size_keeps_the_weights(gpu, cap, n, q_scale, dtype):
+    """Queries with one dimension and one-hot values: a score is one product, exact in fp32, and the rows are the
+    weights themselves. A score is off by three roundings of 2^-24, the polynomial's 2^-24.4 and its
+    evaluation's 2^-22 of itself, or 2^-20.6 where the other form gives it: 2^-20 of the largest capped score, or,
+    for caps up to 88.8 (128 in base 2), by 2^-21.5 of 88.8: 2^-15. That is what a weight is off by,
+    and so is their sum; a weight's 16 bits, the row's, 64 additions and exp2 come on top. Weights are held
+    as fp16 with the largest at 2^7 or more, those under 2^-14 in steps of 2^-24: half of one is 2^-32 of the row."""
+    D = kv = 64
+    s = make(gpu, [(n, kv)], 4, 2, D, dtype=dtype, q_scale=q_scale)
+    keep = np.arange(n * 4).reshape(n, 4, 1) * 7 % D == np.arange(D)
+    s.q = np.where(keep, s.q, 0.0)
+    s.dq = torch.from_numpy(s.q.reshape(n, 4 * D)).to(dtype).to(gpu)
+    s.values[0] = np.repeat(np.eye(kv)[:, None], 2, 1)
+    page = torch.from_numpy(pack_values(np.repeat(np.eye(kv)[None, None], 2, 1))).to(gpu).to(dtype)
+    s.vc[int(s.table[0, 0])] = page[0]
+    got = run(s, gpu, scale=0.5, softcap=cap).double().cpu().numpy().reshape(n, 4, D)
+    ref, _ = attend(s.q, s.keys[0], s.values[0], kv, 0.5, 0, cap)
+    score = np.einsum("nhd,khd->nhk", s.q, np.repeat(s.keys[0].astype(np.float64), 2, 1)) * 0.5
+    most = np.abs(cap * np.tanh(score / cap)).max()
+    off = 2 * (2.0 ** -15 + 2.0 ** -20 * most + 2.0 ** -22) + 2.0 ** -18
+    weight = 2.0 ** -16 if dtype == BF16 else 2.0 ** -11     # two terms where rows leave with more bits
+    assert (np.abs(got - ref) <= (off + weight + 2.0 ** -11) * ref + 2.0 ** -25 + 2.0 ** -32).all(), \
+        np.nanmax(np.abs(got - ref) / (ref + 2.0 ** -14))
