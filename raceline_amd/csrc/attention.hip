@@ -102,11 +102,12 @@ __device__ __forceinline__ float near_capped(const AttnArgs &a, float s, float y
 
 template <int N, typename Scores>
 __device__ __forceinline__ void cap_scores(const AttnArgs &a, Scores &x) {
-  if (a.cap_log2 <= kSmallCap) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = far_capped(a, x[i]);
-    return;
-  }
+  for (int i = 0; i < N; ++i) x[i] = far_capped(a, x[i]);
+}
+
+template <int N, typename Scores>
+__device__ __forceinline__ void large_cap_scores(const AttnArgs &a, Scores &x) {
   float most = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(x[i]));
@@ -435,7 +436,8 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       float x[8], top = -__builtin_inff();
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = sc[n][e >> 2][e & 3];
-      if (a.cap_log2 != 0.0f) cap_scores<8>(a, x);
+      if (a.cap_log2 > kSmallCap) large_cap_scores<8>(a, x);
+      else if (a.cap_log2 != 0.0f) cap_scores<8>(a, x);
       if (masked) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -612,7 +614,8 @@ constexpr int kTileKeys = D >= 128 ? 32 : 64;
 template <int D, int TERMS>
 constexpr int kManyHeld = D == 64 ? (TERMS == 1 ? 4 : 3) : D == 128 && TERMS == 1 ? 3 : 2;
 
-template <typename T, int D, int TERMS>
+// LARGE_CAP: a cap over kSmallCap, whose code would cost the other calls 1 to 3%.
+template <typename T, int D, int TERMS, bool LARGE_CAP>
 __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_kernel(AttnArgs a) {
   constexpr int KB = kTileKeys<D>, NB = KB / kBlockKeys, KS = D / 16, DT = D / 32, ROWS = kManyRows;
   constexpr int kBlockBytes = kBlockKeys * D * 2, kStage = 2 * NB * kBlockBytes, kPieces = kBlockBytes / 1024;
@@ -727,7 +730,10 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
       }
     feed_products<kAhead, NB * KS, 1, 0>();
     __builtin_amdgcn_sched_barrier(0);
-    if (a.cap_log2 != 0.0f) {
+    if constexpr (LARGE_CAP) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) large_cap_scores<16>(a, sc[j]);
+    } else if (a.cap_log2 != 0.0f) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) cap_scores<16>(a, sc[j]);
     }
@@ -1022,9 +1028,10 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
     const int64_t slots = rows / kManyRows + a.c.batch, whole = std::min<int64_t>(p.whole, slots);
     const int64_t grid = (whole + (slots - whole) * p.splits) * a.c.kv_heads;
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
-    static LdsOptIn opt;
-    auto fn = many_rows_kernel<T, D, TERMS>;
-    if (int rc = allow_large_lds(reinterpret_cast<const void *>(fn), opt)) return rc;
+    static LdsOptIn opt[2];
+    const bool large = a.cap_log2 > kSmallCap;
+    auto fn = large ? many_rows_kernel<T, D, TERMS, true> : many_rows_kernel<T, D, TERMS, false>;
+    if (int rc = allow_large_lds(reinterpret_cast<const void *>(fn), opt[large])) return rc;
     fn<<<(unsigned)grid, kThreads, lds, st>>>(a);
     RLQ_HIP(hipGetLastError());
   }
