@@ -25,10 +25,12 @@ constexpr int kManyRows = 128;    // rows of a many_rows_kernel tile
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Weights are exp2(x - ref) with x the score in base-2 units. ref follows the largest score
-// seen, kRefBelow under it, and moves only when a score passes ref + kRefBelow + kRefSlack: most
-// steps then leave the accumulators alone. A weight is at most 2^15, inside fp16, and 2^-14, where
-// fp16 loses bits, lies 2^21 under the largest: what is lost there does not show in the sum.
-constexpr float kRefBelow = 7.0f, kRefSlack = 8.0f;
+// seen, kBelow under it, and moves only when a score passes ref + kBelow + kRefSlack: most
+// steps then leave the accumulators alone. For fp16 (kBelow 7) a weight is at most 2^15, inside fp16, and
+// 2^-14, where fp16 loses bits, lies 2^21 under the largest: what is lost there does not show in the sum.
+// bf16 has no such bound but values up to 2^128: a weight is at most 1 (kBelow -8), so that its
+// product with one stays in range.
+constexpr float kRefSlack = 8.0f;
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -64,6 +66,7 @@ struct Mfma<_Float16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
   static constexpr unsigned kExp = 0x7C00u;
+  static constexpr float kBelow = 7.0f;
 };
 template <>
 struct Mfma<__bf16> {
@@ -75,6 +78,7 @@ struct Mfma<__bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static constexpr unsigned kExp = 0x7F80u;
+  static constexpr float kBelow = -8.0f;
 };
 
 // Capped scores in base-2 units, cap tanh(y) with y = score / cap. 1 - 2 / (1 + e^2y) is off by 2^-21.5
@@ -257,10 +261,10 @@ __device__ __forceinline__ int &run_count(const AttnArgs &a, int row, int head) 
   return a.part_runs[static_cast<int64_t>(row) * a.heads + head];
 }
 
-// What sums over the reference `ref` are multiplied by to join others over m. Never 0, so that an infinity
-// among them stays one; 2^-126 of finite sums is 2^-90 of the others or less.
-__device__ __forceinline__ float share(float ref, float m) {
-  return fmaxf(__builtin_amdgcn_exp2f(ref - m), 0x1p-126f);
+// A sum x over one reference, times the factor f to another's. An infinity stays one where f is 0.
+__device__ __forceinline__ float scaled(float x, float f) {
+  const float y = x * f;
+  return __builtin_isnan(y) ? x : y;
 }
 
 // Adds the infinities and NaN among the values of block `at` (its first key `first`) to o (o[i]:
@@ -449,8 +453,8 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = max_halves(top) * a.unit;
-      if (__any(top > ref[n] + (kRefBelow + kRefSlack))) {
-        const float to = top > ref[n] + (kRefBelow + kRefSlack) ? top - kRefBelow : ref[n];
+      if (__any(top > ref[n] + (Mfma<T>::kBelow + kRefSlack))) {
+        const float to = top > ref[n] + (Mfma<T>::kBelow + kRefSlack) ? top - Mfma<T>::kBelow : ref[n];
         const float f = ref[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref[n] - to);
         ref[n] = to;
         sum[n] *= f;
@@ -532,10 +536,12 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     for (int w2 = 0; w2 < 4; ++w2) top[n] = fmaxf(top[n], stat[w2][n * 16 + r][0]);
     const float m = top[n] == -__builtin_inff() ? 0.0f : top[n];
     for (int w2 = 0; w2 < 4; ++w2)
-      total[n] += stat[w2][n * 16 + r][1] * share(stat[w2][n * 16 + r][0], m);
-    const float f = share(ref[n], m);
+      total[n] += stat[w2][n * 16 + r][1] * __builtin_amdgcn_exp2f(stat[w2][n * 16 + r][0] - m);
+    const float f = __builtin_amdgcn_exp2f(ref[n] - m);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[n][d] *= f;
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][d][i] = scaled(o[n][d][i], f);
   }
   // waves 2 and 3 hand theirs to waves 0 and 1, then wave 1 to wave 0
   for (int step = 2; step; step >>= 1) {
@@ -756,8 +762,8 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[j][i]);
     top = max_halves(top) * a.unit;
-    if (__any(top > ref + (kRefBelow + kRefSlack))) {
-      const float to = top > ref + (kRefBelow + kRefSlack) ? top - kRefBelow : ref;
+    if (__any(top > ref + (Mfma<T>::kBelow + kRefSlack))) {
+      const float to = top > ref + (Mfma<T>::kBelow + kRefSlack) ? top - Mfma<T>::kBelow : ref;
       const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - to);
       ref = to;
       sum *= f;
@@ -878,7 +884,7 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
   if (row < row_start(a.c, 0) || row >= row_start(a.c, a.c.batch) || runs <= 1) return;
   float top = lane < runs ? stat.x : -__builtin_inff();
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  const float mine = lane < runs ? share(stat.x, top == -__builtin_inff() ? 0.0f : top) : 0.0f;
+  const float mine = lane < runs ? __builtin_amdgcn_exp2f(stat.x - (top == -__builtin_inff() ? 0.0f : top)) : 0.0f;
   float total = lane < runs ? stat.y * mine : 0.0f;
   for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off);
   fvec o = {};
@@ -889,9 +895,9 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
       p[i] = *reinterpret_cast<const fvec *>(part_row(a, min(i0 + i, runs - 1), row, head, D) + lane * PER);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const fvec add = p[i] * __shfl(mine, i0 + i);
+      const float f = __shfl(mine, i0 + i);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) o[e] += i0 + i < runs ? add[e] : 0.0f;
+      for (int e = 0; e < PER; ++e) o[e] += i0 + i < runs ? scaled(p[i][e], f) : 0.0f;
     }
   }
   const float f = over_sum(total);

@@ -204,3 +204,43 @@ def test_a_cap_of_any_size_keeps_the_weights(gpu, cap, n, q_scale, dtype):
     weight = 2.0 ** -16 if dtype == BF16 else 2.0 ** -11     # two terms where rows leave with more bits
     assert (np.abs(got - ref) <= (off + weight + 2.0 ** -11) * ref + 2.0 ** -25 + 2.0 ** -32).all(), \
         np.nanmax(np.abs(got - ref) / (ref + 2.0 ** -14))
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("lens", [[(1, 1), (3, 40)], [(2, 6000)], [(70, 90), (1, 1)], [(60, 5000)]],
+                         ids=["few", "few-split", "many", "many-split"])
+def test_values_near_the_largest_of_bf16(gpu, lens, D):
+    """Values of up to 4.5 2^118, the rows' among them; and one key whose value is the largest there is."""
+    s = make(gpu, lens, 4, 2, D, dtype=BF16)
+    s.vc *= 2.0 ** 118
+    s.values = [v.astype(np.float64) * 2.0 ** 118 for v in s.values]
+    for got, ref, tol in rows_of(s, run(s, gpu, out_dtype=BF16), BF16):
+        assert (np.abs(got - ref) <= tol).all()
+    s = make(gpu, [(n, n) for n, _ in lens], 4, 2, D, dtype=BF16)
+    most = float(torch.finfo(BF16).max)
+    for b, (n, _) in enumerate(s.lens):
+        put(s, b, 0, 3, most)
+        s.values[b][0, :, 3] = most
+    out = run(s, gpu, out_dtype=BF16)
+    for got, ref, tol in rows_of(s, out, BF16):
+        assert (np.abs(got - ref) <= tol).all()
+        assert (got[0, :, 3] == most).all()                  # the row that sees it alone
+
+
+def test_large_values_of_no_weight_add_nothing(gpu):
+    """Keys that score 160 under the others (2^-230) hold values of 2^120, in one wave's block and in a run."""
+    for lens, upto in (([(1, 100)], 32), ([(2, 6000)], 2560)):
+        s = make(gpu, lens, 4, 2, 64, dtype=BF16)
+        s.dq.fill_(1.0), s.q.fill(1.0)
+        for pos in range(upto):
+            s.keys[0][pos] = -20.0
+        for at in range(-(-upto // 64)):
+            page, n = int(s.table[0, at]), min(64, upto - at * 64)
+            mark = np.zeros((1, 1, 64, 64), np.float32)
+            mark[0, 0, :n] = 1
+            for c, pack, x in ((s.kc, pack_keys, -20.0), (s.vc, pack_values, 2.0 ** 120)):
+                c[page][:, torch.from_numpy(pack(mark)).to(gpu)[0, 0].bool()] = x
+        # the sums of such values times 2^-230 are 2^-110
+        s.values[0][:upto] = 0.0
+        for got, ref, tol in rows_of(s, run(s, gpu, out_dtype=BF16), BF16):
+            assert (np.abs(got - ref) <= tol).all()
