@@ -602,11 +602,18 @@ def _call_on(dev: int, stream, name: str, *args):
     return lib.call(name, *args, _raw_stream(dev) if stream is None else stream.cuda_stream)
 
 
-def _new(like, shape, dtype, stream) -> torch.Tensor:
-    """An output or scratch tensor that the caching allocator keeps until `stream` is through."""
-    t = torch.empty(shape, dtype=dtype, device=like.device)
-    if stream is not None and t.is_cuda:
-        t.record_stream(stream)
+def _new(like, shape, dtype, stream, scratch=False) -> torch.Tensor:
+    """An output or scratch tensor of a call on `stream`. Its memory is that stream's own: what the
+    current stream's pool gives may still be written by work queued there before it was freed, and
+    nothing makes `stream` wait for that. An output is kept until the current stream, where the
+    caller goes on with it, is through."""
+    if stream is None or not like.is_cuda:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    current = torch.cuda.current_stream(like.device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=like.device)
+    if not scratch and current != stream:
+        t.record_stream(current)
     return t
 
 
@@ -685,7 +692,7 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_
     nbytes = attention_workspace_bytes(T, H, kv_heads, D, B, max_q, max_kv, window)
     if workspace is None:
         if nbytes:
-            workspace = _new(q, nbytes, torch.uint8, stream)
+            workspace = _new(q, nbytes, torch.uint8, stream, scratch=True)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("the workspace must be contiguous, on the cache's device")
     else:
