@@ -489,37 +489,28 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
           o[n][d] = Mfma<T>::mul16(__builtin_bit_cast(op, vr[d]), w[n][t], o[n][d]);
   }
 
-  // NaN beside a sum of weights that is not is one that a value made
+  // Sums that are not finite beside a sum of weights that is: values made them so, and are added once
+  // the waves' shares are scaled.
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     sum[n] += __shfl_xor(sum[n], 16);
     sum[n] += __shfl_xor(sum[n], 32);
-    const bool plain = row[n] >= 0 && !__builtin_isnan(sum[n]);
+    float t[2] = {};
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) odd |= plain && __builtin_isnan(o[n][d][i]);
+      for (int i = 0; i < 4; ++i) t[i & 1] = __builtin_fmaf(o[n][d][i], 0.0f, t[i & 1]);
+    odd |= row[n] >= 0 && !__builtin_isnan(sum[n]) && __builtin_isnan(t[0] + t[1]);
   }
-  if (__builtin_expect(__any(odd), 0)) {
+  const bool any_odd = __any(odd);
+  if (__builtin_expect(any_odd, 0)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][d][i] = __builtin_isnan(o[n][d][i]) && !__builtin_isnan(sum[n]) ? 0.0f : o[n][d][i];
-    for (int i = 0; i < mine; ++i) {
-      const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
-      const int at = block_at(a.c, b, head, blk);
-      if (at < 0) continue;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          float part[4] = {o[n][d][0], o[n][d][1], o[n][d][2], o[n][d][3]};
-          add_odd<T, D, 4>(a, at, first, lo[n], min(hi[n], end - 1), [&](int j) { return 16 * d + 4 * g + j; }, part);
-          o[n][d] = f32x4{part[0], part[1], part[2], part[3]};
-        }
-    }
+        for (int i = 0; i < 4; ++i)
+          o[n][d][i] = !__builtin_isnan(sum[n]) && !__builtin_isfinite(o[n][d][i]) ? 0.0f : o[n][d][i];
   }
 
   // the waves' sums: the largest reference first, then each wave's share scaled to it (where the wave
@@ -539,9 +530,22 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       total[n] += stat[w2][n * 16 + r][1] * __builtin_amdgcn_exp2f(stat[w2][n * 16 + r][0] - m);
     const float f = __builtin_amdgcn_exp2f(ref[n] - m);
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < DT; ++d) o[n][d] *= f;
+  }
+  if (__builtin_expect(any_odd, 0)) {
+    for (int i = 0; i < mine; ++i) {
+      const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
+      const int at = block_at(a.c, b, head, blk);
+      if (at < 0) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][d][i] = scaled(o[n][d][i], f);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          float part[4] = {o[n][d][0], o[n][d][1], o[n][d][2], o[n][d][3]};
+          add_odd<T, D, 4>(a, at, first, lo[n], min(hi[n], end - 1), [&](int j) { return 16 * d + 4 * g + j; }, part);
+          o[n][d] = f32x4{part[0], part[1], part[2], part[3]};
+        }
+    }
   }
   // waves 2 and 3 hand theirs to waves 0 and 1, then wave 1 to wave 0
   for (int step = 2; step; step >>= 1) {
@@ -809,17 +813,19 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
 
   const float total = sum + __shfl_xor(sum, 32);
   __syncthreads();
-  bool found = *odd != 0;
-  const bool plain = row >= 0 && !__builtin_isnan(total);   // NaN beside it is one that a value made
+  // sums that are not finite beside a sum of weights that is: values made them so
+  const bool plain = row >= 0 && !__builtin_isnan(total);
+  float t[4] = {};
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) found |= plain && __builtin_isnan(o[d][i]);
+    for (int i = 0; i < 16; ++i) t[i & 3] = __builtin_fmaf(o[d][i], 0.0f, t[i & 3]);
+  const bool found = *odd || (plain && __builtin_isnan(t[0] + t[1] + (t[2] + t[3])));
   if (__builtin_expect(__any(found), 0)) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] = plain && __builtin_isnan(o[d][i]) ? 0.0f : o[d][i];
+      for (int i = 0; i < 16; ++i) o[d][i] = plain && !__builtin_isfinite(o[d][i]) ? 0.0f : o[d][i];
     for (int i = 0; i < nblk; ++i) {
       const int at = block_at(a.c, b, head, blk0 + i);
       if (at < 0) continue;
