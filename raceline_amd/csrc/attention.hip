@@ -40,14 +40,18 @@ struct AttnArgs {
   void *out;
   PagedCache c;
   int64_t q_stride, out_stride;
-  float *part;                // [splits][rows][heads][D]: a run's sums, not divided; null where no run is split
-  float2 *part_stat;          // [splits][rows][heads]: (ref, sum of weights)
-  int *part_runs;             // [rows][heads]: runs of the row
+  // Sums of tiles whose keys are split: of few_rows_kernel, then of many_rows_kernel. A unit is one of the
+  // split tiles of one key/value head.
+  float *part;                // [unit][run][row of the tile][D]: a run's sums, not divided
+  float2 *part_stat;          // [unit][run][row of the tile]: (ref, sum of weights)
+  int4 *units;                // [unit]: (first row of the sequence, first row of the tile in it, rows of the sequence, runs)
+  int few_units, many_units;
   int heads, group, window, out_bf16, q_wide, out_wide;
-  int whole, splits, span;    // the `whole` longest tiles of a head are not split, the others' keys in runs of `span` (a multiple of 32)
-  int few_splits, few_span;   // the same for sequences of few rows, all of them
+  // of a head's tiles, longest first, the first `whole` are not split, the keys of the next `cut` are, in at
+  // most `splits` runs of `span` (a multiple of 32), and what is left is not
+  int whole, cut, splits, span;
+  int few_splits, few_span, few_rows;   // few_rows_kernel: all tiles, of few_rows rows
   int few, many;              // which kernels this call launches
-  int join_few;               // join_runs_kernel: only sequences of few rows have more than one run
   float unit;                 // base-2 units of a score as the product gives it, or of a capped one (1)
   float cap_log2;             // the cap in base-2 units, 0 for none
   float over_cap, exp_cap;    // score / cap, and the same in the power of tanh's exponential
@@ -194,16 +198,34 @@ __device__ __forceinline__ int runs_of(const AttnArgs &a, const Sequence &s, int
 // call's rows and (d + 1) * 128 / group of them; 64 lanes try 64 lengths at a time for the one past
 // which lie as many tiles as the rank says. The search goes through the sequences, seven times or so:
 // more than kRanked go in the order of the batch, last tile first (63 prompts of 300 tokens searched
-// for 317 us, 64 in order 172).
+// for 317 us, 64 in order 172). Up to 63 by a prefix sum of their tiles, so that no number is without one;
+// more as find_sequence numbers them.
 constexpr int kRanked = 16;
 
 __device__ __forceinline__ Sequence find_tile(const AttnArgs &a, int rank, int slots) {
-  if (a.c.batch > kRanked) return find_sequence(a.c, slots - 1 - rank, a.group, kManyRows, 1);
+  if (a.c.batch > 63) return find_sequence(a.c, slots - 1 - rank, a.group, kManyRows, 1);
   const int lane = threadIdx.x & 63, batch = a.c.batch;
   const int row = row_start(a.c, min(lane, batch)), kv = cached(a.c, min(lane, batch - 1));
   const int tokens = max(0, __shfl(row, lane + 1) - row);
   int tiles = lane < batch ? (tokens * a.group + kManyRows - 1) / kManyRows : 0;
   if (a.few && tokens * a.group <= kFewRows) tiles = 0;   // few_rows_kernel's
+  if (batch > kRanked) {
+    int upto = tiles;                                      // of the sequences up to this lane's
+    for (int off = 1; off < 64; off <<= 1) {
+      const int left = __shfl_up(upto, off);               // by every lane: one that is masked off gives 0
+      upto += lane >= off ? left : 0;
+    }
+    const int at = __builtin_amdgcn_readlane(upto, 63) - 1 - rank;
+    const int b = __popcll(__ballot(upto <= at));
+    Sequence s = {-1, 0, 0, 0, 0};
+    if (at < 0) return s;
+    s.b = b;
+    s.item = at - __builtin_amdgcn_readlane(upto, b) + __builtin_amdgcn_readlane(tiles, b);
+    s.row0 = __builtin_amdgcn_readlane(row, b);
+    s.tokens = __builtin_amdgcn_readlane(tokens, b);
+    s.kv = __builtin_amdgcn_readlane(kv, b);
+    return s;
+  }
   const int before = kv - tokens;
   auto shorter = [&](int length, int b) {                  // tiles of sequence b no longer than that
     const int64_t x = static_cast<int64_t>(length - __builtin_amdgcn_readlane(before, b)) * a.group;
@@ -249,16 +271,13 @@ __device__ __forceinline__ Sequence find_tile(const AttnArgs &a, int rank, int s
   return s;
 }
 
-__device__ __forceinline__ float *part_row(const AttnArgs &a, int split, int row, int head, int D) {
-  return a.part + ((static_cast<int64_t>(split) * a.c.rows + row) * a.heads + head) * D;
+// Row r of a tile's run among the partial sums.
+__device__ __forceinline__ int few_part(const AttnArgs &a, int unit, int run, int r) {
+  return (unit * a.few_splits + run) * a.few_rows + r;
 }
 
-__device__ __forceinline__ float2 &part_stat(const AttnArgs &a, int split, int row, int head) {
-  return a.part_stat[(static_cast<int64_t>(split) * a.c.rows + row) * a.heads + head];
-}
-
-__device__ __forceinline__ int &run_count(const AttnArgs &a, int row, int head) {
-  return a.part_runs[static_cast<int64_t>(row) * a.heads + head];
+__device__ __forceinline__ int many_part(const AttnArgs &a, int unit, int run, int r) {
+  return few_part(a, a.few_units, 0, 0) + (unit * a.splits + run) * kManyRows + r;
 }
 
 // A sum x over one reference, times the factor f to another's. An infinity stays one where f is 0.
@@ -343,8 +362,10 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
   // beside many_rows_kernel a sequence of few rows is one tile: items are the sequences
   const Sequence s = find_sequence(a.c, slot, a.many ? 0 : a.group, ROWS, 1);
   const int b = s.b, tile = s.item * ROWS, rows = s.tokens * a.group;
-  if (b < 0 || tile < 0 || tile >= rows || !is_few(a, s)) return;
-  const int runs = runs_of(a, s, a.few_splits, a.few_span);
+  const int unit = static_cast<int>(blockIdx.x / (KV * a.few_splits)) * KV + head;
+  const bool none = b < 0 || tile < 0 || tile >= rows || !is_few(a, s);
+  const int runs = none ? 0 : runs_of(a, s, a.few_splits, a.few_span);
+  if (a.few_splits > 1 && split == 0 && tid == 0) a.units[unit] = make_int4(s.row0, tile, rows, runs);
   if (split >= runs) return;
 
   // rows of this lane's columns, and what they see
@@ -575,12 +596,11 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
 #pragma unroll
       for (int d = 0; d < DT; ++d) store4(a, row[n], col[n] + d * 16 + 4 * g, o[n][d] * f);
     } else {
-      float *p = part_row(a, split, row[n], col[n] / D, D);
+      const int64_t at = few_part(a, unit, split, n * 16 + r);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p + d * 16 + 4 * g) = o[n][d];
-      if (g == 0) part_stat(a, split, row[n], col[n] / D) = make_float2(top[n], total[n]);
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(a.part + at * D + d * 16 + 4 * g) = o[n][d];
+      if (g == 0) a.part_stat[at] = make_float2(top[n], total[n]);
     }
-    if (split == 0 && g == 0 && a.part) run_count(a, row[n], col[n] / D) = runs;
   }
 }
 
@@ -636,12 +656,14 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
   const int KV = a.c.kv_heads, head = blockIdx.x % KV, item = blockIdx.x / KV, slots = a.c.rows * a.group / kManyRows + a.c.batch;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
-  const bool whole = item < a.whole;
-  const int splits = whole ? 1 : a.splits, split = whole ? 0 : (item - a.whole) % splits;
-  const Sequence s = find_tile(a, whole ? item : a.whole + (item - a.whole) / splits, slots);
+  const int past = item - a.whole;   // items of the split tiles and behind them
+  const bool whole = past < 0 || past >= a.cut * a.splits;
+  const int splits = whole ? 1 : a.splits, split = whole ? 0 : past % splits, nth = past / splits;
+  const Sequence s = find_tile(a, past < 0 ? item : whole ? item - a.cut * (a.splits - 1) : a.whole + nth, slots);
   const int b = s.b, tile = s.item * kManyRows, rows = s.tokens * a.group;
-  if (b < 0 || tile < 0 || tile >= rows || is_few(a, s)) return;
-  const int runs = runs_of(a, s, splits, a.span);
+  const bool none = b < 0 || tile < 0 || tile >= rows || is_few(a, s);
+  const int runs = none ? 0 : runs_of(a, s, splits, a.span), unit = nth * KV + head;
+  if (!whole && split == 0 && tid == 0) a.units[a.few_units + unit] = make_int4(s.row0, tile, rows, runs);
   if (split >= runs) return;
 
   // this lane's rows and what they see
@@ -851,67 +873,72 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
         store4(a, row, col + 32 * d + 8 * i + 4 * h,
                f32x4{o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f});
   } else {
-    float *p = part_row(a, split, row, col / D, D);
+    const int64_t at = many_part(a, unit, split, wave * 32 + n32);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4 *>(p + 32 * d + 8 * i + 4 * h) =
+        *reinterpret_cast<f32x4 *>(a.part + at * D + 32 * d + 8 * i + 4 * h) =
             f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-    if (h == 0) part_stat(a, split, row, col / D) = make_float2(ref, total);
+    if (h == 0) a.part_stat[at] = make_float2(ref, total);
   }
-  if (split == 0 && h == 0 && a.part) run_count(a, row, col / D) = runs;
 }
 
 // ----------------------------------------------------------------------------- the runs' sums
 
-// One wave: one (token, head) row; adds its runs' sums, always in the same order. How many runs a row has
-// its first run's workgroup wrote, so that the wave does not look for its sequence again; the
-// statistics of all runs come with one load (at most 64 runs), the sums eight runs at a time.
+template <int N, int D, typename Row>
+__device__ __forceinline__ void add_runs(Row row, int first, int runs, float mine, float (&o)[D / 64]) {
+  constexpr int PER = D / 64;
+  typedef float fvec __attribute__((ext_vector_type(PER)));
+  fvec p[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = *reinterpret_cast<const fvec *>(row(min(first + i, runs - 1)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float f = __shfl(mine, first + i);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] += first + i < runs ? scaled(p[i][e], f) : 0.0f;
+  }
+}
+
+// One wave: one row of a unit; adds its runs' sums, always in the same order. Where the row is and
+// how many runs it has its tile's first workgroup wrote; the statistics of all runs come with one load (at
+// most 64 runs), the sums eight runs at a time (four where there are no more).
 template <int D>
 __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
   constexpr int PER = D / 64;
-  typedef float fvec __attribute__((ext_vector_type(PER)));
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (item >= (a.join_few ? static_cast<int64_t>(a.c.batch) * a.c.kv_heads * kFewRows
-                          : static_cast<int64_t>(a.c.rows) * a.heads)) return;
-  int row = (int)(item / a.heads), head = (int)(item - (int64_t)row * a.heads);
-  if (a.join_few) {   // only sequences of few rows were split: 32 items for each of them and its heads
-    const int r = (int)item % kFewRows, kvh = (int)(item / kFewRows) % a.c.kv_heads;
-    const int b = (int)(item / kFewRows / a.c.kv_heads), row0 = row_start(a.c, b);
-    const int rows = (row_start(a.c, b + 1) - row0) * a.group;
-    if (r >= rows || rows > kFewRows) return;
-    row = row0 + r / a.group, head = kvh * a.group + r % a.group;
-  }
-  const int most = max(a.splits, a.few_splits);
-  const float2 stat = part_stat(a, min(lane, most - 1), row, head);
-  const int runs = __builtin_amdgcn_readfirstlane(min(run_count(a, row, head), most));
-  if (row < row_start(a.c, 0) || row >= row_start(a.c, a.c.batch) || runs <= 1) return;
+  const int few = a.few_units * a.few_rows, lane = threadIdx.x & 63;
+  int item = static_cast<int>(blockIdx.x) * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= few + a.many_units * kManyRows) return;
+  const bool is_few = item < few;
+  if (!is_few) item -= few;
+  const int rows = is_few ? a.few_rows : kManyRows, most = is_few ? a.few_splits : a.splits;
+  const int unit = item >> __builtin_ctz(rows), r = item & (rows - 1);
+  const int64_t at = is_few ? few_part(a, unit, 0, r) : many_part(a, unit, 0, r);   // run i: at + i * rows
+  const float2 stat = a.part_stat[at + min(lane, most - 1) * rows];
+  const int4 u = a.units[(is_few ? 0 : a.few_units) + unit];
+  const int runs = __builtin_amdgcn_readfirstlane(u.w), R = __builtin_amdgcn_readfirstlane(u.y) + r;
+  if (runs <= 1 || R >= __builtin_amdgcn_readfirstlane(u.z)) return;   // finished by its workgroup, or no row
   float top = lane < runs ? stat.x : -__builtin_inff();
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
   const float mine = lane < runs ? __builtin_amdgcn_exp2f(stat.x - (top == -__builtin_inff() ? 0.0f : top)) : 0.0f;
   float total = lane < runs ? stat.y * mine : 0.0f;
   for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off);
-  fvec o = {};
-  for (int i0 = 0; i0 < runs; i0 += 8) {
-    fvec p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      p[i] = *reinterpret_cast<const fvec *>(part_row(a, min(i0 + i, runs - 1), row, head, D) + lane * PER);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float f = __shfl(mine, i0 + i);
-#pragma unroll
-      for (int e = 0; e < PER; ++e) o[e] += i0 + i < runs ? scaled(p[i][e], f) : 0.0f;
-    }
+  float o[PER] = {};
+  const float *p = a.part + at * D + lane * PER;
+  auto row = [&](int i) { return p + static_cast<int64_t>(i) * rows * D; };
+  if (runs <= 4) {
+    add_runs<4, D>(row, 0, runs, mine, o);
+  } else {
+    for (int i = 0; i < runs; i += 8) add_runs<8, D>(row, i, runs, mine, o);
   }
   const float f = over_sum(total);
-  const int64_t at = row * a.out_stride + head * D + lane * PER;
+  const int tok = R / a.group, kvh = unit % a.c.kv_heads;
+  const int64_t to = static_cast<int64_t>(u.x + tok) * a.out_stride + (kvh * a.group + R - tok * a.group) * D + lane * PER;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    if (a.out_bf16) static_cast<__bf16 *>(a.out)[at + e] = static_cast<__bf16>(o[e] * f);
-    else static_cast<_Float16 *>(a.out)[at + e] = static_cast<_Float16>(o[e] * f);
+    if (a.out_bf16) static_cast<__bf16 *>(a.out)[to + e] = static_cast<__bf16>(o[e] * f);
+    else static_cast<_Float16 *>(a.out)[to + e] = static_cast<_Float16>(o[e] * f);
   }
 }
 
@@ -920,7 +947,10 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
 // How a call is launched, from its sizes alone (max_q and max_kv bound the sequences' new and
 // cached tokens; they choose, they do not limit what is computed).
 struct Plan {
-  int few, many, whole, splits, span, few_splits, few_span, few_tiles;
+  int few, many, whole, cut, splits, span, few_splits, few_span, few_tiles;
+  int64_t few_slots, slots;     // a head's tiles at most, of few_rows_kernel and of many_rows_kernel
+  int few_units, many_units;    // of the partial sums
+  int64_t part_rows;
   size_t bytes;
 };
 
@@ -974,62 +1004,84 @@ double cu_time(const Rates &r, int whole, int keys, int pieces, int run) {
   }
 }
 
+constexpr int64_t kMaxParts = 256 << 20;   // bytes of many_rows_kernel's partial sums
+
 // many_rows_kernel: which tiles are split into how many runs, by the least estimated time of a CU
 // (256 of them). Not all tiles alike: 320 tiles leave a quarter of the CUs with two, so 256 stay
 // whole and the other 64 are split in four; splitting writes and reads the runs' sums once, and
-// joining costs a launch.
-void split_many(int64_t tiles, int kv_heads, int kv, int D, int *whole, int *splits, int *span) {
-  const Rates &r = rates(D);
-  const int64_t per_head = (tiles + kv_heads - 1) / kv_heads;
-  *whole = (int)std::min<int64_t>(per_head, INT32_MAX), *splits = 1, *span = (kv + kBlockKeys - 1) / kBlockKeys * kBlockKeys;
+// joining costs a launch. What is left for splitting are the shortest tiles: `step` keys fewer for
+// every `alike` tiles of a head, the sequences being taken for alike. (A prompt's last tiles hold its first
+// keys, and are not worth splitting.) Up to twice as many tiles are split as the estimate has, for calls
+// whose sequences are not alike; the scratch is for those, kMaxParts at most. Where a sequence has no more than two
+// tiles a head, its keys come from memory for each: a lone workgroup takes 1.25 times as long, two
+// of a CU 1.12 (32 sequences of 40 tokens over 4000 keys in heads of 256: 256 tiles, whole 202 us, in two 170).
+void split_many(int64_t per_head, int kv_heads, int kv, int all, int64_t alike, double step, int D, Plan *p) {
+  Rates r = rates(D);
+  if (per_head <= 2 * alike) r.key[0] *= 1.25, r.key[1] *= 1.12;
+  const int64_t tiles = per_head * kv_heads;
+  p->whole = (int)std::min<int64_t>(per_head, INT32_MAX), p->cut = 0, p->splits = 1;
+  p->span = (kv + kBlockKeys - 1) / kBlockKeys * kBlockKeys;
   if (tiles > 256 * r.most * 3) return;          // the last round is short beside the others
-  double best = cu_time(r, (int)((tiles + 255) / 256), kv, 0, 0);
+  auto keys_of = [&](int64_t tile) { return (int)std::max(1.0, std::min<double>(kv, all - (double)(tile / alike) * step)); };
+  const int64_t most = kMaxParts / ((int64_t)kv_heads * kManyRows * (D + 2) * 4);   // runs of a head's tiles in the scratch
+  const int64_t full = tiles / 256, over = tiles - full * 256;
+  double best = cu_time(r, (int)full, kv, over ? 1 : 0, keys_of(full * 256 / kv_heads));
   for (int pass = 0; pass < 2; ++pass) {
-    const int64_t keep = pass ? tiles / 256 * 256 / kv_heads : 0, rest = tiles - keep * kv_heads;
+    const int64_t keep = pass ? full * 256 / kv_heads : 0, rest = tiles - keep * kv_heads;
     if ((pass && !keep) || rest <= 0) continue;
+    const int left = keys_of(keep);
     for (int pieces = 1; pieces <= 12; ++pieces) {   // of a CU; as many runs as make no CU have more
-      const int64_t n = std::min<int64_t>({64, pieces * 256 / rest, kv / 128});
+      const int64_t n = std::min<int64_t>({64, pieces * 256 / rest, left / 128});
       if (n < 2) continue;
-      const int run = (int)((kv + n * kBlockKeys - 1) / (n * kBlockKeys) * kBlockKeys), runs = (kv + run - 1) / run;
+      const int run = (int)((left + n * kBlockKeys - 1) / (n * kBlockKeys) * kBlockKeys), runs = (left + run - 1) / run;
+      if ((per_head - keep) * runs > most) continue;
       const double us = cu_time(r, (int)((keep * kv_heads + 255) / 256), kv, (int)((rest * runs + 255) / 256), run) + 5 +
                         (double)rest * runs * kManyRows * D * 8 / 4.2e6;
-      if (us < best) best = us, *whole = (int)keep, *splits = runs, *span = run;
+      if (us < best) best = us, p->whole = (int)keep, p->splits = runs, p->span = run;
     }
   }
+  if (p->splits > 1) p->cut = (int)std::min({2 * (per_head - p->whole), p->slots - p->whole, most / p->splits});
 }
 
 Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv, int window) {
   Plan p{};
   const int group = heads / kv_heads;
-  const int64_t rows = (int64_t)max_q * group;
+  const int64_t rows = (int64_t)max_q * group, all_rows = (int64_t)T * group;
   p.many = rows > kFewRows;
   // sequences of few rows beside long ones: their own kernel where they may be long in keys; up to
   // 2048, a tile of them takes no longer than its neighbours, and the launches it saves (the kernel's
   // and the join's) are 8 us
   p.few = !p.many || (B > 1 && (int64_t)B * max_q > T && max_kv > 2048);
   p.few_tiles = !p.many && rows <= 16 ? 1 : 2;
+  const int few_rows = 16 * p.few_tiles;
   int kv = std::max(1, max_kv);
   if (window && window < kMaxPositions && window < kv) kv = (int)std::min<int64_t>(kv, (int64_t)window + max_q + kBlockKeys);
   p.splits = p.few_splits = 1;
   p.span = p.few_span = (kv + 127) / 128 * 128;
   if (p.few) {
-    const int64_t per = std::max<int64_t>(1, (rows + 16 * p.few_tiles - 1) / (16 * p.few_tiles));
-    split_few((int64_t)B * (p.many ? 1 : per) * kv_heads, kv, D, &p.few_splits, &p.few_span);
+    p.few_slots = (p.many ? 0 : all_rows / few_rows) + B;
+    const int64_t per = std::max<int64_t>(1, (rows + few_rows - 1) / few_rows);
+    split_few((p.many ? B : std::max(B * per, all_rows / few_rows)) * kv_heads, kv, D, &p.few_splits, &p.few_span);
   }
   if (p.many) {
-    split_many(((int64_t)T * group + kManyRows - 1) / kManyRows * kv_heads, kv_heads, kv, D, &p.whole, &p.splits, &p.span);
+    p.slots = all_rows / kManyRows + B;
+    // tiles of a head, as if as many sequences as can had max_q new tokens
+    const int64_t longest = std::min<int64_t>(max_q, T), alike = T / longest, tail = T - alike * longest;
+    const int64_t per_head = alike * ((longest * group + kManyRows - 1) / kManyRows) + (tail * group + kManyRows - 1) / kManyRows;
+    split_many(std::min(per_head, p.slots), kv_heads, kv, std::max(1, max_kv), alike, (double)kManyRows / group, D, &p);
   }
-  const int s = std::max(p.splits, p.few_splits);
-  p.bytes = s > 1 ? (size_t)T * heads * ((size_t)s * (D + 2) + 1) * sizeof(float) : 0;
+  // under 2^21 and 2^20 rows: split_few gives at most 511 workgroups and one a tile, split_many 2^20 rows of 64
+  p.few_units = p.few_splits > 1 ? (int)(p.few_slots * kv_heads) : 0;
+  p.many_units = p.cut * kv_heads;
+  p.part_rows = (int64_t)p.few_units * p.few_splits * few_rows + (int64_t)p.many_units * p.splits * kManyRows;
+  p.bytes = (size_t)p.part_rows * (D + 2) * sizeof(float) + (size_t)(p.few_units + p.many_units) * sizeof(int4);
   return p;
 }
 
 template <typename T, int D, int TERMS>
 int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
-  const int64_t rows = (int64_t)a.c.rows * a.group;
   if (p.few) {
-    const int64_t slots = (p.many ? 0 : rows / (16 * p.few_tiles)) + a.c.batch;
-    const int64_t grid = slots * a.c.kv_heads * p.few_splits;
+    const int64_t grid = p.few_slots * a.c.kv_heads * p.few_splits;
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     if (p.few_tiles == 1) few_rows_kernel<T, D, 1><<<(unsigned)grid, kThreads, 0, st>>>(a);
     else few_rows_kernel<T, D, 2><<<(unsigned)grid, kThreads, 0, st>>>(a);
@@ -1037,8 +1089,7 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
   }
   if (p.many) {
     constexpr int lds = 2 * 2 * kTileKeys<D> * D * 2 + 64;
-    const int64_t slots = rows / kManyRows + a.c.batch, whole = std::min<int64_t>(p.whole, slots);
-    const int64_t grid = (whole + (slots - whole) * p.splits) * a.c.kv_heads;
+    const int64_t grid = (p.slots + (int64_t)p.cut * (p.splits - 1)) * a.c.kv_heads;
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     static LdsOptIn opt[2];
     const bool large = a.cap_log2 > kSmallCap;
@@ -1047,9 +1098,8 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
     fn<<<(unsigned)grid, kThreads, lds, st>>>(a);
     RLQ_HIP(hipGetLastError());
   }
-  if (p.splits > 1 || p.few_splits > 1) {
-    const int64_t items = a.join_few ? (int64_t)a.c.batch * a.c.kv_heads * kFewRows : (int64_t)a.c.rows * a.heads;
-    const int64_t grid = (items + 3) / 4;
+  if (p.bytes) {
+    const int64_t grid = ((int64_t)p.few_units * a.few_rows + (int64_t)p.many_units * kManyRows + 3) / 4;
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     join_runs_kernel<D><<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
@@ -1121,16 +1171,17 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
          kv_heads, B, T, table_stride, table_width};
   a.q_stride = q_stride, a.out_stride = out_stride;
   if (p.bytes) {
-    const size_t n = (size_t)std::max(p.splits, p.few_splits) * T * heads;
     a.part = static_cast<float *>(workspace);
-    a.part_stat = reinterpret_cast<float2 *>(a.part + n * D);
-    a.part_runs = reinterpret_cast<int *>(a.part_stat + n);
+    a.part_stat = reinterpret_cast<float2 *>(a.part + p.part_rows * D);
+    a.units = reinterpret_cast<int4 *>(a.part_stat + p.part_rows);
+    a.few_units = p.few_units, a.many_units = p.many_units;
   }
   a.heads = heads, a.group = heads / kv_heads, a.window = window < kMaxPositions ? window : 0, a.out_bf16 = out_dtype == RLQ_BF16;
   a.q_wide = aligned(q, 16) && q_stride % 8 == 0;
   a.out_wide = aligned(out, 8) && out_stride % 4 == 0;
-  a.whole = p.splits > 1 ? p.whole : INT32_MAX, a.splits = p.splits, a.span = p.span, a.few_splits = p.few_splits, a.few_span = p.few_span;
-  a.few = p.few, a.many = p.many, a.join_few = p.many && p.splits == 1;
+  a.whole = p.cut ? p.whole : INT32_MAX, a.cut = p.cut, a.splits = p.splits, a.span = p.span;
+  a.few_splits = p.few_splits, a.few_span = p.few_span, a.few_rows = 16 * p.few_tiles;
+  a.few = p.few, a.many = p.many;
   a.unit = softcap > 0 ? 1.0f : scale * kLog2e;
   if (softcap > 0) {
     constexpr float tanh_over_y[6] = {1.0f, -0.33333284f, 0.13331689f, -0.053768702f, 0.020753626f, -0.0058521652f};
