@@ -382,6 +382,8 @@ int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, 
  *   window > 0. A row that sees no key, or none with a score above -inf, is zero; one that sees a
  *   score that is NaN is NaN. An infinite value makes the rows that see it infinite, whatever
  *   its weight. Infinities and NaN in keys and values that a row does not see do not reach it.
+ *   Uncapped scores have to stay under 2^22 in magnitude, where fp32 holds them to a quarter:
+ *   a row with finite ones past that is not defined.
  * q 16-bit (dtype, the cache's) [T][q_stride]; out 16-bit (out_dtype) [T][out_stride], as the o
  * linear takes its rows; with q's type and stride it may take q's place. Products, softmax and
  * sums in fp32. For the second product weights are rounded to two terms of dtype (2^-16 of a

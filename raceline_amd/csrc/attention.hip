@@ -1148,7 +1148,7 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
               "rlq_attention: a cache of %d pages of %d holds more than 2^31 blocks", n_pages, page_size);
   RLQ_REQUIRE((int64_t)table_width * page_size <= kMaxPositions,
               "rlq_attention: a table of %d pages of %d holds more than 2^29 positions", table_width, page_size);
-  RLQ_REQUIRE(scale > 0 && scale < __builtin_inff(), "rlq_attention: scale=%g must be positive", scale);
+  RLQ_REQUIRE(scale > 0 && scale * kLog2e < __builtin_inff(), "rlq_attention: scale=%g must be positive and under 2.3e38", scale);
   RLQ_REQUIRE(softcap >= 0 && softcap < __builtin_inff(), "rlq_attention: softcap=%g must be 0 or positive", softcap);
   RLQ_REQUIRE(sizes_ok(T, B, heads, kv_heads, D, max_q, max_kv, window),
               "rlq_attention: T=%d, B=%d, heads=%d, max_q=%d, max_kv=%d or window=%d is out of range", T, B, heads, max_q,
