@@ -23,10 +23,10 @@ struct LogitArgs {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// Every wave's LDS operations are done, and what a barrier does not need stays in flight.
+// Every wave's LDS operations are done, and what a barrier does not need stays in flight. One asm
+// block: between a wait and a barrier of their own the compiler may place an LDS operation.
 __device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
-  asm volatile("s_barrier" ::: "memory");
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // One workgroup: a span of 4096 logits of one row. Every workgroup of a row reads all of the row's
