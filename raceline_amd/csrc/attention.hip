@@ -348,7 +348,9 @@ __device__ __forceinline__ typename Mfma<T>::op load_q(const AttnArgs &a, int ro
 // 16 (r / 8) + r % 8 (then + 8), so that a lane's eight weights belong to one 16-byte run of V.
 // Bound by the stream of keys and values, read past the caches: 32 sequences of up to 16384 tokens, 4
 // heads of 256, 1.21 GB in 212 us, 5.7 TB/s (229 us through the L2; a plain read gets 6.9 TB/s).
-template <typename T, int D, int NT>
+// LARGE_CAP: a cap over kSmallCap, whose code would cost the other calls (one token of 1024 keys in heads
+// of 64 9.0 us with it, 8.7 without).
+template <typename T, int D, int NT, bool LARGE_CAP>
 __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kernel(AttnArgs a) {
   constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * NT, TERMS = 2;
   typedef typename Mfma<T>::op op;
@@ -461,7 +463,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
       float x[8], top = -__builtin_inff();
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = sc[n][e >> 2][e & 3];
-      if (a.cap_log2 > kSmallCap) large_cap_scores<8>(a, x);
+      if constexpr (LARGE_CAP) large_cap_scores<8>(a, x);
       else if (a.cap_log2 != 0.0f) cap_scores<8>(a, x);
       if (masked) {
 #pragma unroll
@@ -644,7 +646,7 @@ constexpr int kTileKeys = D >= 128 ? 32 : 64;
 template <int D, int TERMS>
 constexpr int kManyHeld = D == 64 ? (TERMS == 1 ? 4 : 3) : D == 128 && TERMS == 1 ? 3 : 2;
 
-// LARGE_CAP: a cap over kSmallCap, whose code would cost the other calls 1 to 3%.
+// LARGE_CAP as above: 1 to 3% of the other calls.
 template <typename T, int D, int TERMS, bool LARGE_CAP>
 __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_kernel(AttnArgs a) {
   constexpr int KB = kTileKeys<D>, NB = KB / kBlockKeys, KS = D / 16, DT = D / 32, ROWS = kManyRows;
@@ -903,17 +905,19 @@ __device__ __forceinline__ void add_runs(Row row, int first, int runs, float min
 
 // One wave: one row of a unit; adds its runs' sums, always in the same order. Where the row is and
 // how many runs it has its tile's first workgroup wrote; the statistics of all runs come with one load (at
-// most 64 runs), the sums eight runs at a time (four where there are no more).
+// most 64 runs), the sums eight runs at a time (four where there are no more). Neighbouring workgroups
+// are neighbouring heads, as in the kernels that stored the sums: where the heads are a multiple of the 8
+// XCDs, a row is joined from the L2 that holds it (nine sequences' drafts with 8 heads 32.3 -> 30.6 us).
 template <int D>
 __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
   constexpr int PER = D / 64;
-  const int few = a.few_units * a.few_rows, lane = threadIdx.x & 63;
-  int item = static_cast<int>(blockIdx.x) * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= few + a.many_units * kManyRows) return;
-  const bool is_few = item < few;
-  if (!is_few) item -= few;
+  constexpr int kWaves = kThreads / 64;
+  const int few = a.few_units * a.few_rows / kWaves, lane = threadIdx.x & 63, KV = a.c.kv_heads;   // few: workgroups
+  const bool is_few = static_cast<int>(blockIdx.x) < few;
   const int rows = is_few ? a.few_rows : kManyRows, most = is_few ? a.few_splits : a.splits;
-  const int unit = item >> __builtin_ctz(rows), r = item & (rows - 1);
+  const int block = is_few ? blockIdx.x : blockIdx.x - few, head = block % KV, nth = block / KV * kWaves;
+  const int unit = (nth >> __builtin_ctz(rows)) * KV + head;
+  const int r = (nth & (rows - 1)) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t at = is_few ? few_part(a, unit, 0, r) : many_part(a, unit, 0, r);   // run i: at + i * rows
   const float2 stat = a.part_stat[at + min(lane, most - 1) * rows];
   const int4 u = a.units[(is_few ? 0 : a.few_units) + unit];
@@ -933,8 +937,8 @@ __global__ __launch_bounds__(kThreads) void join_runs_kernel(AttnArgs a) {
     for (int i = 0; i < runs; i += 8) add_runs<8, D>(row, i, runs, mine, o);
   }
   const float f = over_sum(total);
-  const int tok = R / a.group, kvh = unit % a.c.kv_heads;
-  const int64_t to = static_cast<int64_t>(u.x + tok) * a.out_stride + (kvh * a.group + R - tok * a.group) * D + lane * PER;
+  const int tok = R / a.group;
+  const int64_t to = static_cast<int64_t>(u.x + tok) * a.out_stride + (head * a.group + R - tok * a.group) * D + lane * PER;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     if (a.out_bf16) static_cast<__bf16 *>(a.out)[to + e] = static_cast<__bf16>(o[e] * f);
@@ -1080,11 +1084,13 @@ Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv
 
 template <typename T, int D, int TERMS>
 int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
+  const bool large_cap = a.cap_log2 > kSmallCap;
   if (p.few) {
     const int64_t grid = p.few_slots * a.c.kv_heads * p.few_splits;
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
-    if (p.few_tiles == 1) few_rows_kernel<T, D, 1><<<(unsigned)grid, kThreads, 0, st>>>(a);
-    else few_rows_kernel<T, D, 2><<<(unsigned)grid, kThreads, 0, st>>>(a);
+    auto fn = p.few_tiles == 1 ? (large_cap ? few_rows_kernel<T, D, 1, true> : few_rows_kernel<T, D, 1, false>)
+                               : (large_cap ? few_rows_kernel<T, D, 2, true> : few_rows_kernel<T, D, 2, false>);
+    fn<<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
   }
   if (p.many) {
@@ -1092,14 +1098,13 @@ int launch_attn(const AttnArgs &a, const Plan &p, hipStream_t st) {
     const int64_t grid = (p.slots + (int64_t)p.cut * (p.splits - 1)) * a.c.kv_heads;
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     static LdsOptIn opt[2];
-    const bool large = a.cap_log2 > kSmallCap;
-    auto fn = large ? many_rows_kernel<T, D, TERMS, true> : many_rows_kernel<T, D, TERMS, false>;
-    if (int rc = allow_large_lds(reinterpret_cast<const void *>(fn), opt[large])) return rc;
+    auto fn = large_cap ? many_rows_kernel<T, D, TERMS, true> : many_rows_kernel<T, D, TERMS, false>;
+    if (int rc = allow_large_lds(reinterpret_cast<const void *>(fn), opt[large_cap])) return rc;
     fn<<<(unsigned)grid, kThreads, lds, st>>>(a);
     RLQ_HIP(hipGetLastError());
   }
   if (p.bytes) {
-    const int64_t grid = ((int64_t)p.few_units * a.few_rows + (int64_t)p.many_units * kManyRows + 3) / 4;
+    const int64_t grid = ((int64_t)p.few_units * a.few_rows + (int64_t)p.many_units * kManyRows) / (kThreads / 64);
     RLQ_REQUIRE(grid <= kMaxGrid, "rlq_attention: %lld workgroups are too many for a launch", (long long)grid);
     join_runs_kernel<D><<<(unsigned)grid, kThreads, 0, st>>>(a);
     RLQ_HIP(hipGetLastError());
