@@ -389,12 +389,14 @@ int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, 
  * sums in fp32. For the second product weights are rounded to two terms of dtype (2^-16 of a
  * weight for bf16, 2^-21 for fp16) where a sequence has at most 32 rows a key/value head (tokens
  * times query heads that share it) and where the cache is RLQ_BF16 and the output RLQ_F16; in
- * other calls to one term.
+ * other calls to one term, unless RLQ_FULL_WEIGHTS is added to out_dtype: rows are then as exact as
+ * their own rounding (2.1e-4 for fp16, in place of 2.9e-4), in 4/3 of the time.
  * max_q and max_kv (host) bound the new and all tokens of a sequence: the kernels and the split
  * of the keys over workgroups are chosen from them, and results stay right past them. Both
  * given as they are, calls of the same sizes give the same bits.
  * The workspace (rlq_attention_workspace_bytes, may be 0; 16-byte aligned, no initialisation)
  * holds the sums of a split call's parts; calls that overlap must not share it. */
+enum { RLQ_FULL_WEIGHTS = 16 };
 size_t rlq_attention_workspace_bytes(int T, int heads, int kv_heads, int D, int B, int max_q, int max_kv, int window);
 int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, int D, int dtype, const void *k_cache,
                   const void *v_cache, int n_pages, int page_size, const int *cu_q, const int *kv_len,

@@ -141,9 +141,10 @@ __device__ __forceinline__ float max_halves(float x) {
 // of a weight for bf16 and 22 for fp16. few_rows_kernel always has it, since it waits for memory (32
 // sequences of up to 16384 tokens 218 us with one term and with two, off by 2.8e-4 of the rows and by
 // 2.07e-4, which is the rows' own rounding to fp16). many_rows_kernel has it where one term would have
-// fewer bits than the rows that leave (bf16 keys, fp16 rows); elsewhere its rounding is as large as the
-// rows' own (2.9e-4 against 2.07e-4, bf16 2.07e-3 against 1.63e-3), and half of the matrix products more
-// cost 33 to 40% (a 27B layer's chunk 351 us against 468, six capped prompts 84 against 113).
+// fewer bits than the rows that leave (bf16 keys, fp16 rows) and where the caller asks for it; elsewhere its
+// rounding is as large as the rows' own (2.9e-4 against 2.07e-4, bf16 2.07e-3 against 1.63e-3), and half
+// of the matrix products more cost 27 to 37% (a 27B layer's chunk 332 us against 439, six capped
+// prompts 84 against 111, a chunk of 333 tokens in heads of 64 49 against 63).
 template <typename T, int TERMS>
 __device__ __forceinline__ void weights(const float (&p)[8], typename Mfma<T>::op (&w)[TERMS]) {
 #pragma unroll
@@ -1143,6 +1144,8 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
   using namespace rlq;
   RLQ_REQUIRE(D == 64 || D == 128 || D == 256, "rlq_attention: head size %d is not 64, 128 or 256", D);
   RLQ_REQUIRE(dtype == RLQ_F16 || dtype == RLQ_BF16, "rlq_attention: unknown dtype %d", dtype);
+  const bool full_weights = (out_dtype & RLQ_FULL_WEIGHTS) != 0;
+  out_dtype &= ~RLQ_FULL_WEIGHTS;
   RLQ_REQUIRE(out_dtype == RLQ_F16 || out_dtype == RLQ_BF16, "rlq_attention: unknown output dtype %d", out_dtype);
   RLQ_REQUIRE(kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0,
               "rlq_attention: %d heads do not share %d key/value heads evenly", heads, kv_heads);
@@ -1195,9 +1198,9 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
     for (int i = 0; i < 6; ++i) a.near_cap[i] = tanh_over_y[i] * (scale * kLog2e);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == RLQ_F16) return launch_size<_Float16, 1>(a, p, D, st);
-  if (out_dtype == RLQ_BF16) return launch_size<__bf16, 1>(a, p, D, st);
-  return launch_size<__bf16, 2>(a, p, D, st);
+  const bool two = full_weights || (dtype == RLQ_BF16 && out_dtype == RLQ_F16);
+  if (dtype == RLQ_F16) return two ? launch_size<_Float16, 2>(a, p, D, st) : launch_size<_Float16, 1>(a, p, D, st);
+  return two ? launch_size<__bf16, 2>(a, p, D, st) : launch_size<__bf16, 1>(a, p, D, st);
 }
 
 }  // extern "C"

@@ -656,6 +656,9 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     return out
 
 
+FULL_WEIGHTS = 16   # include/rlq.h RLQ_FULL_WEIGHTS
+
+
 @functools.lru_cache(maxsize=4096)
 def attention_workspace_bytes(T: int, heads: int, kv_heads: int, head_dim: int, B: int, max_q: int, max_kv: int,
                               window: int = 0) -> int:
@@ -665,13 +668,14 @@ def attention_workspace_bytes(T: int, heads: int, kv_heads: int, head_dim: int, 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
               table: torch.Tensor, max_q: int, max_kv: int, scale: float | None = None, window: int = 0,
               softcap: float = 0.0, out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float16,
-              workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+              workspace: torch.Tensor | None = None, stream=None, full_weights: bool = False) -> torch.Tensor:
     """Causal attention of new rows q [T][heads * head_dim] (the cache's dtype) over their
     sequences' pages, the rows' own keys among them (rlq_attention) -> [T][heads * head_dim] in
     out_dtype. max_q and max_kv bound a sequence's new and all tokens; scale: 1 / sqrt(head_dim)
     by default; window: the last positions a row sees (0: all); softcap: 0 for none. Rows from
     cu_q[B] on are left as they were in `out`. workspace: scratch to use in place of a new
-    tensor; calls that overlap must not share it."""
+    tensor; calls that overlap must not share it. full_weights: softmax weights keep more bits than
+    the rows in calls of many rows too, as they do in those of few, in 4/3 of the time."""
     (n_pages, kv_heads, page, D), code, dev, B = _check_paged(k_cache, v_cache, cu_q, kv_len, table)
     T, width, qs = _rows(q, k_cache.dtype, dev, "q")
     if not width or width % max(kv_heads * D, 1):
@@ -700,7 +704,7 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_
     _call_on(dev, stream, "rlq_attention", q.data_ptr(), qs, T, H, kv_heads, D, code, k_cache.data_ptr(),
              v_cache.data_ptr(), n_pages, page, cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
              max(table.stride(0), table.shape[1]), table.shape[1], B, max_q, max_kv, D ** -0.5 if scale is None else scale,
-             window, softcap, out.data_ptr(), os, out_code, _ptr(workspace), nbytes)
+             window, softcap, out.data_ptr(), os, out_code | (FULL_WEIGHTS if full_weights else 0), _ptr(workspace), nbytes)
     return out
 
 

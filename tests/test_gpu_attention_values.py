@@ -153,11 +153,7 @@ def test_an_infinite_value_of_a_run_of_small_weights_is_infinite(gpu, plan):
         assert (np.abs(got - ref) <= tol).all()
 
 
-@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=["f16", "bf16-f16", "bf16", "f16-bf16"])
-@pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("lens", [[(1, 1), (1, 700), (1, 65)], [(5, 333), (8, 900)], [(2, 6000)]],
-                         ids=["tokens", "drafts", "split"])
-def test_weights_of_few_rows_keep_more_bits_than_the_rows(gpu, lens, D, dtype, out_dtype):
+def check_weights(gpu, lens, D, dtype, out_dtype, **kw):
     """Queries with one dimension, so that a score is one product, exact in fp32 but for two roundings of
     2^-24 of at most 16 (base 2): 2^-19; exp2 2^-22; weights of two terms 2^-16 (bf16) or 2^-21 (fp16); the sum
     over at most 6000 keys, whose partial sums of 4 x 4 x 32 keys and runs are short, 2^-17. The rows are off by half
@@ -167,7 +163,7 @@ def test_weights_of_few_rows_keep_more_bits_than_the_rows(gpu, lens, D, dtype, o
     s.q = np.where(keep, np.clip(s.q, -3, 3), 0.0)
     s.dq = torch.from_numpy(s.q.reshape(s.T, 4 * D)).to(dtype).to(gpu)
     s.q = s.dq.double().cpu().numpy().reshape(s.T, 4, D)
-    out = run(s, gpu, scale=0.5, out_dtype=out_dtype).double().cpu().numpy().reshape(s.T, 4, D)
+    out = run(s, gpu, scale=0.5, out_dtype=out_dtype, **kw).double().cpu().numpy().reshape(s.T, 4, D)
     bits = 10 if out_dtype == F16 else 7
     for b, (n, kv) in enumerate(lens):
         r = slice(s.cu[b], s.cu[b] + n)
@@ -176,6 +172,21 @@ def test_weights_of_few_rows_keep_more_bits_than_the_rows(gpu, lens, D, dtype, o
         _, e = np.frexp(np.abs(ref) + off * size)
         half_step = 2.0 ** np.maximum(e - 2 - bits, -25 if out_dtype == F16 else -134)
         assert (np.abs(out[r] - ref) <= half_step + off * size).all(), np.max((np.abs(out[r] - ref) - half_step) / size)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=["f16", "bf16-f16", "bf16", "f16-bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 1), (1, 700), (1, 65)], [(5, 333), (8, 900)], [(2, 6000)]],
+                         ids=["tokens", "drafts", "split"])
+def test_weights_of_few_rows_keep_more_bits_than_the_rows(gpu, lens, D, dtype, out_dtype):
+    check_weights(gpu, lens, D, dtype, out_dtype)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=["f16", "bf16-f16", "bf16", "f16-bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(70, 333), (129, 129)], [(60, 6000)], [(40, 3000), (1, 5000)]], ids=["many", "split", "both"])
+def test_full_weights_of_many_rows_keep_more_bits_than_the_rows(gpu, lens, D, dtype, out_dtype):
+    check_weights(gpu, lens, D, dtype, out_dtype, full_weights=True)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
