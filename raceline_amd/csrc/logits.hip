@@ -37,7 +37,8 @@ __device__ __forceinline__ void lds_barrier() {
 // Loads return in the order in which they were issued: biases and the first 8192 tokens come
 // before the logits, four neighbours a thread and step, which arrive while the tokens are counted.
 // Bound by HBM without tokens and biases (16 rows of 248,320 in 6.7 us), by the span that most of
-// them fall into with them (8000 tokens and 200 biases a row 14.4 us, a third of them in one span).
+// them fall into with them (8000 tokens and 200 biases a row 14.4 us, half of the tokens and a quarter of
+// the biases in one span).
 // Biases: an id may come twice. Its first entry (found by an integer atomic, whose order changes
 // nothing) adds up all of its entries in list order, so the sum does not depend on which thread
 // came first; the list is looked through only for ids that do come twice.

@@ -56,11 +56,13 @@ __device__ __forceinline__ void load8(const float *p, bool wide, float (&x)[8]) 
 //           sincospi in 32; once per token and pair, kept in LDS for all heads.
 //   values  transposed through LDS into runs of eight keys; a run that is only partly new is
 //           written element by element, so that the other tokens' values stay.
-// Bound by HBM: 2048 tokens of 20 + 2 * 4 heads of 256 (88 MB) in 19.7 us, 4.5 TB/s. Small calls take
+// Bound by HBM for the most part: 2048 tokens of 20 + 2 * 4 heads of 256 (88 MB) in 19.7 us, where a plain
+// conversion of as many numbers takes 16.7; 37 chunks of up to 300 tokens in heads of 128, all of them turned
+// (213 MB), in 56 us and 38: a workgroup forms 2048 angles ahead of its stores there. Small calls take
 // one head a workgroup, in the two cases measured 6.7 us against 9.4 with all heads (5 tokens of
 // 16 + 2 * 4 heads) and 21.5 against 33 (that chunk, before a thread's items were stepped through
-// without divisions); large ones all, so that angles are formed once (37 chunks of up to 300 tokens
-// in heads of 128 57.7 us, one head a workgroup 71.6).
+// without divisions); large ones all, so that angles are formed once (those 37 chunks 57.7 us, one head a
+// workgroup 71.6).
 template <typename T, int D>
 __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
   constexpr int kChunks = D / 8, kRowStep = kRopeThreads / kChunks, kPad = D + 8;
