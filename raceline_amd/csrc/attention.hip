@@ -198,9 +198,10 @@ __device__ __forceinline__ int runs_of(const AttnArgs &a, const Sequence &s, int
 // 87 us, in this order 77). Tile d of a sequence counts as long as the sequence before the
 // call's rows and (d + 1) * 128 / group of them; 64 lanes try 64 lengths at a time for the one past
 // which lie as many tiles as the rank says. The search goes through the sequences, seven times or so:
-// more than kRanked go in the order of the batch, last tile first (63 prompts of 300 tokens searched
-// for 317 us, 64 in order 172). Up to 63 by a prefix sum of their tiles, so that no number is without one;
-// more as find_sequence numbers them.
+// more than kRanked go in the order of the batch, last tile first. (Searched and in order, heads of 128: 63 prompts of
+// 300 tokens 340 us and 131, 32 of up to 900 216 and 142, 20 of up to 1500 188 and 157; but 20 chunks of up to
+// 500 tokens over up to 8000 482 and 606.) Up to 63 by a prefix sum of their tiles, so that no number is
+// without one; more as find_sequence numbers them.
 constexpr int kRanked = 16;
 
 __device__ __forceinline__ Sequence find_tile(const AttnArgs &a, int rank, int slots) {
@@ -348,7 +349,7 @@ __device__ __forceinline__ typename Mfma<T>::op load_q(const AttnArgs &a, int ro
 // v_mfma_f32_16x16x32: S^T (keys x rows) = K Q^T with the operand's row r standing for key
 // 16 (r / 8) + r % 8 (then + 8), so that a lane's eight weights belong to one 16-byte run of V.
 // Bound by the stream of keys and values, read past the caches: 32 sequences of up to 16384 tokens, 4
-// heads of 256, 1.21 GB in 212 us, 5.7 TB/s (229 us through the L2; a plain read gets 6.9 TB/s).
+// heads of 256, 1.21 GB in 210 us, 5.8 TB/s (229 us through the L2; a plain read gets 6.9 TB/s).
 // LARGE_CAP: a cap over kSmallCap, whose code would cost the other calls (one token of 1024 keys in heads
 // of 64 9.0 us with it, 8.7 without).
 template <typename T, int D, int NT, bool LARGE_CAP>
@@ -964,24 +965,28 @@ constexpr int64_t kMaxGrid = (int64_t)UINT32_MAX / kThreads;   // a launch count
 // few_rows_kernel: how the keys are split into runs (of whole blocks for the four waves, 64 at most).
 // Where the keys and values take 8 us or more at 5.5 TB/s, as many runs as give 512 workgroups, two a
 // CU: fewer leave memory idle and sequences of different lengths uneven (nine sequences' drafts 29.6
-// us with 576 workgroups, 35 with 288). Below that a call is a chain of latencies: a run of 128 keys
-// (a block a wave) takes `first`, each further 128 keys `step`, joining 2.5 us and 0.14 a run, and
-// the least sum is taken. So one token of 1024 keys in heads of 64 is one run (7.7 us, eight runs 7.8),
-// in heads of 256 eight (10.1, one run 15.5), and of 4096 keys 16 (12.4, 32 runs 14.2).
+// us with 576 workgroups, 35 with 288). (Heads of 256 with more than 16 rows hold one workgroup a CU; 256
+// workgroups were from 31% faster, 4 sequences of up to 16000 tokens, to 22% slower, 16 of up to 8000, as their
+// lengths fall.) Below that a call is a chain of latencies: a run of 128 keys (a block a wave)
+// takes `first`, each further 128 keys `step`, joining 2.1 us and 0.13 a run, and the least sum is taken. So
+// one token of 512 keys in heads of 64 is one run (6.2 us, four runs 7.3), of 1024 keys eight (7.7, one
+// run 9.3), in heads of 256 eight as well (10.6, one run 22.9), and of 4096 keys 16 (13.9, 32 runs 13.3, eight 18.1).
 void split_few(int64_t tiles, int kv, int D, int *splits, int *span) {
-  const double first = D == 256 ? 7.5 : D == 128 ? 5.5 : 4.5, step = D == 256 ? 1.15 : D == 128 ? 0.56 : 0.45;
+  const double first = D == 256 ? 7.5 : D == 128 ? 5.5 : 4.6, step = D == 256 ? 1.9 : D == 128 ? 1.0 : 0.75;
   const bool streams = (double)tiles * kv * D * 4 / 5.5e6 >= 8;
   const int block = 4 * kBlockKeys, most = (int)std::min<int64_t>(64, (511 + tiles) / tiles);
   double best = 0;
   for (int n = streams ? most : 1; n <= most; ++n) {
     const int run = (int)(((int64_t)kv + (int64_t)n * block - 1) / ((int64_t)n * block) * block), runs = (kv + run - 1) / run;
-    const double us = first + step * (run / block - 1) + (runs > 1 ? 2.5 + 0.14 * runs : 0);
+    const double us = first + step * (run / block - 1) + (runs > 1 ? 2.1 + 0.13 * runs : 0);
     if (best == 0 || us < best) best = us, *splits = runs, *span = run;
   }
 }
 
 // many_rows_kernel's microseconds a key for one of 1, 2, .. workgroups that share a CU (measured over
-// 8192 keys, whole chips of them); as many as its registers let in.
+// 8192 keys, whole chips of them); as many as its registers let in. With weights of one term: with two a
+// key takes a third longer and heads of 64 and 128 hold one workgroup less, but the plan is the same, since
+// the scratch's size is asked for without the types (a 27B chunk 423 us, 332 with one term).
 struct Rates {
   int most;
   double key[4];
@@ -1055,7 +1060,9 @@ Plan plan_of(int T, int B, int heads, int kv_heads, int D, int max_q, int max_kv
   p.many = rows > kFewRows;
   // sequences of few rows beside long ones: their own kernel where they may be long in keys; up to
   // 2048, a tile of them takes no longer than its neighbours, and the launches it saves (the kernel's
-  // and the join's) are 8 us
+  // and the join's) are 8 us. (One kernel and two, a chunk of 512 tokens beside 32 single ones of up to
+  // 2000 keys, 27B heads: 94 us and 104, of up to 4000 230 and 158, heads of 128 93 and 82, 176 and 138;
+  // beside 8 of up to 4000 91 and 111, a chunk of 2048 beside 32 of them 229 and 274: the keys alone do not decide.)
   p.few = !p.many || (B > 1 && (int64_t)B * max_q > T && max_kv > 2048);
   p.few_tiles = !p.many && rows <= 16 ? 1 : 2;
   const int few_rows = 16 * p.few_tiles;
