@@ -395,7 +395,8 @@ int rlq_rope_append(const float *q, int q_stride, const float *k, int k_stride, 
  * of the keys over workgroups are chosen from them, and results stay right past them. Both
  * given as they are, calls of the same sizes give the same bits.
  * The workspace (rlq_attention_workspace_bytes, may be 0; 16-byte aligned, no initialisation)
- * holds the sums of a split call's parts; calls that overlap must not share it. */
+ * holds the sums of a split call's parts; calls that overlap must not share it. What a call needs does
+ * not rise with its sizes; 340 MB (10^6 bytes) are enough for any. */
 enum { RLQ_FULL_WEIGHTS = 16 };
 size_t rlq_attention_workspace_bytes(int T, int heads, int kv_heads, int D, int B, int max_q, int max_kv, int window);
 int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, int D, int dtype, const void *k_cache,
