@@ -117,6 +117,37 @@ def test_an_infinite_value_is_infinite_in_the_rows_that_see_it(gpu, plan, dtype,
             assert (np.abs(got - ref) <= tol).all()
 
 
+@pytest.mark.parametrize("dtype,full", [(F16, False), (F16, True), (BF16, True)], ids=["f16", "f16-full", "bf16-full"])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("plan", PLANS)
+def test_infinite_values_in_every_tile_of_dimensions(gpu, plan, D, dtype, full):
+    """In the first and last dimensions of larger heads, seen by the rows from one position on (in one plan not
+    by its first 20, whose positions are 50 to 69) and by the last alone, beside a row whose scores are NaN."""
+    s = planned(gpu, plan, D, dtype)
+    n, kv = s.lens[0]
+    place = 70 if kv > 100 else 40
+    for dim in (0, 31, 32, D // 2 + 5, D - 1):
+        put(s, 0, place, dim, INF)
+    put(s, 0, kv - 1, D - 2, -INF)
+    s.dq[0, D + 5] = float("nan")                            # row 0, head 1
+    for b, (got, ref, tol) in enumerate(rows_of(s, run(s, gpu, out_dtype=dtype, full_weights=full), dtype)):
+        ok = np.abs(got - ref) <= tol
+        if b == 0:
+            assert np.isnan(got[0, 1]).all()
+            rest = np.ones(got.shape[:2], bool)
+            rest[0, 1] = False
+            seen = rest & (np.arange(kv - n, kv) >= place)[:, None]
+            for dim in (0, 31, 32, D // 2 + 5, D - 1):
+                assert (got[:, :, dim][seen] == INF).all()
+                ok[:, :, dim][seen] = True
+            last = rest.copy()
+            last[:-1] = False
+            assert (got[:, :, D - 2][last] == -INF).all()
+            ok[:, :, D - 2][last] = True
+            ok[0, 1] = True
+        assert ok.all()
+
+
 @pytest.mark.parametrize("dtype,out_dtype", TYPES, ids=["f16", "bf16-f16", "bf16", "f16-bf16"])
 @pytest.mark.parametrize("plan", PLANS)
 @pytest.mark.parametrize("below", [-6, -20])
