@@ -28,8 +28,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // seen, kBelow under it, and moves only when a score passes ref + kBelow + kRefSlack: most
 // steps then leave the accumulators alone. For fp16 (kBelow 7) a weight is at most 2^15, inside fp16, and
 // 2^-14, where fp16 loses bits, lies 2^21 under the largest: what is lost there does not show in the sum.
-// bf16 has no such bound but values up to 2^128: a weight is at most 1 (kBelow -8), so that its
-// product with one stays in range.
+// bf16 has no such bound but values up to 2^128: a weight is at most 2^-12 (kBelow -20), so that the sums
+// of thousands of such values stay in range.
 constexpr float kRefSlack = 8.0f;
 
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -82,7 +82,7 @@ struct Mfma<__bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static constexpr unsigned kExp = 0x7F80u;
-  static constexpr float kBelow = -8.0f;
+  static constexpr float kBelow = -20.0f;
 };
 
 // Capped scores in base-2 units, cap tanh(y) with y = score / cap. 1 - 2 / (1 + e^2y) is off by 2^-21.5
@@ -161,7 +161,8 @@ __device__ __forceinline__ void weights(const float (&p)[8], typename Mfma<T>::o
 // behind a sequence's end is never read into a result. In blocks that every row sees the product is
 // formed with them, and is NaN where a weight, or its second term, rounds to 0 or below. In both
 // cases they are added at the end to the rows that see them (add_odd), whose sums they alone
-// decide: an infinity makes the rows that see it infinite, wherever it lies.
+// decide: an infinity makes the rows that see it infinite, wherever it lies. (NaN that finite values made, by
+// sums past fp32 of both signs, stays: it is kMade until then, which nothing is added to.)
 template <typename T>
 __device__ __forceinline__ u32x4 finite8(u32x4 v, unsigned seen, bool &odd) {
   constexpr unsigned E = Mfma<T>::kExp;
@@ -287,6 +288,14 @@ __device__ __forceinline__ float scaled(float x, float f) {
   const float y = x * f;
   return __builtin_isnan(y) ? x : y;
 }
+
+constexpr unsigned kMade = 1;   // bits of a sum that was NaN beside a sum of weights that is not
+
+__device__ __forceinline__ float marked(float o, float sum) {
+  return __builtin_isnan(o) && !__builtin_isnan(sum) ? __uint_as_float(kMade) : o;
+}
+
+__device__ __forceinline__ float unmarked(float o) { return __float_as_uint(o) == kMade ? __builtin_nanf("") : o; }
 
 // Adds the infinities and NaN among the values of block `at` (its first key `first`) to o (o[i]:
 // dimension dim(i)) for the keys that a row sees.
@@ -528,15 +537,6 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     odd |= row[n] >= 0 && !__builtin_isnan(sum[n]) && __builtin_isnan(t[0] + t[1]);
   }
   const bool any_odd = __any(odd);
-  if (__builtin_expect(any_odd, 0)) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o[n][d][i] = !__builtin_isnan(sum[n]) && !__builtin_isfinite(o[n][d][i]) ? 0.0f : o[n][d][i];
-  }
 
   // the waves' sums: the largest reference first, then each wave's share scaled to it (where the wave
   // found no score, its sums are 0, or NaN where what it saw was)
@@ -554,8 +554,15 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     for (int w2 = 0; w2 < 4; ++w2)
       total[n] += stat[w2][n * 16 + r][1] * __builtin_amdgcn_exp2f(stat[w2][n * 16 + r][0] - m);
     const float f = __builtin_amdgcn_exp2f(ref[n] - m);
+    if (__builtin_expect(any_odd, 0)) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[n][d] *= f;
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][d][i] = marked(scaled(o[n][d][i], f), sum[n]);
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[n][d] *= f;
+    }
   }
   if (__builtin_expect(any_odd, 0)) {
     for (int i = 0; i < mine; ++i) {
@@ -571,6 +578,12 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
           o[n][d] = f32x4{part[0], part[1], part[2], part[3]};
         }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][d][i] = unmarked(o[n][d][i]);
   }
   // waves 2 and 3 hand theirs to waves 0 and 1, then wave 1 to wave 0
   for (int step = 2; step; step >>= 1) {
@@ -851,7 +864,7 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] = plain && !__builtin_isfinite(o[d][i]) ? 0.0f : o[d][i];
+      for (int i = 0; i < 16; ++i) o[d][i] = marked(o[d][i], total);
     for (int i = 0; i < nblk; ++i) {
       const int at = block_at(a.c, b, head, blk0 + i);
       if (at < 0) continue;
@@ -866,6 +879,10 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
         for (int e = 0; e < 16; ++e) o[d][e] = part[e];
       }
     }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = unmarked(o[d][i]);
   }
   if (row < 0) return;
   if (runs == 1) {

@@ -286,3 +286,17 @@ def test_large_values_of_no_weight_add_nothing(gpu):
         s.values[0][:upto] = 0.0
         for got, ref, tol in rows_of(s, run(s, gpu, out_dtype=BF16), BF16):
             assert (np.abs(got - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("plan", PLANS)
+def test_sums_of_the_largest_values_of_bf16_stay_in_range(gpu, plan, D):
+    """Every value one of the largest bf16 numbers, all of one sign in a dimension: rows of them."""
+    s = planned(gpu, plan, D, BF16)
+    most = float(torch.finfo(BF16).max)
+    for b in range(len(s.lens)):
+        s.values[b] = np.broadcast_to(np.where(np.arange(D) % 3 == 0, -most, most), s.values[b].shape)
+    big = np.broadcast_to(np.where(np.arange(D) % 3 == 0, -most, most).astype(np.float32), (s.vc.shape[0], 2, s.page, D))
+    s.vc = torch.from_numpy(pack_values(np.ascontiguousarray(big))).to(gpu).to(BF16)
+    for got, ref, tol in rows_of(s, run(s, gpu, out_dtype=BF16), BF16):
+        assert (np.abs(got - ref) <= tol).all()
