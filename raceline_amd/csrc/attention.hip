@@ -297,6 +297,21 @@ __device__ __forceinline__ float marked(float o, float sum) {
 
 __device__ __forceinline__ float unmarked(float o) { return __float_as_uint(o) == kMade ? __builtin_nanf("") : o; }
 
+// Whether a block holds any infinity or NaN; a wave looks at it a kilobyte at a time.
+template <typename T, int D>
+__device__ __forceinline__ bool block_odd(const AttnArgs &a, int at) {
+  constexpr unsigned E = Mfma<T>::kExp;
+  const u32x4 *v = reinterpret_cast<const u32x4 *>(static_cast<const T *>(a.c.v) + static_cast<int64_t>(at) * (kBlockKeys * D));
+  bool odd = false;
+#pragma unroll 4
+  for (int i = 0; i < D / 16; ++i) {
+    const u32x4 x = v[i * 64 + (threadIdx.x & 63)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd |= (x[e] & E) == E || (x[e] & (E << 16)) == E << 16;
+  }
+  return __any(odd);
+}
+
 // Adds the infinities and NaN among the values of block `at` (its first key `first`) to o (o[i]:
 // dimension dim(i)) for the keys that a row sees.
 template <typename T, int D, int N, typename Dim>
@@ -568,7 +583,7 @@ __global__ __launch_bounds__(kThreads, D * NT > 256 ? 1 : 2) void few_rows_kerne
     for (int i = 0; i < mine; ++i) {
       const int blk = blk0 + wave + 4 * i, first = blk * kBlockKeys;
       const int at = block_at(a.c, b, head, blk);
-      if (at < 0) continue;
+      if (at < 0 || !block_odd<T, D>(a, at)) continue;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -867,7 +882,7 @@ __global__ __launch_bounds__(kThreads, (kManyHeld<D, TERMS>)) void many_rows_ker
       for (int i = 0; i < 16; ++i) o[d][i] = marked(o[d][i], total);
     for (int i = 0; i < nblk; ++i) {
       const int at = block_at(a.c, b, head, blk0 + i);
-      if (at < 0) continue;
+      if (at < 0 || !block_odd<T, D>(a, at)) continue;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         float part[16];
