@@ -7,7 +7,8 @@
  * kernels/params.h:6-32. Here the same operations are plain C functions over device
  * pointers, so an engine, ctypes (raceline/engine.py:67-125 style) or a test can call them.
  * At the end: the operators of a decoding step between those products (rotary positions with
- * the write into a paged cache, attention, adjustments of logits).
+ * the write into a paged cache, attention, the causal convolution and the gated delta rule of
+ * linear-attention layers, adjustments of logits, sampling).
  *
  * Conventions
  *  - Every pointer argument is device memory (hipMalloc'd or a torch CUDA tensor), except
@@ -405,6 +406,51 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
                   int window, float softcap, void *out, int out_stride, int out_dtype, void *workspace,
                   size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------- linear attention */
+
+/* The two operators below keep a state of each sequence in a slot of an array: slots[b] (int32 [B])
+ * is sequence b's. Rows and sequences are given by cu_q and kv_len as above (device memory): a
+ * sequence whose rows are all its tokens (kv_len[b] <= its rows) begins from a state of zeros,
+ * whatever its slot holds; one without rows leaves its slot as it is. A slot outside
+ * [0, n_slots) names no state: such a sequence begins from zeros and nothing is stored. keep[b]
+ * (int32 [B], NULL: all) is how many of the sequence's rows go into the stored state, for drafts
+ * that are taken back: their rows are computed, 0 stores nothing, and the call for what comes next
+ * goes on from the rows that were kept. No two sequences with rows may name the same slot.
+ * Rows from cu_q[B] on are neither read nor written. T at most 2^26, B at most 2^20. */
+
+/* Causal convolution of each channel with `taps` (2 .. 4) taps of its own
+ * (kernels/ops.metal:281, dispatched by src/engine.mm:1086-1154):
+ *   y_t[c] = act(bias[c] + sum_j w[c][j] x_{t - (taps-1) + j}[c]),  act = SiLU with `silu`, else none.
+ * x fp32 [T][x_stride] (a slice of the in projection's rows, say); w fp32 [channels][taps]; bias fp32
+ * [channels] or NULL; out 16-bit (out_dtype) [T][out_stride]. state fp32 [n_slots][taps-1][channels]:
+ * the last taps-1 rows of a sequence's inputs, the newest last. Sums in fp32. */
+int rlq_causal_conv(const float *x, int x_stride, int T, int channels, int taps, const float *w, const float *bias,
+                    int silu, float *state, int n_slots, const int *cu_q, const int *kv_len, const int *slots,
+                    const int *keep, int B, void *out, int out_stride, int out_dtype, void *stream);
+
+/* The gated delta rule (kernels/ops.metal:320,338,362,424, dispatched by src/engine.mm:1086-1154). For a
+ * token of value head h, with q and k of key head h / (v_heads / k_heads) and the head's S, Dk x Dv:
+ *   q^ = scale q / sqrt(q.q + eps),  k^ = k / sqrt(k.k + eps),
+ *   g = exp(-exp(a_log[h]) softplus(a[h] + dt_bias[h])),  beta = 1 / (1 + exp(-b[h])),
+ *   S = g S,  d = beta (v - S^T k^),  S = S + k^ d^T,  o = S^T q^;
+ * out = o, or with z and norm (both or neither) o / sqrt(mean o^2 + norm_eps) * norm * z / (1 + exp(-z)).
+ * q, k 16-bit (dtype) [T][stride] with k_heads * Dk elements a row, v with v_heads * Dv (slices of
+ * rlq_causal_conv's rows, say); a, b fp32 [T][stride], v_heads a row; a_log, dt_bias fp32 [v_heads]; z fp32
+ * [T][z_stride]; norm fp32 [Dv]; out 16-bit (out_dtype) [T][out_stride]. state fp32
+ * [n_slots][v_heads][Dk][Dv], 16-byte aligned. Dk 64 or 128; Dv 64, 128 or 256; v_heads a multiple of
+ * k_heads. State, products and sums in fp32; rows of q and k have lengths below 2^63.
+ * max_q (host) bounds the rows of a sequence: it chooses between the rule token by token and its form in
+ * chunks of 64 tokens, and results stay right past it. The workspace
+ * (rlq_gated_delta_workspace_bytes, may be 0; 16-byte aligned, no initialisation) holds what the chunks
+ * hand on; calls that overlap must not share it. */
+size_t rlq_gated_delta_workspace_bytes(int T, int k_heads, int v_heads, int Dk, int Dv, int B, int max_q);
+int rlq_gated_delta(const void *q, int q_stride, const void *k, int k_stride, const void *v, int v_stride, int T,
+                    int k_heads, int v_heads, int Dk, int Dv, int dtype, const float *a, int a_stride, const float *b,
+                    int b_stride, const float *a_log, const float *dt_bias, float eps, float scale, const float *z,
+                    int z_stride, const float *norm, float norm_eps, float *state, int n_slots, const int *cu_q,
+                    const int *kv_len, const int *slots, const int *keep, int B, int max_q, void *out, int out_stride,
+                    int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------- logits */
 
 /* Adjusts rows of logits before a token is chosen from them (rl_top_k_device, rl_argmax); out may
@@ -424,6 +470,26 @@ int rlq_adjust_logits(const float *logits, int64_t stride, int rows, int vocab, 
                       const float *repetition, const float *presence, const float *frequency, const int *bias_ids,
                       const float *bias, int n_bias, int64_t bias_stride, const uint32_t *allowed,
                       int64_t allowed_stride, float *out, int64_t out_stride, void *stream);
+
+/* A token from each row of logits (rl_head's, or rlq_adjust_logits's out) and a number from [0, 1)
+ * given for the row. With l the row's logits and T its temperature, token v weighs
+ * w_v = exp((l_v - max l) / T). The row's tokens in falling order of l, equal ones by rising
+ * index, are cut to the first top_k; of these to the shortest prefix that has at least top_p of their
+ * weight (one token at least); of these to those with w_v >= min_p. The token is the first in order
+ * of index up to which the kept tokens have more than `uniform` of their weight.
+ * uniform fp64 [rows]; temperature fp32 [rows] (NULL: 1; 0 or less: the largest logit is taken, the
+ * first of equal ones), top_k int32 [rows] (NULL, 0 or less: all), top_p fp32 [rows] (NULL, 1 or
+ * more: all), min_p fp32 [rows] (NULL, 0 or less: all; 1 or more: those equal to the largest); NaN
+ * is as NULL, for the temperature as 0. tokens int32 [rows]; probs fp32 [rows] or NULL: the token's share of the
+ * kept weight. Logits of -inf and NaN are never taken; a row of nothing else gives token -1 and
+ * share 0. Weights are formed in fp64 and summed as whole numbers of steps of 2^-(62 - ceil(log2 vocab))
+ * of the largest: the same row gives the same token in every call. vocab at most 2^22.
+ * The workspace (rlq_sample_workspace_bytes; 16-byte aligned, no initialisation) must not be shared by
+ * calls that overlap. */
+size_t rlq_sample_workspace_bytes(int rows, int vocab);
+int rlq_sample(const float *logits, int64_t stride, int rows, int vocab, const double *uniform,
+               const float *temperature, const int *top_k, const float *top_p, const float *min_p, int *tokens,
+               float *probs, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

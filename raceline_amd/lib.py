@@ -88,6 +88,16 @@ SIGNATURES = {
     "rlq_adjust_logits": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64,
                                   c_void_p, c_int64, c_void_p]),
+    "rlq_causal_conv": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p]),
+    "rlq_gated_delta_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "rlq_gated_delta": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                                c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_float, c_float, c_void_p,
+                                c_int, c_void_p, c_float, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                c_int, c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "rlq_sample_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "rlq_sample": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                           c_void_p, c_void_p, c_size_t, c_void_p]),
     # include/rl_engine.h: the model file reader and the engine layer
     "rlm_open": (c_void_p, [c_char_p]),
     "rlm_close": (None, [c_void_p]),

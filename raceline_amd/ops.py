@@ -708,6 +708,150 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_
     return out
 
 
+# ------------------------------------------------------------------ linear attention
+
+def _check_sequences(cu_q, kv_len, slots, keep, dev):
+    """Types, shapes and places of the sequences of a call with states -> B."""
+    i32 = torch.int32
+    if cu_q.dtype is not i32 or kv_len.dtype is not i32 or slots.dtype is not i32 or (
+            keep is not None and keep.dtype is not i32):
+        raise TypeError("cu_q, kv_len, slots and keep must be int32")
+    B = kv_len.numel()
+    if kv_len.shape != (B,) or cu_q.shape != (B + 1,) or slots.shape != (B,) or not (
+            cu_q.is_contiguous() and kv_len.is_contiguous() and slots.is_contiguous()):
+        raise ValueError("kv_len and slots must be contiguous vectors [B], cu_q [B + 1]")
+    if keep is not None and (keep.shape != (B,) or not keep.is_contiguous() or keep.get_device() != dev):
+        raise ValueError("keep must be a contiguous vector [B] on the device of the call's other tensors")
+    if cu_q.get_device() != dev or kv_len.get_device() != dev or slots.get_device() != dev:
+        raise ValueError("the sequences must be on the device of the call's other tensors")
+    return B
+
+
+def conv_state(n_slots: int, channels: int, taps: int = 4, device="cuda") -> torch.Tensor:
+    """The states of causal_conv, [n_slots][taps - 1][channels] fp32. They need no filling: a sequence
+    begins from zeros."""
+    return torch.empty((n_slots, taps - 1, channels), dtype=torch.float32, device=device)
+
+
+def delta_state(n_slots: int, v_heads: int, k_dim: int, v_dim: int, device="cuda") -> torch.Tensor:
+    """The states of gated_delta, [n_slots][v_heads][k_dim][v_dim] fp32. They need no filling either."""
+    return torch.empty((n_slots, v_heads, k_dim, v_dim), dtype=torch.float32, device=device)
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+                slots: torch.Tensor, bias: torch.Tensor | None = None, silu: bool = True,
+                keep: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.float16, stream=None) -> torch.Tensor:
+    """The short causal convolution of a linear-attention layer (rlq_causal_conv): rows x fp32
+    [T][channels] (a slice of the in projection's rows, say) with weight fp32 [channels][taps] ->
+    [T][channels] in out_dtype, and the sequences' last inputs in state (conv_state), in place.
+    cu_q and kv_len as for rope_append; slots int32 [B]: the states' places, one outside the array for
+    none. A sequence whose rows are all its tokens begins from zeros. keep int32 [B]: how many of a
+    sequence's rows go into its state (all by default; a draft's rows are computed with 0, then again
+    with what was taken). Rows from cu_q[B] on are left as they were in `out`."""
+    f32, dev = torch.float32, state.get_device()
+    T, C, xs = _rows(x, f32, dev, "x")
+    if weight.dtype is not f32 or weight.dim() != 2 or weight.shape[0] != C or not weight.is_contiguous() or (
+            weight.get_device() != dev):
+        raise ValueError(f"weight must be a contiguous float32 matrix [{C}][taps] on the state's device")
+    taps = weight.shape[1]
+    if bias is not None and (bias.dtype is not f32 or bias.shape != (C,) or not bias.is_contiguous() or (
+            bias.get_device() != dev)):
+        raise ValueError(f"bias must be a contiguous float32 vector of {C} on the state's device")
+    if state.dtype is not f32 or state.dim() != 3 or state.shape[1:] != (taps - 1, C) or not state.is_contiguous():
+        raise ValueError(f"state must be contiguous float32 [n_slots][{taps - 1}][{C}]")
+    B = _check_sequences(cu_q, kv_len, slots, keep, dev)
+    if out is None:
+        out = _new(x, (T, C), out_dtype, stream)
+        os = C
+    else:
+        To, ow, os = _rows(out, out.dtype, dev, "out")
+        if To != T or ow != C:
+            raise ValueError("out must be shaped like x")
+    out_code = _CODES.get(out.dtype)
+    if out_code is None:
+        raise ValueError(f"out must be float16 or bfloat16, not {out.dtype}")
+    _call_on(dev, stream, "rlq_causal_conv", x.data_ptr(), xs, T, C, taps, weight.data_ptr(), _ptr(bias),
+             1 if silu else 0, state.data_ptr(), state.shape[0], cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(),
+             _ptr(keep), B, out.data_ptr(), os, out_code)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def gated_delta_workspace_bytes(T: int, k_heads: int, v_heads: int, k_dim: int, v_dim: int, B: int, max_q: int) -> int:
+    return int(lib.load().rlq_gated_delta_workspace_bytes(T, k_heads, v_heads, k_dim, v_dim, B, max_q))
+
+
+def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                a_log: torch.Tensor, dt_bias: torch.Tensor, state: torch.Tensor, cu_q: torch.Tensor,
+                kv_len: torch.Tensor, slots: torch.Tensor, max_q: int, scale: float | None = None, eps: float = 1e-6,
+                z: torch.Tensor | None = None, norm: torch.Tensor | None = None, norm_eps: float = 1e-6,
+                keep: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.float16, workspace: torch.Tensor | None = None,
+                stream=None) -> torch.Tensor:
+    """The gated delta rule of a linear-attention layer (rlq_gated_delta): rows q, k [T][k_heads * k_dim]
+    and v [T][v_heads * v_dim] (float16 or bfloat16, slices of causal_conv's rows, say) with a, b fp32
+    [T][v_heads] and a_log, dt_bias fp32 [v_heads] -> [T][v_heads * v_dim] in out_dtype, and state
+    (delta_state) updated in place. q and k are brought to length 1 here, q times scale
+    (1 / sqrt(k_dim) by default). z fp32 [T][v_heads * v_dim] and norm fp32 [v_dim]: the rows' heads
+    normalised and gated for the out projection. max_q bounds a sequence's rows; cu_q, kv_len, slots and keep
+    as for causal_conv. workspace: scratch to use in place of a new tensor; calls that overlap must
+    not share it. Rows from cu_q[B] on are left as they were in `out`."""
+    f32, dev, shape = torch.float32, state.get_device(), state.shape
+    if state.dtype is not f32 or len(shape) != 4 or not state.is_contiguous():
+        raise ValueError("state must be contiguous float32 [n_slots][v_heads][k_dim][v_dim]")
+    n_slots, Hv, Dk, Dv = shape
+    code = _CODES.get(q.dtype)
+    if code is None:
+        raise ValueError(f"q, k and v must be float16 or bfloat16, not {q.dtype}")
+    T, width, qs = _rows(q, q.dtype, dev, "q")
+    Tk, kw, ks = _rows(k, q.dtype, dev, "k")
+    Tv, vw, vs = _rows(v, q.dtype, dev, "v")
+    Ta, aw, as_ = _rows(a, f32, dev, "a")
+    Tb, bw, bs = _rows(b, f32, dev, "b")
+    if Tk != T or Tv != T or kw != width or vw != Hv * Dv or not width or width % max(Dk, 1):
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match states of "
+                         f"{Hv} heads of {Dk} x {Dv}")
+    if Ta != T or Tb != T or aw != Hv or bw != Hv:
+        raise ValueError(f"a and b must be [{T}][{Hv}]")
+    for t, n, what in ((a_log, Hv, "a_log"), (dt_bias, Hv, "dt_bias"), (norm, Dv, "norm")):
+        if t is not None and (t.dtype is not f32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != dev):
+            raise ValueError(f"{what} must be a contiguous float32 vector of {n} on the state's device")
+    if (z is None) != (norm is None):
+        raise ValueError("z and norm come together")
+    zs = 0
+    if z is not None:
+        Tz, zw, zs = _rows(z, f32, dev, "z")
+        if Tz != T or zw != Hv * Dv:
+            raise ValueError("z must be shaped like v")
+    B = _check_sequences(cu_q, kv_len, slots, keep, dev)
+    if out is None:
+        out = _new(q, (T, Hv * Dv), out_dtype, stream)
+        os = Hv * Dv
+    else:
+        To, ow, os = _rows(out, out.dtype, dev, "out")
+        if To != T or ow != Hv * Dv:
+            raise ValueError("out must be shaped like v")
+    out_code = _CODES.get(out.dtype)
+    if out_code is None:
+        raise ValueError(f"out must be float16 or bfloat16, not {out.dtype}")
+    max_q = min(max_q, 2**31 - 1)
+    nbytes = gated_delta_workspace_bytes(T, width // Dk, Hv, Dk, Dv, B, max_q)
+    if workspace is None:
+        if nbytes:
+            workspace = _new(q, nbytes, torch.uint8, stream, scratch=True)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous, on the state's device")
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+    _call_on(dev, stream, "rlq_gated_delta", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, T, width // Dk, Hv, Dk,
+             Dv, code, a.data_ptr(), as_, b.data_ptr(), bs, a_log.data_ptr(), dt_bias.data_ptr(), eps,
+             Dk ** -0.5 if scale is None else scale, _ptr(z), zs, _ptr(norm), norm_eps, state.data_ptr(), n_slots,
+             cu_q.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), _ptr(keep), B, max_q, out.data_ptr(), os, out_code,
+             _ptr(workspace), nbytes)
+    return out
+
+
 # ------------------------------------------------------------------ logits
 
 def _row_vector(t, rows, dtype, what, dev) -> int:
@@ -774,4 +918,41 @@ def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, n_to
              _row_vector(repetition, rows, torch.float32, "repetition", dev),
              _row_vector(presence, rows, torch.float32, "presence", dev),
              _row_vector(frequency, rows, torch.float32, "frequency", dev), ip, bp, nb, bs, mp, ms, out.data_ptr(), ys)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    return int(lib.load().rlq_sample_workspace_bytes(rows, vocab))
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None,
+           top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+           out: torch.Tensor | None = None, probs: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+           stream=None) -> torch.Tensor:
+    """A token from each row of logits (fp32 [rows][vocab], adjust_logits's out, say) and a number of
+    [0, 1) given for it (uniform, fp64 [rows]) -> int32 [rows] (rlq_sample). temperature, top_p and min_p
+    fp32 [rows], top_k int32 [rows]; None: 1 and all tokens. Temperature 0 takes the largest logit.
+    Cut to the top_k, of these to the shortest prefix of top_p of the weight, of these to min_p of
+    the largest weight. probs (fp32 [rows]) gets the tokens' shares of the kept weight. A row without a logit
+    above -inf gives -1. workspace: scratch to use in place of a new tensor; calls that overlap must
+    not share it."""
+    dev = logits.get_device()
+    rows, vocab, xs = _rows(logits, torch.float32, dev, "logits")
+    f32, i32 = torch.float32, torch.int32
+    if out is None:
+        out = _new(logits, (rows,), i32, stream)
+    nbytes = sample_workspace_bytes(rows, vocab)
+    if workspace is None:
+        if nbytes:
+            workspace = _new(logits, nbytes, torch.uint8, stream, scratch=True)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous, on the logits' device")
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+    _call_on(dev, stream, "rlq_sample", logits.data_ptr(), xs, rows, vocab,
+             _row_vector(uniform, rows, torch.float64, "uniform", dev),
+             _row_vector(temperature, rows, f32, "temperature", dev), _row_vector(top_k, rows, i32, "top_k", dev),
+             _row_vector(top_p, rows, f32, "top_p", dev), _row_vector(min_p, rows, f32, "min_p", dev),
+             _row_vector(out, rows, i32, "out", dev), _row_vector(probs, rows, f32, "probs", dev), _ptr(workspace), nbytes)
     return out
