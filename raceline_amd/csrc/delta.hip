@@ -5,6 +5,7 @@
 #include "paged.h"
 #include "../../include/rlq.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace rlq {
@@ -179,8 +180,628 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
   }
 }
 
+// ------------------------------------------------------------------ chunks of 64 tokens
+
+// With G_i the sum of log g up to row i of a chunk, L_ij = beta_i e^(G_i - G_j) k_i.k_j below the diagonal and
+// S the state in front of the chunk, the rule over the chunk's rows is
+//   R = beta (V - e^G (K S)),   U = (I + L)^-1 R,
+//   O = e^G (Q S) + P U,        P_ij = e^(G_i - G_j) q_i.k_j on and below the diagonal,
+//   S <- e^(G_64) S + (e^(G_64 - G) K)^T U.
+// delta_chunks_kernel forms what does not depend on S, of all chunks at once: T = (I + L)^-1, P, and the rows
+// as operands. delta_chain_kernel goes through a sequence's chunks with S.
+//
+// The products are to keep the state to fp32: rows of q and k, brought to a length of 2^13 .. 2^14 by a power of
+// two, are exact in fp16 (what bf16 loses there lies 2^-38 below the length); T, P, R, U and S are two fp16
+// terms (2^-22), T and P, at most 1, times 2^14, so that what has faded keeps its bits. Operands stand in the order in which sums leave the matrix cores: slot 8 h + 4 a + b of a step of
+// 32 is row 16 a + 4 h + b, so that what a lane holds of a result is what it holds of the next product.
+
+constexpr int kChunk = 64, kChunkThreads = 256, kHeadsPer = 2, kMatPad = 68;
+constexpr int kBlock = 64 * 8;                       // halves of a 16 x 32 operand
+constexpr float kUnit = 16384.0f, kLength = 8192.0f; // T and P are held times kUnit, rows of q and k at this length or twice it
+constexpr int64_t kMostScratch = 256 << 20;
+
+// What a chunk leaves for the chain, in bytes from its place.
+struct ChunkLayout {
+  int dk, k_heads, v_heads, dv;
+  __host__ __device__ int64_t k_head() const { return 3 * kChunk * dk * 2; }       // K, Q, K^T
+  __host__ __device__ int64_t v_head() const { return 4 * 8 * kBlock * 2 + 5 * kChunk * 4; }   // T, P (two terms), factors
+  __host__ __device__ int64_t rows_at() const { return k_heads * k_head() + v_heads * v_head(); }
+  __host__ __device__ int64_t bytes() const { return rows_at() + (int64_t)kChunk * v_heads * dv * 4; }
+  __host__ __device__ int64_t state() const { return (int64_t)v_heads * dk * dv * 4; }
+};
+
+struct ChunkArgs {
+  DeltaArgs d;
+  ChunkLayout at;
+  char *chunks;       // of the chunks first .. first + count - 1
+  float *carry[2];    // states that go from one run of chunks to the next
+  int first, count, run;
+};
+
+struct Chunk {
+  int start, rows;
+};
+
+// A sequence's rows up to the kept ones, then the others, in chunks.
+__device__ __forceinline__ int kept_rows(const DeltaArgs &a, int b, int n) {
+  const int slot = a.slots[b], kept = a.keep ? a.keep[b] : n;
+  return slot >= 0 && slot < a.n_slots && kept > 0 && kept < n ? kept : n;
+}
+
+__device__ __forceinline__ int chunks_of(int n, int kept) {
+  return (kept + kChunk - 1) / kChunk + (n - kept + kChunk - 1) / kChunk;
+}
+
+__device__ __forceinline__ Chunk chunk_of(int n, int kept, int item) {
+  const int head = (kept + kChunk - 1) / kChunk;
+  const int start = item < head ? item * kChunk : kept + (item - head) * kChunk;
+  return {start, min(kChunk, (item < head ? kept : n) - start)};
+}
+
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+
+// x as two fp16 terms. The barrier keeps the product that x may come from out of the conversion: fused, it
+// is rounded once, and where that differs the second term was that of another first one (one value in
+// ten thousand was off by 2^-11).
+__device__ __forceinline__ void split(const float (&x)[4], half4 &high, half4 &low) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v = x[i];
+    asm("" : "+v"(v));
+    high[i] = static_cast<_Float16>(v);
+    low[i] = static_cast<_Float16>(v - static_cast<float>(high[i]));
+  }
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p) {
+  constexpr int kPad = DK + 8, kSteps = DK / 32, kPer = DK / 4;
+  const DeltaArgs &a = p.d;
+  __shared__ __align__(16) _Float16 ks[kChunk][kPad], qs[kChunk][kPad];
+  __shared__ __align__(16) float kk[kChunk][kMatPad], qk[kChunk][kMatPad], m[kChunk][kMatPad];
+  __shared__ double total[kChunk];
+  __shared__ float rk[kChunk], rq[kChunk], beta[kChunk];
+
+  const Sequence s = find_sequence(a.c, p.first + blockIdx.x, 1, kChunk, 2);
+  if (s.b < 0 || s.tokens <= 0) return;
+  const int kept = kept_rows(a, s.b, s.tokens);
+  if (s.item >= chunks_of(s.tokens, kept)) return;
+  const Chunk c = chunk_of(s.tokens, kept, s.item);
+  const int group = a.v_heads / a.k_heads, parts = (group + kHeadsPer - 1) / kHeadsPer;
+  const int k_head = blockIdx.y / parts, part = blockIdx.y - k_head * parts;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row0 = s.row0 + c.start;
+  char *place = p.chunks + blockIdx.x * p.at.bytes();
+
+  {  // rows to lengths of 2^13 .. 2^14, in fp16; four threads a row
+    const int row = tid >> 2, d0 = (tid & 3) * kPer;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float x[kPer], sum = 0.0f;
+      if (row < c.rows) {
+        const T *from = which ? static_cast<const T *>(a.q) + (row0 + row) * a.q_stride
+                              : static_cast<const T *>(a.k) + (row0 + row) * a.k_stride;
+        load_narrow<T, kPer>(from + k_head * DK + d0, a.wide, x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += x[i] * x[i];
+      sum += dpp<0xB1>(sum);
+      sum += dpp<0x4E>(sum);
+      // the power of two that brings the length to 2^13 .. 2^14, and back
+      const int ex = max(14, min(253, (int)(__float_as_uint(sqrtf(sum)) >> 23)));
+      const float up = __uint_as_float((254 + 13 - ex) << 23), down = __uint_as_float((ex - 13) << 23);
+      _Float16 *to = which ? &qs[row][d0] : &ks[row][d0];
+#pragma unroll
+      for (int i = 0; i < kPer; i += 8) {
+        half8 y;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = static_cast<_Float16>(x[i + j] * up);
+        *reinterpret_cast<half8 *>(to + i) = y;
+      }
+      if ((tid & 3) == 0) (which ? rq : rk)[row] = down / sqrtf(sum + a.eps);
+    }
+  }
+  __syncthreads();
+  {  // K K^T and Q K^T, 16 rows a wave
+    f32x4 ck[4] = {}, cq[4] = {};
+    const int r = lane & 15, h = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      const half8 ka = *reinterpret_cast<const half8 *>(&ks[wave * 16 + r][t * 32 + h * 8]);
+      const half8 qa = *reinterpret_cast<const half8 *>(&qs[wave * 16 + r][t * 32 + h * 8]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const half8 kb = *reinterpret_cast<const half8 *>(&ks[n * 16 + r][t * 32 + h * 8]);
+        ck[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, kb, ck[n], 0, 0, 0);
+        cq[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa, kb, cq[n], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        kk[wave * 16 + h * 4 + i][n * 16 + r] = ck[n][i];
+        qk[wave * 16 + h * 4 + i][n * 16 + r] = cq[n][i];
+      }
+  }
+  if (part == 0) {  // the rows as operands
+    _Float16 *to = reinterpret_cast<_Float16 *>(place + k_head * p.at.k_head());
+    for (int i = tid; i < 4 * kSteps * 64; i += kChunkThreads) {
+      const int l = i & 63, t = (i >> 6) % kSteps, tile = (i >> 6) / kSteps, row = tile * 16 + (l & 15);
+      const int d = t * 32 + (l >> 4) * 4;
+      const half4 k0 = *reinterpret_cast<const half4 *>(&ks[row][d]), k1 = *reinterpret_cast<const half4 *>(&ks[row][d + 16]);
+      const half4 q0 = *reinterpret_cast<const half4 *>(&qs[row][d]), q1 = *reinterpret_cast<const half4 *>(&qs[row][d + 16]);
+      *reinterpret_cast<half8 *>(to + i * 8) = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
+      *reinterpret_cast<half8 *>(to + kChunk * DK + i * 8) = __builtin_shufflevector(q0, q1, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    for (int i = tid; i < (DK / 16) * 2 * 64; i += kChunkThreads) {
+      const int l = i & 63, t = (i >> 6) & 1, d = (i >> 7) * 16 + (l & 15), row = t * 32 + (l >> 4) * 4;
+      half8 y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = ks[row + (e >> 2) * 16 + (e & 3)][d];
+      *reinterpret_cast<half8 *>(to + 2 * kChunk * DK + i * 8) = y;
+    }
+  }
+  for (int v = part * kHeadsPer; v < min(group, (part + 1) * kHeadsPer); ++v) {
+    const int head = k_head * group + v;
+    char *mine = place + p.at.k_heads * p.at.k_head() + head * p.at.v_head();
+    _Float16 *to = reinterpret_cast<_Float16 *>(mine);
+    float *factors = reinterpret_cast<float *>(mine + 4 * 8 * kBlock * 2);
+    __syncthreads();
+    if (wave == 0) {
+      // sums of logarithms in 64 bits: what they differ by between rows that forget little is to be exact
+      // beside rows that forget all (e^-128 is nothing in fp32)
+      double sum = 0.0;
+      float w = 0.0f;
+      if (lane < c.rows) {
+        const float x = log_fade(a.a[(row0 + lane) * a.a_stride + head], a.dt_bias[head], expf(a.a_log[head]));
+        sum = x < -128.0f ? -128.0f : x;
+        w = sigmoid(a.b[(row0 + lane) * a.b_stride + head]);
+      }
+      for (int off = 1; off < 64; off <<= 1) {
+        const double o = __shfl_up(sum, off);
+        if (lane >= off) sum += o;
+      }
+      total[lane] = sum;
+      beta[lane] = w;
+      const double last = __shfl(sum, 63);
+      const float fade = expf(static_cast<float>(sum));
+      factors[lane] = w;
+      factors[kChunk + lane] = w * fade * rk[lane];
+      factors[2 * kChunk + lane] = rk[lane] * kLength * expf(static_cast<float>(last - sum));
+      factors[3 * kChunk + lane] = rq[lane] * fade;
+      factors[4 * kChunk + lane] = expf(static_cast<float>(last));
+    }
+    __syncthreads();
+    {  // L, and P as operands: sixteen columns of one row a thread
+      const int i = tid >> 2, m0 = (tid & 3) * 16;
+      const double ti = total[i];
+      const float bi = beta[i] * rk[i], qi = rq[i] * kUnit;
+      _Float16 *block = to + 2 * 8 * kBlock + ((i >> 4) * 2 + (m0 >> 5)) * kBlock + (i & 15) * 8 + (m0 >> 4 & 1) * 4;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        float x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = m0 + h * 4 + e;
+          const float f = j <= i ? expf(static_cast<float>(ti - total[j])) * rk[j] : 0.0f;
+          x[e] = j < i ? bi * f * kk[i][j] : 0.0f;
+          y[e] = j <= i ? qi * f * qk[i][j] : 0.0f;
+        }
+        *reinterpret_cast<f32x4 *>(&m[i][m0 + h * 4]) = f32x4{x[0], x[1], x[2], x[3]};
+        half4 high, low;
+        split(y, high, low);
+        *reinterpret_cast<half4 *>(block + h * 128) = high;
+        *reinterpret_cast<half4 *>(block + 8 * kBlock + h * 128) = low;
+      }
+    }
+    __syncthreads();
+    const int r = lane & 15, h = lane >> 4;
+    {  // the inverses of the 16 x 16 blocks on the diagonal, one a wave: a lane solves for column r
+      float x[16];
+      const int at = wave * 16;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float sum = i == r ? 1.0f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < i; ++j) sum -= m[at + i][at + j] * x[j];
+        x[i] = sum;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (h == i >> 2) m[at + i][at + r] = x[i];
+    }
+    __syncthreads();
+    // -T22 (L21 T11) joins two inverses; in fp32 products of 16 x 16 x 4, whose result is the second's operand
+    auto times = [&](int row, int col, const f32x4 &right, f32x4 sum) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m[row * 16 + r][col * 16 + h * 4 + e], right[e], sum, 0, 0, 0);
+      return sum;
+    };
+    auto block_at_ = [&](int row, int col) {
+      return f32x4{m[row * 16 + h * 4][col * 16 + r], m[row * 16 + h * 4 + 1][col * 16 + r],
+                   m[row * 16 + h * 4 + 2][col * 16 + r], m[row * 16 + h * 4 + 3][col * 16 + r]};
+    };
+    auto put = [&](int row, int col, const f32x4 &x) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m[row * 16 + h * 4 + e][col * 16 + r] = -x[e];
+    };
+    if (wave < 2) {
+      const int at = wave * 2;
+      const f32x4 x = times(at + 1, at, block_at_(at, at), f32x4{});
+      put(at + 1, at, times(at + 1, at + 1, x, f32x4{}));
+    }
+    __syncthreads();
+    f32x4 low0 = {}, low1 = {};
+    if (wave < 2) {
+      const f32x4 t0 = wave ? f32x4{} : block_at_(0, 0), t1 = block_at_(1, wave);
+      const f32x4 x0 = times(2, 1, t1, times(2, 0, t0, f32x4{})), x1 = times(3, 1, t1, times(3, 0, t0, f32x4{}));
+      low0 = times(2, 2, x0, f32x4{});
+      low1 = times(3, 3, x1, times(3, 2, x0, f32x4{}));
+    }
+    __syncthreads();
+    if (wave < 2) put(2, wave, low0), put(3, wave, low1);
+    __syncthreads();
+    {
+      const int i = tid >> 2, m0 = (tid & 3) * 16;
+      _Float16 *block = to + ((i >> 4) * 2 + (m0 >> 5)) * kBlock + (i & 15) * 8 + (m0 >> 4 & 1) * 4;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(&m[i][m0 + g * 4]);
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = m0 + g * 4 + e <= i ? y[e] * kUnit : 0.0f;
+        half4 high, low;
+        split(x, high, low);
+        *reinterpret_cast<half4 *>(block + g * 128) = high;
+        *reinterpret_cast<half4 *>(block + 8 * kBlock + g * 128) = low;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float most_of_wave(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));
+  x = fmaxf(x, dpp<0x4E>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  x = fmaxf(x, dpp<0x128>(x));
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// What a wave reads of a chunk: its 16 rows of the rows' products, its rows of the state's.
+template <int DK>
+struct ChunkOperands {
+  half8 k[DK / 32], q[DK / 32], kt[DK / 64][2], t[2][2], p[2][2];   // t, p: term, step
+  f32x4 take, seen, left, read;                                      // factors of its rows of V, K S, U, Q S
+  float v[4], fade;
+};
+
+// A workgroup goes through a sequence's chunks with 16 columns of one head's state: a wave has 16 of a chunk's rows
+// and a quarter of the state's, and S, R and U go between the waves as operands in LDS.
+// Values are held times a power of two that keeps them in fp16's range: with keys of length 1 and beta at most 1
+// a column of S is never longer than what its square and those of the values v add up to, and R and U never larger
+// than S and 9 of the largest v.
+template <typename T, typename TO, int DK>
+__global__ __launch_bounds__(kChunkThreads) void delta_chain_kernel(ChunkArgs p) {
+  constexpr int kSteps = DK / 32, kTiles = DK / 64;   // steps over the state's rows, tiles of 16 of them a wave has
+  const DeltaArgs &a = p.d;
+  __shared__ __align__(16) _Float16 sb[2][kSteps][64][8], rb[2][2][64][8], ub[2][2][64][8], wb[2][2][64][8];
+  __shared__ float most[2][4];
+
+  // workgroups of one head run on one XCD, whose L2 then holds its chunk for all of them
+  const int slices = a.dv / 16, xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
+  const int slice = rest % slices;
+  const int64_t pair = static_cast<int64_t>(rest / slices) * 8 + xcd;
+  if (pair >= static_cast<int64_t>(a.c.batch) * a.v_heads) return;
+  const int b = static_cast<int>(pair / a.v_heads), head = static_cast<int>(pair - static_cast<int64_t>(b) * a.v_heads);
+  const int row0 = row_start(a.c, b), n = row_start(a.c, b + 1) - row0;
+  if (n <= 0) return;
+  const int kept = kept_rows(a, b, n), chunks = chunks_of(n, kept), kept_chunks = (kept + kChunk - 1) / kChunk;
+  const int64_t base = first_item(row0, b, 1, kChunk, 2);
+  const int c0 = static_cast<int>(max((int64_t)0, p.first - base));
+  const int c1 = static_cast<int>(min((int64_t)chunks, p.first + p.count - base));
+  if (c0 >= c1) return;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, h = lane >> 4;
+  const int k_head = head / (a.v_heads / a.k_heads), slot = a.slots[b], col = slice * 16 + r;
+  const bool has_state = slot >= 0 && slot < a.n_slots;
+  const int64_t in_state = (static_cast<int64_t>(head) * DK + wave * 16 * kTiles + h * 4) * a.dv + col;
+  float *state = has_state ? a.state + static_cast<int64_t>(slot) * a.v_heads * DK * a.dv + in_state : nullptr;
+
+  float s[kTiles][4], size = 0.0f;   // size: a bound of the length of a column of S
+  {
+    const float *from = c0 ? p.carry[p.run & 1] + in_state : has_state && cached(a.c, b) > n ? state : nullptr;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[t][i] = from ? from[(t * 16 + i) * a.dv] : 0.0f;
+        size = fmaxf(size, fabsf(s[t][i]));
+      }
+  }
+  const T *values = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + col;
+
+  auto load = [&](int at, ChunkOperands<DK> &o) {
+    const Chunk c = chunk_of(n, kept, at);
+    const int row = wave * 16 + h * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o.v[i] = row + i < c.rows ? static_cast<float>(values[(c.start + row + i) * a.v_stride]) : 0.0f;
+    const char *place = p.chunks + (base + at - p.first) * p.at.bytes();
+    const _Float16 *rows = reinterpret_cast<const _Float16 *>(place + k_head * p.at.k_head()) + lane * 8;
+    const char *mine = place + p.at.k_heads * p.at.k_head() + head * p.at.v_head();
+    const _Float16 *mats = reinterpret_cast<const _Float16 *>(mine) + lane * 8;
+    const float *factors = reinterpret_cast<const float *>(mine + 4 * 8 * kBlock * 2);
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      o.k[t] = *reinterpret_cast<const half8 *>(rows + (wave * kSteps + t) * kBlock);
+      o.q[t] = *reinterpret_cast<const half8 *>(rows + kChunk * DK + (wave * kSteps + t) * kBlock);
+    }
+    o.take = *reinterpret_cast<const f32x4 *>(factors + row);
+    o.seen = *reinterpret_cast<const f32x4 *>(factors + kChunk + row);
+    o.left = *reinterpret_cast<const f32x4 *>(factors + 2 * kChunk + row);
+    o.read = *reinterpret_cast<const f32x4 *>(factors + 3 * kChunk + row);
+    o.fade = factors[4 * kChunk];
+#pragma unroll
+    for (int term = 0; term < 2; ++term)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (t > wave >> 1) continue;               // above the diagonal
+        o.t[term][t] = *reinterpret_cast<const half8 *>(mats + (term * 8 + wave * 2 + t) * kBlock);
+        o.p[term][t] = *reinterpret_cast<const half8 *>(mats + (16 + term * 8 + wave * 2 + t) * kBlock);
+      }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        o.kt[t][u] = *reinterpret_cast<const half8 *>(rows + 2 * kChunk * DK + ((wave * kTiles + t) * 2 + u) * kBlock);
+  };
+  auto most_value = [&](const ChunkOperands<DK> &o) {
+    return most_of_wave(fmaxf(fmaxf(fabsf(o.v[0]), fabsf(o.v[1])), fmaxf(fabsf(o.v[2]), fabsf(o.v[3]))));
+  };
+  auto of_waves = [&](int which) { return fmaxf(fmaxf(most[which][0], most[which][1]), fmaxf(most[which][2], most[which][3])); };
+  // the power of two that brings what is below `x` under 2^15, and its inverse
+  auto scale_of = [&](float x, float &inverse) {
+    const int ex = max(40, min(254, (int)(__float_as_uint(x) >> 23)));
+    inverse = __uint_as_float((ex - 14) << 23);
+    return __uint_as_float((268 - ex) << 23);
+  };
+  auto give = [&](_Float16 (&to)[2][2][64][8], const float (&x)[4]) {
+    half4 high, low;
+    split(x, high, low);
+    *reinterpret_cast<half4 *>(&to[0][wave >> 1][lane][(wave & 1) * 4]) = high;
+    *reinterpret_cast<half4 *>(&to[1][wave >> 1][lane][(wave & 1) * 4]) = low;
+  };
+  auto give_state = [&]() {
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      half4 high, low;
+      split(s[t], high, low);
+      const int part = wave * kTiles + t;
+      *reinterpret_cast<half4 *>(&sb[0][part >> 1][lane][(part & 1) * 4]) = high;
+      *reinterpret_cast<half4 *>(&sb[1][part >> 1][lane][(part & 1) * 4]) = low;
+    }
+  };
+
+  ChunkOperands<DK> now, next;
+  load(c0, now);
+  {
+    const float x = most_of_wave(size), y = most_value(now);
+    if (lane == 0) most[0][wave] = x, most[1][wave] = y;
+  }
+  __syncthreads();
+  size = of_waves(0) * (DK == 128 ? 11.32f : 8.0f);
+  float value = of_waves(1), inverse, scale = scale_of(size + 9.0f * value, inverse);
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] *= scale;
+  give_state();
+  __syncthreads();
+
+  auto step = [&](int at, const ChunkOperands<DK> &now, ChunkOperands<DK> &next) {
+    const bool more = at + 1 < c1;
+    if (more) load(at + 1, next);
+    f32x4 ks = {}, ks_low = {}, qs = {}, qs_low = {};
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      const half8 high = *reinterpret_cast<const half8 *>(&sb[0][t][lane][0]);
+      const half8 low = *reinterpret_cast<const half8 *>(&sb[1][t][lane][0]);
+      ks = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.k[t], high, ks, 0, 0, 0);
+      ks_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.k[t], low, ks_low, 0, 0, 0);
+      qs = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.q[t], high, qs, 0, 0, 0);
+      qs_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.q[t], low, qs_low, 0, 0, 0);
+    }
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = now.take[i] * (now.v[i] * scale) - now.seen[i] * (ks[i] + ks_low[i]);
+    give(rb, x);
+    __syncthreads();
+
+    f32x4 u = {}, u_low = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t > wave >> 1) continue;
+      const half8 high = *reinterpret_cast<const half8 *>(&rb[0][t][lane][0]);
+      const half8 low = *reinterpret_cast<const half8 *>(&rb[1][t][lane][0]);
+      u = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.t[0][t], high, u, 0, 0, 0);
+      u_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.t[0][t], low, u_low, 0, 0, 0);
+      u_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.t[1][t], high, u_low, 0, 0, 0);
+    }
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = (u[i] + u_low[i]) * (1.0f / kUnit);
+      w[i] = now.left[i] * x[i];
+    }
+    give(ub, x);
+    give(wb, w);
+    if (more) {
+      const float y = most_value(next);
+      if (lane == 0) most[at & 1][wave] = y;
+    }
+    __syncthreads();
+
+    // the state first: the next chunk waits for it
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      f32x4 sum, sum_low = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = now.fade * kLength * s[t][i];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const half8 high = *reinterpret_cast<const half8 *>(&wb[0][e][lane][0]);
+        const half8 low = *reinterpret_cast<const half8 *>(&wb[1][e][lane][0]);
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.kt[t][e], high, sum, 0, 0, 0);
+        sum_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.kt[t][e], low, sum_low, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] = (sum[i] + sum_low[i]) * (1.0f / kLength);
+    }
+    f32x4 o, o_low = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = now.read[i] * kUnit * (qs[i] + qs_low[i]);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t > wave >> 1) continue;
+      const half8 high = *reinterpret_cast<const half8 *>(&ub[0][t][lane][0]);
+      const half8 low = *reinterpret_cast<const half8 *>(&ub[1][t][lane][0]);
+      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.p[0][t], high, o, 0, 0, 0);
+      o_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.p[0][t], low, o_low, 0, 0, 0);
+      o_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.p[1][t], high, o_low, 0, 0, 0);
+    }
+    // lengths add up as squares do; sqrt(64) of the largest value for the chunk's
+    const float was = now.fade * size, came = 8.0f * value, large = fmaxf(was, came), small = fminf(was, came);
+    size = large > 0.0f ? large * sqrtf(1.0f + (small / large) * (small / large)) : 0.0f;
+    const float back = inverse;
+    if (more) {
+      value = of_waves(at & 1);
+      scale = scale_of(size + 9.0f * value, inverse);
+    }
+    if (at + 1 == kept_chunks && state && (!a.keep || a.keep[b] > 0)) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) state[(t * 16 + i) * a.dv] = s[t][i] * back;
+    }
+    if (!more && at + 1 < chunks) {
+      float *to = p.carry[(p.run + 1) & 1] + in_state;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(t * 16 + i) * a.dv] = s[t][i] * back;
+    }
+    if (more) {
+      const float ratio = back * scale;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][i] *= ratio;
+      give_state();
+    }
+    const Chunk c = chunk_of(n, kept, at);
+    const float unit = a.scale * back * (1.0f / kUnit);
+    const int row = wave * 16 + h * 4;
+    if (a.z) {
+      float *to = reinterpret_cast<float *>(p.chunks + (base + at - p.first) * p.at.bytes() + p.at.rows_at()) +
+                  static_cast<int64_t>(row) * a.v_heads * a.dv + head * a.dv + col;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row + i < c.rows) to[static_cast<int64_t>(i) * a.v_heads * a.dv] = (o[i] + o_low[i]) * unit;
+    } else {
+      TO *to = static_cast<TO *>(a.out) + (static_cast<int64_t>(row0) + c.start + row) * a.out_stride + head * a.dv + col;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row + i < c.rows) to[i * a.out_stride] = static_cast<TO>((o[i] + o_low[i]) * unit);
+    }
+    __syncthreads();
+  };
+  for (int at = c0; at < c1; at += 2) {
+    step(at, now, next);
+    if (at + 1 < c1) step(at + 1, next, now);
+  }
+}
+
+// The chunks' rows, fp32, normalised and gated: a workgroup a row, four neighbouring values a lane.
+template <typename TO>
+__global__ __launch_bounds__(kChunkThreads) void delta_gate_kernel(ChunkArgs p) {
+  const DeltaArgs &a = p.d;
+  const Sequence s = find_sequence(a.c, p.first + blockIdx.x, 1, kChunk, 2);
+  if (s.b < 0 || s.tokens <= 0) return;
+  const int kept = kept_rows(a, s.b, s.tokens), row = blockIdx.y;
+  if (s.item >= chunks_of(s.tokens, kept)) return;
+  const Chunk c = chunk_of(s.tokens, kept, s.item);
+  if (row >= c.rows) return;
+  const int width = a.v_heads * a.dv, lanes = a.dv / 4;
+  const float *o = reinterpret_cast<const float *>(p.chunks + blockIdx.x * p.at.bytes() + p.at.rows_at()) + static_cast<int64_t>(row) * width;
+  const int64_t out_row = static_cast<int64_t>(s.row0) + c.start + row;
+  for (int i = threadIdx.x * 4; i < width; i += kChunkThreads * 4) {   // whole heads: a head's lanes are of one wave
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(o + i);
+    float sum = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+    for (int off = lanes / 2; off; off >>= 1) sum += __shfl_xor(sum, off);
+    const float f = 1.0f / sqrtf(sum / a.dv + a.norm_eps);
+    const float *z = a.z + out_row * a.z_stride + i, *w = a.norm + i % a.dv;
+    TO *to = static_cast<TO *>(a.out) + out_row * a.out_stride + i;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = static_cast<TO>(x[e] * f * w[e] * (z[e] * sigmoid(z[e])));
+  }
+}
+
+// Calls whose sequences have more rows than this go in chunks.
+constexpr int kMostTokens = 16;
+
+struct ChunkPlan {
+  int64_t slots;
+  int count;      // chunks that the scratch holds at a time
+  int64_t bytes;
+};
+
+ChunkPlan plan_chunks(const ChunkLayout &at, int T, int B) {
+  ChunkPlan r;
+  r.slots = T / kChunk + 2 * (int64_t)B;
+  r.count = (int)std::min<int64_t>(r.slots, std::max<int64_t>(1, kMostScratch / at.bytes()));
+  r.bytes = r.count * at.bytes() + (r.count < r.slots ? 2 * at.state() : 0);
+  return r;
+}
+
+template <typename T, typename TO, int DK>
+int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
+  ChunkArgs p{};
+  p.d = a;
+  p.at = {DK, a.k_heads, a.v_heads, a.dv};
+  const ChunkPlan plan = plan_chunks(p.at, a.c.rows, a.c.batch);
+  p.chunks = static_cast<char *>(workspace);
+  p.carry[0] = reinterpret_cast<float *>(p.chunks + plan.count * p.at.bytes());
+  p.carry[1] = reinterpret_cast<float *>(reinterpret_cast<char *>(p.carry[0]) + p.at.state());
+  const int parts = (a.v_heads / a.k_heads + kHeadsPer - 1) / kHeadsPer;
+  const int64_t pairs = ((int64_t)a.c.batch * a.v_heads + 7) / 8 * 8;
+  RLQ_REQUIRE(a.k_heads * (int64_t)parts <= 65535 && pairs * (a.dv / 16) <= INT32_MAX,
+              "rlq_gated_delta: %d heads of %d sequences are too many for chunks", a.v_heads, a.c.batch);
+  for (int64_t first = 0; first < plan.slots; first += plan.count, ++p.run) {
+    p.first = (int)first;
+    p.count = (int)std::min<int64_t>(plan.count, plan.slots - first);
+    delta_chunks_kernel<T, DK><<<dim3(p.count, a.k_heads * parts), kChunkThreads, 0, st>>>(p);
+    RLQ_HIP(hipGetLastError());
+    delta_chain_kernel<T, TO, DK><<<(unsigned)(pairs * (a.dv / 16)), kChunkThreads, 0, st>>>(p);
+    RLQ_HIP(hipGetLastError());
+    if (a.z) {
+      delta_gate_kernel<TO><<<dim3(p.count, kChunk), kChunkThreads, 0, st>>>(p);
+      RLQ_HIP(hipGetLastError());
+    }
+  }
+  return 0;
+}
+
 template <typename T, typename TO>
-int launch_delta(const DeltaArgs &a, int DK, hipStream_t st) {
+int launch_delta(const DeltaArgs &a, int DK, int max_q, void *workspace, hipStream_t st) {
+  if (max_q > kMostTokens) return DK == 64 ? launch_chunks<T, TO, 64>(a, workspace, st) : launch_chunks<T, TO, 128>(a, workspace, st);
   const unsigned grid = (unsigned)a.c.batch * (unsigned)a.v_heads;
   if (DK == 64) delta_tokens_kernel<T, TO, 64><<<grid, a.dv * 2, 0, st>>>(a);
   else delta_tokens_kernel<T, TO, 128><<<grid, a.dv * 2, 0, st>>>(a);
@@ -194,7 +815,8 @@ int launch_delta(const DeltaArgs &a, int DK, hipStream_t st) {
 extern "C" {
 
 size_t rlq_gated_delta_workspace_bytes(int T, int k_heads, int v_heads, int Dk, int Dv, int B, int max_q) {
-  return 0;
+  if (T <= 0 || B <= 0 || max_q <= rlq::kMostTokens || k_heads < 1 || v_heads < k_heads || Dk <= 0 || Dv <= 0) return 0;
+  return (size_t)rlq::plan_chunks({Dk, k_heads, v_heads, Dv}, T, B).bytes;
 }
 
 int rlq_gated_delta(const void *q, int q_stride, const void *k, int k_stride, const void *v, int v_stride, int T,
@@ -225,6 +847,9 @@ int rlq_gated_delta(const void *q, int q_stride, const void *k, int k_stride, co
                   b_stride >= v_heads && out_stride >= v_heads * Dv && (!z || z_stride >= v_heads * Dv),
               "rlq_gated_delta: a row stride is shorter than the row (q %d, k %d, v %d, a %d, b %d, z %d, out %d)", q_stride,
               k_stride, v_stride, a_stride, b_stride, z_stride, out_stride);
+  const size_t need = rlq_gated_delta_workspace_bytes(T, k_heads, v_heads, Dk, Dv, B, max_q);
+  RLQ_REQUIRE(need == 0 || (workspace && rlq::aligned(workspace, 16) && workspace_bytes >= need),
+              "rlq_gated_delta: needs %zu bytes of 16-byte aligned workspace, got %zu", need, workspace_bytes);
   rlq::DeltaArgs x{};
   x.q = q, x.k = k, x.v = v, x.a = a, x.b = b, x.a_log = a_log, x.dt_bias = dt_bias, x.z = z, x.norm = norm;
   x.state = state, x.out = out, x.slots = slots, x.keep = keep;
@@ -237,9 +862,9 @@ int rlq_gated_delta(const void *q, int q_stride, const void *k, int k_stride, co
            q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0 && out_stride % 4 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == RLQ_F16) {
-    return out_dtype == RLQ_F16 ? rlq::launch_delta<_Float16, _Float16>(x, Dk, st) : rlq::launch_delta<_Float16, __bf16>(x, Dk, st);
+    return out_dtype == RLQ_F16 ? rlq::launch_delta<_Float16, _Float16>(x, Dk, max_q, workspace, st) : rlq::launch_delta<_Float16, __bf16>(x, Dk, max_q, workspace, st);
   }
-  return out_dtype == RLQ_F16 ? rlq::launch_delta<__bf16, _Float16>(x, Dk, st) : rlq::launch_delta<__bf16, __bf16>(x, Dk, st);
+  return out_dtype == RLQ_F16 ? rlq::launch_delta<__bf16, _Float16>(x, Dk, max_q, workspace, st) : rlq::launch_delta<__bf16, __bf16>(x, Dk, max_q, workspace, st);
 }
 
 }  // extern "C"
