@@ -482,8 +482,9 @@ int rlq_adjust_logits(const float *logits, int64_t stride, int rows, int vocab, 
  * more: all), min_p fp32 [rows] (NULL, 0 or less: all; 1 or more: those equal to the largest); NaN
  * is as NULL, for the temperature as 0. tokens int32 [rows]; probs fp32 [rows] or NULL: the token's share of the
  * kept weight. Logits of -inf and NaN are never taken; a row of nothing else gives token -1 and
- * share 0. Weights are formed in fp64 and summed as whole numbers of steps of 2^-(62 - ceil(log2 vocab))
- * of the largest: the same row gives the same token in every call. vocab at most 2^22.
+ * share 0. Weights are formed in fp64 and summed as whole numbers of steps of 2^-44 of the
+ * largest (2^-(62 - ceil(log2 vocab)) past 2^18 tokens): the same row gives the same token in every
+ * call. vocab at most 2^22.
  * The workspace (rlq_sample_workspace_bytes; 16-byte aligned, no initialisation) must not be shared by
  * calls that overlap. */
 size_t rlq_sample_workspace_bytes(int rows, int vocab);

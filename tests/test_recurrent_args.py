@@ -50,10 +50,29 @@ def test_gated_delta_refuses(change, message):
 @pytest.mark.parametrize("change,message", [
     (dict(rows=-1), "rows=-1"), (dict(rows=70000), "rows=70000"), (dict(vocab=0), "vocab=0"),
     (dict(vocab=(1 << 22) + 1, stride=1 << 23), "vocab="), (dict(logits=None), "null pointer"),
-    (dict(uniform=None), "null pointer"), (dict(tokens=None), "null pointer"), (dict(stride=999), "stride")])
+    (dict(uniform=None), "null pointer"), (dict(tokens=None), "null pointer"), (dict(stride=999), "stride"),
+    (dict(workspace=None), "16-byte aligned workspace"), (dict(workspace=24), "16-byte aligned workspace"),
+    (dict(workspace_bytes=100), "16-byte aligned workspace")])
 def test_sample_refuses(change, message):
     with pytest.raises(lib.RlqError, match=message):
         lib.call("rlq_sample", *{**SAMPLE, **change}.values())
+
+
+@pytest.mark.parametrize("change", [dict(workspace=None, workspace_bytes=1 << 40), dict(workspace=24, workspace_bytes=1 << 40),
+                                    dict(workspace=16, workspace_bytes=1000)])
+def test_gated_delta_in_chunks_refuses_other_scratch(change):
+    with pytest.raises(lib.RlqError, match="16-byte aligned workspace"):
+        lib.call("rlq_gated_delta", *{**DELTA, "max_q": 1000, **change}.values())
+
+
+def test_workspace_queries():
+    assert ops.gated_delta_workspace_bytes(1, 16, 32, 128, 128, 1, 1) == 0                # token by token
+    one, two, long = (ops.gated_delta_workspace_bytes(T, 16, 32, 128, 128, 1, T) for T in (1000, 2000, 1 << 20))
+    assert 0 < one < two < long < 400 << 20                                               # bounded, however long
+    assert ops.gated_delta_workspace_bytes(0, 16, 32, 128, 128, 1, 100) == 0
+    assert ops.gated_delta_workspace_bytes(100, 16, 8, 128, 128, 1, 100) == 0             # no such heads
+    assert ops.sample_workspace_bytes(3, 1000) == 3 * ops.sample_workspace_bytes(1, 1000) > 0
+    assert ops.sample_workspace_bytes(1, 1 << 23) == ops.sample_workspace_bytes(-1, 100) == 0
 
 
 def test_calls_without_rows_do_nothing():
