@@ -7,7 +7,7 @@
 namespace rlq {
 namespace {
 
-constexpr int kConvThreads = 64, kConvRun = 16, kMaxTaps = 4;
+constexpr int kConvThreads = 64, kMaxTaps = 4, kLongRun = 16, kShortRun = 4, kManyWaves = 2048;
 
 struct ConvArgs {
   const float *x, *w, *bias;
@@ -50,10 +50,10 @@ __device__ __forceinline__ void store_floats(float *p, const Floats<VEC> &x) {
 // A thread takes VEC neighbouring channels of one sequence over a run of tokens, whose inputs slide
 // through its registers; the run in front is read again for TAPS - 1 rows. The state is read and
 // written by the threads of a sequence's first run alone, so no other has to be waited for.
-template <typename T, int TAPS, int VEC>
+template <typename T, int TAPS, int VEC, int RUN>
 __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
-  const Sequence s = find_sequence(a.c, blockIdx.x, 1, kConvRun, 1);
-  const int t0 = s.item * kConvRun, tokens = min(s.tokens - t0, kConvRun);
+  const Sequence s = find_sequence(a.c, blockIdx.x, 1, RUN, 1);
+  const int t0 = s.item * RUN, tokens = min(s.tokens - t0, RUN);
   const int c0 = (blockIdx.y * kConvThreads + threadIdx.x) * VEC;
   if (s.b < 0 || tokens <= 0 || c0 >= a.channels) return;
   const float *x = a.x + s.row0 * a.x_stride + c0;
@@ -61,10 +61,10 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
   const bool has_state = slot >= 0 && slot < a.n_slots;
   float *state = a.state + (has_state ? static_cast<int64_t>(slot) * (TAPS - 1) * a.channels + c0 : 0);
 
-  Floats<VEC> in[TAPS - 1 + kConvRun];
+  // behind a short run its last row again: without branches all loads are on their way at once
+  Floats<VEC> in[TAPS - 1 + RUN];
 #pragma unroll
-  for (int i = 0; i < kConvRun; ++i)
-    if (i < tokens) in[TAPS - 1 + i] = load_floats<VEC>(x + (t0 + i) * a.x_stride);
+  for (int i = 0; i < RUN; ++i) in[TAPS - 1 + i] = load_floats<VEC>(x + (t0 + min(i, tokens - 1)) * a.x_stride);
 #pragma unroll
   for (int j = 0; j < TAPS - 1; ++j) {
     in[j] = {};
@@ -87,6 +87,7 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
       for (int j = 0; j < TAPS; ++j) w[e][j] = a.w[(c0 + e) * static_cast<int64_t>(TAPS) + j];
     }
   }
+  __builtin_amdgcn_sched_barrier(0);   // the compiler would put each load in front of its use
   if (t0 == 0 && has_state) {
     // after `end` tokens: inputs end - (TAPS-1) .. end - 1, from the old state where that is negative
     const int end = a.keep ? max(0, min(a.keep[s.b], s.tokens)) : s.tokens;
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
   }
   T *out = static_cast<T *>(a.out) + (s.row0 + t0) * a.out_stride + c0;
 #pragma unroll
-  for (int i = 0; i < kConvRun; ++i) {
+  for (int i = 0; i < RUN; ++i) {
     if (i >= tokens) break;
     T y[VEC];
 #pragma unroll
@@ -132,22 +133,26 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
   }
 }
 
-template <typename T, int TAPS>
-int launch_conv(const ConvArgs &a, bool wide, hipStream_t st) {
-  const int per = kConvThreads * (wide ? 4 : 1);
-  const dim3 grid((unsigned)(a.c.rows / kConvRun + a.c.batch), (unsigned)((a.channels + per - 1) / per));
+template <typename T, int TAPS, int VEC, int RUN>
+int launch_run(const ConvArgs &a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.c.rows / RUN + a.c.batch), (unsigned)((a.channels + kConvThreads * VEC - 1) / (kConvThreads * VEC)));
   RLQ_REQUIRE(grid.y <= 65535, "rlq_causal_conv: %d channels are too many", a.channels);
-  if (wide) causal_conv_kernel<T, TAPS, 4><<<grid, kConvThreads, 0, st>>>(a);
-  else causal_conv_kernel<T, TAPS, 1><<<grid, kConvThreads, 0, st>>>(a);
+  causal_conv_kernel<T, TAPS, VEC, RUN><<<grid, kConvThreads, 0, st>>>(a);
   RLQ_HIP(hipGetLastError());
   return 0;
 }
 
+template <typename T, int TAPS, int VEC>
+int launch_conv(const ConvArgs &a, hipStream_t st) {
+  const int64_t waves = (int64_t)a.c.rows / kLongRun * ((a.channels + kConvThreads * VEC - 1) / (kConvThreads * VEC));
+  return waves >= kManyWaves ? launch_run<T, TAPS, VEC, kLongRun>(a, st) : launch_run<T, TAPS, VEC, kShortRun>(a, st);
+}
+
 template <typename T>
 int launch_taps(const ConvArgs &a, int taps, bool wide, hipStream_t st) {
-  if (taps == 2) return launch_conv<T, 2>(a, wide, st);
-  if (taps == 3) return launch_conv<T, 3>(a, wide, st);
-  return launch_conv<T, 4>(a, wide, st);
+  if (taps == 2) return wide ? launch_conv<T, 2, 4>(a, st) : launch_conv<T, 2, 1>(a, st);
+  if (taps == 3) return wide ? launch_conv<T, 3, 4>(a, st) : launch_conv<T, 3, 1>(a, st);
+  return wide ? launch_conv<T, 4, 4>(a, st) : launch_conv<T, 4, 1>(a, st);
 }
 
 }  // namespace

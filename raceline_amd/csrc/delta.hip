@@ -19,7 +19,7 @@ struct DeltaArgs {
   const int *slots, *keep;
   PagedCache c;   // rows and sequences alone
   int64_t q_stride, k_stride, v_stride, a_stride, b_stride, z_stride, out_stride;
-  int k_heads, v_heads, dv, n_slots, wide;
+  int k_heads, v_heads, dv, n_slots, wide, wide_z;
   float eps, scale, norm_eps;
 };
 
@@ -55,18 +55,19 @@ __device__ __forceinline__ float sum_low(float x) {
 }
 
 template <typename T, int N>
-__device__ __forceinline__ void load_narrow(const T *p, bool wide, float (&x)[N]) {
-  typedef T pack __attribute__((ext_vector_type(N < 8 ? N : 8)));
+__device__ __forceinline__ void load_row(const T *p, bool wide, T (&x)[N]) {
+  constexpr int kPack = N < 8 ? N : 8;
+  typedef T pack __attribute__((ext_vector_type(kPack)));
   if (wide) {
 #pragma unroll
-    for (int i = 0; i < N; i += 8) {
+    for (int i = 0; i < N; i += kPack) {
       const pack v = *reinterpret_cast<const pack *>(p + i);
 #pragma unroll
-      for (int j = 0; j < 8 && j < N; ++j) x[i + j] = static_cast<float>(v[j]);
+      for (int j = 0; j < kPack; ++j) x[i + j] = v[j];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = static_cast<float>(p[i]);
+    for (int i = 0; i < N; ++i) x[i] = p[i];
   }
 }
 
@@ -115,16 +116,37 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = a.norm[col + e];
   }
+  // a token's rows are on their way while the one in front is worked on
+  struct Rows {
+    T q[kRows], k[kRows], v[4];
+    float a, b, z[4];
+  };
+  auto fetch = [&](int t, Rows &x) {
+    load_row<T, kRows>(qp + t * a.q_stride, a.wide, x.q);
+    load_row<T, kRows>(kp + t * a.k_stride, a.wide, x.k);
+    load_row<T, 4>(vp + t * a.v_stride, a.wide, x.v);
+    x.a = ap[t * a.a_stride], x.b = bp[t * a.b_stride];
+    if (zp) {
+      if (a.wide_z) {
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(zp + t * a.z_stride);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.z[e] = y[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.z[e] = zp[t * a.z_stride + e];
+      }
+    }
+  };
+  Rows next;
+  fetch(0, next);
   for (int t = 0; t < n; ++t) {
     float q[kRows], k[kRows], v[4], z[4];
-    load_narrow<T, kRows>(qp + t * a.q_stride, a.wide, q);
-    load_narrow<T, kRows>(kp + t * a.k_stride, a.wide, k);
-    load_narrow<T, 4>(vp + t * a.v_stride, a.wide, v);
-    if (zp) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = zp[t * a.z_stride + e];
-    }
-    const float fade = expf(log_fade(ap[t * a.a_stride], dt_bias, rate)), beta = sigmoid(bp[t * a.b_stride]);
+    for (int i = 0; i < kRows; ++i) q[i] = static_cast<float>(next.q[i]), k[i] = static_cast<float>(next.k[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(next.v[e]), z[e] = next.z[e];
+    const float fade = expf(log_fade(next.a, dt_bias, rate)), beta = sigmoid(next.b);
+    if (t + 1 < n) fetch(t + 1, next);
     // to length 1 before the products: those of raw rows with a state could pass fp32
     float kk = 0.0f, qq = 0.0f, kq = 0.0f, p[4] = {}, r[4] = {};
 #pragma unroll
@@ -160,7 +182,7 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
     if (zp) {
       const float mine = sum_low(o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3]);
       if (lane == 0) squares[t & 1][wave] = mine;
-      __syncthreads();          // the other half is free: its last readers are past the barrier before
+      lds_barrier();          // the other half is free: its last readers are past the barrier before
       float sum = 0.0f;
       for (int i = 0; i < a.dv / 32; ++i) sum += squares[t & 1][i];
       const float r = 1.0f / sqrtf(sum / a.dv + a.norm_eps);
@@ -253,6 +275,17 @@ __device__ __forceinline__ void split(const float (&x)[4], half4 &high, half4 &l
   }
 }
 
+__device__ __forceinline__ float most_of_wave(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));
+  x = fmaxf(x, dpp<0x4E>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  x = fmaxf(x, dpp<0x128>(x));
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 template <typename T, int DK>
 __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p) {
   constexpr int kPad = DK + 8, kSteps = DK / 32, kPer = DK / 4;
@@ -260,7 +293,7 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
   __shared__ __align__(16) _Float16 ks[kChunk][kPad], qs[kChunk][kPad];
   __shared__ __align__(16) float kk[kChunk][kMatPad], qk[kChunk][kMatPad], m[kChunk][kMatPad];
   __shared__ double total[kChunk];
-  __shared__ float rk[kChunk], rq[kChunk], beta[kChunk];
+  __shared__ float rk[kChunk], rq[kChunk], beta[kChunk], most[4];
 
   const Sequence s = find_sequence(a.c, p.first + blockIdx.x, 1, kChunk, 2);
   if (s.b < 0 || s.tokens <= 0) return;
@@ -279,9 +312,12 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
     for (int which = 0; which < 2; ++which) {
       float x[kPer], sum = 0.0f;
       if (row < c.rows) {
+        T y[kPer];
         const T *from = which ? static_cast<const T *>(a.q) + (row0 + row) * a.q_stride
                               : static_cast<const T *>(a.k) + (row0 + row) * a.k_stride;
-        load_narrow<T, kPer>(from + k_head * DK + d0, a.wide, x);
+        load_row<T, kPer>(from + k_head * DK + d0, a.wide, y);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] = static_cast<float>(y[i]);
       } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
@@ -304,7 +340,7 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
       if ((tid & 3) == 0) (which ? rq : rk)[row] = down / sqrtf(sum + a.eps);
     }
   }
-  __syncthreads();
+  lds_barrier();
   {  // K K^T and Q K^T, 16 rows a wave
     f32x4 ck[4] = {}, cq[4] = {};
     const int r = lane & 15, h = lane >> 4;
@@ -350,7 +386,7 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
     char *mine = place + p.at.k_heads * p.at.k_head() + head * p.at.v_head();
     _Float16 *to = reinterpret_cast<_Float16 *>(mine);
     float *factors = reinterpret_cast<float *>(mine + 4 * 8 * kBlock * 2);
-    __syncthreads();
+    lds_barrier();
     if (wave == 0) {
       // sums of logarithms in 64 bits: what they differ by between rows that forget little is to be exact
       // beside rows that forget all (e^-128 is nothing in fp32)
@@ -372,10 +408,10 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
       factors[lane] = w;
       factors[kChunk + lane] = w * fade * rk[lane];
       factors[2 * kChunk + lane] = rk[lane] * kLength * expf(static_cast<float>(last - sum));
-      factors[3 * kChunk + lane] = rq[lane] * fade;
-      factors[4 * kChunk + lane] = expf(static_cast<float>(last));
+      factors[3 * kChunk + lane] = rq[lane] * fade * kUnit;
+      if (lane == 0) factors[4 * kChunk] = expf(static_cast<float>(last));
     }
-    __syncthreads();
+    lds_barrier();
     {  // L, and P as operands: sixteen columns of one row a thread
       const int i = tid >> 2, m0 = (tid & 3) * 16;
       const double ti = total[i];
@@ -398,7 +434,22 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
         *reinterpret_cast<half4 *>(block + 8 * kBlock + h * 128) = low;
       }
     }
-    __syncthreads();
+    lds_barrier();
+    {  // the largest value
+      const T *from = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv;
+      float x = 0.0f;
+      for (int i = tid; i < c.rows * (a.dv / 8); i += kChunkThreads) {
+        const int row = i / (a.dv / 8);
+        T y[8];
+        load_row<T, 8>(from + row * a.v_stride + (i - row * (a.dv / 8)) * 8, a.wide, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf(static_cast<float>(y[e])));
+      }
+      x = most_of_wave(x);
+      if (lane == 0) most[wave] = x;
+    }
+    lds_barrier();
+    if (tid == 0) factors[4 * kChunk + 1] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
     const int r = lane & 15, h = lane >> 4;
     {  // the inverses of the 16 x 16 blocks on the diagonal, one a wave: a lane solves for column r
       float x[16];
@@ -414,7 +465,7 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
       for (int i = 0; i < 16; ++i)
         if (h == i >> 2) m[at + i][at + r] = x[i];
     }
-    __syncthreads();
+    lds_barrier();
     // -T22 (L21 T11) joins two inverses; in fp32 products of 16 x 16 x 4, whose result is the second's operand
     auto times = [&](int row, int col, const f32x4 &right, f32x4 sum) {
 #pragma unroll
@@ -435,7 +486,7 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
       const f32x4 x = times(at + 1, at, block_at_(at, at), f32x4{});
       put(at + 1, at, times(at + 1, at + 1, x, f32x4{}));
     }
-    __syncthreads();
+    lds_barrier();
     f32x4 low0 = {}, low1 = {};
     if (wave < 2) {
       const f32x4 t0 = wave ? f32x4{} : block_at_(0, 0), t1 = block_at_(1, wave);
@@ -443,9 +494,9 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
       low0 = times(2, 2, x0, f32x4{});
       low1 = times(3, 3, x1, times(3, 2, x0, f32x4{}));
     }
-    __syncthreads();
+    lds_barrier();
     if (wave < 2) put(2, wave, low0), put(3, wave, low1);
-    __syncthreads();
+    lds_barrier();
     {
       const int i = tid >> 2, m0 = (tid & 3) * 16;
       _Float16 *block = to + ((i >> 4) * 2 + (m0 >> 5)) * kBlock + (i & 15) * 8 + (m0 >> 4 & 1) * 4;
@@ -464,36 +515,22 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
   }
 }
 
-__device__ __forceinline__ float most_of_wave(float x) {
-  x = fmaxf(x, dpp<0xB1>(x));
-  x = fmaxf(x, dpp<0x4E>(x));
-  x = fmaxf(x, dpp<0x141>(x));
-  x = fmaxf(x, dpp<0x128>(x));
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
+constexpr int kChainThreads = 512;
 
-// What a wave reads of a chunk: its 16 rows of the rows' products, its rows of the state's.
-template <int DK>
-struct ChunkOperands {
-  half8 k[DK / 32], q[DK / 32], kt[DK / 64][2], t[2][2], p[2][2];   // t, p: term, step
-  f32x4 take, seen, left, read;                                      // factors of its rows of V, K S, U, Q S
-  float v[4], fade;
-};
-
-// A workgroup goes through a sequence's chunks with 16 columns of one head's state: a wave has 16 of a chunk's rows
-// and a quarter of the state's, and S, R and U go between the waves as operands in LDS.
-// Values are held times a power of two that keeps them in fp16's range: with keys of length 1 and beta at most 1
-// a column of S is never longer than what its square and those of the values v add up to, and R and U never larger
-// than S and 9 of the largest v.
+// A workgroup goes through a sequence's chunks with 16 columns of one head's state. Four waves are the chain: each
+// has 16 of a chunk's rows and a quarter of the state's, and S, R and U go between them as operands in LDS, a barrier
+// after each. Four others read the state out (O) beside them, 16 rows each.
+// Values are held times a power of two that keeps them in fp16's range: with keys of length 1 and beta at most 1 a
+// chunk lengthens a column of S by at most the sum of its values' squares (8 of the largest), and R and U are never
+// larger than a column of S and 9 of the largest value.
+// What a wave reads of the next chunk is asked for as soon as this chunk's has been used, so every load has a whole
+// step to arrive; no branch stands between a load and its use, or the wait there would be for all of them.
 template <typename T, typename TO, int DK>
-__global__ __launch_bounds__(kChunkThreads) void delta_chain_kernel(ChunkArgs p) {
+__global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs p) {
   constexpr int kSteps = DK / 32, kTiles = DK / 64;   // steps over the state's rows, tiles of 16 of them a wave has
   const DeltaArgs &a = p.d;
   __shared__ __align__(16) _Float16 sb[2][kSteps][64][8], rb[2][2][64][8], ub[2][2][64][8], wb[2][2][64][8];
-  __shared__ float most[2][4];
+  __shared__ __align__(16) float most[4];
 
   // workgroups of one head run on one XCD, whose L2 then holds its chunk for all of them
   const int slices = a.dv / 16, xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
@@ -509,223 +546,252 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chain_kernel(ChunkArgs p)
   const int c1 = static_cast<int>(min((int64_t)chunks, p.first + p.count - base));
   if (c0 >= c1) return;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, h = lane >> 4;
-  const int k_head = head / (a.v_heads / a.k_heads), slot = a.slots[b], col = slice * 16 + r;
-  const bool has_state = slot >= 0 && slot < a.n_slots;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+  const bool chain = __builtin_amdgcn_readfirstlane(tid >> 6) < 4;
+  const int r = lane & 15, h = lane >> 4, col = slice * 16 + r, row = wave * 16 + h * 4;
+  const bool below = wave >= 2;     // rows 32 and on: the second step over a chunk's rows is not above the diagonal
+  const int k_head = head / (a.v_heads / a.k_heads), slot = a.slots[b];
+  const bool has_state = slot >= 0 && slot < a.n_slots, stored = has_state && (!a.keep || a.keep[b] > 0);
   const int64_t in_state = (static_cast<int64_t>(head) * DK + wave * 16 * kTiles + h * 4) * a.dv + col;
   float *state = has_state ? a.state + static_cast<int64_t>(slot) * a.v_heads * DK * a.dv + in_state : nullptr;
 
-  float s[kTiles][4], size = 0.0f;   // size: a bound of the length of a column of S
-  {
-    const float *from = c0 ? p.carry[p.run & 1] + in_state : has_state && cached(a.c, b) > n ? state : nullptr;
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = from ? from[(t * 16 + i) * a.dv] : 0.0f;
-        size = fmaxf(size, fabsf(s[t][i]));
-      }
-  }
-  const T *values = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + col;
-
-  auto load = [&](int at, ChunkOperands<DK> &o) {
-    const Chunk c = chunk_of(n, kept, at);
-    const int row = wave * 16 + h * 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      o.v[i] = row + i < c.rows ? static_cast<float>(values[(c.start + row + i) * a.v_stride]) : 0.0f;
-    const char *place = p.chunks + (base + at - p.first) * p.at.bytes();
-    const _Float16 *rows = reinterpret_cast<const _Float16 *>(place + k_head * p.at.k_head()) + lane * 8;
-    const char *mine = place + p.at.k_heads * p.at.k_head() + head * p.at.v_head();
-    const _Float16 *mats = reinterpret_cast<const _Float16 *>(mine) + lane * 8;
-    const float *factors = reinterpret_cast<const float *>(mine + 4 * 8 * kBlock * 2);
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      o.k[t] = *reinterpret_cast<const half8 *>(rows + (wave * kSteps + t) * kBlock);
-      o.q[t] = *reinterpret_cast<const half8 *>(rows + kChunk * DK + (wave * kSteps + t) * kBlock);
-    }
-    o.take = *reinterpret_cast<const f32x4 *>(factors + row);
-    o.seen = *reinterpret_cast<const f32x4 *>(factors + kChunk + row);
-    o.left = *reinterpret_cast<const f32x4 *>(factors + 2 * kChunk + row);
-    o.read = *reinterpret_cast<const f32x4 *>(factors + 3 * kChunk + row);
-    o.fade = factors[4 * kChunk];
+  // the places of this head's data in a chunk's
+  const int64_t step_bytes = p.at.bytes();
+  const char *place = p.chunks + (base + c0 - p.first) * step_bytes;
+  const int64_t rows_at = k_head * p.at.k_head() + (wave * kSteps * kBlock + lane * 8) * 2;
+  const int64_t head_at = p.at.k_heads * p.at.k_head() + head * p.at.v_head();
+  const int64_t mats_at = head_at + (wave * 2 * kBlock + lane * 8) * 2, factors_at = head_at + 4 * 8 * kBlock * 2;
+  auto load8 = [](const char *from) { return *reinterpret_cast<const half8 *>(from); };
+  auto load4 = [](const char *from) { return *reinterpret_cast<const f32x4 *>(from); };
+  auto load_mats = [&](const char *from, int which, half8 (&to)[2][2]) {     // term, step
+    from += mats_at + which * 16 * kBlock * 2;
 #pragma unroll
     for (int term = 0; term < 2; ++term)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (t > wave >> 1) continue;               // above the diagonal
-        o.t[term][t] = *reinterpret_cast<const half8 *>(mats + (term * 8 + wave * 2 + t) * kBlock);
-        o.p[term][t] = *reinterpret_cast<const half8 *>(mats + (16 + term * 8 + wave * 2 + t) * kBlock);
-      }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        o.kt[t][u] = *reinterpret_cast<const half8 *>(rows + 2 * kChunk * DK + ((wave * kTiles + t) * 2 + u) * kBlock);
+      for (int e = 0; e < 2; ++e) to[term][e] = load8(from + (term * 8 + e) * kBlock * 2);
   };
-  auto most_value = [&](const ChunkOperands<DK> &o) {
-    return most_of_wave(fmaxf(fmaxf(fabsf(o.v[0]), fabsf(o.v[1])), fmaxf(fabsf(o.v[2]), fabsf(o.v[3]))));
+  auto operand = [&](const _Float16 (&from)[64][8]) { return *reinterpret_cast<const half8 *>(&from[lane][0]); };
+  auto mfma = [](const half8 &x, const half8 &y, const f32x4 &sum) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, sum, 0, 0, 0);
   };
-  auto of_waves = [&](int which) { return fmaxf(fmaxf(most[which][0], most[which][1]), fmaxf(most[which][2], most[which][3])); };
+  // a chunk's 64 x 64 matrix in two terms times 64 x 16 values in two, this wave's rows
+  auto times = [&](const half8 (&x)[2][2], const _Float16 (&y)[2][2][64][8], f32x4 sum) {
+    f32x4 low_sum = {};
+    const half8 high = operand(y[0][0]), low = operand(y[1][0]);
+    sum = mfma(x[0][0], high, sum);
+    low_sum = mfma(x[0][0], low, low_sum);
+    low_sum = mfma(x[1][0], high, low_sum);
+    if (below) {
+      const half8 high = operand(y[0][1]), low = operand(y[1][1]);
+      sum = mfma(x[0][1], high, sum);
+      low_sum = mfma(x[0][1], low, low_sum);
+      low_sum = mfma(x[1][1], high, low_sum);
+    }
+    return sum + low_sum;
+  };
   // the power of two that brings what is below `x` under 2^15, and its inverse
   auto scale_of = [&](float x, float &inverse) {
     const int ex = max(40, min(254, (int)(__float_as_uint(x) >> 23)));
     inverse = __uint_as_float((ex - 14) << 23);
     return __uint_as_float((268 - ex) << 23);
   };
-  auto give = [&](_Float16 (&to)[2][2][64][8], const float (&x)[4]) {
-    half4 high, low;
-    split(x, high, low);
-    *reinterpret_cast<half4 *>(&to[0][wave >> 1][lane][(wave & 1) * 4]) = high;
-    *reinterpret_cast<half4 *>(&to[1][wave >> 1][lane][(wave & 1) * 4]) = low;
-  };
-  auto give_state = [&]() {
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      half4 high, low;
-      split(s[t], high, low);
-      const int part = wave * kTiles + t;
-      *reinterpret_cast<half4 *>(&sb[0][part >> 1][lane][(part & 1) * 4]) = high;
-      *reinterpret_cast<half4 *>(&sb[1][part >> 1][lane][(part & 1) * 4]) = low;
-    }
-  };
 
-  ChunkOperands<DK> now, next;
-  load(c0, now);
-  {
-    const float x = most_of_wave(size), y = most_value(now);
-    if (lane == 0) most[0][wave] = x, most[1][wave] = y;
+  float s[kTiles][4], size = 0.0f;   // size: a bound of the length of a column of S
+  if (chain) {
+    const float *from = c0 ? p.carry[p.run & 1] + in_state : has_state && cached(a.c, b) > n ? state : nullptr;
+#pragma unroll
+    for (int e = 0; e < kTiles; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[e][i] = from ? from[(e * 16 + i) * a.dv] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < kTiles; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) size = fmaxf(size, fabsf(s[e][i]));
+    size = most_of_wave(size);
+    if (lane == 0) most[wave] = size;
   }
-  __syncthreads();
-  size = of_waves(0) * (DK == 128 ? 11.32f : 8.0f);
-  float value = of_waves(1), inverse, scale = scale_of(size + 9.0f * value, inverse);
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[t][i] *= scale;
-  give_state();
-  __syncthreads();
+  f32x4 about = load4(place + factors_at + 4 * kChunk * 4);          // the chunk's fade and its largest value
+  Chunk c = chunk_of(n, kept, c0);
+  lds_barrier();
+  size = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * (DK == 128 ? 11.32f : 8.0f);
+  float inverse, scale = scale_of(size + 9.0f * about[1], inverse);
 
-  auto step = [&](int at, const ChunkOperands<DK> &now, ChunkOperands<DK> &next) {
-    const bool more = at + 1 < c1;
-    if (more) load(at + 1, next);
-    f32x4 ks = {}, ks_low = {}, qs = {}, qs_low = {};
+  if (chain) {
+    half8 k[kSteps], t[2][2], kt[kTiles][2];
+    f32x4 take, seen, left;            // factors of this wave's rows of V, K S and U
+    T v[4], v_next[4];
+    const T *values = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + col;
+    auto load_values = [&](int start, T (&to)[4]) {                  // behind the sequence its last row again
 #pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      const half8 high = *reinterpret_cast<const half8 *>(&sb[0][t][lane][0]);
-      const half8 low = *reinterpret_cast<const half8 *>(&sb[1][t][lane][0]);
-      ks = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.k[t], high, ks, 0, 0, 0);
-      ks_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.k[t], low, ks_low, 0, 0, 0);
-      qs = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.q[t], high, qs, 0, 0, 0);
-      qs_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.q[t], low, qs_low, 0, 0, 0);
-    }
-    float x[4];
+      for (int i = 0; i < 4; ++i) to[i] = values[min(start + row + i, n - 1) * a.v_stride];
+    };
+    auto load_rows = [&](const char *from) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = now.take[i] * (now.v[i] * scale) - now.seen[i] * (ks[i] + ks_low[i]);
-    give(rb, x);
-    __syncthreads();
-
-    f32x4 u = {}, u_low = {};
+      for (int e = 0; e < kSteps; ++e) k[e] = load8(from + rows_at + e * kBlock * 2);
+      take = load4(from + factors_at + row * 4);
+      seen = load4(from + factors_at + (kChunk + row) * 4);
+    };
+    auto load_left = [&](const char *from) {
+      load_mats(from, 0, t);
+      left = load4(from + factors_at + (2 * kChunk + row) * 4);
+    };
+    auto load_last = [&](const char *from) {
+      from += k_head * p.at.k_head() + (2 * kChunk * DK + wave * kTiles * 2 * kBlock + lane * 8) * 2;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t > wave >> 1) continue;
-      const half8 high = *reinterpret_cast<const half8 *>(&rb[0][t][lane][0]);
-      const half8 low = *reinterpret_cast<const half8 *>(&rb[1][t][lane][0]);
-      u = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.t[0][t], high, u, 0, 0, 0);
-      u_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.t[0][t], low, u_low, 0, 0, 0);
-      u_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.t[1][t], high, u_low, 0, 0, 0);
-    }
-    float w[4];
+      for (int e = 0; e < kTiles; ++e)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = (u[i] + u_low[i]) * (1.0f / kUnit);
-      w[i] = now.left[i] * x[i];
-    }
-    give(ub, x);
-    give(wb, w);
-    if (more) {
-      const float y = most_value(next);
-      if (lane == 0) most[at & 1][wave] = y;
-    }
-    __syncthreads();
-
-    // the state first: the next chunk waits for it
+        for (int u = 0; u < 2; ++u) kt[e][u] = load8(from + (e * 2 + u) * kBlock * 2);
+    };
+    auto give = [&](_Float16 (&to)[2][2][64][8], const float (&x)[4]) {
+      half4 high, low;
+      split(x, high, low);
+      *reinterpret_cast<half4 *>(&to[0][wave >> 1][lane][(wave & 1) * 4]) = high;
+      *reinterpret_cast<half4 *>(&to[1][wave >> 1][lane][(wave & 1) * 4]) = low;
+    };
+    auto give_state = [&]() {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      f32x4 sum, sum_low = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = now.fade * kLength * s[t][i];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const half8 high = *reinterpret_cast<const half8 *>(&wb[0][e][lane][0]);
-        const half8 low = *reinterpret_cast<const half8 *>(&wb[1][e][lane][0]);
-        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.kt[t][e], high, sum, 0, 0, 0);
-        sum_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.kt[t][e], low, sum_low, 0, 0, 0);
+      for (int e = 0; e < kTiles; ++e) {
+        half4 high, low;
+        split(s[e], high, low);
+        const int part = wave * kTiles + e;
+        *reinterpret_cast<half4 *>(&sb[0][part >> 1][lane][(part & 1) * 4]) = high;
+        *reinterpret_cast<half4 *>(&sb[1][part >> 1][lane][(part & 1) * 4]) = low;
       }
+    };
+    load_values(c.start, v);
+    load_values(c.start + c.rows, v_next);
+    load_rows(place);
+    load_left(place);
+    load_last(place);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[t][i] = (sum[i] + sum_low[i]) * (1.0f / kLength);
-    }
-    f32x4 o, o_low = {};
+    for (int e = 0; e < kTiles; ++e)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = now.read[i] * kUnit * (qs[i] + qs_low[i]);
+      for (int i = 0; i < 4; ++i) s[e][i] *= scale;
+    give_state();
+    lds_barrier();
+
+    for (int at = c0; at < c1; ++at) {
+      place += at + 1 < c1 ? step_bytes : 0;             // the last chunk's data come again, unused
+      const int start = c.start + c.rows, rows = min(kChunk, (start < kept ? kept : n) - start);
+      f32x4 ks = {}, ks_low = {};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t > wave >> 1) continue;
-      const half8 high = *reinterpret_cast<const half8 *>(&ub[0][t][lane][0]);
-      const half8 low = *reinterpret_cast<const half8 *>(&ub[1][t][lane][0]);
-      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.p[0][t], high, o, 0, 0, 0);
-      o_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.p[0][t], low, o_low, 0, 0, 0);
-      o_low = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.p[1][t], high, o_low, 0, 0, 0);
-    }
-    // lengths add up as squares do; sqrt(64) of the largest value for the chunk's
-    const float was = now.fade * size, came = 8.0f * value, large = fmaxf(was, came), small = fminf(was, came);
-    size = large > 0.0f ? large * sqrtf(1.0f + (small / large) * (small / large)) : 0.0f;
-    const float back = inverse;
-    if (more) {
-      value = of_waves(at & 1);
-      scale = scale_of(size + 9.0f * value, inverse);
-    }
-    if (at + 1 == kept_chunks && state && (!a.keep || a.keep[b] > 0)) {
+      for (int e = 0; e < kSteps; ++e) {
+        ks = mfma(k[e], operand(sb[0][e]), ks);
+        ks_low = mfma(k[e], operand(sb[1][e]), ks_low);
+      }
+      float x[4];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
+      for (int i = 0; i < 4; ++i) {
+        const float mine = row + i < c.rows ? static_cast<float>(v[i]) : 0.0f;
+        x[i] = take[i] * (mine * scale) - seen[i] * (ks[i] + ks_low[i]);
+        v[i] = v_next[i];
+      }
+      give(rb, x);
+      load_rows(place);
+      load_values(start + rows, v_next);
+      lds_barrier();
+
+      const f32x4 u = times(t, rb, f32x4{});
+      float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) state[(t * 16 + i) * a.dv] = s[t][i] * back;
-    }
-    if (!more && at + 1 < chunks) {
-      float *to = p.carry[(p.run + 1) & 1] + in_state;
+      for (int i = 0; i < 4; ++i) {
+        x[i] = u[i] * (1.0f / kUnit);
+        w[i] = left[i] * x[i];
+      }
+      give(wb, w);
+      give(ub, x);
+      load_left(place);
+      const float fade = about[0];
+      size = fade * size + 8.0f * about[1];
+      about = load4(place + factors_at + 4 * kChunk * 4);
+      lds_barrier();
+
+      f32x4 sum[kTiles];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
+      for (int e = 0; e < kTiles; ++e) {
+        f32x4 low = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) to[(t * 16 + i) * a.dv] = s[t][i] * back;
-    }
-    if (more) {
-      const float ratio = back * scale;
+        for (int i = 0; i < 4; ++i) sum[e][i] = (fade * kLength) * s[e][i];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
+        for (int u = 0; u < 2; ++u) {
+          sum[e] = mfma(kt[e][u], operand(wb[0][u]), sum[e]);
+          low = mfma(kt[e][u], operand(wb[1][u]), low);
+        }
+        sum[e] += low;
+      }
+      load_last(place);
+      const float back = inverse * (1.0f / kLength);
+      scale = scale_of(size + 9.0f * about[1], inverse);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][i] *= ratio;
+      for (int e = 0; e < kTiles; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[e][i] = sum[e][i] * (back * scale);
       give_state();
-    }
-    const Chunk c = chunk_of(n, kept, at);
-    const float unit = a.scale * back * (1.0f / kUnit);
-    const int row = wave * 16 + h * 4;
-    if (a.z) {
-      float *to = reinterpret_cast<float *>(p.chunks + (base + at - p.first) * p.at.bytes() + p.at.rows_at()) +
-                  static_cast<int64_t>(row) * a.v_heads * a.dv + head * a.dv + col;
+      float *to = at + 1 == kept_chunks && stored ? state : nullptr;
+      float *on = at + 1 == c1 && at + 1 < chunks ? p.carry[(p.run + 1) & 1] + in_state : nullptr;
+      if (to || on) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (row + i < c.rows) to[static_cast<int64_t>(i) * a.v_heads * a.dv] = (o[i] + o_low[i]) * unit;
-    } else {
-      TO *to = static_cast<TO *>(a.out) + (static_cast<int64_t>(row0) + c.start + row) * a.out_stride + head * a.dv + col;
+        for (int e = 0; e < kTiles; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (row + i < c.rows) to[i * a.out_stride] = static_cast<TO>((o[i] + o_low[i]) * unit);
+          for (int i = 0; i < 4; ++i) {
+            if (to) to[(e * 16 + i) * a.dv] = sum[e][i] * back;
+            if (on) on[(e * 16 + i) * a.dv] = sum[e][i] * back;
+          }
+      }
+      c = {start, rows};
+      lds_barrier();
     }
-    __syncthreads();
-  };
-  for (int at = c0; at < c1; at += 2) {
-    step(at, now, next);
-    if (at + 1 < c1) step(at + 1, next, now);
+  } else {
+    half8 q[kSteps], pm[2][2];
+    f32x4 read;                        // factors of this wave's rows of Q S
+    auto load_rows = [&](const char *from) {
+#pragma unroll
+      for (int e = 0; e < kSteps; ++e) q[e] = load8(from + rows_at + (kChunk * DK + e * kBlock) * 2);
+    };
+    auto load_last = [&](const char *from) {
+      load_mats(from, 1, pm);
+      read = load4(from + factors_at + (3 * kChunk + row) * 4);
+    };
+    load_rows(place);
+    load_last(place);
+    const int64_t width = a.z ? static_cast<int64_t>(a.v_heads) * a.dv : a.out_stride;
+    float *scratch = reinterpret_cast<float *>(p.chunks + (base + c0 - p.first) * step_bytes + p.at.rows_at()) + row * width +
+                     head * a.dv + col;
+    TO *out = static_cast<TO *>(a.out) + (static_cast<int64_t>(row0) + c.start + row) * a.out_stride + head * a.dv + col;
+    lds_barrier();
+
+    for (int at = c0; at < c1; ++at) {
+      place += at + 1 < c1 ? step_bytes : 0;
+      f32x4 qs = {}, qs_low = {};
+#pragma unroll
+      for (int e = 0; e < kSteps; ++e) {
+        qs = mfma(q[e], operand(sb[0][e]), qs);
+        qs_low = mfma(q[e], operand(sb[1][e]), qs_low);
+      }
+      load_rows(place);
+      lds_barrier();
+      const float unit = a.scale * (1.0f / kUnit) * inverse;
+      size = about[0] * size + 8.0f * about[1];
+      about = load4(place + factors_at + 4 * kChunk * 4);
+      lds_barrier();
+      const f32x4 o = times(pm, ub, read * (qs + qs_low)) * unit;
+      load_last(place);
+      scale = scale_of(size + 9.0f * about[1], inverse);
+      lds_barrier();        // nothing of LDS is read behind it: the rows are stored beside the next step
+      if (a.z) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row + i < c.rows) scratch[i * width] = o[i];
+        scratch = reinterpret_cast<float *>(reinterpret_cast<char *>(scratch) + step_bytes);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row + i < c.rows) out[i * width] = static_cast<TO>(o[i]);
+        out += c.rows * width;
+      }
+      const int start = c.start + c.rows;
+      c = {start, min(kChunk, (start < kept ? kept : n) - start)};
+    }
   }
 }
 
@@ -789,7 +855,7 @@ int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
     p.count = (int)std::min<int64_t>(plan.count, plan.slots - first);
     delta_chunks_kernel<T, DK><<<dim3(p.count, a.k_heads * parts), kChunkThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
-    delta_chain_kernel<T, TO, DK><<<(unsigned)(pairs * (a.dv / 16)), kChunkThreads, 0, st>>>(p);
+    delta_chain_kernel<T, TO, DK><<<(unsigned)(pairs * (a.dv / 16)), kChainThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
     if (a.z) {
       delta_gate_kernel<TO><<<dim3(p.count, kChunk), kChunkThreads, 0, st>>>(p);
@@ -860,6 +926,7 @@ int rlq_gated_delta(const void *q, int q_stride, const void *k, int k_stride, co
   x.eps = eps, x.scale = scale, x.norm_eps = norm_eps;
   x.wide = rlq::aligned(q, 16) && rlq::aligned(k, 16) && rlq::aligned(v, 16) && rlq::aligned(out, 8) &&
            q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0 && out_stride % 4 == 0;
+  x.wide_z = rlq::aligned(z, 16) && z_stride % 4 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == RLQ_F16) {
     return out_dtype == RLQ_F16 ? rlq::launch_delta<_Float16, _Float16>(x, Dk, max_q, workspace, st) : rlq::launch_delta<_Float16, __bf16>(x, Dk, max_q, workspace, st);

@@ -23,12 +23,6 @@ struct LogitArgs {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// Every wave's LDS operations are done, and what a barrier does not need stays in flight. One asm
-// block: between a wait and a barrier of their own the compiler may place an LDS operation.
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 // One workgroup: a span of 4096 logits of one row. Every workgroup of a row reads all of the row's
 // tokens (from L2 but for the first) and counts those that fall into its span with integer LDS
 // atomics, whose order changes nothing; so the row needs neither a second launch nor counters in

@@ -220,15 +220,6 @@ __device__ int block_exclusive_scan(int v, int *wave_tot, int *total) {
   return ex;
 }
 
-// A workgroup barrier that orders LDS accesses only: __syncthreads also waits for every
-// global store in flight (its release fence), which the sort's later phases never read back
-// (the work items, rows and slots are for the next kernels); that wait took about 1 us at
-// each such barrier.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_s_waitcnt(0xC07F);             // lgkmcnt(0): this thread's LDS accesses are done
-  asm volatile("s_barrier" ::: "memory");
-}
-
 // One workgroup of 1024 threads sorts all T*S assignments by expert (a counting sort,
 // moe.metal:109-139) and writes the work list. Within an expert, rows follow token order:
 // token t's row for expert e is off[e] + (tokens before t that chose e). The tokens go in

@@ -46,6 +46,13 @@ int allow_large_lds(const void *fn, LdsOptIn &done);
 
 // ----------------------------------------------------------------- device helpers
 
+// A workgroup's barrier for what goes through LDS: every wave's LDS operations are done, and global loads and
+// stores stay in flight (__syncthreads waits for those too, about 1 us where stores are on their way). One
+// asm block: between a wait and a barrier of their own the compiler may place an LDS operation.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
