@@ -217,7 +217,7 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
 // terms (2^-22), T and P, at most 1, times 2^14, so that what has faded keeps its bits. Operands stand in the order in which sums leave the matrix cores: slot 8 h + 4 a + b of a step of
 // 32 is row 16 a + 4 h + b, so that what a lane holds of a result is what it holds of the next product.
 
-constexpr int kChunk = 64, kChunkThreads = 256, kHeadsPer = 2, kMatPad = 68;
+constexpr int kChunk = 64, kGateThreads = 256, kHeadsPer = 2, kPrepareThreads = 256 * kHeadsPer, kMatPad = 68;
 constexpr int kBlock = 64 * 8;                       // halves of a 16 x 32 operand
 constexpr float kUnit = 16384.0f, kLength = 8192.0f; // T and P are held times kUnit, rows of q and k at this length or twice it
 constexpr int64_t kMostScratch = 256 << 20;
@@ -286,14 +286,24 @@ __device__ __forceinline__ float most_of_wave(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// 2^x; what x loses in fp32 is nothing beside 2^x where x is large.
+__device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); }
+
+// A workgroup forms what the chain needs of one chunk and one key head: the rows of q and k as operands, and of
+// two of the value heads that share it, four waves each, T, P and the rows' factors.
+// T = (I + L)^-1 in fp32: the inverses of the four 16 x 16 blocks on the diagonal, a lane a column, joined by
+// -T22 (L21 T11) to blocks of 32 and of 64 with fp32 matrix products, whose result is the next one's operand.
 template <typename T, int DK>
-__global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p) {
-  constexpr int kPad = DK + 8, kSteps = DK / 32, kPer = DK / 4;
+__global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkArgs p) {
+  constexpr int kPad = DK + 8, kSteps = DK / 32, kPer = DK / 8;
   const DeltaArgs &a = p.d;
-  __shared__ __align__(16) _Float16 ks[kChunk][kPad], qs[kChunk][kPad];
-  __shared__ __align__(16) float kk[kChunk][kMatPad], qk[kChunk][kMatPad], m[kChunk][kMatPad];
-  __shared__ double total[kChunk];
-  __shared__ float rk[kChunk], rq[kChunk], beta[kChunk], most[4];
+  // rows of k and q, then, when they have been read, L and its inverse of both heads
+  __shared__ __align__(16) char pool[kHeadsPer * kChunk * kMatPad * 4];
+  __shared__ __align__(16) float kk[kChunk][kMatPad], qk[kChunk][kMatPad];
+  __shared__ double totals[kHeadsPer][kChunk];
+  __shared__ float rk[kChunk], rq[kChunk], betas[kHeadsPer][kChunk], most[kHeadsPer][4];
+  static_assert(2 * kChunk * kPad * 2 <= (int)sizeof(pool), "the rows fit");
+  _Float16(*ks)[kPad] = reinterpret_cast<_Float16(*)[kPad]>(pool), (*qs)[kPad] = ks + kChunk;
 
   const Sequence s = find_sequence(a.c, p.first + blockIdx.x, 1, kChunk, 2);
   if (s.b < 0 || s.tokens <= 0) return;
@@ -302,70 +312,107 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
   const Chunk c = chunk_of(s.tokens, kept, s.item);
   const int group = a.v_heads / a.k_heads, parts = (group + kHeadsPer - 1) / kHeadsPer;
   const int k_head = blockIdx.y / parts, part = blockIdx.y - k_head * parts;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, mine = wave & 3, own = tid & 255;
+  const int head = k_head * group + min(part * kHeadsPer + half, group - 1);
+  const bool there = part * kHeadsPer + half < group;      // an odd group's last pair has one head
   const int64_t row0 = s.row0 + c.start;
   char *place = p.chunks + blockIdx.x * p.at.bytes();
+  char *head_place = place + p.at.k_heads * p.at.k_head() + head * p.at.v_head();
+  float *factors = reinterpret_cast<float *>(head_place + 4 * 8 * kBlock * 2);
 
-  {  // rows to lengths of 2^13 .. 2^14, in fp16; four threads a row
-    const int row = tid >> 2, d0 = (tid & 3) * kPer;
+  {  // rows to lengths of 2^13 .. 2^14, in fp16; eight threads a row
+    const int row = tid >> 3, d0 = (tid & 7) * kPer;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
+      T y[kPer];
       float x[kPer], sum = 0.0f;
-      if (row < c.rows) {
-        T y[kPer];
-        const T *from = which ? static_cast<const T *>(a.q) + (row0 + row) * a.q_stride
-                              : static_cast<const T *>(a.k) + (row0 + row) * a.k_stride;
-        load_row<T, kPer>(from + k_head * DK + d0, a.wide, y);
+      const T *from = which ? static_cast<const T *>(a.q) + (row0 + min(row, c.rows - 1)) * a.q_stride
+                            : static_cast<const T *>(a.k) + (row0 + min(row, c.rows - 1)) * a.k_stride;
+      load_row<T, kPer>(from + k_head * DK + d0, a.wide, y);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] = static_cast<float>(y[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
+      for (int i = 0; i < kPer; ++i) {
+        x[i] = row < c.rows ? static_cast<float>(y[i]) : 0.0f;
+        sum += x[i] * x[i];
       }
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += x[i] * x[i];
-      sum += dpp<0xB1>(sum);
-      sum += dpp<0x4E>(sum);
+      sum = sum_low(sum);
       // the power of two that brings the length to 2^13 .. 2^14, and back
       const int ex = max(14, min(253, (int)(__float_as_uint(sqrtf(sum)) >> 23)));
       const float up = __uint_as_float((254 + 13 - ex) << 23), down = __uint_as_float((ex - 13) << 23);
       _Float16 *to = which ? &qs[row][d0] : &ks[row][d0];
 #pragma unroll
       for (int i = 0; i < kPer; i += 8) {
-        half8 y;
+        half8 z;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = static_cast<_Float16>(x[i + j] * up);
-        *reinterpret_cast<half8 *>(to + i) = y;
+        for (int j = 0; j < 8; ++j) z[j] = static_cast<_Float16>(x[i + j] * up);
+        *reinterpret_cast<half8 *>(to + i) = z;
       }
-      if ((tid & 3) == 0) (which ? rq : rk)[row] = down / sqrtf(sum + a.eps);
+      if ((tid & 7) == 0) (which ? rq : rk)[row] = down / sqrtf(sum + a.eps);
     }
   }
+  {  // the largest value of the head
+    const T *from = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv;
+    const int per = a.dv / 8;
+    float x = 0.0f;
+    for (int i = own; i < c.rows * per; i += 256) {
+      T y[8];
+      load_row<T, 8>(from + i / per * a.v_stride + i % per * 8, a.wide, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf(static_cast<float>(y[e])));
+    }
+    x = most_of_wave(x);
+    if (lane == 0) most[half][mine] = x;
+  }
   lds_barrier();
-  {  // K K^T and Q K^T, 16 rows a wave
-    f32x4 ck[4] = {}, cq[4] = {};
-    const int r = lane & 15, h = lane >> 4;
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      const half8 ka = *reinterpret_cast<const half8 *>(&ks[wave * 16 + r][t * 32 + h * 8]);
-      const half8 qa = *reinterpret_cast<const half8 *>(&qs[wave * 16 + r][t * 32 + h * 8]);
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const half8 kb = *reinterpret_cast<const half8 *>(&ks[n * 16 + r][t * 32 + h * 8]);
-        ck[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, kb, ck[n], 0, 0, 0);
-        cq[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa, kb, cq[n], 0, 0, 0);
+  if (mine == 0) {
+    // sums of logarithms (base 2) in 64 bits: what they differ by between rows that forget little is to be exact
+    // beside rows that forget all (2^-184 is nothing in fp32)
+    double sum = 0.0;
+    float w = 0.0f;
+    if (lane < c.rows) {
+      const float x = log_fade(a.a[(row0 + lane) * a.a_stride + head], a.dt_bias[head], expf(a.a_log[head]));
+      sum = (x < -128.0f ? -128.0f : x) * 1.4426950408889634;
+      w = sigmoid(a.b[(row0 + lane) * a.b_stride + head]);
+    }
+    for (int off = 1; off < 64; off <<= 1) {
+      const double o = __shfl_up(sum, off);
+      if (lane >= off) sum += o;
+    }
+    totals[half][lane] = sum;
+    betas[half][lane] = w;
+    const double last = __shfl(sum, 63);
+    const float fade = exp2_of(sum);
+    if (there) {
+      factors[lane] = w;
+      factors[kChunk + lane] = w * fade * rk[lane];
+      factors[2 * kChunk + lane] = rk[lane] * kLength * exp2_of(last - sum);
+      factors[3 * kChunk + lane] = rq[lane] * fade * kUnit;
+      if (lane == 0) {
+        factors[4 * kChunk] = exp2_of(last);
+        factors[4 * kChunk + 1] = fmaxf(fmaxf(most[half][0], most[half][1]), fmaxf(most[half][2], most[half][3]));
       }
     }
+  }
+  {  // K K^T of one half, Q K^T of the other, 16 rows a wave, on and below the diagonal
+    f32x4 x[4] = {};
+    const _Float16(*rows)[kPad] = half ? qs : ks;
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      const half8 left = *reinterpret_cast<const half8 *>(&rows[mine * 16 + r][t * 32 + h * 8]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (n <= mine) x[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(left, *reinterpret_cast<const half8 *>(&ks[n * 16 + r][t * 32 + h * 8]), x[n], 0, 0, 0);
+    }
+    float(*to)[kMatPad] = half ? qk : kk;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        kk[wave * 16 + h * 4 + i][n * 16 + r] = ck[n][i];
-        qk[wave * 16 + h * 4 + i][n * 16 + r] = cq[n][i];
-      }
+      for (int i = 0; i < 4; ++i)
+        if (n <= mine) to[mine * 16 + h * 4 + i][n * 16 + r] = x[n][i];
   }
   if (part == 0) {  // the rows as operands
     _Float16 *to = reinterpret_cast<_Float16 *>(place + k_head * p.at.k_head());
-    for (int i = tid; i < 4 * kSteps * 64; i += kChunkThreads) {
+    for (int i = tid; i < 4 * kSteps * 64; i += kPrepareThreads) {
       const int l = i & 63, t = (i >> 6) % kSteps, tile = (i >> 6) / kSteps, row = tile * 16 + (l & 15);
       const int d = t * 32 + (l >> 4) * 4;
       const half4 k0 = *reinterpret_cast<const half4 *>(&ks[row][d]), k1 = *reinterpret_cast<const half4 *>(&ks[row][d + 16]);
@@ -373,7 +420,7 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
       *reinterpret_cast<half8 *>(to + i * 8) = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
       *reinterpret_cast<half8 *>(to + kChunk * DK + i * 8) = __builtin_shufflevector(q0, q1, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    for (int i = tid; i < (DK / 16) * 2 * 64; i += kChunkThreads) {
+    for (int i = tid; i < (DK / 16) * 2 * 64; i += kPrepareThreads) {
       const int l = i & 63, t = (i >> 6) & 1, d = (i >> 7) * 16 + (l & 15), row = t * 32 + (l >> 4) * 4;
       half8 y;
 #pragma unroll
@@ -381,137 +428,91 @@ __global__ __launch_bounds__(kChunkThreads) void delta_chunks_kernel(ChunkArgs p
       *reinterpret_cast<half8 *>(to + 2 * kChunk * DK + i * 8) = y;
     }
   }
-  for (int v = part * kHeadsPer; v < min(group, (part + 1) * kHeadsPer); ++v) {
-    const int head = k_head * group + v;
-    char *mine = place + p.at.k_heads * p.at.k_head() + head * p.at.v_head();
-    _Float16 *to = reinterpret_cast<_Float16 *>(mine);
-    float *factors = reinterpret_cast<float *>(mine + 4 * 8 * kBlock * 2);
-    lds_barrier();
-    if (wave == 0) {
-      // sums of logarithms in 64 bits: what they differ by between rows that forget little is to be exact
-      // beside rows that forget all (e^-128 is nothing in fp32)
-      double sum = 0.0;
-      float w = 0.0f;
-      if (lane < c.rows) {
-        const float x = log_fade(a.a[(row0 + lane) * a.a_stride + head], a.dt_bias[head], expf(a.a_log[head]));
-        sum = x < -128.0f ? -128.0f : x;
-        w = sigmoid(a.b[(row0 + lane) * a.b_stride + head]);
+  lds_barrier();
+
+  float(*m)[kMatPad] = reinterpret_cast<float(*)[kMatPad]>(pool) + half * kChunk;
+  const double *total = totals[half];
+  const int i = own >> 2, m0 = (own & 3) * 16;              // sixteen columns of one row a thread
+  // its place in operands of T and P: the row's tile, the step of 32 columns, and the half of its slots
+  _Float16 *block = reinterpret_cast<_Float16 *>(head_place) + ((i >> 4) * 2 + (m0 >> 5)) * kBlock + (i & 15) * 8 + (m0 >> 4 & 1) * 4;
+  const bool used = there && (i >= 32 || m0 < 32);           // above the diagonal nothing is read
+  auto put_operand = [&](const float (&x)[4], int which, int g) {
+    half4 high, low;
+    split(x, high, low);
+    *reinterpret_cast<half4 *>(block + which * 16 * kBlock + g * 128) = high;
+    *reinterpret_cast<half4 *>(block + (which * 16 + 8) * kBlock + g * 128) = low;
+  };
+  {  // L, and P as operands
+    const double ti = total[i];
+    const float bi = betas[half][i] * rk[i], qi = rq[i] * kUnit;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float x[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = m0 + g * 4 + e;
+        const float f = j <= i ? exp2_of(ti - total[j]) * rk[j] : 0.0f;
+        x[e] = j < i ? bi * f * kk[i][j] : 0.0f;
+        y[e] = j <= i ? qi * f * qk[i][j] : 0.0f;
       }
-      for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(sum, off);
-        if (lane >= off) sum += o;
-      }
-      total[lane] = sum;
-      beta[lane] = w;
-      const double last = __shfl(sum, 63);
-      const float fade = expf(static_cast<float>(sum));
-      factors[lane] = w;
-      factors[kChunk + lane] = w * fade * rk[lane];
-      factors[2 * kChunk + lane] = rk[lane] * kLength * expf(static_cast<float>(last - sum));
-      factors[3 * kChunk + lane] = rq[lane] * fade * kUnit;
-      if (lane == 0) factors[4 * kChunk] = expf(static_cast<float>(last));
+      *reinterpret_cast<f32x4 *>(&m[i][m0 + g * 4]) = f32x4{x[0], x[1], x[2], x[3]};
+      if (used) put_operand(y, 1, g);
     }
-    lds_barrier();
-    {  // L, and P as operands: sixteen columns of one row a thread
-      const int i = tid >> 2, m0 = (tid & 3) * 16;
-      const double ti = total[i];
-      const float bi = beta[i] * rk[i], qi = rq[i] * kUnit;
-      _Float16 *block = to + 2 * 8 * kBlock + ((i >> 4) * 2 + (m0 >> 5)) * kBlock + (i & 15) * 8 + (m0 >> 4 & 1) * 4;
+  }
+  lds_barrier();
+  {  // a lane solves for column r of its wave's block
+    float x[16];
+    const int at = mine * 16;
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        float x[4], y[4];
+    for (int i = 0; i < 16; ++i) {
+      float sum = i == r ? 1.0f : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = m0 + h * 4 + e;
-          const float f = j <= i ? expf(static_cast<float>(ti - total[j])) * rk[j] : 0.0f;
-          x[e] = j < i ? bi * f * kk[i][j] : 0.0f;
-          y[e] = j <= i ? qi * f * qk[i][j] : 0.0f;
-        }
-        *reinterpret_cast<f32x4 *>(&m[i][m0 + h * 4]) = f32x4{x[0], x[1], x[2], x[3]};
-        half4 high, low;
-        split(y, high, low);
-        *reinterpret_cast<half4 *>(block + h * 128) = high;
-        *reinterpret_cast<half4 *>(block + 8 * kBlock + h * 128) = low;
-      }
+      for (int j = 0; j < i; ++j) sum -= m[at + i][at + j] * x[j];
+      x[i] = sum;
     }
-    lds_barrier();
-    {  // the largest value
-      const T *from = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv;
-      float x = 0.0f;
-      for (int i = tid; i < c.rows * (a.dv / 8); i += kChunkThreads) {
-        const int row = i / (a.dv / 8);
-        T y[8];
-        load_row<T, 8>(from + row * a.v_stride + (i - row * (a.dv / 8)) * 8, a.wide, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf(static_cast<float>(y[e])));
-      }
-      x = most_of_wave(x);
-      if (lane == 0) most[wave] = x;
-    }
-    lds_barrier();
-    if (tid == 0) factors[4 * kChunk + 1] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-    const int r = lane & 15, h = lane >> 4;
-    {  // the inverses of the 16 x 16 blocks on the diagonal, one a wave: a lane solves for column r
-      float x[16];
-      const int at = wave * 16;
+    for (int i = 0; i < 16; ++i)
+      if (h == i >> 2) m[at + i][at + r] = x[i];
+  }
+  lds_barrier();
+  auto times = [&](int row, int col, const f32x4 &right, f32x4 sum) {
+    const f32x4 left = *reinterpret_cast<const f32x4 *>(&m[row * 16 + r][col * 16 + h * 4]);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float sum = i == r ? 1.0f : 0.0f;
+    for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(left[e], right[e], sum, 0, 0, 0);
+    return sum;
+  };
+  auto block_of = [&](int row, int col) {
+    return f32x4{m[row * 16 + h * 4][col * 16 + r], m[row * 16 + h * 4 + 1][col * 16 + r],
+                 m[row * 16 + h * 4 + 2][col * 16 + r], m[row * 16 + h * 4 + 3][col * 16 + r]};
+  };
+  auto put = [&](int row, int col, const f32x4 &x) {
 #pragma unroll
-        for (int j = 0; j < i; ++j) sum -= m[at + i][at + j] * x[j];
-        x[i] = sum;
-      }
+    for (int e = 0; e < 4; ++e) m[row * 16 + h * 4 + e][col * 16 + r] = -x[e];
+  };
+  if (mine < 2) {
+    const int at = mine * 2;
+    const f32x4 x = times(at + 1, at, block_of(at, at), f32x4{});
+    put(at + 1, at, times(at + 1, at + 1, x, f32x4{}));
+  }
+  lds_barrier();
+  f32x4 low0 = {}, low1 = {};
+  if (mine < 2) {
+    const f32x4 t0 = mine ? f32x4{} : block_of(0, 0), t1 = block_of(1, mine);
+    const f32x4 x0 = times(2, 1, t1, times(2, 0, t0, f32x4{})), x1 = times(3, 1, t1, times(3, 0, t0, f32x4{}));
+    low0 = times(2, 2, x0, f32x4{});
+    low1 = times(3, 3, x1, times(3, 2, x0, f32x4{}));
+  }
+  lds_barrier();
+  if (mine < 2) put(2, mine, low0), put(3, mine, low1);
+  lds_barrier();
+  if (!used) return;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (h == i >> 2) m[at + i][at + r] = x[i];
-    }
-    lds_barrier();
-    // -T22 (L21 T11) joins two inverses; in fp32 products of 16 x 16 x 4, whose result is the second's operand
-    auto times = [&](int row, int col, const f32x4 &right, f32x4 sum) {
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(&m[i][m0 + g * 4]);
+    float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m[row * 16 + r][col * 16 + h * 4 + e], right[e], sum, 0, 0, 0);
-      return sum;
-    };
-    auto block_at_ = [&](int row, int col) {
-      return f32x4{m[row * 16 + h * 4][col * 16 + r], m[row * 16 + h * 4 + 1][col * 16 + r],
-                   m[row * 16 + h * 4 + 2][col * 16 + r], m[row * 16 + h * 4 + 3][col * 16 + r]};
-    };
-    auto put = [&](int row, int col, const f32x4 &x) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) m[row * 16 + h * 4 + e][col * 16 + r] = -x[e];
-    };
-    if (wave < 2) {
-      const int at = wave * 2;
-      const f32x4 x = times(at + 1, at, block_at_(at, at), f32x4{});
-      put(at + 1, at, times(at + 1, at + 1, x, f32x4{}));
-    }
-    lds_barrier();
-    f32x4 low0 = {}, low1 = {};
-    if (wave < 2) {
-      const f32x4 t0 = wave ? f32x4{} : block_at_(0, 0), t1 = block_at_(1, wave);
-      const f32x4 x0 = times(2, 1, t1, times(2, 0, t0, f32x4{})), x1 = times(3, 1, t1, times(3, 0, t0, f32x4{}));
-      low0 = times(2, 2, x0, f32x4{});
-      low1 = times(3, 3, x1, times(3, 2, x0, f32x4{}));
-    }
-    lds_barrier();
-    if (wave < 2) put(2, wave, low0), put(3, wave, low1);
-    lds_barrier();
-    {
-      const int i = tid >> 2, m0 = (tid & 3) * 16;
-      _Float16 *block = to + ((i >> 4) * 2 + (m0 >> 5)) * kBlock + (i & 15) * 8 + (m0 >> 4 & 1) * 4;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 y = *reinterpret_cast<const f32x4 *>(&m[i][m0 + g * 4]);
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = m0 + g * 4 + e <= i ? y[e] * kUnit : 0.0f;
-        half4 high, low;
-        split(x, high, low);
-        *reinterpret_cast<half4 *>(block + g * 128) = high;
-        *reinterpret_cast<half4 *>(block + 8 * kBlock + g * 128) = low;
-      }
-    }
+    for (int e = 0; e < 4; ++e) x[e] = m0 + g * 4 + e <= i ? y[e] * kUnit : 0.0f;
+    put_operand(x, 0, g);
   }
 }
 
@@ -563,12 +564,13 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   const int64_t mats_at = head_at + (wave * 2 * kBlock + lane * 8) * 2, factors_at = head_at + 4 * 8 * kBlock * 2;
   auto load8 = [](const char *from) { return *reinterpret_cast<const half8 *>(from); };
   auto load4 = [](const char *from) { return *reinterpret_cast<const f32x4 *>(from); };
+  const int second = below ? kBlock * 2 : 0;         // above the diagonal the first step's again, unused
   auto load_mats = [&](const char *from, int which, half8 (&to)[2][2]) {     // term, step
     from += mats_at + which * 16 * kBlock * 2;
 #pragma unroll
     for (int term = 0; term < 2; ++term)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) to[term][e] = load8(from + (term * 8 + e) * kBlock * 2);
+      for (int e = 0; e < 2; ++e) to[term][e] = load8(from + term * 8 * kBlock * 2 + (e ? second : 0));
   };
   auto operand = [&](const _Float16 (&from)[64][8]) { return *reinterpret_cast<const half8 *>(&from[lane][0]); };
   auto mfma = [](const half8 &x, const half8 &y, const f32x4 &sum) {
@@ -797,7 +799,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
 
 // The chunks' rows, fp32, normalised and gated: a workgroup a row, four neighbouring values a lane.
 template <typename TO>
-__global__ __launch_bounds__(kChunkThreads) void delta_gate_kernel(ChunkArgs p) {
+__global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
   const DeltaArgs &a = p.d;
   const Sequence s = find_sequence(a.c, p.first + blockIdx.x, 1, kChunk, 2);
   if (s.b < 0 || s.tokens <= 0) return;
@@ -808,7 +810,7 @@ __global__ __launch_bounds__(kChunkThreads) void delta_gate_kernel(ChunkArgs p) 
   const int width = a.v_heads * a.dv, lanes = a.dv / 4;
   const float *o = reinterpret_cast<const float *>(p.chunks + blockIdx.x * p.at.bytes() + p.at.rows_at()) + static_cast<int64_t>(row) * width;
   const int64_t out_row = static_cast<int64_t>(s.row0) + c.start + row;
-  for (int i = threadIdx.x * 4; i < width; i += kChunkThreads * 4) {   // whole heads: a head's lanes are of one wave
+  for (int i = threadIdx.x * 4; i < width; i += kGateThreads * 4) {   // whole heads: a head's lanes are of one wave
     const f32x4 x = *reinterpret_cast<const f32x4 *>(o + i);
     float sum = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
     for (int off = lanes / 2; off; off >>= 1) sum += __shfl_xor(sum, off);
@@ -853,12 +855,12 @@ int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
   for (int64_t first = 0; first < plan.slots; first += plan.count, ++p.run) {
     p.first = (int)first;
     p.count = (int)std::min<int64_t>(plan.count, plan.slots - first);
-    delta_chunks_kernel<T, DK><<<dim3(p.count, a.k_heads * parts), kChunkThreads, 0, st>>>(p);
+    delta_chunks_kernel<T, DK><<<dim3(p.count, a.k_heads * parts), kPrepareThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
     delta_chain_kernel<T, TO, DK><<<(unsigned)(pairs * (a.dv / 16)), kChainThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
     if (a.z) {
-      delta_gate_kernel<TO><<<dim3(p.count, kChunk), kChunkThreads, 0, st>>>(p);
+      delta_gate_kernel<TO><<<dim3(p.count, kChunk), kGateThreads, 0, st>>>(p);
       RLQ_HIP(hipGetLastError());
     }
   }
