@@ -261,17 +261,22 @@ __device__ __forceinline__ Chunk chunk_of(int n, int kept, int item) {
 }
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // x as two fp16 terms. The barrier keeps the product that x may come from out of the conversion: fused, it
 // is rounded once, and where that differs the second term was that of another first one (one value in
 // ten thousand was off by 2^-11).
 __device__ __forceinline__ void split(const float (&x)[4], half4 &high, half4 &low) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float v = x[i];
-    asm("" : "+v"(v));
-    high[i] = static_cast<_Float16>(v);
-    low[i] = static_cast<_Float16>(v - static_cast<float>(high[i]));
+  for (int i = 0; i < 4; i += 2) {
+    f32x2 v = {x[i], x[i + 1]};
+    asm("" : "+v"(v[0]), "+v"(v[1]));
+    const half2v h = __builtin_convertvector(v, half2v);
+    const f32x2 rest = {__builtin_fmaf(static_cast<float>(h[0]), -1.0f, v[0]), __builtin_fmaf(static_cast<float>(h[1]), -1.0f, v[1])};
+    const half2v l = __builtin_convertvector(rest, half2v);
+    high[i] = h[0], high[i + 1] = h[1];
+    low[i] = l[0], low[i + 1] = l[1];
   }
 }
 
@@ -385,7 +390,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
     if (there) {
       factors[lane] = w;
       factors[kChunk + lane] = w * fade * rk[lane];
-      factors[2 * kChunk + lane] = rk[lane] * kLength * exp2_of(last - sum);
+      factors[2 * kChunk + lane] = rk[lane] * (kLength / kUnit) * exp2_of(last - sum);
       factors[3 * kChunk + lane] = rq[lane] * fade * kUnit;
       if (lane == 0) {
         factors[4 * kChunk] = exp2_of(last);
@@ -519,8 +524,9 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
 constexpr int kChainThreads = 512;
 
 // A workgroup goes through a sequence's chunks with 16 columns of one head's state. Four waves are the chain: each
-// has 16 of a chunk's rows and a quarter of the state's, and S, R and U go between them as operands in LDS, a barrier
-// after each. Four others read the state out (O) beside them, 16 rows each.
+// has 16 of a chunk's rows, K S, R and U; four others read the rows out (Q S and, a step later, P U), 16 rows
+// each; and every wave has a tile of 16 of the state's rows (64 of them: the chain's waves). S, R and U go between
+// the waves as operands in LDS, a barrier after each.
 // Values are held times a power of two that keeps them in fp16's range: with keys of length 1 and beta at most 1 a
 // chunk lengthens a column of S by at most the sum of its values' squares (8 of the largest), and R and U are never
 // larger than a column of S and 9 of the largest value.
@@ -528,10 +534,10 @@ constexpr int kChainThreads = 512;
 // step to arrive; no branch stands between a load and its use, or the wait there would be for all of them.
 template <typename T, typename TO, int DK>
 __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs p) {
-  constexpr int kSteps = DK / 32, kTiles = DK / 64;   // steps over the state's rows, tiles of 16 of them a wave has
+  constexpr int kSteps = DK / 32;   // steps over the state's rows
   const DeltaArgs &a = p.d;
   __shared__ __align__(16) _Float16 sb[2][kSteps][64][8], rb[2][2][64][8], ub[2][2][64][8], wb[2][2][64][8];
-  __shared__ __align__(16) float most[4];
+  __shared__ float most[8];
 
   // workgroups of one head run on one XCD, whose L2 then holds its chunk for all of them
   const int slices = a.dv / 16, xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
@@ -547,252 +553,267 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   const int c1 = static_cast<int>(min((int64_t)chunks, p.first + p.count - base));
   if (c0 >= c1) return;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-  const bool chain = __builtin_amdgcn_readfirstlane(tid >> 6) < 4;
+  const int tid = threadIdx.x, lane = tid & 63, tile = __builtin_amdgcn_readfirstlane(tid >> 6), wave = tile & 3;
+  const bool chain = tile < 4, has_tile = tile < DK / 16;
   const int r = lane & 15, h = lane >> 4, col = slice * 16 + r, row = wave * 16 + h * 4;
   const bool below = wave >= 2;     // rows 32 and on: the second step over a chunk's rows is not above the diagonal
   const int k_head = head / (a.v_heads / a.k_heads), slot = a.slots[b];
-  const bool has_state = slot >= 0 && slot < a.n_slots, stored = has_state && (!a.keep || a.keep[b] > 0);
-  const int64_t in_state = (static_cast<int64_t>(head) * DK + wave * 16 * kTiles + h * 4) * a.dv + col;
+  const bool has_state = slot >= 0 && slot < a.n_slots, stored = has_state && has_tile && (!a.keep || a.keep[b] > 0);
+  const int64_t in_state = (static_cast<int64_t>(head) * DK + tile * 16 + h * 4) * a.dv + col;
   float *state = has_state ? a.state + static_cast<int64_t>(slot) * a.v_heads * DK * a.dv + in_state : nullptr;
 
-  // the places of this head's data in a chunk's
+  // the places of this head's data in a chunk's: a uniform place and a lane's offset of 32 bits
   const int64_t step_bytes = p.at.bytes();
   const char *place = p.chunks + (base + c0 - p.first) * step_bytes;
-  const int64_t rows_at = k_head * p.at.k_head() + (wave * kSteps * kBlock + lane * 8) * 2;
+  const int64_t k_at = k_head * p.at.k_head(), rows_at = k_at + (chain ? 0 : kChunk * DK * 2) + wave * kSteps * kBlock * 2;
+  const int64_t tile_at = k_at + (2 * kChunk * DK + tile * 2 * kBlock) * 2;
   const int64_t head_at = p.at.k_heads * p.at.k_head() + head * p.at.v_head();
-  const int64_t mats_at = head_at + (wave * 2 * kBlock + lane * 8) * 2, factors_at = head_at + 4 * 8 * kBlock * 2;
-  auto load8 = [](const char *from) { return *reinterpret_cast<const half8 *>(from); };
-  auto load4 = [](const char *from) { return *reinterpret_cast<const f32x4 *>(from); };
-  const int second = below ? kBlock * 2 : 0;         // above the diagonal the first step's again, unused
-  auto load_mats = [&](const char *from, int which, half8 (&to)[2][2]) {     // term, step
-    from += mats_at + which * 16 * kBlock * 2;
+  const int64_t mats_at = head_at + ((chain ? 0 : 16) + wave * 2) * kBlock * 2, factors_at = head_at + 4 * 8 * kBlock * 2;
+  const int row_bytes = wave * 16 * 4;          // a wave's rows among 64 factors
+  const int second = below ? kBlock * 2 : 0;    // above the diagonal the first step's again, unused
+  uint32_t lane_at = lane * 16, row_at = h * 16, zero = 0;
+  asm("" : "+v"(zero));             // a vector load, which is waited for with the others
+  auto load8 = [&](const char *from) { return *reinterpret_cast<const half8 *>(from + lane_at); };
+  auto load4 = [&](const char *from) { return *reinterpret_cast<const f32x4 *>(from + row_at); };
+  auto load_pair = [&](const char *from) { return *reinterpret_cast<const f32x2 *>(from + factors_at + 4 * kChunk * 4 + zero); };
+
+  half8 rows[kSteps], mats[2][2], kt[2];      // K and T, or Q and P (term, step); the tile of K^T
+  auto load_rows = [&]() {
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) rows[e] = load8(place + rows_at + e * kBlock * 2);
+  };
+  auto load_mats = [&]() {
 #pragma unroll
     for (int term = 0; term < 2; ++term)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) to[term][e] = load8(from + term * 8 * kBlock * 2 + (e ? second : 0));
+      for (int e = 0; e < 2; ++e) mats[term][e] = load8(place + mats_at + term * 8 * kBlock * 2 + (e ? second : 0));
+  };
+  auto load_tile = [&]() {
+    if (!has_tile) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) kt[e] = load8(place + tile_at + e * kBlock * 2);
   };
   auto operand = [&](const _Float16 (&from)[64][8]) { return *reinterpret_cast<const half8 *>(&from[lane][0]); };
   auto mfma = [](const half8 &x, const half8 &y, const f32x4 &sum) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, sum, 0, 0, 0);
   };
-  // a chunk's 64 x 64 matrix in two terms times 64 x 16 values in two, this wave's rows
-  auto times = [&](const half8 (&x)[2][2], const _Float16 (&y)[2][2][64][8], f32x4 sum) {
-    f32x4 low_sum = {};
+  // this wave's rows times the state
+  auto times_state = [&]() {
+    f32x4 sum = {}, low = {};
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) {
+      sum = mfma(rows[e], operand(sb[0][e]), sum);
+      low = mfma(rows[e], operand(sb[1][e]), low);
+    }
+    return sum + low;
+  };
+  // its rows of a chunk's 64 x 64 matrix in two terms times 64 x 16 values in two
+  auto times_mats = [&](const _Float16 (&y)[2][2][64][8], f32x4 sum) {
     const half8 high = operand(y[0][0]), low = operand(y[1][0]);
-    sum = mfma(x[0][0], high, sum);
-    low_sum = mfma(x[0][0], low, low_sum);
-    low_sum = mfma(x[1][0], high, low_sum);
+    f32x4 low_sum = mfma(mats[0][0], low, f32x4{}), last = mfma(mats[1][0], high, f32x4{});
+    sum = mfma(mats[0][0], high, sum);
     if (below) {
       const half8 high = operand(y[0][1]), low = operand(y[1][1]);
-      sum = mfma(x[0][1], high, sum);
-      low_sum = mfma(x[0][1], low, low_sum);
-      low_sum = mfma(x[1][1], high, low_sum);
+      low_sum = mfma(mats[0][1], low, low_sum);
+      last = mfma(mats[1][1], high, last);
+      sum = mfma(mats[0][1], high, sum);
     }
-    return sum + low_sum;
+    return sum + (low_sum + last);
   };
-  // the power of two that brings what is below `x` under 2^15, and its inverse
-  auto scale_of = [&](float x, float &inverse) {
-    const int ex = max(40, min(254, (int)(__float_as_uint(x) >> 23)));
+  auto give = [&](_Float16 (&to)[2][2][64][8], const float (&x)[4]) {
+    half4 high, low;
+    split(x, high, low);
+    *reinterpret_cast<half4 *>(&to[0][wave >> 1][lane][(wave & 1) * 4]) = high;
+    *reinterpret_cast<half4 *>(&to[1][wave >> 1][lane][(wave & 1) * 4]) = low;
+  };
+  float s[4];
+  auto give_state = [&]() {
+    half4 high, low;
+    split(s, high, low);
+    *reinterpret_cast<half4 *>(&sb[0][tile >> 1][lane][(tile & 1) * 4]) = high;
+    *reinterpret_cast<half4 *>(&sb[1][tile >> 1][lane][(tile & 1) * 4]) = low;
+  };
+
+  float size = 0.0f, inverse, scale, fade, value;   // size: a bound of the length of a column of S
+  // the power of two that brings R, U and S of the next step under 2^15, and its inverse
+  auto set_scale = [&]() {
+    const int ex = max(40, min(254, (int)(__float_as_uint(size + 9.0f * value) >> 23)));
     inverse = __uint_as_float((ex - 14) << 23);
-    return __uint_as_float((268 - ex) << 23);
+    scale = __uint_as_float((268 - ex) << 23);
+  };
+  // a chunk's fade and its largest value; the next one's give the scale of what this one hands on
+  const char *second_place = place + (c0 + 1 < c1 ? step_bytes : 0);
+  f32x2 next = load_pair(place);
+  fade = next[0], value = next[1];
+  next = load_pair(second_place);
+  Chunk c = chunk_of(n, kept, c0);
+  {
+    const float *from = !has_tile ? nullptr : c0 ? p.carry[p.run & 1] + in_state : has_state && cached(a.c, b) > n ? state : nullptr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = from ? from[i * a.dv] : 0.0f;
+      size = fmaxf(size, fabsf(s[i]));
+    }
+    size = most_of_wave(size);
+    if (lane == 0) most[tile] = size;
+  }
+  load_rows();
+  load_mats();
+  load_tile();
+  lds_barrier();
+  size = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) size = fmaxf(size, most[i]);
+  size *= DK == 128 ? 11.32f : 8.0f;
+  set_scale();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] *= scale;
+  if (has_tile) give_state();
+
+  // S <- fade S + K^T W, of this wave's tile, and the next chunk's scale
+  auto update_state = [&](int at) {
+    const float faded = fade * kLength, back = inverse * (1.0f / kLength);
+    f32x4 sum, low = {};
+    if (has_tile) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = faded * s[i];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sum = mfma(kt[e], operand(wb[0][e]), sum);
+        low = mfma(kt[e], operand(wb[1][e]), low);
+      }
+      load_tile();
+    }
+    size = fade * size + 8.0f * value;
+    fade = next[0], value = next[1];
+    asm("" : "+v"(fade), "+v"(value));     // registers of their own: those of a load stay its own from step to step
+    set_scale();
+    second_place += at + 2 < c1 ? step_bytes : 0;
+    next = load_pair(second_place);
+    if (has_tile) {
+      sum += low;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = sum[i] * (back * scale);
+      give_state();
+      if (at + 1 == kept_chunks && stored) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) state[i * a.dv] = sum[i] * back;
+      }
+      if (at + 1 == c1 && at + 1 < chunks) {
+        float *to = p.carry[(p.run + 1) & 1] + in_state;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i * a.dv] = sum[i] * back;
+      }
+    }
   };
 
-  float s[kTiles][4], size = 0.0f;   // size: a bound of the length of a column of S
   if (chain) {
-    const float *from = c0 ? p.carry[p.run & 1] + in_state : has_state && cached(a.c, b) > n ? state : nullptr;
-#pragma unroll
-    for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[e][i] = from ? from[(e * 16 + i) * a.dv] : 0.0f;
-#pragma unroll
-    for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) size = fmaxf(size, fabsf(s[e][i]));
-    size = most_of_wave(size);
-    if (lane == 0) most[wave] = size;
-  }
-  f32x4 about = load4(place + factors_at + 4 * kChunk * 4);          // the chunk's fade and its largest value
-  Chunk c = chunk_of(n, kept, c0);
-  lds_barrier();
-  size = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * (DK == 128 ? 11.32f : 8.0f);
-  float inverse, scale = scale_of(size + 9.0f * about[1], inverse);
-
-  if (chain) {
-    half8 k[kSteps], t[2][2], kt[kTiles][2];
     f32x4 take, seen, left;            // factors of this wave's rows of V, K S and U
-    T v[4], v_next[4];
-    const T *values = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + col;
-    auto load_values = [&](int start, T (&to)[4]) {                  // behind the sequence its last row again
+    T v[4];
+    const T *values = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + slice * 16;
+    int64_t value_at[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) to[i] = values[min(start + row + i, n - 1) * a.v_stride];
-    };
-    auto load_rows = [&](const char *from) {
+    for (int i = 0; i < 4; ++i) value_at[i] = (row + i) * a.v_stride + r;
+    auto load_values = [&](int start) {                              // behind the chunk's rows its last one again
+      const int end = start < kept ? kept : n;
+      const T *from = values + start * a.v_stride;
+      if (start + kChunk <= end) {
 #pragma unroll
-      for (int e = 0; e < kSteps; ++e) k[e] = load8(from + rows_at + e * kBlock * 2);
-      take = load4(from + factors_at + row * 4);
-      seen = load4(from + factors_at + (kChunk + row) * 4);
-    };
-    auto load_left = [&](const char *from) {
-      load_mats(from, 0, t);
-      left = load4(from + factors_at + (2 * kChunk + row) * 4);
-    };
-    auto load_last = [&](const char *from) {
-      from += k_head * p.at.k_head() + (2 * kChunk * DK + wave * kTiles * 2 * kBlock + lane * 8) * 2;
+        for (int i = 0; i < 4; ++i) v[i] = from[value_at[i]];
+      } else {
 #pragma unroll
-      for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) kt[e][u] = load8(from + (e * 2 + u) * kBlock * 2);
-    };
-    auto give = [&](_Float16 (&to)[2][2][64][8], const float (&x)[4]) {
-      half4 high, low;
-      split(x, high, low);
-      *reinterpret_cast<half4 *>(&to[0][wave >> 1][lane][(wave & 1) * 4]) = high;
-      *reinterpret_cast<half4 *>(&to[1][wave >> 1][lane][(wave & 1) * 4]) = low;
-    };
-    auto give_state = [&]() {
-#pragma unroll
-      for (int e = 0; e < kTiles; ++e) {
-        half4 high, low;
-        split(s[e], high, low);
-        const int part = wave * kTiles + e;
-        *reinterpret_cast<half4 *>(&sb[0][part >> 1][lane][(part & 1) * 4]) = high;
-        *reinterpret_cast<half4 *>(&sb[1][part >> 1][lane][(part & 1) * 4]) = low;
+        for (int i = 0; i < 4; ++i) v[i] = values[min(start + row + i, end - 1) * a.v_stride + r];
       }
     };
-    load_values(c.start, v);
-    load_values(c.start + c.rows, v_next);
-    load_rows(place);
-    load_left(place);
-    load_last(place);
-#pragma unroll
-    for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[e][i] *= scale;
-    give_state();
+    auto load_factors = [&]() {
+      take = load4(place + factors_at + row_bytes);
+      seen = load4(place + factors_at + kChunk * 4 + row_bytes);
+    };
+    load_factors();
+    load_values(c.start);
+    left = load4(place + factors_at + 2 * kChunk * 4 + row_bytes);
+    __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0): the loop's own waits are then for loads of a step before
+    __builtin_amdgcn_s_setprio(2);           // the other waves have slack
     lds_barrier();
 
     for (int at = c0; at < c1; ++at) {
       place += at + 1 < c1 ? step_bytes : 0;             // the last chunk's data come again, unused
-      const int start = c.start + c.rows, rows = min(kChunk, (start < kept ? kept : n) - start);
-      f32x4 ks = {}, ks_low = {};
+      const f32x4 ks = times_state();
+      float x[4], w[4];
 #pragma unroll
-      for (int e = 0; e < kSteps; ++e) {
-        ks = mfma(k[e], operand(sb[0][e]), ks);
-        ks_low = mfma(k[e], operand(sb[1][e]), ks_low);
-      }
-      float x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float mine = row + i < c.rows ? static_cast<float>(v[i]) : 0.0f;
-        x[i] = take[i] * (mine * scale) - seen[i] * (ks[i] + ks_low[i]);
-        v[i] = v_next[i];
-      }
+      for (int i = 0; i < 4; ++i) x[i] = take[i] * (static_cast<float>(v[i]) * scale) - seen[i] * ks[i];   // take: 0 behind the rows
       give(rb, x);
-      load_rows(place);
-      load_values(start + rows, v_next);
+      c.start += c.rows;
+      c.rows = min(kChunk, (c.start < kept ? kept : n) - c.start);
+      load_rows();
+      load_factors();
+      load_values(c.start);
       lds_barrier();
 
-      const f32x4 u = times(t, rb, f32x4{});
-      float w[4];
+      const f32x4 u = times_mats(rb, f32x4{});
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[i] = u[i] * (1.0f / kUnit);
-        w[i] = left[i] * x[i];
+        w[i] = left[i] * u[i];
       }
       give(wb, w);
       give(ub, x);
-      load_left(place);
-      const float fade = about[0];
-      size = fade * size + 8.0f * about[1];
-      about = load4(place + factors_at + 4 * kChunk * 4);
+      load_mats();
+      left = load4(place + factors_at + 2 * kChunk * 4 + row_bytes);
       lds_barrier();
 
-      f32x4 sum[kTiles];
-#pragma unroll
-      for (int e = 0; e < kTiles; ++e) {
-        f32x4 low = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[e][i] = (fade * kLength) * s[e][i];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          sum[e] = mfma(kt[e][u], operand(wb[0][u]), sum[e]);
-          low = mfma(kt[e][u], operand(wb[1][u]), low);
-        }
-        sum[e] += low;
-      }
-      load_last(place);
-      const float back = inverse * (1.0f / kLength);
-      scale = scale_of(size + 9.0f * about[1], inverse);
-#pragma unroll
-      for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[e][i] = sum[e][i] * (back * scale);
-      give_state();
-      float *to = at + 1 == kept_chunks && stored ? state : nullptr;
-      float *on = at + 1 == c1 && at + 1 < chunks ? p.carry[(p.run + 1) & 1] + in_state : nullptr;
-      if (to || on) {
-#pragma unroll
-        for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (to) to[(e * 16 + i) * a.dv] = sum[e][i] * back;
-            if (on) on[(e * 16 + i) * a.dv] = sum[e][i] * back;
-          }
-      }
-      c = {start, rows};
+      update_state(at);
       lds_barrier();
     }
   } else {
-    half8 q[kSteps], pm[2][2];
-    f32x4 read;                        // factors of this wave's rows of Q S
-    auto load_rows = [&](const char *from) {
-#pragma unroll
-      for (int e = 0; e < kSteps; ++e) q[e] = load8(from + rows_at + (kChunk * DK + e * kBlock) * 2);
-    };
-    auto load_last = [&](const char *from) {
-      load_mats(from, 1, pm);
-      read = load4(from + factors_at + (3 * kChunk + row) * 4);
-    };
-    load_rows(place);
-    load_last(place);
+    f32x4 read = load4(place + factors_at + 3 * kChunk * 4 + row_bytes), qs = {};      // factors of this wave's rows of Q S
     const int64_t width = a.z ? static_cast<int64_t>(a.v_heads) * a.dv : a.out_stride;
     float *scratch = reinterpret_cast<float *>(p.chunks + (base + c0 - p.first) * step_bytes + p.at.rows_at()) + row * width +
                      head * a.dv + col;
     TO *out = static_cast<TO *>(a.out) + (static_cast<int64_t>(row0) + c.start + row) * a.out_stride + head * a.dv + col;
+    float unit = 0.0f;
+    // the rows of the chunk whose U lies in LDS
+    auto finish = [&]() {
+      const f32x4 o = times_mats(ub, read * qs) * unit;
+      if (a.z) {
+        if (c.rows == kChunk) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) scratch[i * width] = o[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row + i < c.rows) scratch[i * width] = o[i];
+        }
+        scratch = reinterpret_cast<float *>(reinterpret_cast<char *>(scratch) + step_bytes);
+      } else {
+        if (c.rows == kChunk) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) out[i * width] = static_cast<TO>(o[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row + i < c.rows) out[i * width] = static_cast<TO>(o[i]);
+        }
+        out += c.rows * width;
+      }
+      c.start += c.rows;
+      c.rows = min(kChunk, (c.start < kept ? kept : n) - c.start);
+    };
+    __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0), as above
     lds_barrier();
 
     for (int at = c0; at < c1; ++at) {
       place += at + 1 < c1 ? step_bytes : 0;
-      f32x4 qs = {}, qs_low = {};
-#pragma unroll
-      for (int e = 0; e < kSteps; ++e) {
-        qs = mfma(q[e], operand(sb[0][e]), qs);
-        qs_low = mfma(q[e], operand(sb[1][e]), qs_low);
-      }
-      load_rows(place);
       lds_barrier();
-      const float unit = a.scale * (1.0f / kUnit) * inverse;
-      size = about[0] * size + 8.0f * about[1];
-      about = load4(place + factors_at + 4 * kChunk * 4);
+      qs = times_state();
+      unit = a.scale * (1.0f / kUnit) * inverse;
+      load_rows();
       lds_barrier();
-      const f32x4 o = times(pm, ub, read * (qs + qs_low)) * unit;
-      load_last(place);
-      scale = scale_of(size + 9.0f * about[1], inverse);
-      lds_barrier();        // nothing of LDS is read behind it: the rows are stored beside the next step
-      if (a.z) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (row + i < c.rows) scratch[i * width] = o[i];
-        scratch = reinterpret_cast<float *>(reinterpret_cast<char *>(scratch) + step_bytes);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (row + i < c.rows) out[i * width] = static_cast<TO>(o[i]);
-        out += c.rows * width;
-      }
-      const int start = c.start + c.rows;
-      c = {start, min(kChunk, (start < kept ? kept : n) - start)};
+      update_state(at);
+      lds_barrier();
+      finish();              // beside the chain's next K S
+      load_mats();
+      read = load4(place + factors_at + 3 * kChunk * 4 + row_bytes);
     }
   }
 }
