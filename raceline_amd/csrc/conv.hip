@@ -61,19 +61,16 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
   const bool has_state = slot >= 0 && slot < a.n_slots;
   float *state = a.state + (has_state ? static_cast<int64_t>(slot) * (TAPS - 1) * a.channels + c0 : 0);
 
-  // behind a short run its last row again: without branches all loads are on their way at once
+  // no branch stands between the loads, so all are on their way at once: behind a short run its last row comes
+  // again, in front of a sequence without a state its first
   Floats<VEC> in[TAPS - 1 + RUN];
+  const bool begins = t0 == 0, from_state = begins && has_state && s.kv > s.tokens;
+  const float *before = from_state ? state : begins ? x : x + (t0 - (TAPS - 1)) * a.x_stride;   // a run is longer than the taps
+  const int64_t step = from_state ? a.channels : begins ? 0 : a.x_stride;
+#pragma unroll
+  for (int j = 0; j < TAPS - 1; ++j) in[j] = load_floats<VEC>(before + j * step);
 #pragma unroll
   for (int i = 0; i < RUN; ++i) in[TAPS - 1 + i] = load_floats<VEC>(x + (t0 + min(i, tokens - 1)) * a.x_stride);
-#pragma unroll
-  for (int j = 0; j < TAPS - 1; ++j) {
-    in[j] = {};
-    if (t0) {
-      in[j] = load_floats<VEC>(x + (t0 - (TAPS - 1) + j) * a.x_stride);   // a run is longer than the taps
-    } else if (has_state && s.kv > s.tokens) {
-      in[j] = load_floats<VEC>(state + static_cast<int64_t>(j) * a.channels);
-    }
-  }
   float w[VEC][TAPS], bias[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
@@ -88,7 +85,11 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
     }
   }
   __builtin_amdgcn_sched_barrier(0);   // the compiler would put each load in front of its use
-  if (t0 == 0 && has_state) {
+  if (begins && !from_state) {
+#pragma unroll
+    for (int j = 0; j < TAPS - 1; ++j) in[j] = {};
+  }
+  if (begins && has_state) {
     // after `end` tokens: inputs end - (TAPS-1) .. end - 1, from the old state where that is negative
     const int end = a.keep ? max(0, min(a.keep[s.b], s.tokens)) : s.tokens;
     if (end) {
@@ -108,22 +109,21 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(ConvArgs a) {
       for (int j = 0; j < TAPS - 1; ++j) store_floats<VEC>(state + static_cast<int64_t>(j) * a.channels, now[j]);
     }
   }
+  const bool silu = a.silu;
   T *out = static_cast<T *>(a.out) + (s.row0 + t0) * a.out_stride + c0;
 #pragma unroll
   for (int i = 0; i < RUN; ++i) {
-    if (i >= tokens) break;
     T y[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       float sum = bias[e];
 #pragma unroll
       for (int j = 0; j < TAPS; ++j) sum += w[e][j] * in[i + j].v[e];
-      if (a.silu) {
-        const float t = __expf(-fabsf(sum));          // at most 1: no overflow on either side
-        sum *= (sum >= 0.0f ? 1.0f : t) / (1.0f + t);
-      }
-      y[e] = static_cast<T>(sum);
+      // at most 1: no overflow on either side; formed for every row, so that no branch stands between them
+      const float t = __expf(-fabsf(sum)), f = (sum >= 0.0f ? 1.0f : t) * __builtin_amdgcn_rcpf(1.0f + t);
+      y[e] = static_cast<T>(sum * (silu ? f : 1.0f));
     }
+    if (i >= tokens) continue;
     if constexpr (VEC == 4) {
       typedef T pack4 __attribute__((ext_vector_type(4)));
       *reinterpret_cast<pack4 *>(out + i * a.out_stride) = pack4{y[0], y[1], y[2], y[3]};
