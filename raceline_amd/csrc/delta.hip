@@ -2,6 +2,7 @@
 // faded by each token and corrected towards its value at its key, and read at its query; the rows
 // normalised and gated for the out projection. Plays the parts of lin_prep_qk, lin_gates, gated_delta and
 // lin_out_norm (kernels/ops.metal:320,338,362,424, dispatched by src/engine.mm:1086-1154).
+#include "lanes.h"
 #include "paged.h"
 #include "../../include/rlq.h"
 
@@ -32,26 +33,6 @@ __device__ __forceinline__ float log_fade(float a, float dt_bias, float rate) {
 __device__ __forceinline__ float sigmoid(float x) {
   const float t = expf(-fabsf(x));
   return (x >= 0.0f ? 1.0f : t) / (1.0f + t);
-}
-
-// Sums over the lanes that differ in bits 3 to 5 (0 to 2) of their number; every lane gets the sum.
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
-}
-
-__device__ __forceinline__ float sum_high(float x) {
-  x += dpp<0x128>(x);   // row_ror:8
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-__device__ __forceinline__ float sum_low(float x) {
-  x += dpp<0xB1>(x);    // quad_perm 1 0 3 2
-  x += dpp<0x4E>(x);    // quad_perm 2 3 0 1
-  return x + dpp<0x141>(x);   // row_half_mirror
 }
 
 template <typename T, int N>
@@ -278,17 +259,6 @@ __device__ __forceinline__ void split(const float (&x)[4], half4 &high, half4 &l
     high[i] = h[0], high[i + 1] = h[1];
     low[i] = l[0], low[i + 1] = l[1];
   }
-}
-
-__device__ __forceinline__ float most_of_wave(float x) {
-  x = fmaxf(x, dpp<0xB1>(x));
-  x = fmaxf(x, dpp<0x4E>(x));
-  x = fmaxf(x, dpp<0x141>(x));
-  x = fmaxf(x, dpp<0x128>(x));
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // 2^x; what x loses in fp32 is nothing beside 2^x where x is large.
