@@ -438,7 +438,8 @@ int rlq_causal_conv(const float *x, int x_stride, int T, int channels, int taps,
  * rlq_causal_conv's rows, say); a, b fp32 [T][stride], v_heads a row; a_log, dt_bias fp32 [v_heads]; z fp32
  * [T][z_stride]; norm fp32 [Dv]; out 16-bit (out_dtype) [T][out_stride]. state fp32
  * [n_slots][v_heads][Dk][Dv], 16-byte aligned. Dk 64 or 128; Dv 64, 128 or 256; v_heads a multiple of
- * k_heads. State, products and sums in fp32; rows of q and k have lengths below 2^63.
+ * k_heads; eps and norm_eps at least 1e-37. State, products and sums in fp32; rows of q and k have
+ * lengths below 2^63.
  * max_q (host) bounds the rows of a sequence: it chooses between the rule token by token and its form in
  * chunks of 64 tokens, and results stay right past it. The workspace
  * (rlq_gated_delta_workspace_bytes, may be 0; 16-byte aligned, no initialisation) holds what the chunks

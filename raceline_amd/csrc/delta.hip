@@ -35,6 +35,12 @@ __device__ __forceinline__ float sigmoid(float x) {
   return (x >= 0.0f ? 1.0f : t) / (1.0f + t);
 }
 
+// z sigmoid(z), to a few roundings of fp32: the rows it gates are rounded to 16 bits.
+__device__ __forceinline__ float gate_of(float z) {
+  const float t = __expf(-fabsf(z));
+  return z * ((z >= 0.0f ? 1.0f : t) * __builtin_amdgcn_rcpf(1.0f + t));
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void load_row(const T *p, bool wide, T (&x)[N]) {
   constexpr int kPack = N < 8 ? N : 8;
@@ -71,6 +77,8 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
   float *state = a.state + (has_state ? (static_cast<int64_t>(slot) * a.v_heads + head) * DK * a.dv + k0 * a.dv + col : 0);
   const int end = has_state ? (a.keep ? max(0, min(a.keep[b], n)) : n) : 0;
 
+  const float *ap = a.a + row0 * a.a_stride + head, *bp = a.b + row0 * a.b_stride + head;
+  float fades = ap[min(lane, n - 1) * a.a_stride], betas = bp[min(lane, n - 1) * a.b_stride];   // of 64 tokens, one a lane
   float s[kRows][4];
   if (has_state && cached(a.c, b) > n) {
 #pragma unroll
@@ -88,7 +96,6 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
   const T *qp = static_cast<const T *>(a.q) + row0 * a.q_stride + k_head * DK + k0;
   const T *kp = static_cast<const T *>(a.k) + row0 * a.k_stride + k_head * DK + k0;
   const T *vp = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + col;
-  const float *ap = a.a + row0 * a.a_stride + head, *bp = a.b + row0 * a.b_stride + head;
   const float *zp = a.z ? a.z + row0 * a.z_stride + head * a.dv + col : nullptr;
   TO *op = static_cast<TO *>(a.out) + row0 * a.out_stride + head * a.dv + col;
   const float rate = expf(a.a_log[head]), dt_bias = a.dt_bias[head];
@@ -100,13 +107,12 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
   // a token's rows are on their way while the one in front is worked on
   struct Rows {
     T q[kRows], k[kRows], v[4];
-    float a, b, z[4];
+    float z[4];
   };
   auto fetch = [&](int t, Rows &x) {
     load_row<T, kRows>(qp + t * a.q_stride, a.wide, x.q);
     load_row<T, kRows>(kp + t * a.k_stride, a.wide, x.k);
     load_row<T, 4>(vp + t * a.v_stride, a.wide, x.v);
-    x.a = ap[t * a.a_stride], x.b = bp[t * a.b_stride];
     if (zp) {
       if (a.wide_z) {
         const f32x4 y = *reinterpret_cast<const f32x4 *>(zp + t * a.z_stride);
@@ -121,18 +127,24 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
   Rows next;
   fetch(0, next);
   for (int t = 0; t < n; ++t) {
+    if ((t & 63) == 0) {
+      if (t) fades = ap[min(t + lane, n - 1) * a.a_stride], betas = bp[min(t + lane, n - 1) * a.b_stride];
+      fades = expf(log_fade(fades, dt_bias, rate));
+      betas = sigmoid(betas);
+    }
     float q[kRows], k[kRows], v[4], z[4];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) q[i] = static_cast<float>(next.q[i]), k[i] = static_cast<float>(next.k[i]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(next.v[e]), z[e] = next.z[e];
-    const float fade = expf(log_fade(next.a, dt_bias, rate)), beta = sigmoid(next.b);
+    const float fade = __uint_as_float(of_lane(__float_as_uint(fades), t & 63));
+    const float beta = __uint_as_float(of_lane(__float_as_uint(betas), t & 63));
     if (t + 1 < n) fetch(t + 1, next);
     // to length 1 before the products: those of raw rows with a state could pass fp32
     float kk = 0.0f, qq = 0.0f, kq = 0.0f, p[4] = {}, r[4] = {};
 #pragma unroll
     for (int i = 0; i < kRows; ++i) kk += k[i] * k[i], qq += q[i] * q[i];
-    const float rk = 1.0f / sqrtf(sum_high(kk) + a.eps), rq = a.scale / sqrtf(sum_high(qq) + a.eps);
+    const float rk = __builtin_amdgcn_rsqf(sum_high(kk) + a.eps), rq = a.scale * __builtin_amdgcn_rsqf(sum_high(qq) + a.eps);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       k[i] *= rk;
@@ -166,9 +178,9 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
       lds_barrier();          // the other half is free: its last readers are past the barrier before
       float sum = 0.0f;
       for (int i = 0; i < a.dv / 32; ++i) sum += squares[t & 1][i];
-      const float r = 1.0f / sqrtf(sum / a.dv + a.norm_eps);
+      const float r = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + a.norm_eps);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = o[e] * r * w[e] * (z[e] * sigmoid(z[e]));
+      for (int e = 0; e < 4; ++e) o[e] = o[e] * r * w[e] * gate_of(z[e]);
     }
     if (lane < 8) {
       if (a.wide) {
@@ -805,11 +817,11 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
     const f32x4 x = *reinterpret_cast<const f32x4 *>(o + i);
     float sum = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
     for (int off = lanes / 2; off; off >>= 1) sum += __shfl_xor(sum, off);
-    const float f = 1.0f / sqrtf(sum / a.dv + a.norm_eps);
+    const float f = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + a.norm_eps);
     const float *z = a.z + out_row * a.z_stride + i, *w = a.norm + i % a.dv;
     TO *to = static_cast<TO *>(a.out) + out_row * a.out_stride + i;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = static_cast<TO>(x[e] * f * w[e] * (z[e] * sigmoid(z[e])));
+    for (int e = 0; e < 4; ++e) to[e] = static_cast<TO>(x[e] * f * w[e] * gate_of(z[e]));
   }
 }
 
@@ -894,10 +906,11 @@ int rlq_gated_delta(const void *q, int q_stride, const void *k, int k_stride, co
               "rlq_gated_delta: %d value heads do not share %d key heads evenly", v_heads, k_heads);
   RLQ_REQUIRE((int64_t)v_heads * Dv <= INT32_MAX && (int64_t)B * v_heads <= INT32_MAX,
               "rlq_gated_delta: %d heads of %d sequences are too many", v_heads, B);
-  RLQ_REQUIRE(eps > 0 && std::isfinite(eps), "rlq_gated_delta: eps=%g must be above 0", eps);
+  RLQ_REQUIRE(eps >= 1e-37f && std::isfinite(eps), "rlq_gated_delta: eps=%g must be at least 1e-37", eps);
   RLQ_REQUIRE(std::isfinite(scale), "rlq_gated_delta: scale=%g", scale);
   RLQ_REQUIRE((z == nullptr) == (norm == nullptr), "rlq_gated_delta: z and norm come together");
-  RLQ_REQUIRE(!norm || (norm_eps > 0 && std::isfinite(norm_eps)), "rlq_gated_delta: norm_eps=%g must be above 0", norm_eps);
+  RLQ_REQUIRE(!norm || (norm_eps >= 1e-37f && std::isfinite(norm_eps)), "rlq_gated_delta: norm_eps=%g must be at least 1e-37",
+              norm_eps);
   RLQ_REQUIRE(n_slots >= 0 && max_q >= 0, "rlq_gated_delta: n_slots=%d, max_q=%d", n_slots, max_q);
   if (T == 0 || B == 0) return 0;
   RLQ_REQUIRE(q && k && v && a && b && a_log && dt_bias && out && cu_q && kv_len && slots, "rlq_gated_delta: null pointer");

@@ -380,25 +380,34 @@ __device__ uint64_t cut_list(Load load, Listed &x, int rounds, int first, int la
   __shared__ uint64_t found[4];
   const int tid = threadIdx.x;
   auto taken = [&](int e) { return x.place[e] && x.bin[e] >= first && x.bin[e] <= last && x.place[e] >= from; };
-  if (tid == 0) found[2] = found[3] = 0;
+  if (tid == 0) found[0] = found[2] = found[3] = 0;
   lds_barrier();
   uint32_t high = 0, low = 0;              // of the logits; low: the largest complement
+  int count = 0;
   for (int round = 0; round < rounds; ++round) {
     if (rounds > 1) load(round);
 #pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (taken(e)) high = max(high, static_cast<uint32_t>(x.place[e] >> 32)), low = max(low, ~static_cast<uint32_t>(x.place[e] >> 32));
+    for (int e = 0; e < kEach; ++e) {
+      const bool one = taken(e);
+      count += __popcll(__ballot(one));
+      if (!one) continue;
+      high = max(high, x.key[e]), low = max(low, ~x.key[e]);
+      found[1] = x.place[e];
+    }
   }
   high = most_of_wave(high), low = most_of_wave(low);
-  if ((tid & 63) == 0 && high) {
+  if ((tid & 63) == 0 && count) {
     atomicMax(reinterpret_cast<uint32_t *>(&found[2]), low);
     atomicMax(reinterpret_cast<uint32_t *>(&found[3]), high);
+    add(&found[0], count);
   }
   lds_barrier();
+  if (found[0] == 1) return found[1];      // a bin of its own, as the likeliest tokens have
   low = ~static_cast<uint32_t>(found[2]), high = static_cast<uint32_t>(found[3]);
   int open = 32 + (low == high ? 0 : 32 - __builtin_clz(low ^ high));     // bits that are not known
   uint64_t prefix = static_cast<uint64_t>(high) << 32;
   prefix = open < 64 ? prefix >> open : 0;
+  lds_barrier();
   while (open) {
     const int width = min(open, kDigit), shift = open - width;
     hist[tid] = 0, hist[tid + kSampleThreads] = 0;
