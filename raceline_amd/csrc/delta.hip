@@ -287,8 +287,8 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
   // rows of k and q, then, when they have been read, L and its inverse of both heads
   __shared__ __align__(16) char pool[kHeadsPer * kChunk * kMatPad * 4];
   __shared__ __align__(16) float kk[kChunk][kMatPad], qk[kChunk][kMatPad];
-  __shared__ double totals[kHeadsPer][kChunk];
-  __shared__ float rk[kChunk], rq[kChunk], betas[kHeadsPer][kChunk], most[kHeadsPer][4];
+  __shared__ __align__(16) double totals[kHeadsPer][kChunk];
+  __shared__ __align__(16) float rk[kChunk], rq[kChunk], betas[kHeadsPer][kChunk], most[kHeadsPer][4];
   static_assert(2 * kChunk * kPad * 2 <= (int)sizeof(pool), "the rows fit");
   _Float16(*ks)[kPad] = reinterpret_cast<_Float16(*)[kPad]>(pool), (*qs)[kPad] = ks + kChunk;
 
@@ -434,13 +434,16 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
     const float bi = betas[half][i] * rk[i], qi = rq[i] * kUnit;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
+      // without branches: above the diagonal what was read is thrown away
+      const int j0 = m0 + g * 4;
+      const f32x4 kr = *reinterpret_cast<const f32x4 *>(&kk[i][j0]), qr = *reinterpret_cast<const f32x4 *>(&qk[i][j0]);
+      const f32x4 r4 = *reinterpret_cast<const f32x4 *>(&rk[j0]);
       float x[4], y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int j = m0 + g * 4 + e;
-        const float f = j <= i ? exp2_of(ti - total[j]) * rk[j] : 0.0f;
-        x[e] = j < i ? bi * f * kk[i][j] : 0.0f;
-        y[e] = j <= i ? qi * f * qk[i][j] : 0.0f;
+        const float f = exp2_of(ti - total[j0 + e]) * r4[e], l = bi * f * kr[e], m = qi * f * qr[e];
+        x[e] = j0 + e < i ? l : 0.0f;
+        y[e] = j0 + e <= i ? m : 0.0f;
       }
       *reinterpret_cast<f32x4 *>(&m[i][m0 + g * 4]) = f32x4{x[0], x[1], x[2], x[3]};
       if (used) put_operand(y, 1, g);
