@@ -207,19 +207,20 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
 //
 // The products are to keep the state to fp32: rows of q and k, brought to a length of 2^13 .. 2^14 by a power of
 // two, are exact in fp16 (what bf16 loses there lies 2^-38 below the length); T, P, R, U and S are two fp16
-// terms (2^-22), T and P, at most 1, times 2^14, so that what has faded keeps its bits. Operands stand in the order in which sums leave the matrix cores: slot 8 h + 4 a + b of a step of
+// terms (2^-22), T, at most 1, times 2^14, and P before the length of q is taken out, so that what has faded
+// keeps its bits. Operands stand in the order in which sums leave the matrix cores: slot 8 h + 4 a + b of a step of
 // 32 is row 16 a + 4 h + b, so that what a lane holds of a result is what it holds of the next product.
 
 constexpr int kChunk = 64, kGateThreads = 256, kHeadsPer = 2, kPrepareThreads = 256 * kHeadsPer, kMatPad = 68;
 constexpr int kBlock = 64 * 8;                       // halves of a 16 x 32 operand
-constexpr float kUnit = 16384.0f, kLength = 8192.0f; // T and P are held times kUnit, rows of q and k at this length or twice it
+constexpr float kUnit = 16384.0f, kLength = 8192.0f; // T is held times kUnit, rows of q and k at this length or twice it
 constexpr int64_t kMostScratch = 256 << 20;
 
 // What a chunk leaves for the chain, in bytes from its place.
 struct ChunkLayout {
   int dk, k_heads, v_heads, dv;
   __host__ __device__ int64_t k_head() const { return 3 * kChunk * dk * 2; }       // K, Q, K^T
-  __host__ __device__ int64_t v_head() const { return 4 * 8 * kBlock * 2 + 5 * kChunk * 4; }   // T, P (two terms), factors
+  __host__ __device__ int64_t v_head() const { return 4 * 8 * kBlock * 2 + 6 * kChunk * 4; }   // T, P (two terms), factors
   __host__ __device__ int64_t rows_at() const { return k_heads * k_head() + v_heads * v_head(); }
   __host__ __device__ int64_t bytes() const { return rows_at() + (int64_t)kChunk * v_heads * dv * 4; }
   __host__ __device__ int64_t state() const { return (int64_t)v_heads * dk * dv * 4; }
@@ -313,19 +314,29 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       T y[kPer];
-      float x[kPer], sum = 0.0f;
+      float x[kPer], sum = 0.0f, largest = 0.0f;
       const T *from = which ? static_cast<const T *>(a.q) + (row0 + min(row, c.rows - 1)) * a.q_stride
                             : static_cast<const T *>(a.k) + (row0 + min(row, c.rows - 1)) * a.k_stride;
       load_row<T, kPer>(from + k_head * DK + d0, a.wide, y);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         x[i] = row < c.rows ? static_cast<float>(y[i]) : 0.0f;
+        largest = fmaxf(largest, fabsf(x[i]));
+      }
+      largest = fmaxf(largest, dpp<kQuadSwap1>(largest));
+      largest = fmaxf(largest, dpp<kQuadSwap2>(largest));
+      largest = fmaxf(largest, dpp<kHalfMirror>(largest));
+      // to 1 .. 2 by the largest, so that no square passes fp32, then to the length
+      const int ex = max(1, min(253, (int)(__float_as_uint(largest) >> 23)));
+      const float unit = __uint_as_float(ex << 23);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        x[i] *= __uint_as_float((254 - ex) << 23);
         sum += x[i] * x[i];
       }
       sum = sum_low(sum);
-      // the power of two that brings the length to 2^13 .. 2^14, and back
-      const int ex = max(14, min(253, (int)(__float_as_uint(sqrtf(sum)) >> 23)));
-      const float up = __uint_as_float((254 + 13 - ex) << 23), down = __uint_as_float((ex - 13) << 23);
+      const int length = max(127, (int)(__float_as_uint(sqrtf(sum)) >> 23));
+      const float up = __uint_as_float((267 - min(length, 254)) << 23), down = unit * __uint_as_float((min(length, 254) - 13) << 23);
       _Float16 *to = which ? &qs[row][d0] : &ks[row][d0];
 #pragma unroll
       for (int i = 0; i < kPer; i += 8) {
@@ -334,7 +345,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
         for (int j = 0; j < 8; ++j) z[j] = static_cast<_Float16>(x[i + j] * up);
         *reinterpret_cast<half8 *>(to + i) = z;
       }
-      if ((tid & 7) == 0) (which ? rq : rk)[row] = down / sqrtf(sum + a.eps);
+      if ((tid & 7) == 0) (which ? rq : rk)[row] = down / sqrtf(sum * unit * unit + a.eps);
     }
   }
   {  // the largest value of the head
@@ -373,10 +384,11 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
       factors[lane] = w;
       factors[kChunk + lane] = w * fade * rk[lane];
       factors[2 * kChunk + lane] = rk[lane] * (kLength / kUnit) * exp2_of(last - sum);
-      factors[3 * kChunk + lane] = rq[lane] * fade * kUnit;
+      factors[3 * kChunk + lane] = fade;
+      factors[4 * kChunk + lane] = rq[lane];
       if (lane == 0) {
-        factors[4 * kChunk] = exp2_of(last);
-        factors[4 * kChunk + 1] = fmaxf(fmaxf(most[half][0], most[half][1]), fmaxf(most[half][2], most[half][3]));
+        factors[5 * kChunk] = exp2_of(last);
+        factors[5 * kChunk + 1] = fmaxf(fmaxf(most[half][0], most[half][1]), fmaxf(most[half][2], most[half][3]));
       }
     }
   }
@@ -431,7 +443,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
   };
   {  // L, and P as operands
     const double ti = total[i];
-    const float bi = betas[half][i] * rk[i], qi = rq[i] * kUnit;
+    const float bi = betas[half][i] * rk[i];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       // without branches: above the diagonal what was read is thrown away
@@ -441,7 +453,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
       float x[4], y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float f = exp2_of(ti - total[j0 + e]) * r4[e], l = bi * f * kr[e], m = qi * f * qr[e];
+        const float f = exp2_of(ti - total[j0 + e]) * r4[e], l = bi * f * kr[e], m = f * qr[e];
         x[e] = j0 + e < i ? l : 0.0f;
         y[e] = j0 + e <= i ? m : 0.0f;
       }
@@ -560,7 +572,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   asm("" : "+v"(zero));             // a vector load, which is waited for with the others
   auto load8 = [&](const char *from) { return *reinterpret_cast<const half8 *>(from + lane_at); };
   auto load4 = [&](const char *from) { return *reinterpret_cast<const f32x4 *>(from + row_at); };
-  auto load_pair = [&](const char *from) { return *reinterpret_cast<const f32x2 *>(from + factors_at + 4 * kChunk * 4 + zero); };
+  auto load_pair = [&](const char *from) { return *reinterpret_cast<const f32x2 *>(from + factors_at + 5 * kChunk * 4 + zero); };
 
   half8 rows[kSteps], mats[2][2], kt[2];      // K and T, or Q and P (term, step); the tile of K^T
   auto load_rows = [&]() {
@@ -622,7 +634,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   float size = 0.0f, inverse, scale, fade, value;   // size: a bound of the length of a column of S
   // the power of two that brings R, U and S of the next step under 2^15, and its inverse
   auto set_scale = [&]() {
-    const int ex = max(40, min(254, (int)(__float_as_uint(size + 9.0f * value) >> 23)));
+    const int ex = max(15, min(254, (int)(__float_as_uint(size + 9.0f * value) >> 23)));
     inverse = __uint_as_float((ex - 14) << 23);
     scale = __uint_as_float((268 - ex) << 23);
   };
@@ -751,7 +763,12 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
       lds_barrier();
     }
   } else {
-    f32x4 read = load4(place + factors_at + 3 * kChunk * 4 + row_bytes), qs = {};      // factors of this wave's rows of Q S
+    f32x4 read, length, qs = {};           // factors of this wave's rows of Q S, and of all of them
+    auto load_factors = [&]() {
+      read = load4(place + factors_at + 3 * kChunk * 4 + row_bytes);
+      length = load4(place + factors_at + 4 * kChunk * 4 + row_bytes);
+    };
+    load_factors();
     const int64_t width = a.z ? static_cast<int64_t>(a.v_heads) * a.dv : a.out_stride;
     float *scratch = reinterpret_cast<float *>(p.chunks + (base + c0 - p.first) * step_bytes + p.at.rows_at()) + row * width +
                      head * a.dv + col;
@@ -759,7 +776,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
     float unit = 0.0f;
     // the rows of the chunk whose U lies in LDS
     auto finish = [&]() {
-      const f32x4 o = times_mats(ub, read * qs) * unit;
+      const f32x4 o = times_mats(ub, read * qs) * (length * unit);
       if (a.z) {
         if (c.rows == kChunk) {
 #pragma unroll
@@ -791,14 +808,14 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
       place += at + 1 < c1 ? step_bytes : 0;
       lds_barrier();
       qs = times_state();
-      unit = a.scale * (1.0f / kUnit) * inverse;
+      unit = a.scale * inverse;
       load_rows();
       lds_barrier();
       update_state(at);
       lds_barrier();
       finish();              // beside the chain's next K S
       load_mats();
-      read = load4(place + factors_at + 3 * kChunk * 4 + row_bytes);
+      load_factors();
     }
   }
 }
@@ -828,8 +845,13 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
   }
 }
 
-// Calls whose sequences have more rows than this go in chunks.
-constexpr int kMostTokens = 16;
+// Whether a call goes token by token. Heads of 128 x 128, 16 key and 32 value heads, kernels alone (us, tokens and
+// chunks): one sequence of 8 rows 17.8 and 22.4, of 16 rows 31.5 and 22.6; four of 16 rows 32.5 and 41.8, of 24 46
+// and 42; sixteen of 32 rows 91 and 103, of 48 131 and 106. A token takes its 1.7 us in all heads at
+// once as long as they find room; the chunks of one sequence fill the chip.
+bool by_tokens(int B, int v_heads, int max_q) {
+  return max_q <= std::min<int64_t>(40, 8 + (int64_t)B * v_heads / 16);
+}
 
 struct ChunkPlan {
   int64_t slots;
@@ -875,7 +897,7 @@ int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
 
 template <typename T, typename TO>
 int launch_delta(const DeltaArgs &a, int DK, int max_q, void *workspace, hipStream_t st) {
-  if (max_q > kMostTokens) return DK == 64 ? launch_chunks<T, TO, 64>(a, workspace, st) : launch_chunks<T, TO, 128>(a, workspace, st);
+  if (!by_tokens(a.c.batch, a.v_heads, max_q)) return DK == 64 ? launch_chunks<T, TO, 64>(a, workspace, st) : launch_chunks<T, TO, 128>(a, workspace, st);
   const unsigned grid = (unsigned)a.c.batch * (unsigned)a.v_heads;
   if (DK == 64) delta_tokens_kernel<T, TO, 64><<<grid, a.dv * 2, 0, st>>>(a);
   else delta_tokens_kernel<T, TO, 128><<<grid, a.dv * 2, 0, st>>>(a);
@@ -889,7 +911,7 @@ int launch_delta(const DeltaArgs &a, int DK, int max_q, void *workspace, hipStre
 extern "C" {
 
 size_t rlq_gated_delta_workspace_bytes(int T, int k_heads, int v_heads, int Dk, int Dv, int B, int max_q) {
-  if (T <= 0 || B <= 0 || max_q <= rlq::kMostTokens || k_heads < 1 || v_heads < k_heads || Dk <= 0 || Dv <= 0) return 0;
+  if (T <= 0 || B <= 0 || rlq::by_tokens(B, v_heads, max_q) || k_heads < 1 || v_heads < k_heads || Dk <= 0 || Dv <= 0) return 0;
   return (size_t)rlq::plan_chunks({Dk, k_heads, v_heads, Dv}, T, B).bytes;
 }
 

@@ -107,6 +107,7 @@ def test_strides(gpu, pad):
 def test_kept_rows(gpu):
     s, c = draw([(5, 30)] * 6 + [(5, 5)], "k128", F16, seed=1)
     check(gpu, s, c, F16, True, keep=[0, 1, 4, 5, 9, -2, 3])
+    check(gpu, s, c, F16, True, keep=[0, 1, 4, 5, 9, -2, 3], max_q=1000)
     s, c = draw([(150, 300)] * 6 + [(1, 9), (70, 70)], "h64", F16, seed=2)
     check(gpu, s, c, F16, False, keep=[0, 1, 63, 64, 65, 149, 0, 69])
 
@@ -175,6 +176,47 @@ def test_sizes_of_bf16_rows(gpu, size):
     c["v"] = torch.from_numpy(c["v"] * size).bfloat16().double().numpy()
     c["state"] = (c["state"] * size).astype(np.float32).astype(np.float64)
     check(gpu, s, c, BF16, out_dtype=BF16, eps=1e-30)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -70, 2.0 ** -90, 2.0 ** -120])
+def test_rows_whose_squares_pass_below_fp32(gpu, size):
+    """Keys and queries far shorter than eps: the state takes next to nothing, and nothing overflows."""
+    s, c = draw([(90, 100), (70, 70)], "h64", BF16, seed=4)
+    c["k"][::3] *= size
+    c["q"][::2] *= size
+    check(gpu, s, c, BF16, out_dtype=BF16)
+    check(gpu, s, c, BF16, out_dtype=BF16, max_q=1)
+
+
+def test_runs_of_chunks(gpu):
+    """A prompt of more chunks than the scratch holds at a time, in one call and in two: the state goes from run to
+    run as it goes from call to call, but for the power of two its parts are held at (two terms of 2^-22)."""
+    from raceline_amd import ops
+
+    Hk, Hv, Dk, Dv, T, cut = 16, 32, 128, 128, 6400, 64 * 40
+    assert ops.gated_delta_workspace_bytes(T, Hk, Hv, Dk, Dv, 1, T) == ops.gated_delta_workspace_bytes(2 * T, Hk, Hv, Dk, Dv, 1, T)
+    g = torch.Generator(device=gpu)
+    g.manual_seed(1)
+    rnd = lambda *n: torch.randn(n, generator=g, device=gpu)                             # noqa: E731
+    x, ba, z = rnd(T, 2 * Hk * Dk + Hv * Dv).half(), rnd(T, 2 * Hv), rnd(T, Hv * Dv)
+    a_log, dt, norm, start = rnd(Hv) - 2, rnd(Hv) - 3, rnd(Dv), rnd(1, Hv, Dk, Dv) * 0.3
+
+    def run(state, lo, hi, slot=0):
+        ints = dict(dtype=torch.int32, device=gpu)
+        r = slice(lo, hi)
+        return ops.gated_delta(x[r, :Hk * Dk], x[r, Hk * Dk:2 * Hk * Dk], x[r, 2 * Hk * Dk:], ba[r, :Hv], ba[r, Hv:], a_log, dt,
+                               state, torch.tensor([0, hi - lo], **ints), torch.tensor([hi + 9], **ints),
+                               torch.tensor([slot], **ints), max_q=T, z=z[r], norm=norm, out_dtype=BF16)
+
+    one, two, none = start.clone(), start.clone(), start.clone()
+    whole = run(one, 0, T)
+    parts = torch.cat([run(two, 0, cut), run(two, cut, T)])
+    assert (one - two).norm() <= 2.0 ** -18 * two.norm()
+    assert (whole.float() - parts.float()).norm() <= 2.0 ** -8 * parts.float().norm()
+    # a sequence without a slot goes through the runs all the same, from zeros
+    free = run(none, 0, T, slot=-1)
+    zeros = torch.zeros_like(start)
+    assert torch.equal(none, start) and torch.equal(free, run(zeros, 0, T))
 
 
 def test_zero_rows_and_eps(gpu):
