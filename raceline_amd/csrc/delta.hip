@@ -62,16 +62,21 @@ __device__ __forceinline__ void load_row(const T *p, bool wide, T (&x)[N]) {
 //   p = S^T k, r = S^T q,  d = beta (v - g p),  o = g r + (k.q) d,  S <- g S + k d^T,
 // so that both reads of the state go side by side. A workgroup takes one value head of one sequence, a
 // wave 32 columns of its state: lane 8 i + c the rows i DK/8 .. and the columns 4 c .. 4 c + 3, in registers
-// for all of the call's tokens. Sums over the rows go over the lanes of a column without LDS; only the norm of
-// the output needs the other waves.
+// for all of the call's tokens; sums over the rows go over the lanes of a column without LDS. What does not depend on
+// the state goes beside it, eight tokens at a time: keys and queries to length 1, a token a wave, before; the norm of
+// the rows and their gate, four values a thread, behind.
+// Bound by HBM for many sequences (48 of 32 heads of 128 x 128: 203 MB in 34.8 us, 5.8 TB/s), else by the chain of a
+// token's sums, 1 us each (one token 6.9 us, nine drafts of five 10.5).
 template <typename T, typename TO, int DK>
 __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
-  constexpr int kRows = DK / 8;
-  __shared__ float squares[2][8];
+  constexpr int kRows = DK / 8, kOf = DK / 64, kBatch = 8, kMostDv = 256;
+  __shared__ __align__(16) float ks[kBatch][DK], qs[kBatch][DK], vs[kBatch][kMostDv], os[kBatch][kMostDv];
+  __shared__ float squares[kBatch][kMostDv / 32], kqs[kBatch];
   const int b = blockIdx.x / a.v_heads, head = blockIdx.x - b * a.v_heads;
   const int row0 = row_start(a.c, b), n = row_start(a.c, b + 1) - row0;
   if (n <= 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k0 = (lane >> 3) * kRows, col = wave * 32 + (lane & 7) * 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = a.dv / 32;
+  const int k0 = (lane >> 3) * kRows, col = wave * 32 + (lane & 7) * 4;
   const int k_head = head / (a.v_heads / a.k_heads), slot = a.slots[b];
   const bool has_state = slot >= 0 && slot < a.n_slots;
   float *state = a.state + (has_state ? (static_cast<int64_t>(slot) * a.v_heads + head) * DK * a.dv + k0 * a.dv + col : 0);
@@ -80,116 +85,140 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
   const float *ap = a.a + row0 * a.a_stride + head, *bp = a.b + row0 * a.b_stride + head;
   float fades = ap[min(lane, n - 1) * a.a_stride], betas = bp[min(lane, n - 1) * a.b_stride];   // of 64 tokens, one a lane
   float s[kRows][4];
-  if (has_state && cached(a.c, b) > n) {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const f32x4 x = *reinterpret_cast<const f32x4 *>(state + i * a.dv);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = x[e];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = 0.0f;
-  }
-  const T *qp = static_cast<const T *>(a.q) + row0 * a.q_stride + k_head * DK + k0;
-  const T *kp = static_cast<const T *>(a.k) + row0 * a.k_stride + k_head * DK + k0;
-  const T *vp = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + col;
-  const float *zp = a.z ? a.z + row0 * a.z_stride + head * a.dv + col : nullptr;
-  TO *op = static_cast<TO *>(a.out) + row0 * a.out_stride + head * a.dv + col;
+  const T *qp = static_cast<const T *>(a.q) + row0 * a.q_stride + k_head * DK;
+  const T *kp = static_cast<const T *>(a.k) + row0 * a.k_stride + k_head * DK;
   const float rate = expf(a.a_log[head]), dt_bias = a.dt_bias[head];
-  float w[4] = {};
+  // a thread's token of eight, and four of its values
+  const int quads = a.dv / 4, mine = tid / quads, at = (tid - mine * quads) * 4;
+  const T *vp = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + at;
+  const float *zp = a.z ? a.z + row0 * a.z_stride + head * a.dv + at : nullptr;
+  TO *op = static_cast<TO *>(a.out) + row0 * a.out_stride + head * a.dv + at;
+  f32x4 w = {};
   if (zp) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = a.norm[col + e];
+    for (int e = 0; e < 4; ++e) w[e] = a.norm[at + e];
   }
-  // a token's rows are on their way while the one in front is worked on
-  struct Rows {
-    T q[kRows], k[kRows], v[4];
-    float z[4];
-  };
-  auto fetch = [&](int t, Rows &x) {
-    load_row<T, kRows>(qp + t * a.q_stride, a.wide, x.q);
-    load_row<T, kRows>(kp + t * a.k_stride, a.wide, x.k);
-    load_row<T, 4>(vp + t * a.v_stride, a.wide, x.v);
+  for (int t0 = 0; t0 < n; t0 += kBatch) {
+    const int m = min(kBatch, n - t0);
+    if (t0) lds_barrier();               // the rows in front have been read
+    // loads return in order: the rows first, whose work then goes beside the state's arrival
+    const int token = t0 + min(mine, m - 1);
+    f32x4 z = {};
+    T v[4], qr[kOf], kr[kOf];
+    auto fetch = [&](int t) {
+      load_row<T, kOf>(qp + (t0 + t) * a.q_stride + lane * kOf, a.wide, qr);
+      load_row<T, kOf>(kp + (t0 + t) * a.k_stride + lane * kOf, a.wide, kr);
+    };
+    fetch(min(wave, m - 1));
+    load_row<T, 4>(vp + token * a.v_stride, a.wide, v);
     if (zp) {
-      if (a.wide_z) {
-        const f32x4 y = *reinterpret_cast<const f32x4 *>(zp + t * a.z_stride);
+      const float *from = zp + token * a.z_stride;
+      if (a.wide_z) z = *reinterpret_cast<const f32x4 *>(from);
+      else z = f32x4{from[0], from[1], from[2], from[3]};
+    }
+    if (t0 == 0) {
+      if (has_state && cached(a.c, b) > n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.z[e] = y[e];
+        for (int i = 0; i < kRows; ++i) {
+          const f32x4 x = *reinterpret_cast<const f32x4 *>(state + i * a.dv);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = x[e];
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.z[e] = zp[t * a.z_stride + e];
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = 0.0f;
       }
     }
-  };
-  Rows next;
-  fetch(0, next);
-  for (int t = 0; t < n; ++t) {
-    if ((t & 63) == 0) {
-      if (t) fades = ap[min(t + lane, n - 1) * a.a_stride], betas = bp[min(t + lane, n - 1) * a.b_stride];
+    if (mine < m) {
+      *reinterpret_cast<f32x4 *>(&vs[mine][at]) = f32x4{static_cast<float>(v[0]), static_cast<float>(v[1]), static_cast<float>(v[2]),
+                                                        static_cast<float>(v[3])};
+    }
+    for (int t = wave; t < m; t += waves) {
+      if (t != wave) fetch(t);
+      float kk = 0.0f, qq = 0.0f, kq = 0.0f, k[kOf], q[kOf];
+#pragma unroll
+      for (int i = 0; i < kOf; ++i) {
+        k[i] = static_cast<float>(kr[i]), q[i] = static_cast<float>(qr[i]);
+        kk += k[i] * k[i], qq += q[i] * q[i];
+      }
+      // to length 1 before the products: those of raw rows could pass fp32
+      const float rk = __builtin_amdgcn_rsqf(sum_high(sum_low(kk)) + a.eps);
+      const float rq = a.scale * __builtin_amdgcn_rsqf(sum_high(sum_low(qq)) + a.eps);
+#pragma unroll
+      for (int i = 0; i < kOf; ++i) {
+        k[i] *= rk, q[i] *= rq;
+        kq += k[i] * q[i];
+        ks[t][lane * kOf + i] = k[i];
+        qs[t][lane * kOf + i] = q[i];
+      }
+      kq = sum_high(sum_low(kq));
+      if (lane == 0) kqs[t] = kq;
+    }
+    if ((t0 & 63) == 0) {
+      if (t0) fades = ap[min(t0 + lane, n - 1) * a.a_stride], betas = bp[min(t0 + lane, n - 1) * a.b_stride];
       fades = expf(log_fade(fades, dt_bias, rate));
       betas = sigmoid(betas);
     }
-    float q[kRows], k[kRows], v[4], z[4];
+    lds_barrier();
+    for (int t = 0; t < m; ++t) {
+      const float fade = __uint_as_float(of_lane(__float_as_uint(fades), t0 + t & 63));
+      const float beta = __uint_as_float(of_lane(__float_as_uint(betas), t0 + t & 63));
+      float k[kRows], q[kRows], p[4] = {}, r[4] = {};
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) q[i] = static_cast<float>(next.q[i]), k[i] = static_cast<float>(next.k[i]);
+      for (int i = 0; i < kRows; i += 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(&ks[t][k0 + i]), y = *reinterpret_cast<const f32x4 *>(&qs[t][k0 + i]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(next.v[e]), z[e] = next.z[e];
-    const float fade = __uint_as_float(of_lane(__float_as_uint(fades), t & 63));
-    const float beta = __uint_as_float(of_lane(__float_as_uint(betas), t & 63));
-    if (t + 1 < n) fetch(t + 1, next);
-    // to length 1 before the products: those of raw rows with a state could pass fp32
-    float kk = 0.0f, qq = 0.0f, kq = 0.0f, p[4] = {}, r[4] = {};
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) kk += k[i] * k[i], qq += q[i] * q[i];
-    const float rk = __builtin_amdgcn_rsqf(sum_high(kk) + a.eps), rq = a.scale * __builtin_amdgcn_rsqf(sum_high(qq) + a.eps);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      k[i] *= rk;
-      q[i] *= rq;
-      kq += k[i] * q[i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[e] += s[i][e] * k[i];
-        r[e] += s[i][e] * q[i];
+        for (int e = 0; e < 4; ++e) k[i + e] = x[e], q[i + e] = y[e];
       }
-    }
-    kq = sum_high(kq);
-    float o[4], d[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      d[e] = beta * (v[e] - fade * sum_high(p[e]));
-      o[e] = fade * sum_high(r[e]) + kq * d[e];
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = fade * s[i][e] + k[i] * d[e];
-    if (t + 1 == end) {
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(&vs[t][col]);
 #pragma unroll
       for (int i = 0; i < kRows; ++i)
-        *reinterpret_cast<f32x4 *>(state + i * a.dv) = f32x4{s[i][0], s[i][1], s[i][2], s[i][3]};
-    }
-    if (zp) {
-      const float mine = sum_low(o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3]);
-      if (lane == 0) squares[t & 1][wave] = mine;
-      lds_barrier();          // the other half is free: its last readers are past the barrier before
-      float sum = 0.0f;
-      for (int i = 0; i < a.dv / 32; ++i) sum += squares[t & 1][i];
-      const float r = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + a.norm_eps);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = o[e] * r * w[e] * gate_of(z[e]);
+        for (int e = 0; e < 4; ++e) {
+          p[e] += s[i][e] * k[i];
+          r[e] += s[i][e] * q[i];
+        }
+      const float kq = kqs[t];
+      f32x4 o;
+      float d[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d[e] = beta * (v[e] - fade * sum_high(p[e]));
+        o[e] = fade * sum_high(r[e]) + kq * d[e];
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = fade * s[i][e] + k[i] * d[e];
+      if (lane < 8) *reinterpret_cast<f32x4 *>(&os[t][col]) = o;
+      const float sum = sum_low(o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3]);
+      if (lane == 0) squares[t][wave] = sum;
+      if (t0 + t + 1 == end) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          *reinterpret_cast<f32x4 *>(state + i * a.dv) = f32x4{s[i][0], s[i][1], s[i][2], s[i][3]};
+      }
     }
-    if (lane < 8) {
+    lds_barrier();
+    if (mine < m) {
+      f32x4 o = *reinterpret_cast<const f32x4 *>(&os[mine][at]);
+      if (zp) {
+        float sum = 0.0f;
+        for (int i = 0; i < waves; ++i) sum += squares[mine][i];
+        const float r = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + a.norm_eps);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * r * w[e] * gate_of(z[e]);
+      }
+      TO *to = op + (t0 + mine) * a.out_stride;
       if (a.wide) {
         typedef TO pack4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<pack4 *>(op + t * a.out_stride) =
+        *reinterpret_cast<pack4 *>(to) =
             pack4{static_cast<TO>(o[0]), static_cast<TO>(o[1]), static_cast<TO>(o[2]), static_cast<TO>(o[3])};
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) op[t * a.out_stride + e] = static_cast<TO>(o[e]);
+        for (int e = 0; e < 4; ++e) to[e] = static_cast<TO>(o[e]);
       }
     }
   }
@@ -846,11 +875,11 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
 }
 
 // Whether a call goes token by token. Heads of 128 x 128, 16 key and 32 value heads, kernels alone (us, tokens and
-// chunks): one sequence of 8 rows 17.8 and 22.4, of 16 rows 31.5 and 22.6; four of 16 rows 32.5 and 41.8, of 24 46
-// and 42; sixteen of 32 rows 91 and 103, of 48 131 and 106. A token takes its 1.7 us in all heads at
-// once as long as they find room; the chunks of one sequence fill the chip.
+// chunks): one sequence of 16 rows 21 and 22.6, of 24 rows 29 and 22.8; four of 32 rows 38 and 42, of 48 rows 55 and
+// 44; sixteen of 48 rows 85 and 106, of 64 rows 110 and 107. A token takes its 1 us in all heads at once as long as they find
+// room; the chunks of one sequence fill the chip.
 bool by_tokens(int B, int v_heads, int max_q) {
-  return max_q <= std::min<int64_t>(40, 8 + (int64_t)B * v_heads / 16);
+  return max_q <= std::min<int64_t>(56, 12 + (int64_t)B * v_heads / 6);
 }
 
 struct ChunkPlan {
