@@ -438,10 +438,13 @@ int rlq_causal_conv(const float *x, int x_stride, int T, int channels, int taps,
  * rlq_causal_conv's rows, say); a, b fp32 [T][stride], v_heads a row; a_log, dt_bias fp32 [v_heads]; z fp32
  * [T][z_stride]; norm fp32 [Dv]; out 16-bit (out_dtype) [T][out_stride]. state fp32
  * [n_slots][v_heads][Dk][Dv], 16-byte aligned. Dk 64 or 128; Dv 64, 128 or 256; v_heads a multiple of
- * k_heads; eps and norm_eps at least 1e-37. State, products and sums in fp32; rows of q and k have
- * lengths below 2^63.
+ * k_heads; eps and norm_eps at least 1e-37. State and sums in fp32; rows of q and k have lengths below 2^63.
  * max_q (host) bounds the rows of a sequence: it chooses between the rule token by token and its form in
- * chunks of 64 tokens, and results stay right past it. The workspace
+ * chunks of 64 tokens (from a sequence's first row on, and anew behind the kept ones), and results stay right past
+ * it. In chunks the factors of a product hold 22 bits and values and state are held by the largest finite value
+ * that the head has met, as it faded: what is smaller than its 2^-14 begins to lose bits; finite values are to be below
+ * 2^120. An infinity or NaN in a row of a chunk also reaches the rows in front of it in that chunk, in the values it
+ * touches; in v or the state it stays in its column (with z in its head), and it never reaches another sequence. The workspace
  * (rlq_gated_delta_workspace_bytes, may be 0; 16-byte aligned, no initialisation) holds what the chunks
  * hand on; calls that overlap must not share it. */
 size_t rlq_gated_delta_workspace_bytes(int T, int k_heads, int v_heads, int Dk, int Dv, int B, int max_q);

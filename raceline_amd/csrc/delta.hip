@@ -303,6 +303,9 @@ __device__ __forceinline__ void split(const float (&x)[4], half4 &high, half4 &l
   }
 }
 
+// An infinity or NaN stays in its own column, so it has no part in a size that other columns are held by.
+__device__ __forceinline__ float finite_size(float x) { return fabsf(x) < __builtin_inff() ? fabsf(x) : 0.0f; }
+
 // 2^x; what x loses in fp32 is nothing beside 2^x where x is large.
 __device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); }
 
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
       if ((tid & 7) == 0) (which ? rq : rk)[row] = down / sqrtf(sum * unit * unit + a.eps);
     }
   }
-  {  // the largest value of the head
+  {  // the largest finite value of the head
     const T *from = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv;
     const int per = a.dv / 8;
     float x = 0.0f;
@@ -385,7 +388,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
       T y[8];
       load_row<T, 8>(from + i / per * a.v_stride + i % per * 8, a.wide, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf(static_cast<float>(y[e])));
+      for (int e = 0; e < 8; ++e) x = fmaxf(x, finite_size(static_cast<float>(y[e])));
     }
     x = most_of_wave(x);
     if (lane == 0) most[half][mine] = x;
@@ -548,6 +551,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
 }
 
 constexpr int kChainThreads = 512;
+constexpr float kMostSize = 3.0e38f;   // a bound past fp32 has to come back as it fades
 
 // A workgroup goes through a sequence's chunks with 16 columns of one head's state. Four waves are the chain: each
 // has 16 of a chunk's rows, K S, R and U; four others read the rows out (Q S and, a step later, P U), 16 rows
@@ -678,7 +682,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       s[i] = from ? from[i * a.dv] : 0.0f;
-      size = fmaxf(size, fabsf(s[i]));
+      size = fmaxf(size, finite_size(s[i]));
     }
     size = most_of_wave(size);
     if (lane == 0) most[tile] = size;
@@ -710,7 +714,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
       }
       load_tile();
     }
-    size = fade * size + 8.0f * value;
+    size = fminf(fade * size + 8.0f * value, kMostSize);
     fade = next[0], value = next[1];
     asm("" : "+v"(fade), "+v"(value));     // registers of their own: those of a load stay its own from step to step
     set_scale();
@@ -907,7 +911,7 @@ int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
   p.carry[1] = reinterpret_cast<float *>(reinterpret_cast<char *>(p.carry[0]) + p.at.state());
   const int parts = (a.v_heads / a.k_heads + kHeadsPer - 1) / kHeadsPer;
   const int64_t pairs = ((int64_t)a.c.batch * a.v_heads + 7) / 8 * 8;
-  RLQ_REQUIRE(a.k_heads * (int64_t)parts <= 65535 && pairs * (a.dv / 16) <= INT32_MAX,
+  RLQ_REQUIRE(a.k_heads * (int64_t)parts <= 65535 && pairs * (a.dv / 16) * kChainThreads <= UINT32_MAX,
               "rlq_gated_delta: %d heads of %d sequences are too many for chunks", a.v_heads, a.c.batch);
   for (int64_t first = 0; first < plan.slots; first += plan.count, ++p.run) {
     p.first = (int)first;
@@ -928,6 +932,8 @@ template <typename T, typename TO>
 int launch_delta(const DeltaArgs &a, int DK, int max_q, void *workspace, hipStream_t st) {
   if (!by_tokens(a.c.batch, a.v_heads, max_q)) return DK == 64 ? launch_chunks<T, TO, 64>(a, workspace, st) : launch_chunks<T, TO, 128>(a, workspace, st);
   const unsigned grid = (unsigned)a.c.batch * (unsigned)a.v_heads;
+  RLQ_REQUIRE(a.c.batch * (int64_t)a.v_heads * a.dv * 2 <= UINT32_MAX, "rlq_gated_delta: %d heads of %d sequences are too many",
+              a.v_heads, a.c.batch);
   if (DK == 64) delta_tokens_kernel<T, TO, 64><<<grid, a.dv * 2, 0, st>>>(a);
   else delta_tokens_kernel<T, TO, 128><<<grid, a.dv * 2, 0, st>>>(a);
   RLQ_HIP(hipGetLastError());

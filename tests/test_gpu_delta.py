@@ -258,3 +258,55 @@ def test_the_same_call_gives_the_same_bits(gpu):
     first = check(gpu, s, c, F16, True)
     again = check(gpu, s, c, F16, True)
     assert all(np.array_equal(x, y) for x, y in zip(first, again))
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("where", ["value", "state", "kept"])
+def test_what_is_not_finite_stays_in_its_column(gpu, where, value):
+    """In chunks a head's values are held by the size of the largest one; the others keep their bits beside an infinity."""
+    from raceline_amd import ops
+
+    s, c = draw([(70, 90), (130, 130)], "k128", BF16, seed=6)
+    f = lambda n, t=torch.float32: torch.from_numpy(c[n]).to(t).to(gpu)                  # noqa: E731
+    keep = torch.tensor([66, 100], dtype=torch.int32, device=gpu) if where == "kept" else None
+
+    def run(x):
+        v, state = f("v", BF16), f("state")
+        if where == "state":
+            state[int(s.slots[0]), 1, :, 5] = x
+        else:
+            v[67, 1, 5] = v[70 + 69, 2, 100] = x
+        out = ops.gated_delta(f("q", BF16).flatten(1), f("k", BF16).flatten(1), v.flatten(1), f("a"), f("b"), f("a_log"),
+                              f("dt_bias"), state, *s.dev(gpu), max_q=s.max_q, keep=keep)
+        return out.reshape(s.T, 4, 128), state
+
+    (out, state), (want, kept) = run(value), run(0.0)
+    touched = torch.zeros_like(want, dtype=torch.bool)
+    of_state = torch.zeros_like(kept, dtype=torch.bool)
+    first = 0 if where == "state" else 66 if where == "kept" else 64
+    touched[first:70, 1, 5] = of_state[int(s.slots[0]), 1, :, 5] = True
+    if where != "state":
+        touched[70 + 64:, 2, 100] = of_state[int(s.slots[1]), 2, :, 100] = True
+    if where == "kept":
+        of_state[int(s.slots[0])] = False                      # the row lies behind the kept ones
+    assert torch.equal(out[~touched], want[~touched]) and torch.equal(state[~of_state], kept[~of_state])
+    assert not out[69, 1, 5].isfinite() and (not of_state.any() or not state[of_state].isfinite().any())
+
+
+def test_a_largest_value_is_forgotten_with_its_rows(gpu):
+    """Rates are 0.01 at least, so a token fades by e^-9.9 or more: the first chunk's last tokens, which are held by its
+    largest value, still reach the second chunk, and nothing of them the third (e^-600 is 0 in fp32)."""
+    from raceline_amd import ops
+
+    s, c = draw([(200, 200)], "h64", BF16, seed=7)
+    f = lambda n, t=torch.float32: torch.from_numpy(c[n]).to(t).to(gpu)                  # noqa: E731
+
+    def run(x):
+        v, state = f("v", BF16), f("state")
+        v[3, 1, 5] = x
+        out = ops.gated_delta(f("q", BF16).flatten(1), f("k", BF16).flatten(1), v.flatten(1), f("a") + 1e3, f("b"), f("a_log"),
+                              f("dt_bias"), state, *s.dev(gpu), max_q=s.max_q)
+        return out[128:], state
+
+    for x, y in zip(run(torch.finfo(BF16).max), run(0.0)):
+        assert x.isfinite().all() and torch.equal(x, y)

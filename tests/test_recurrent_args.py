@@ -41,7 +41,10 @@ def test_causal_conv_refuses(change, message):
     (dict(state=None), "16-byte aligned"), (dict(state=20), "16-byte aligned"), (dict(q_stride=127), "stride"),
     (dict(v_stride=255), "stride"), (dict(a_stride=3), "stride"), (dict(b_stride=3), "stride"), (dict(z_stride=255), "stride"),
     (dict(out_stride=255), "stride"), (dict(B=1 << 20, v_heads=4096, v_stride=1 << 18, a_stride=4096, b_stride=4096,
-                                            z_stride=1 << 18, out_stride=1 << 18), "too many")])
+                                            z_stride=1 << 18, out_stride=1 << 18), "too many"),
+    (dict(B=1 << 20, v_heads=64, v_stride=4096, a_stride=64, b_stride=64, z_stride=4096, out_stride=4096), "too many"),
+    (dict(B=1 << 20, v_heads=16, v_stride=1024, a_stride=16, b_stride=16, z_stride=1024, out_stride=1024, max_q=1 << 24,
+          workspace=16, workspace_bytes=1 << 40), "too many")])
 def test_gated_delta_refuses(change, message):
     with pytest.raises(lib.RlqError, match=message):
         lib.call("rlq_gated_delta", *{**DELTA, **change}.values())
