@@ -565,16 +565,18 @@ constexpr float kMostSize = 3.0e38f;   // a bound past fp32 has to come back as 
 // chunk lengthens a column of S by at most the sum of its values' squares (8 of the largest), and R and U are never
 // larger than a column of S and 9 of the largest value.
 // What a wave reads of the next chunk is asked for as soon as this chunk's has been used, so every load has a whole
-// step to arrive; no branch stands between a load and its use, or the wait there would be for all of them.
-// Bound by the chain: a step is 1.5 us, K S, R, U and S with three barriers, each a few dependent products (32 steps 52 us;
-// 256 workgroups of two waves a SIMD, MFMA 0.16, VALU 0.34, LDS 0.24). A 16-column slice fills the chip from one
-// sequence of 32 heads of 128; two slices a CU share its cycles. Without the reading waves' slack in use (their loads behind
-// the barriers) 54 us, at four waves a SIMD 92 (spills).
+// step to arrive; no branch stands between a load and its use, or the wait there would be for all of them. The values
+// come by way of the reading waves, which have slack: their loads and addresses cost the chain 3 of 50 us.
+// Bound by the chain: a step is 1.4 us, K S, R, U and S with three barriers, each a few dependent products (32 steps 47.7 us,
+// 39 without any load; 256 workgroups of two waves a SIMD, MFMA 0.16, VALU 0.34, LDS 0.24). A 16-column slice fills the chip
+// from one sequence of 32 heads of 128; two slices a CU share its cycles. With the reading waves' Q asked for beside the
+// state's step 50.7, without loads above T's diagonal 49.2 (branches), at four waves a SIMD 92 (spills).
 template <typename T, typename TO, int DK>
 __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs p) {
   constexpr int kSteps = DK / 32;   // steps over the state's rows
   const DeltaArgs &a = p.d;
   __shared__ __align__(16) _Float16 sb[2][kSteps][64][8], rb[2][2][64][8], ub[2][2][64][8], wb[2][2][64][8];
+  __shared__ f32x4 vb[4][64];       // a chunk's values, as the chain's lanes hold its rows
   __shared__ float most[8];
 
   // workgroups of one head run on one XCD, whose L2 then holds its chunk for all of them
@@ -592,7 +594,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   if (c0 >= c1) return;
 
   const int tid = threadIdx.x, lane = tid & 63, tile = __builtin_amdgcn_readfirstlane(tid >> 6), wave = tile & 3;
-  const bool chain = tile < 4, has_tile = tile < DK / 16;
+  const bool chain = tile < 4, has_tile = DK == 128 || chain;
   const int r = lane & 15, h = lane >> 4, col = slice * 16 + r, row = wave * 16 + h * 4;
   const bool below = wave >= 2;     // rows 32 and on: the second step over a chunk's rows is not above the diagonal
   const int k_head = head / (a.v_heads / a.k_heads), slot = a.slots[b];
@@ -635,26 +637,36 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   auto mfma = [](const half8 &x, const half8 &y, const f32x4 &sum) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, sum, 0, 0, 0);
   };
-  // this wave's rows times the state
-  auto times_state = [&]() {
-    f32x4 sum = {}, low = {};
+  // A product's operands are asked for together, and `beside` (the next loads) is issued while they come: the compiler would
+  // wait for LDS three times in a row, and issue the loads behind the product, where the others wait for it.
+  // This wave's rows times the state:
+  auto times_state = [&](auto beside) {
+    half8 high[kSteps], low[kSteps];
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) high[e] = operand(sb[0][e]), low[e] = operand(sb[1][e]);
+    __builtin_amdgcn_sched_barrier(0);
+    beside();
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 sum = {}, low_sum = {};
 #pragma unroll
     for (int e = 0; e < kSteps; ++e) {
-      sum = mfma(rows[e], operand(sb[0][e]), sum);
-      low = mfma(rows[e], operand(sb[1][e]), low);
+      sum = mfma(rows[e], high[e], sum);
+      low_sum = mfma(rows[e], low[e], low_sum);
     }
-    return sum + low;
+    return sum + low_sum;
   };
   // its rows of a chunk's 64 x 64 matrix in two terms times 64 x 16 values in two
-  auto times_mats = [&](const _Float16 (&y)[2][2][64][8], f32x4 sum) {
-    const half8 high = operand(y[0][0]), low = operand(y[1][0]);
+  auto times_mats = [&](const _Float16 (&y)[2][2][64][8], f32x4 sum, auto beside) {
+    const half8 high = operand(y[0][0]), low = operand(y[1][0]), high2 = operand(y[0][1]), low2 = operand(y[1][1]);
+    __builtin_amdgcn_sched_barrier(0);
+    beside();
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 low_sum = mfma(mats[0][0], low, f32x4{}), last = mfma(mats[1][0], high, f32x4{});
     sum = mfma(mats[0][0], high, sum);
     if (below) {
-      const half8 high = operand(y[0][1]), low = operand(y[1][1]);
-      low_sum = mfma(mats[0][1], low, low_sum);
-      last = mfma(mats[1][1], high, last);
-      sum = mfma(mats[0][1], high, sum);
+      low_sum = mfma(mats[0][1], low2, low_sum);
+      last = mfma(mats[1][1], high2, last);
+      sum = mfma(mats[0][1], high2, sum);
     }
     return sum + (low_sum + last);
   };
@@ -681,9 +693,8 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   };
   // a chunk's fade and its largest value; the next one's give the scale of what this one hands on
   const char *second_place = place + (c0 + 1 < c1 ? step_bytes : 0);
-  f32x2 next = load_pair(place);
+  f32x2 next = load_pair(place);         // then the next chunk's
   fade = next[0], value = next[1];
-  next = load_pair(second_place);
   Chunk c = chunk_of(n, kept, c0);
   {
     const float *from = !has_tile ? nullptr : c0 ? p.carry[p.run & 1] + in_state : has_state && cached(a.c, b) > n ? state : nullptr;
@@ -697,7 +708,6 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   }
   load_rows();
   load_mats();
-  load_tile();
   lds_barrier();
   size = 0.0f;
 #pragma unroll
@@ -708,26 +718,37 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   for (int i = 0; i < 4; ++i) s[i] *= scale;
   if (has_tile) give_state();
 
+  // what the step behind needs for its S
+  auto load_update = [&]() {
+    load_tile();
+    next = load_pair(second_place);
+  };
   // S <- fade S + K^T W, of this wave's tile, and the next chunk's scale
-  auto update_state = [&](int at) {
+  auto update_state = [&](int at, auto beside) {
     const float faded = fade * kLength, back = inverse * (1.0f / kLength);
     f32x4 sum, low = {};
+    half8 w[2][2];
+    if (has_tile) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) w[0][e] = operand(wb[0][e]), w[1][e] = operand(wb[1][e]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    beside();
+    __builtin_amdgcn_sched_barrier(0);
     if (has_tile) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = faded * s[i];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        sum = mfma(kt[e], operand(wb[0][e]), sum);
-        low = mfma(kt[e], operand(wb[1][e]), low);
+        sum = mfma(kt[e], w[0][e], sum);
+        low = mfma(kt[e], w[1][e], low);
       }
-      load_tile();
     }
     size = fminf(fade * size + 8.0f * value, kMostSize);
     fade = next[0], value = next[1];
     asm("" : "+v"(fade), "+v"(value));     // registers of their own: those of a load stay its own from step to step
     set_scale();
     second_place += at + 2 < c1 ? step_bytes : 0;
-    next = load_pair(second_place);
     if (has_tile) {
       sum += low;
 #pragma unroll
@@ -745,50 +766,56 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
     }
   };
 
+  // of the next chunk, by the waves that have slack
+  T v[4];
+  const T *values = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + slice * 16;
+  int64_t value_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) value_at[i] = (row + i) * a.v_stride + r;
+  auto load_values = [&](int start) {                              // behind the chunk's rows its last one again
+    const int end = start < kept ? kept : n;
+    const T *from = values + start * a.v_stride;
+    if (start + kChunk <= end) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = from[value_at[i]];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = values[min(start + row + i, end - 1) * a.v_stride + r];
+    }
+  };
+  auto give_values = [&]() {
+    vb[wave][lane] = f32x4{static_cast<float>(v[0]), static_cast<float>(v[1]), static_cast<float>(v[2]), static_cast<float>(v[3])};
+  };
+
   if (chain) {
     f32x4 take, seen, left;            // factors of this wave's rows of V, K S and U
-    T v[4];
-    const T *values = static_cast<const T *>(a.v) + row0 * a.v_stride + head * a.dv + slice * 16;
-    int64_t value_at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) value_at[i] = (row + i) * a.v_stride + r;
-    auto load_values = [&](int start) {                              // behind the chunk's rows its last one again
-      const int end = start < kept ? kept : n;
-      const T *from = values + start * a.v_stride;
-      if (start + kChunk <= end) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = from[value_at[i]];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = values[min(start + row + i, end - 1) * a.v_stride + r];
-      }
-    };
     auto load_factors = [&]() {
       take = load4(place + factors_at + row_bytes);
       seen = load4(place + factors_at + kChunk * 4 + row_bytes);
     };
     load_factors();
-    load_values(c.start);
     left = load4(place + factors_at + 2 * kChunk * 4 + row_bytes);
     __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0): the loop's own waits are then for loads of a step before
     __builtin_amdgcn_s_setprio(2);           // the other waves have slack
     lds_barrier();
 
     for (int at = c0; at < c1; ++at) {
+      f32x4 y;
+      const f32x4 ks = times_state([&]() {
+        y = vb[wave][lane];
+        load_update();
+      });
       place += at + 1 < c1 ? step_bytes : 0;             // the last chunk's data come again, unused
-      const f32x4 ks = times_state();
       float x[4], w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = take[i] * (static_cast<float>(v[i]) * scale) - seen[i] * ks[i];   // take: 0 behind the rows
+      for (int i = 0; i < 4; ++i) x[i] = take[i] * (y[i] * scale) - seen[i] * ks[i];   // take: 0 behind the rows
       give(rb, x);
-      c.start += c.rows;
-      c.rows = min(kChunk, (c.start < kept ? kept : n) - c.start);
-      load_rows();
-      load_factors();
-      load_values(c.start);
       lds_barrier();
 
-      const f32x4 u = times_mats(rb, f32x4{});
+      const f32x4 u = times_mats(rb, f32x4{}, [&]() {
+        load_rows();
+        load_factors();
+      });
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[i] = u[i] * (1.0f / kUnit);
@@ -796,11 +823,12 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
       }
       give(wb, w);
       give(ub, x);
-      load_mats();
-      left = load4(place + factors_at + 2 * kChunk * 4 + row_bytes);
       lds_barrier();
 
-      update_state(at);
+      update_state(at, [&]() {
+        load_mats();
+        left = load4(place + factors_at + 2 * kChunk * 4 + row_bytes);
+      });
       lds_barrier();
     }
   } else {
@@ -817,7 +845,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
     float unit = 0.0f;
     // the rows of the chunk whose U lies in LDS
     auto finish = [&]() {
-      const f32x4 o = times_mats(ub, read * qs) * (length * unit);
+      const f32x4 o = times_mats(ub, read * qs, load_update) * (length * unit);
       if (a.z) {
         if (c.rows == kChunk) {
 #pragma unroll
@@ -842,17 +870,29 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
       c.start += c.rows;
       c.rows = min(kChunk, (c.start < kept ? kept : n) - c.start);
     };
+    load_update();
+    load_values(c.start);
+    give_values();
+    int ahead = c.start + c.rows;
+    auto next_values = [&]() {
+      load_values(ahead);
+      ahead += min(kChunk, (ahead < kept ? kept : n) - ahead);
+    };
+    next_values();
     __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0), as above
     lds_barrier();
 
     for (int at = c0; at < c1; ++at) {
       place += at + 1 < c1 ? step_bytes : 0;
       lds_barrier();
-      qs = times_state();
+      qs = times_state([] {});
       unit = a.scale * inverse;
       load_rows();
+      give_values();
+      next_values();
+
       lds_barrier();
-      update_state(at);
+      update_state(at, [] {});
       lds_barrier();
       finish();              // beside the chain's next K S
       load_mats();
