@@ -233,7 +233,7 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
 //   S <- e^(G_64) S + (e^(G_64 - G) K)^T U.
 // delta_chunks_kernel forms what does not depend on S, of all chunks at once: T = (I + L)^-1, P, and the rows
 // as operands. delta_chain_kernel goes through a sequence's chunks with S. A 2048-token chunk of a prompt, 16 key and 32
-// value heads of 128: 22.6 + 52 us, and 15 for the rows' norm and gate; token by token it took 5870.
+// value heads of 128: 23 + 47.7 us, and 16 for the rows' norm and gate; token by token it took 5870.
 //
 // The products are to keep the state to fp32: rows of q and k, brought to a length of 2^13 .. 2^14 by a power of
 // two, are exact in fp16 (what bf16 loses there lies 2^-38 below the length); T, P, R, U and S are two fp16
@@ -570,7 +570,7 @@ constexpr float kMostSize = 3.0e38f;   // a bound past fp32 has to come back as 
 // step to arrive; no branch stands between a load and its use, or the wait there would be for all of them. The values
 // come by way of the reading waves, which have slack: their loads and addresses cost the chain 3 of 50 us.
 // Bound by the chain: a step is 1.4 us, K S, R, U and S with three barriers, each a few dependent products (32 steps 47.7 us,
-// 39 without any load; 256 workgroups of two waves a SIMD, MFMA 0.16, VALU 0.34, LDS 0.24). A 16-column slice fills the chip
+// 39 without any load; 256 workgroups of two waves a SIMD, MFMA 0.18, VALU 0.39, LDS 0.30). A 16-column slice fills the chip
 // from one sequence of 32 heads of 128; two slices a CU share its cycles. With the reading waves' Q asked for beside the
 // state's step 50.7, without loads above T's diagonal 49.2 (branches), at four waves a SIMD 92 (spills).
 template <typename T, typename TO, int DK>
