@@ -264,6 +264,7 @@ struct ChunkArgs {
   char *chunks;       // of the chunks first .. first + count - 1
   float *carry[2];    // states that go from one run of chunks to the next
   int first, count, run;
+  int sequences;      // that a run can touch
 };
 
 struct Chunk {
@@ -585,8 +586,13 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   const int slices = a.dv / 16, xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
   const int slice = rest % slices;
   const int64_t pair = static_cast<int64_t>(rest / slices) * 8 + xcd;
-  if (pair >= static_cast<int64_t>(a.c.batch) * a.v_heads) return;
-  const int b = static_cast<int>(pair / a.v_heads), head = static_cast<int>(pair - static_cast<int64_t>(b) * a.v_heads);
+  if (pair >= static_cast<int64_t>(p.sequences) * a.v_heads) return;
+  int b = static_cast<int>(pair / a.v_heads);
+  const int head = static_cast<int>(pair - static_cast<int64_t>(b) * a.v_heads);
+  if (p.sequences < a.c.batch) {
+    b += max(0, find_sequence(a.c, p.first, 1, kChunk, 2).b);
+    if (b >= a.c.batch) return;
+  }
   const int row0 = row_start(a.c, b), n = row_start(a.c, b + 1) - row0;
   if (n <= 0) return;
   const int kept = kept_rows(a, b, n), chunks = chunks_of(n, kept), kept_chunks = (kept + kChunk - 1) / kChunk;
@@ -966,12 +972,15 @@ int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
   const int64_t pairs = ((int64_t)a.c.batch * a.v_heads + 7) / 8 * 8;
   RLQ_REQUIRE(a.k_heads * (int64_t)parts <= 65535 && pairs * (a.dv / 16) * kChainThreads <= UINT32_MAX,
               "rlq_gated_delta: %d heads of %d sequences are too many for chunks", a.v_heads, a.c.batch);
+  // a sequence has two chunks' places or more, so the chain of a run need not look at all of many sequences
+  p.sequences = (int)std::min<int64_t>(a.c.batch, plan.count / 2 + 2);
+  const unsigned chain_grid = (unsigned)(((int64_t)p.sequences * a.v_heads + 7) / 8 * 8 * (a.dv / 16));
   for (int64_t first = 0; first < plan.slots; first += plan.count, ++p.run) {
     p.first = (int)first;
     p.count = (int)std::min<int64_t>(plan.count, plan.slots - first);
     delta_chunks_kernel<T, DK><<<dim3(p.count, a.k_heads * parts), kPrepareThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
-    delta_chain_kernel<T, TO, DK><<<(unsigned)(pairs * (a.dv / 16)), kChainThreads, 0, st>>>(p);
+    delta_chain_kernel<T, TO, DK><<<chain_grid, kChainThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
     if (a.z) {
       delta_gate_kernel<TO><<<dim3(p.count, kChunk), kGateThreads, 0, st>>>(p);

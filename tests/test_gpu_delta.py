@@ -219,6 +219,50 @@ def test_runs_of_chunks(gpu):
     assert torch.equal(none, start) and torch.equal(free, run(zeros, 0, T))
 
 
+def test_runs_of_chunks_over_many_sequences(gpu):
+    """More sequences than a run of chunks can touch, some without rows, one longer than a run: each as if alone (as in
+    test_runs_of_chunks where a run ends inside one, else to the bit)."""
+    from raceline_amd import ops
+
+    Hk, Hv, Dk, Dv = 16, 32, 128, 128
+    rng = np.random.default_rng(5)
+    lens = [int(n) for n in rng.integers(0, 150, 100)]
+    lens[3], lens[40], lens[99] = 0, 64 * 70 + 5, 1
+    B, cu = len(lens), np.concatenate([[0], np.cumsum(lens)])
+    T = int(cu[-1]) + 3                                        # rows behind the last sequence too
+    ints = dict(dtype=torch.int32, device=gpu)
+    g = torch.Generator(device=gpu)
+    g.manual_seed(2)
+    rnd = lambda *n: torch.randn(n, generator=g, device=gpu)                             # noqa: E731
+    x, ba = rnd(T, 2 * Hk * Dk + Hv * Dv).half(), rnd(T, 2 * Hv)
+    a_log, dt, start = rnd(Hv) - 2, rnd(Hv) - 3, rnd(B, Hv, Dk, Dv) * 0.3
+    most = 1 << 20
+    assert ops.gated_delta_workspace_bytes(T, Hk, Hv, Dk, Dv, B, most) == ops.gated_delta_workspace_bytes(2 * T, Hk, Hv, Dk, Dv, B, most)
+
+    def run(state, lo, hi, cu, kv, slots):
+        r = slice(lo, hi)
+        out = torch.full((hi - lo, Hv * Dv), 7.0, dtype=F16, device=gpu)
+        return ops.gated_delta(x[r, :Hk * Dk], x[r, Hk * Dk:2 * Hk * Dk], x[r, 2 * Hk * Dk:], ba[r, :Hv], ba[r, Hv:], a_log, dt,
+                               state, torch.tensor(cu, **ints), torch.tensor(kv, **ints), torch.tensor(slots, **ints),
+                               max_q=most, out=out)
+
+    kv = [n + 5 * (i % 2) for i, n in enumerate(lens)]
+    together, alone = start.clone(), start.clone()
+    whole = run(together, 0, T, cu.tolist(), kv, list(range(B)))
+    assert (whole[cu[-1]:] == 7).all()
+    same = 0
+    for i, n in enumerate(lens):
+        if not n:
+            assert torch.equal(together[i], start[i])
+            continue
+        rows = run(alone, int(cu[i]), int(cu[i + 1]), [0, n], [kv[i]], [i])
+        same += torch.equal(rows, whole[cu[i]:cu[i + 1]]) and torch.equal(alone[i], together[i])
+        assert (alone[i] - together[i]).norm() <= 2.0 ** -18 * alone[i].norm(), i
+        assert (rows.float() - whole[cu[i]:cu[i + 1]].float()).norm() <= 2.0 ** -10 * rows.float().norm(), i
+    runs = -(-(T // 64 + 2 * B) // 60)                         # a run holds 60 chunks or more
+    assert same >= sum(n > 0 for n in lens) - runs
+
+
 def test_zero_rows_and_eps(gpu):
     s, c = draw([(80, 100), (2, 5)], "k128", F16, seed=3)
     c["k"][5:9] = 0
