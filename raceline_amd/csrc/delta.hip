@@ -937,10 +937,12 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
 
 // Whether a call goes token by token. Heads of 128 x 128, 16 key and 32 value heads, kernels alone (us, tokens and
 // chunks): one sequence of 16 rows 21 and 22.6, of 24 rows 29 and 22.8; four of 32 rows 38 and 42, of 48 rows 55 and
-// 44; sixteen of 48 rows 85 and 106, of 64 rows 110 and 107. A token takes its 1 us in all heads at once as long as they find
-// room; the chunks of one sequence fill the chip.
+// 44; sixteen of 48 rows 85 and 106, of 64 rows 110 and 107; 32 of 64 rows 211 and 217, of 100 318 and 289; 64 of 64 rows 400 and
+// 483, of 100 604 and 645; 128 of 100 rows 1173 and 1273, of 200 2266 and 1829; 512 of 100 rows 4551 and 5754. A token takes its 1 us
+// in all heads at once as long as they find room; the chunks of one sequence fill the chip, those of many short ones are half empty.
 bool by_tokens(int B, int v_heads, int max_q) {
-  return max_q <= std::min<int64_t>(56, 12 + (int64_t)B * v_heads / 6);
+  const int64_t heads = (int64_t)B * v_heads;
+  return max_q <= std::min<int64_t>({112, 50 + heads / 48, 12 + heads / 6});
 }
 
 struct ChunkPlan {
