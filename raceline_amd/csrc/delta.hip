@@ -559,6 +559,7 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
 
 constexpr int kChainThreads = 512;
 constexpr float kMostSize = 3.0e38f;   // a bound past fp32 has to come back as it fades
+constexpr float kFarScale = 0x1p20f;   // 2^33 from one chunk's scale to the next, less the 2^13 of kLength
 
 // A workgroup goes through a sequence's chunks with 16 columns of one head's state. Four waves are the chain: each
 // has 16 of a chunk's rows, K S, R and U; four others read the rows out (Q S and, a step later, P U), 16 rows
@@ -756,11 +757,24 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
     fade = next[0], value = next[1];
     asm("" : "+v"(fade), "+v"(value));     // registers of their own: those of a load stay its own from step to step
     set_scale();
+    const float up = back * scale;
+    const bool far = __builtin_amdgcn_readfirstlane(__float_as_int(up)) > __float_as_int(kFarScale);   // the same in every lane
     second_place += at + 2 < c1 ? step_bytes : 0;
     if (has_tile) {
       sum += low;
+      // To the next scale. What the operands' last bits leave in a state that has faded away, 64 times 2^-25 at most, stays in its
+      // range where the scales lie less than 2^33 apart. Past that it is held there, so that it does not grow into an
+      // infinity, and the factors come one by one, as their product can pass fp32 (0 times it is NaN, for good).
+      if (!far) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = sum[i] * (back * scale);
+        for (int i = 0; i < 4; ++i) s[i] = sum[i] * up;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float t = sum[i] * back;
+          s[i] = __builtin_fmaf(t, 0.0f, __builtin_amdgcn_fmed3f(t * scale, -2.0f * kUnit, 2.0f * kUnit));   // t: NaN where it is not finite
+        }
+      }
       give_state();
       if (at + 1 == kept_chunks && stored) {
 #pragma unroll

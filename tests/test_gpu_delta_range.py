@@ -1,0 +1,41 @@
+"""gated_delta over the range of fp32: values that fade by more than fp32 spans."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests import recurrent as R
+from tests.test_gpu_delta import BF16, draw
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("max_q", [1, 300], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("state,first,later", [
+    (1e6, 0.0, 0.0), (1e8, 0.0, 0.0), (1e9, 0.0, 0.0), (2.0 ** 116, 0.0, 0.0), (2.0 ** 116, 0.0, 2.0 ** -30),
+    (0.3, 2.0 ** 116, 2.0 ** -30), (0.0, 2.0 ** 116, 2.0 ** -60), (2.0 ** 100, 2.0 ** 100, 2.0 ** -100)])
+@pytest.mark.parametrize("heads", ["h64", "k128"])
+def test_what_is_forgotten_leaves_no_trace(gpu, heads, state, first, later, max_q):
+    """A chunk that forgets all, in front of values that may be smaller by more than fp32 spans. Every token fades by e^-9.9
+    or more, so nothing of the first 64 rows reaches those behind the next 64 (e^-630), and these and the state are held to
+    the rule's own bounds; what stands in front has to be finite."""
+    from raceline_amd import ops
+
+    s, c = draw([(200, 300), (70, 70)], heads, BF16, seed=11, state=1.0)
+    Hv, Dk, Dv = c["state"].shape[1:]
+    c["a"] = c["a"] + 1e3
+    c["state"] = (np.clip(c["state"], -4, 4) * state).astype(np.float32).astype(np.float64)
+    size = np.where(np.arange(len(c["v"])) < 64, first, later)[:, None, None]
+    c["v"] = torch.from_numpy(np.clip(c["v"], -4, 4) * size).bfloat16().double().numpy()
+    f = lambda n, t=torch.float32: torch.from_numpy(c[n]).to(t).to(gpu)                  # noqa: E731
+    st = f("state")
+    out = ops.gated_delta(*(f(n, BF16).flatten(1) for n in "qkv"), f("a"), f("b"), f("a_log"), f("dt_bias"), st, *s.dev(gpu),
+                          max_q=max_q, out_dtype=BF16)
+    torch.cuda.synchronize()
+    assert out.isfinite().all() and st.isfinite().all()
+    args = [c[n][:200] for n in "qkvab"]
+    ref, S, tol, off = R.delta(*args, c["a_log"], c["dt_bias"], c["state"][s.slots[0]], Dk ** -0.5)
+    tol = (tol + R.half_step(BF16, np.abs(ref) + tol))[128:]
+    got = out[128:200].double().cpu().numpy().reshape(72, Hv, Dv)
+    assert (np.abs(got - ref[128:]) <= tol).all()
+    assert (np.abs(st[int(s.slots[0])].double().cpu().numpy() - S) <= off[:, None, :] + 1e-37).all()
