@@ -41,6 +41,9 @@ __device__ __forceinline__ float gate_of(float z) {
   return z * ((z >= 0.0f ? 1.0f : t) * __builtin_amdgcn_rcpf(1.0f + t));
 }
 
+// The squares of a row of 2^64 pass fp32: where their sum did, it is formed again of the row made smaller by this.
+constexpr float kSmaller = 0x1p-96f;
+
 template <typename T, int N>
 __device__ __forceinline__ void load_row(const T *p, bool wide, T (&x)[N]) {
   constexpr int kPack = N < 8 ? N : 8;
@@ -207,7 +210,15 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
       if (zp) {
         float sum = 0.0f;
         for (int i = 0; i < waves; ++i) sum += squares[mine][i];
-        const float r = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + a.norm_eps);
+        float eps = a.norm_eps;
+        if (sum == __builtin_inff()) {
+          sum = 0.0f, eps *= kSmaller * kSmaller, o *= kSmaller;
+          for (int i = 0; i < a.dv; ++i) {
+            const float x = os[mine][i] * kSmaller;
+            sum += x * x;
+          }
+        }
+        const float r = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + eps);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = o[e] * r * w[e] * gate_of(z[e]);
       }
@@ -938,10 +949,19 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
   const float *o = reinterpret_cast<const float *>(p.chunks + blockIdx.x * p.at.bytes() + p.at.rows_at()) + static_cast<int64_t>(row) * width;
   const int64_t out_row = static_cast<int64_t>(s.row0) + c.start + row;
   for (int i = threadIdx.x * 4; i < width; i += kGateThreads * 4) {   // whole heads: a head's lanes are of one wave
-    const f32x4 x = *reinterpret_cast<const f32x4 *>(o + i);
-    float sum = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
-    for (int off = lanes / 2; off; off >>= 1) sum += __shfl_xor(sum, off);
-    const float f = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + a.norm_eps);
+    f32x4 x = *reinterpret_cast<const f32x4 *>(o + i);
+    float eps = a.norm_eps;
+    auto squares = [&]() {
+      float sum = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+      for (int off = lanes / 2; off; off >>= 1) sum += __shfl_xor(sum, off);
+      return sum;
+    };
+    float sum = squares();
+    if (sum == __builtin_inff()) {       // in all lanes of a head
+      x *= kSmaller, eps *= kSmaller * kSmaller;
+      sum = squares();
+    }
+    const float f = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + eps);
     const float *z = a.z + out_row * a.z_stride + i, *w = a.norm + i % a.dv;
     TO *to = static_cast<TO *>(a.out) + out_row * a.out_stride + i;
 #pragma unroll

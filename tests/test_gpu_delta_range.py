@@ -1,11 +1,12 @@
-"""gated_delta over the range of fp32: values that fade by more than fp32 spans."""
+"""gated_delta over the range of fp32: values that fade by more than fp32 spans, rows
+whose squares pass fp32."""
 
 import numpy as np
 import pytest
 import torch
 
 from tests import recurrent as R
-from tests.test_gpu_delta import BF16, draw
+from tests.test_gpu_delta import BF16, check, draw
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,15 @@ def test_what_is_forgotten_leaves_no_trace(gpu, heads, state, first, later, max_
     got = out[128:200].double().cpu().numpy().reshape(72, Hv, Dv)
     assert (np.abs(got - ref[128:]) <= tol).all()
     assert (np.abs(st[int(s.slots[0])].double().cpu().numpy() - S) <= off[:, None, :] + 1e-37).all()
+
+
+@pytest.mark.parametrize("max_q", [1, 300], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("heads", ["h64", "wide", "256", "one"])
+@pytest.mark.parametrize("size", [2.0 ** 58, 2.0 ** 70, 2.0 ** 110])
+def test_rows_whose_squares_pass_fp32_are_normalised(gpu, size, heads, max_q):
+    s, c = draw([(90, 100), (2, 5), (70, 70)], heads, BF16, seed=5)
+    c["v"] = torch.from_numpy(c["v"] * size).bfloat16().double().numpy()
+    c["state"] = (c["state"] * size).astype(np.float32).astype(np.float64)
+    c["v"][:, 0] /= 2.0 ** 60                                  # another head of ordinary rows beside them
+    c["state"][:, 0] /= 2.0 ** 60
+    check(gpu, s, c, BF16, True, out_dtype=BF16, max_q=max_q)
