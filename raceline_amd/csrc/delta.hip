@@ -878,7 +878,8 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
     float unit = 0.0f;
     // the rows of the chunk whose U lies in LDS
     auto finish = [&]() {
-      const f32x4 o = times_mats(ub, read * qs, load_update) * (length * unit);
+      // one by one: their product can lie below fp32's last bits where the row does not
+      const f32x4 o = times_mats(ub, read * qs, load_update) * length * unit;
       if (a.z) {
         if (c.rows == kChunk) {
 #pragma unroll

@@ -1,5 +1,5 @@
 """gated_delta over the range of fp32: values that fade by more than fp32 spans, rows
-whose squares pass fp32."""
+whose squares pass fp32, values next to the smallest ones."""
 
 import numpy as np
 import pytest
@@ -52,3 +52,13 @@ def test_rows_whose_squares_pass_fp32_are_normalised(gpu, size, heads, max_q):
     c["v"][:, 0] /= 2.0 ** 60                                  # another head of ordinary rows beside them
     c["state"][:, 0] /= 2.0 ** 60
     check(gpu, s, c, BF16, True, out_dtype=BF16, max_q=max_q)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -112, 2.0 ** -118])
+@pytest.mark.parametrize("heads", ["h64", "k128"])
+def test_values_next_to_the_smallest(gpu, size, heads):
+    s, c = draw([(90, 100), (2, 5), (70, 70)], heads, BF16, seed=6)
+    c["v"] = torch.from_numpy(c["v"] * size).bfloat16().double().numpy()
+    c["state"] = (c["state"] * size).astype(np.float32).astype(np.float64)
+    for max_q in (1, 300):
+        check(gpu, s, c, BF16, out_dtype=BF16, max_q=max_q)
