@@ -441,9 +441,11 @@ int rlq_causal_conv(const float *x, int x_stride, int T, int channels, int taps,
  * k_heads; eps and norm_eps at least 1e-37. State and sums in fp32; rows of q and k have lengths below 2^63.
  * max_q (host) bounds the rows of a sequence: it chooses between the rule token by token and its form in
  * chunks of 64 tokens (from a sequence's first row on, and anew behind the kept ones), and results stay right past
- * it. In chunks the factors of a product hold 22 bits and values and state are held by the largest finite value
- * that the head has met, as it faded: what is smaller than its 2^-14 begins to lose bits; finite values are to be below
- * 2^120. An infinity or NaN in a row of a chunk also reaches the rows in front of it in that chunk, in the values it
+ * it. In chunks the factors of a product hold 22 bits, and in a chunk values and state are held to 2^-39 of a bound of their
+ * head: 9 of the chunk's largest finite value and what a column of the state can be long, which is sqrt(Dk) of its largest finite
+ * element where the call begins, and behind each chunk the root of that, faded, squared and the square of 8 of the chunk's
+ * largest value. So what is smaller than 2^-17 of the bound begins to lose bits: in a first chunk from zeros 2^-13 of the largest value, in the
+ * n-th without any fade 2^-13 sqrt(n) of it. Finite values are to be below 2^120. An infinity or NaN in a row of a chunk also reaches the rows in front of it in that chunk, in the values it
  * touches; in v or the state it stays in its column (with z in its head), and it never reaches another sequence. The workspace
  * (rlq_gated_delta_workspace_bytes, may be 0; 16-byte aligned, no initialisation) holds what the chunks
  * hand on; calls that overlap must not share it. */

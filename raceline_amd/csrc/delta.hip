@@ -568,6 +568,14 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
   }
 }
 
+// sqrt(x^2 + y^2) of two that are not negative, by a power of two so that neither square passes fp32.
+__device__ __forceinline__ float length_of(float x, float y) {
+  const int ex = max(1, min(253, (int)(__float_as_uint(fmaxf(x, y)) >> 23)));
+  const float down = __uint_as_float((254 - ex) << 23);
+  x *= down, y *= down;
+  return __builtin_amdgcn_sqrtf(x * x + y * y) * __uint_as_float(ex << 23);
+}
+
 constexpr int kChainThreads = 512;
 constexpr float kMostSize = 3.0e38f;   // a bound past fp32 has to come back as it fades
 constexpr float kFarScale = 0x1p20f;   // 2^33 from one chunk's scale to the next, less the 2^13 of kLength
@@ -576,9 +584,10 @@ constexpr float kFarScale = 0x1p20f;   // 2^33 from one chunk's scale to the nex
 // has 16 of a chunk's rows, K S, R and U; four others read the rows out (Q S and, a step later, P U), 16 rows
 // each; and every wave has a tile of 16 of the state's rows (64 of them: the chain's waves). S, R and U go between
 // the waves as operands in LDS, a barrier after each.
-// Values are held times a power of two that keeps them in fp16's range: with keys of length 1 and beta at most 1 a
-// chunk lengthens a column of S by at most the sum of its values' squares (8 of the largest), and R and U are never
-// larger than a column of S and 9 of the largest value.
+// Values are held times a power of two that keeps them in fp16's range: with keys of length 1 and beta at most 1 the square
+// of a column's length in S grows by at most the values' squares (64 of the largest a chunk), and R and U are never
+// larger than a column of S and 9 of the largest value. Without a fade that bound is 8 sqrt(n) of the largest value after n chunks
+// (lengths added up, not their squares, would be 8 n, and 512 chunks would cost values of 2^-18 of the largest their last bits).
 // What a wave reads of the next chunk is asked for as soon as this chunk's has been used, so every load has a whole
 // step to arrive; no branch stands between a load and its use, or the wait there would be for all of them. The values
 // come by way of the reading waves, which have slack: their loads and addresses cost the chain 3 of 50 us.
@@ -743,6 +752,8 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
     load_tile();
     next = load_pair(second_place);
   };
+  // the bound behind this chunk: beside a product, as nothing of it waits for one
+  auto grow = [&]() { size = fminf(length_of(fade * size, 8.0f * value), kMostSize); };
   // S <- fade S + K^T W, of this wave's tile, and the next chunk's scale
   auto update_state = [&](int at, auto beside) {
     const float faded = fade * kLength, back = inverse * (1.0f / kLength);
@@ -764,7 +775,6 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
         low = mfma(kt[e], w[1][e], low);
       }
     }
-    size = fminf(fade * size + 8.0f * value, kMostSize);
     fade = next[0], value = next[1];
     asm("" : "+v"(fade), "+v"(value));     // registers of their own: those of a load stay its own from step to step
     set_scale();
@@ -848,6 +858,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
       const f32x4 u = times_mats(rb, f32x4{}, [&]() {
         load_rows();
         load_factors();
+        grow();
       });
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -924,6 +935,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
       load_rows();
       give_values();
       next_values();
+      grow();
 
       lds_barrier();
       update_state(at, [] {});

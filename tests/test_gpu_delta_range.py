@@ -1,5 +1,5 @@
 """gated_delta over the range of fp32: values that fade by more than fp32 spans, rows
-whose squares pass fp32, values next to the smallest ones."""
+whose squares pass fp32, values next to the smallest ones, columns far smaller than others of their head."""
 
 import numpy as np
 import pytest
@@ -62,3 +62,36 @@ def test_values_next_to_the_smallest(gpu, size, heads):
     c["state"] = (c["state"] * size).astype(np.float32).astype(np.float64)
     for max_q in (1, 300):
         check(gpu, s, c, BF16, out_dtype=BF16, max_q=max_q)
+
+
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("gate", [False, True], ids=["plain", "gated"])
+def test_small_columns_keep_their_bits_without_a_fade(gpu, dk, gate):
+    """Keys and queries of one element, weights of 1 and no fade: after each token the state's row of its key is its value,
+    and its output that row. Every number on the way is a whole one of at most 8 bits times a power of two, so fp32 and
+    the operands of chunks hold it exactly, unless its unit lies below the last bit that they keep: 2^-39 of the bound that
+    a head's values are held by. Values here are up to 127; after n chunks the bound is 127 (9 + 8 sqrt(n)) at most,
+    and units of 2^-21 (2^-28 of the largest value) are kept for 32768 rows; 127 (9 + 8 n), a sum of lengths in place of their
+    squares', would lose them from 130 chunks on."""
+    from raceline_amd import ops
+
+    T, dv = 32768, 64
+    g = torch.Generator(device=gpu)
+    g.manual_seed(3)
+    order = torch.cat([torch.randperm(dk, generator=g, device=gpu) for _ in range(T // dk)])
+    rows = torch.zeros(T, dk, device=gpu, dtype=BF16)
+    rows[torch.arange(T, device=gpu), order] = 1
+    v = torch.randint(-127, 128, (T, dv), generator=g, device=gpu).float()
+    v[:, 0] = 127
+    v[:, 1::2] *= 2.0 ** -21
+    ints = dict(dtype=torch.int32, device=gpu)
+    a, b, zero = torch.full((T, 1), -1e30, device=gpu), torch.full((T, 1), 1e30, device=gpu), torch.zeros(1, device=gpu)
+    state = ops.delta_state(1, 1, dk, dv)
+    extra = dict(z=torch.full((T, dv), 1e30, device=gpu), norm=torch.ones(dv, device=gpu)) if gate else {}
+    out = ops.gated_delta(rows, rows, v.bfloat16(), a, b, zero, zero, state, torch.tensor([0, T], **ints), torch.tensor([T], **ints),
+                          torch.tensor([0], **ints), max_q=T, scale=1.0, eps=1e-37, out_dtype=BF16, **extra)
+    want = torch.empty(dk, dv, device=gpu)
+    want[order[-dk:]] = v[-dk:]
+    assert torch.equal(state[0, 0], want)
+    if not gate:
+        assert torch.equal(out.float(), v)
