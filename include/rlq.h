@@ -439,9 +439,10 @@ int rlq_causal_conv(const float *x, int x_stride, int T, int channels, int taps,
  * [T][z_stride]; norm fp32 [Dv]; out 16-bit (out_dtype) [T][out_stride]. state fp32
  * [n_slots][v_heads][Dk][Dv], 16-byte aligned. Dk 64 or 128; Dv 64, 128 or 256; v_heads a multiple of
  * k_heads; eps and norm_eps at least 1e-37. State and sums in fp32; rows of q and k have lengths below 2^63.
+ * B * v_heads * Dv is below 2^31, B * v_heads below 2^24 where max_q asks for chunks.
  * max_q (host) bounds the rows of a sequence: it chooses between the rule token by token and its form in
  * chunks of 64 tokens (from a sequence's first row on, and anew behind the kept ones), and results stay right past
- * it. In chunks the factors of a product hold 22 bits, and in a chunk values and state are held to 2^-39 of a bound of their
+ * it; from B * v_heads * Dv = 2^27 on it is token by token. In chunks the factors of a product hold 22 bits, and in a chunk values and state are held to 2^-39 of a bound of their
  * head: 9 of the chunk's largest finite value and what a column of the state can be long, which is sqrt(Dk) of its largest finite
  * element where the call begins, and behind each chunk the root of that, faded, squared and the square of 8 of the chunk's
  * largest value. So what is smaller than 2^-17 of the bound begins to lose bits: in a first chunk from zeros 2^-13 of the largest value, in the

@@ -987,9 +987,13 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
 // 44; sixteen of 48 rows 85 and 106, of 64 rows 110 and 107; 32 of 64 rows 211 and 217, of 100 318 and 289; 64 of 64 rows 400 and
 // 483, of 100 604 and 645; 128 of 100 rows 1173 and 1273, of 200 2266 and 1829; 512 of 100 rows 4551 and 5754. A token takes its 1 us
 // in all heads at once as long as they find room; the chunks of one sequence fill the chip, those of many short ones are half empty.
-bool by_tokens(int B, int v_heads, int max_q) {
+// Batches of 2^27 columns and more (32768 sequences of 32 heads of 128) are past what the chunks are for, whatever max_q says: each run's
+// workgroups look through all sequences. 32700 of 32 heads of 64 x 128, a row each: 13 ms and 2386; with one of 20000 rows
+// beside them 26 and 2395.
+constexpr int64_t kMostColumns = 1 << 27, kMostHeads = 1 << 24;
+bool by_tokens(int B, int v_heads, int dv, int max_q) {
   const int64_t heads = (int64_t)B * v_heads;
-  return max_q <= std::min<int64_t>({112, 50 + heads / 48, 12 + heads / 6});
+  return max_q <= std::min<int64_t>({112, 50 + heads / 48, 12 + heads / 6}) || ((heads + 7) / 8 * 8 * dv >= kMostColumns && heads < kMostHeads);
 }
 
 struct ChunkPlan {
@@ -1018,18 +1022,17 @@ int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
   p.carry[0] = reinterpret_cast<float *>(p.chunks + plan.most * p.at.bytes());
   p.carry[1] = reinterpret_cast<float *>(reinterpret_cast<char *>(p.carry[0]) + p.at.state());
   const int parts = (a.v_heads / a.k_heads + kHeadsPer - 1) / kHeadsPer;
-  const int64_t pairs = ((int64_t)a.c.batch * a.v_heads + 7) / 8 * 8;
-  RLQ_REQUIRE(a.k_heads * (int64_t)parts <= 65535 && pairs * (a.dv / 16) * kChainThreads <= UINT32_MAX,
-              "rlq_gated_delta: %d heads of %d sequences are too many for chunks", a.v_heads, a.c.batch);
   // a sequence has two chunks' places or more, so the chain of a run need not look at all of many sequences
   p.sequences = (int)std::min<int64_t>(a.c.batch, plan.count / 2 + 2);
-  const unsigned chain_grid = (unsigned)(((int64_t)p.sequences * a.v_heads + 7) / 8 * 8 * (a.dv / 16));
+  const int64_t chain_grid = ((int64_t)p.sequences * a.v_heads + 7) / 8 * 8 * (a.dv / 16);
+  RLQ_REQUIRE((int64_t)a.c.batch * a.v_heads < kMostHeads && a.k_heads * (int64_t)parts <= 65535 && chain_grid * kChainThreads <= UINT32_MAX,
+              "rlq_gated_delta: %d heads of %d sequences are too many for chunks", a.v_heads, a.c.batch);
   for (int64_t first = 0; first < plan.slots; first += plan.count, ++p.run) {
     p.first = (int)first;
     p.count = (int)std::min<int64_t>(plan.count, plan.slots - first);
     delta_chunks_kernel<T, DK><<<dim3(p.count, a.k_heads * parts), kPrepareThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
-    delta_chain_kernel<T, TO, DK><<<chain_grid, kChainThreads, 0, st>>>(p);
+    delta_chain_kernel<T, TO, DK><<<(unsigned)chain_grid, kChainThreads, 0, st>>>(p);
     RLQ_HIP(hipGetLastError());
     if (a.z) {
       delta_gate_kernel<TO><<<dim3(p.count, kChunk), kGateThreads, 0, st>>>(p);
@@ -1041,7 +1044,7 @@ int launch_chunks(const DeltaArgs &a, void *workspace, hipStream_t st) {
 
 template <typename T, typename TO>
 int launch_delta(const DeltaArgs &a, int DK, int max_q, void *workspace, hipStream_t st) {
-  if (!by_tokens(a.c.batch, a.v_heads, max_q)) return DK == 64 ? launch_chunks<T, TO, 64>(a, workspace, st) : launch_chunks<T, TO, 128>(a, workspace, st);
+  if (!by_tokens(a.c.batch, a.v_heads, a.dv, max_q)) return DK == 64 ? launch_chunks<T, TO, 64>(a, workspace, st) : launch_chunks<T, TO, 128>(a, workspace, st);
   const unsigned grid = (unsigned)a.c.batch * (unsigned)a.v_heads;
   RLQ_REQUIRE(a.c.batch * (int64_t)a.v_heads * a.dv * 2 <= UINT32_MAX, "rlq_gated_delta: %d heads of %d sequences are too many",
               a.v_heads, a.c.batch);
@@ -1057,7 +1060,7 @@ int launch_delta(const DeltaArgs &a, int DK, int max_q, void *workspace, hipStre
 extern "C" {
 
 size_t rlq_gated_delta_workspace_bytes(int T, int k_heads, int v_heads, int Dk, int Dv, int B, int max_q) {
-  if (T <= 0 || B <= 0 || rlq::by_tokens(B, v_heads, max_q) || k_heads < 1 || v_heads < k_heads || Dk <= 0 || Dv <= 0) return 0;
+  if (T <= 0 || B <= 0 || rlq::by_tokens(B, v_heads, Dv, max_q) || k_heads < 1 || v_heads < k_heads || Dk <= 0 || Dv <= 0) return 0;
   return (size_t)rlq::plan_chunks({Dk, k_heads, v_heads, Dv}, T, B).bytes;
 }
 

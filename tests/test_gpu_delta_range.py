@@ -95,3 +95,38 @@ def test_small_columns_keep_their_bits_without_a_fade(gpu, dk, gate):
     assert torch.equal(state[0, 0], want)
     if not gate:
         assert torch.equal(out.float(), v)
+
+
+def test_more_sequences_than_chunks_are_for(gpu):
+    """A batch whose heads are past the chunked form takes a large max_q too: every sequence as in a call of its own."""
+    from raceline_amd import ops
+
+    Hk, Hv, Dk, Dv, B, most = 1, 32, 64, 128, 33000, 1 << 20
+    rng = np.random.default_rng(8)
+    lens = np.zeros(B, np.int64)
+    lens[rng.choice(B, 40, replace=False)] = rng.integers(1, 4, 40)
+    lens[[0, 777, B - 1]] = 5, 150, 2
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    T, used = int(cu[-1]), np.nonzero(lens)[0]
+    slots = np.full(B, -1)
+    slots[used] = rng.permutation(len(used))
+    assert ops.gated_delta_workspace_bytes(T, Hk, Hv, Dk, Dv, B, most) == 0
+    ints = dict(dtype=torch.int32, device=gpu)
+    g = torch.Generator(device=gpu)
+    g.manual_seed(4)
+    rnd = lambda *n: torch.randn(n, generator=g, device=gpu)                             # noqa: E731
+    x, ba = rnd(T, 2 * Hk * Dk + Hv * Dv).bfloat16(), rnd(T, 2 * Hv)
+    a_log, dt, start = rnd(Hv) - 2, rnd(Hv) - 3, rnd(len(used), Hv, Dk, Dv)
+
+    def run(state, lo, hi, cu, kv, slots, max_q):
+        r = slice(lo, hi)
+        return ops.gated_delta(x[r, :Dk], x[r, Dk:2 * Dk], x[r, 2 * Dk:], ba[r, :Hv], ba[r, Hv:], a_log, dt, state,
+                               torch.tensor(cu, **ints), torch.tensor(kv, **ints), torch.tensor(slots, **ints), max_q=max_q,
+                               out_dtype=BF16)
+
+    together, alone = start.clone(), start.clone()
+    whole = run(together, 0, T, cu, lens + 3, slots, most)
+    for b in used:
+        rows = run(alone, int(cu[b]), int(cu[b + 1]), [0, lens[b]], [lens[b] + 3], [slots[b]], 1)
+        assert torch.equal(rows, whole[cu[b]:cu[b + 1]]), b
+    assert torch.equal(together, alone)

@@ -145,3 +145,10 @@ def sample_args(**change):
 def test_sample_checks_its_tensors(change):
     with pytest.raises(ValueError):
         ops.sample(**sample_args(**change))
+
+
+def test_gated_delta_goes_token_by_token_where_chunks_have_no_room():
+    """32768 sequences of 32 heads of 128 and more: whatever max_q is, and without scratch. Below, max_q chooses."""
+    for heads, dv, border in ((32, 128, 1 << 15), (16, 256, 1 << 15), (8, 64, 1 << 18)):
+        assert ops.gated_delta_workspace_bytes(1 << 20, 1, heads, 64, dv, border - 1, 1 << 20) > 0
+        assert ops.gated_delta_workspace_bytes(1 << 20, 1, heads, 64, dv, border, 1 << 20) == 0
