@@ -105,3 +105,20 @@ def test_other_sequences_do_not_reach_a_row(gpu):
     assert torch.equal(got[:6], want[:6]) and torch.equal(got[13:], want[13:]) and got[6:13].isnan().all()
     for b in (0, 2):
         assert torch.equal(state[int(s.slots[b])], want_state[int(s.slots[b])])
+
+
+LONG = [(15, 15), (16, 40), (17, 17), (33, 60), (0, 3), (1, 9), (1050, 1050), (31, 32), (2, 2), (1040, 3000)]
+
+
+@pytest.mark.parametrize("taps,C,pad", [(4, 8192, 0), (3, 8192, 0), (2, 8192, 4), (4, 2051, 0), (3, 2048, 1), (2, 2048, 3), (4, 8196, 0)])
+def test_long_calls_in_runs_of_sixteen(gpu, taps, C, pad):
+    """Calls of 2048 waves and more take runs of 16 tokens: with wide loads 8192 channels a wave of 256, else a wave of 64."""
+    rows = sum(n for n, _ in LONG)
+    wide = C % 4 == 0 and pad % 4 == 0
+    assert rows // 16 * -(-C // (64 * (4 if wide else 1))) >= 2048
+    check(gpu, LONG, C, taps, torch.bfloat16 if taps == 3 else torch.float16, bias=taps != 2, pad=pad, seed=C + taps, more_rows=9)
+
+
+@pytest.mark.parametrize("C", [8192, 2049])
+def test_kept_rows_of_long_calls(gpu, C):
+    check(gpu, LONG, C, keep=[15, 3, 0, 32, 7, 1, 1049, 16, 1, 2], silu=C != 2049, seed=C, slots=[0, 1, 2, 3, 4, 5, 6, -1, 7, 8])
