@@ -170,3 +170,29 @@ def test_after_adjust_logits(gpu):
     y = ops.adjust_logits(x, allowed=torch.from_numpy(mask).to(gpu))
     got = check(gpu, y.cpu().numpy(), rng.random(4), p=0.9)
     assert got[3] == -1 and all(mask.view(np.uint32)[r][t // 32] >> (t % 32) & 1 for r, t in enumerate(got[:3]))
+
+
+@pytest.mark.parametrize("V", [2**18 + 1, 2**22])
+def test_the_largest_vocabularies(gpu, V):
+    """Past 2^18 tokens a weight is held in steps of 2^-(62 - ceil(log2 V)) of the largest: each is off by half a step and their
+    sum by V / 2 of them, so a share of a weight of W is off by less than V steps / W, and a number that lies farther from a
+    border is on the right side of it."""
+    rng = np.random.default_rng(V)
+    step = 2.0 ** -(62 - int(np.ceil(np.log2(V))))
+    flat = np.full((2, V), 2.5, np.float32)
+    x = np.concatenate([rows_of(rng, 1, V), np.round(rows_of(rng, 1, V))])
+    u = rng.random(2)
+    told = 0
+    for rows, f in ((flat, {}), (flat, dict(p=0.7)), (flat, dict(k=V - 1000)), (flat, dict(k=V // 3, p=0.5)), (x, {}), (x, dict(p=0.9)),
+                    (x, dict(m=0.001)), (x, dict(k=100000, p=0.99, m=1e-4, T=0.9)), (x, dict(T=0.0))):
+        tokens, probs = run(gpu, rows, u, **f)
+        for r in range(2):
+            T, p, m = (float(np.float32(f.get(n, d))) for n, d in (("T", 1.0), ("p", 1.0), ("m", 0.0)))
+            want, share, border = R.choose(rows[r], u[r], T, f.get("k", 0), p, m)
+            w = 1.0 if not T > 0 else np.exp((float(rows[r][want]) - float(rows[r].max())) / T)
+            near = V * step * share / w
+            if border > near:
+                told += 1
+                assert tokens[r] == want, (f, r)
+                assert abs(probs[r] - share) <= share * 2.0 ** -23 + near, (f, r)
+    assert told >= 16                                              # of 18
