@@ -839,7 +839,6 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
     load_factors();
     left = load4(place + factors_at + 2 * kChunk * 4 + row_bytes);
     __builtin_amdgcn_s_waitcnt(0x0F70);      // vmcnt(0): the loop's own waits are then for loads of a step before
-    __builtin_amdgcn_s_setprio(2);           // the other waves have slack
     lds_barrier();
 
     for (int at = c0; at < c1; ++at) {
