@@ -423,7 +423,8 @@ int rlq_attention(const void *q, int q_stride, int T, int heads, int kv_heads, i
  *   y_t[c] = act(bias[c] + sum_j w[c][j] x_{t - (taps-1) + j}[c]),  act = SiLU with `silu`, else none.
  * x fp32 [T][x_stride] (a slice of the in projection's rows, say); w fp32 [channels][taps]; bias fp32
  * [channels] or NULL; out 16-bit (out_dtype) [T][out_stride]. state fp32 [n_slots][taps-1][channels]:
- * the last taps-1 rows of a sequence's inputs, the newest last. Sums in fp32. */
+ * the last taps-1 rows of a sequence's inputs, the newest last. Sums in fp32.
+ * out must not share memory with the other arrays. */
 int rlq_causal_conv(const float *x, int x_stride, int T, int channels, int taps, const float *w, const float *bias,
                     int silu, float *state, int n_slots, const int *cu_q, const int *kv_len, const int *slots,
                     const int *keep, int B, void *out, int out_stride, int out_dtype, void *stream);
@@ -442,12 +443,15 @@ int rlq_causal_conv(const float *x, int x_stride, int T, int channels, int taps,
  * B * v_heads * Dv is below 2^31, B * v_heads below 2^24 where max_q asks for chunks.
  * max_q (host) bounds the rows of a sequence: it chooses between the rule token by token and its form in
  * chunks of 64 tokens (from a sequence's first row on, and anew behind the kept ones), and results stay right past
- * it; from B * v_heads * Dv = 2^27 on it is token by token. In chunks the factors of a product hold 22 bits, and in a chunk values and state are held to 2^-39 of a bound of their
- * head: 9 of the chunk's largest finite value and what a column of the state can be long, which is sqrt(Dk) of its largest finite
- * element where the call begins, and behind each chunk the root of that, faded, squared and the square of 8 of the chunk's
- * largest value. So what is smaller than 2^-17 of the bound begins to lose bits: in a first chunk from zeros 2^-13 of the largest value, in the
- * n-th without any fade 2^-13 sqrt(n) of it. Finite values are to be below 2^120. An infinity or NaN in a row of a chunk also reaches the rows in front of it in that chunk, in the values it
- * touches; in v or the state it stays in its column (with z in its head), and it never reaches another sequence. The workspace
+ * it, but for what is not finite; from B * v_heads * Dv = 2^27 on it is token by token.
+ * In chunks the factors of a product hold 22 bits, and values and state are held to 2^-39 of a bound of their head: 9 of the
+ * chunk's largest finite value and what a column of the state can be long. That is sqrt(Dk) of its largest finite element where
+ * the call begins (and where the scratch of a long one is used anew), and behind each chunk the root of its square, faded, and the
+ * square of 8 of the chunk's largest value. So what is smaller than 2^-17 of the bound begins to lose bits: in a first chunk from
+ * zeros 2^-13 of the largest value, in the n-th without any fade 2^-13 sqrt(n) of it. Finite values are to be below 2^120.
+ * In chunks an infinity or NaN in a row also reaches the rows in front of it in its chunk, in the values it touches (token by
+ * token it does not); in v or the state it stays in its column (with z in its head), and it never reaches another sequence.
+ * out must not share memory with the other arrays. The workspace
  * (rlq_gated_delta_workspace_bytes, may be 0; 16-byte aligned, no initialisation) holds what the chunks
  * hand on; calls that overlap must not share it. */
 size_t rlq_gated_delta_workspace_bytes(int T, int k_heads, int v_heads, int Dk, int Dv, int B, int max_q);

@@ -68,8 +68,9 @@ __device__ __forceinline__ void load_row(const T *p, bool wide, T (&x)[N]) {
 // for all of the call's tokens; sums over the rows go over the lanes of a column without LDS. What does not depend on
 // the state goes beside it, eight tokens at a time: keys and queries to length 1, a token a wave, before; the norm of
 // the rows and their gate, four values a thread, behind.
-// Bound by HBM for many sequences (48 of 32 heads of 128 x 128: 203 MB in 34.8 us, 5.8 TB/s), else by the chain of a
-// token's sums, 1 us each (one token 6.9 us, nine drafts of five 10.5).
+// Bound by HBM for many sequences (48 of 32 heads of 128 x 128: 203 MB in 43.9 us, 4.6 TB/s), else by a token's 1 us, of which
+// half is the issue of its work on 64 elements a lane (VALU share 0.45 at one wave a SIMD) and half the chain of its sums (one token
+// 6.8 us, nine drafts of five 10.5).
 template <typename T, typename TO, int DK>
 __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
   constexpr int kRows = DK / 8, kOf = DK / 64, kBatch = 8, kMostDv = 256;
@@ -237,14 +238,14 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
 
 // ------------------------------------------------------------------ chunks of 64 tokens
 
-// With G_i the sum of log g up to row i of a chunk, L_ij = beta_i e^(G_i - G_j) k_i.k_j below the diagonal and
-// S the state in front of the chunk, the rule over the chunk's rows is
+// The published triangular (WY) form of the rule. With G_i the sum of log g up to row i of a chunk,
+// L_ij = beta_i e^(G_i - G_j) k_i.k_j below the diagonal and S the state in front of the chunk, the rule over the chunk's rows is
 //   R = beta (V - e^G (K S)),   U = (I + L)^-1 R,
 //   O = e^G (Q S) + P U,        P_ij = e^(G_i - G_j) q_i.k_j on and below the diagonal,
 //   S <- e^(G_64) S + (e^(G_64 - G) K)^T U.
 // delta_chunks_kernel forms what does not depend on S, of all chunks at once: T = (I + L)^-1, P, and the rows
 // as operands. delta_chain_kernel goes through a sequence's chunks with S. A 2048-token chunk of a prompt, 16 key and 32
-// value heads of 128: 23 + 47.7 us, and 16 for the rows' norm and gate; token by token it took 5870.
+// value heads of 128: 24 + 50 us, and 17 for the rows' norm and gate; token by token it took 5870.
 //
 // The products are to keep the state to fp32: rows of q and k, brought to a length of 2^13 .. 2^14 by a power of
 // two, are exact in fp16 (what bf16 loses there lies 2^-38 below the length); T, P, R, U and S are two fp16
@@ -591,8 +592,8 @@ constexpr float kFarScale = 0x1p20f;   // 2^33 from one chunk's scale to the nex
 // What a wave reads of the next chunk is asked for as soon as this chunk's has been used, so every load has a whole
 // step to arrive; no branch stands between a load and its use, or the wait there would be for all of them. The values
 // come by way of the reading waves, which have slack: their loads and addresses cost the chain 3 of 50 us.
-// Bound by the chain: a step is 1.4 us, K S, R, U and S with three barriers, each a few dependent products (32 steps 47.7 us,
-// 39 without any load; 256 workgroups of two waves a SIMD, MFMA 0.18, VALU 0.39, LDS 0.30). A 16-column slice fills the chip
+// Bound by the chain: a step is 1.5 us, K S, R, U and S with three barriers, each a few dependent products (32 steps 50 us,
+// 39 without any load; 256 workgroups of two waves a SIMD, MFMA 0.17, VALU 0.41, LDS 0.29). A 16-column slice fills the chip
 // from one sequence of 32 heads of 128; two slices a CU share its cycles. With the reading waves' Q asked for beside the
 // state's step 50.7, without loads above T's diagonal 49.2 (branches), at four waves a SIMD 92 (spills).
 template <typename T, typename TO, int DK>
@@ -986,6 +987,9 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
 // 44; sixteen of 48 rows 85 and 106, of 64 rows 110 and 107; 32 of 64 rows 211 and 217, of 100 318 and 289; 64 of 64 rows 400 and
 // 483, of 100 604 and 645; 128 of 100 rows 1173 and 1273, of 200 2266 and 1829; 512 of 100 rows 4551 and 5754. A token takes its 1 us
 // in all heads at once as long as they find room; the chunks of one sequence fill the chip, those of many short ones are half empty.
+// The rule gives 64 of 100 rows to the chunks (7% lost). It goes by these heads for all: of 150 sizes in five geometries (12 to 160
+// rows, 1 to 256 sequences) it is within 3% of the better form in all but eight, which lose 14 to 41% (256 of 112 rows, 8 heads of 64 x 128:
+// 392 and 552; heads of 128 x 256 1.3 times in 12 rows of one sequence, 23 and 18).
 // Batches of 2^27 columns and more (32768 sequences of 32 heads of 128) are past what the chunks are for, whatever max_q says: each run's
 // workgroups look through all sequences. 32700 of 32 heads of 64 x 128, a row each: 13 ms and 2386; with one of 20000 rows
 // beside them 26 and 2395.
