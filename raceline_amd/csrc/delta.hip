@@ -41,7 +41,8 @@ __device__ __forceinline__ float gate_of(float z) {
   return z * ((z >= 0.0f ? 1.0f : t) * __builtin_amdgcn_rcpf(1.0f + t));
 }
 
-// The squares of a row of 2^64 pass fp32: where their sum did, it is formed again of the row made smaller by this.
+// The squares of a row of 2^64 pass fp32: where their mean and eps did, they are formed again of the row made smaller by this
+// (and eps by its square, which is no float).
 constexpr float kSmaller = 0x1p-96f;
 
 template <typename T, int N>
@@ -211,15 +212,16 @@ __global__ __launch_bounds__(512) void delta_tokens_kernel(DeltaArgs a) {
       if (zp) {
         float sum = 0.0f;
         for (int i = 0; i < waves; ++i) sum += squares[mine][i];
-        float eps = a.norm_eps;
-        if (sum == __builtin_inff()) {
-          sum = 0.0f, eps *= kSmaller * kSmaller, o *= kSmaller;
+        float square = sum * (1.0f / a.dv) + a.norm_eps;
+        if (square == __builtin_inff()) {
+          sum = 0.0f, o *= kSmaller;
           for (int i = 0; i < a.dv; ++i) {
             const float x = os[mine][i] * kSmaller;
             sum += x * x;
           }
+          square = sum * (1.0f / a.dv) + a.norm_eps * kSmaller * kSmaller;
         }
-        const float r = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + eps);
+        const float r = __builtin_amdgcn_rsqf(square);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = o[e] * r * w[e] * gate_of(z[e]);
       }
@@ -963,18 +965,17 @@ __global__ __launch_bounds__(kGateThreads) void delta_gate_kernel(ChunkArgs p) {
   const int64_t out_row = static_cast<int64_t>(s.row0) + c.start + row;
   for (int i = threadIdx.x * 4; i < width; i += kGateThreads * 4) {   // whole heads: a head's lanes are of one wave
     f32x4 x = *reinterpret_cast<const f32x4 *>(o + i);
-    float eps = a.norm_eps;
-    auto squares = [&]() {
+    auto mean = [&]() {
       float sum = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
       for (int off = lanes / 2; off; off >>= 1) sum += __shfl_xor(sum, off);
-      return sum;
+      return sum * (1.0f / a.dv);
     };
-    float sum = squares();
-    if (sum == __builtin_inff()) {       // in all lanes of a head
-      x *= kSmaller, eps *= kSmaller * kSmaller;
-      sum = squares();
+    float square = mean() + a.norm_eps;
+    if (square == __builtin_inff()) {    // in all lanes of a head
+      x *= kSmaller;
+      square = mean() + a.norm_eps * kSmaller * kSmaller;
     }
-    const float f = __builtin_amdgcn_rsqf(sum * (1.0f / a.dv) + eps);
+    const float f = __builtin_amdgcn_rsqf(square);
     const float *z = a.z + out_row * a.z_stride + i, *w = a.norm + i % a.dv;
     TO *to = static_cast<TO *>(a.out) + out_row * a.out_stride + i;
 #pragma unroll

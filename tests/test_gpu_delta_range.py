@@ -130,3 +130,14 @@ def test_more_sequences_than_chunks_are_for(gpu):
         rows = run(alone, int(cu[b]), int(cu[b + 1]), [0, lens[b]], [lens[b] + 3], [slots[b]], 1)
         assert torch.equal(rows, whole[cu[b]:cu[b + 1]]), b
     assert torch.equal(together, alone)
+
+
+@pytest.mark.parametrize("max_q", [1, 300], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("heads,size,norm_eps", [("256", 2.0 ** 61, 1e38), ("256", 2.0 ** 62, 3e38), ("h64", 2.0 ** 64, 3e38), ("h64", 1.0, 3e38)])
+def test_large_rows_beside_a_large_norm_eps(gpu, heads, size, norm_eps, max_q):
+    """Squares whose sum, or whose mean with eps, passes fp32."""
+    s, c = draw([(90, 100), (2, 5), (70, 70)], heads, BF16, seed=5)
+    c["v"] = torch.from_numpy(c["v"] * size).bfloat16().double().numpy()
+    c["state"] = (c["state"] * size).astype(np.float32).astype(np.float64)
+    c["norm"] = c["norm"] * 2.0 ** 10
+    check(gpu, s, c, BF16, True, out_dtype=BF16, max_q=max_q, scale=1.0, norm_eps=float(np.float32(norm_eps)))
