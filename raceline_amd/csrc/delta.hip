@@ -571,12 +571,13 @@ __global__ __launch_bounds__(kPrepareThreads, 2) void delta_chunks_kernel(ChunkA
   }
 }
 
-// sqrt(x^2 + y^2) of two that are not negative, by a power of two so that neither square passes fp32.
+// sqrt(x^2 + y^2) of two that are not negative, by a power of two so that neither square passes fp32. The fused operations are
+// spelled out here and in set_scale: all waves have to come to the same bits, in code that the compiler makes more than once.
 __device__ __forceinline__ float length_of(float x, float y) {
   const int ex = max(1, min(253, (int)(__float_as_uint(fmaxf(x, y)) >> 23)));
   const float down = __uint_as_float((254 - ex) << 23);
   x *= down, y *= down;
-  return __builtin_amdgcn_sqrtf(x * x + y * y) * __uint_as_float(ex << 23);
+  return __builtin_amdgcn_sqrtf(__builtin_fmaf(x, x, y * y)) * __uint_as_float(ex << 23);
 }
 
 constexpr int kChainThreads = 512;
@@ -719,7 +720,7 @@ __global__ __launch_bounds__(kChainThreads, 2) void delta_chain_kernel(ChunkArgs
   float size = 0.0f, inverse, scale, fade, value;   // size: a bound of the length of a column of S
   // the power of two that brings R, U and S of the next step under 2^15, and its inverse
   auto set_scale = [&]() {
-    const int ex = max(15, min(254, (int)(__float_as_uint(size + 9.0f * value) >> 23)));
+    const int ex = max(15, min(254, (int)(__float_as_uint(__builtin_fmaf(9.0f, value, size)) >> 23)));
     inverse = __uint_as_float((ex - 14) << 23);
     scale = __uint_as_float((268 - ex) << 23);
   };
